@@ -1,0 +1,435 @@
+// sda_bwd.hip -- softmax differential attention, backward.  With P_b the softmax maps, O_b = P_b v,
+// dP = dO v^T, r_b = rowsum(dO O_b) and lambda per row:
+//   dS_1 = P_1 (dP - r_1),  dS_2 = -lambda P_2 (dP - r_2),  dq_b = s dS_b k_b,  dk_b = s dS_b^T q_b,
+//   dv = (P_1 - lambda P_2)^T dO,  dlambda_i = -r_2.
+// One dP and one dv product serve both branches.  r_1 comes from the outputs: dO O = r_1 - lambda r_2.
+//
+//   bwd_rows   r_1, r_2 and lambda of every row (f32)
+//   bwd_keys   key-major: a wave owns 32 keys and walks the query rows that see them
+//   bwd_query  query-major: a wave owns 32 query rows and walks the keys they see
+//   bwd_sum    adds the key pass' partial sums where several workgroups share a key head
+//   bwd_lambda sums dlambda over the axes lambda is broadcast along
+// Both passes recompute the weights from the forward's log-sums: no atomics, so results do not depend
+// on the order of execution.
+#include "sda_common.hpp"
+
+namespace sda {
+
+// ------------------------------------------------------------------ row sums
+// 16 lanes per row, 16 rows per workgroup.
+template <class T, int DV>
+__global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
+  const int64_t rows = (int64_t)P.B * P.H * P.Nq;
+  const int64_t row = (int64_t)tda::grid_bid<256>() * 16 + (threadIdx.x >> 4);
+  const int c = threadIdx.x & 15;
+  if (row >= rows) return;
+  const int i = (int)(row % P.Nq);
+  const int64_t bh = row / P.Nq;
+  const int b = (int)(bh / P.H), h = (int)(bh % P.H);
+  const T* d = row_of<T>(P.dout, b, h, i);
+  const T* x = row_of<T>(P.out, b, h, i);
+  const T* y = row_of<T>(P.out2, b, h, i);
+  float rx = 0.f, ry = 0.f;
+#pragma unroll
+  for (int u = 0; u < DV / 64; ++u) {
+    const f32x4 dd = tda::load4(d + 64 * u + 4 * c), xx = tda::load4(x + 64 * u + 4 * c), yy = tda::load4(y + 64 * u + 4 * c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      rx = __builtin_fmaf(dd[e], xx[e], rx);
+      ry = __builtin_fmaf(dd[e], yy[e], ry);
+    }
+  }
+  rx = tda::group_sum<16>(rx);
+  ry = tda::group_sum<16>(ry);
+  if (c == 0) {
+    const float lam = lambda_of(P.lam, b, h, i);
+    P.stat[row] = __builtin_fmaf(lam, ry, rx);
+    P.stat[rows + row] = ry;
+    P.stat[2 * rows + row] = lam;
+  }
+}
+
+// ------------------------------------------------------------------ key-major pass
+constexpr int kKeyRows = 128;  // keys of a workgroup: 4 waves of 32
+
+template <class Tr, int D, int DV>
+struct KeyShape {
+  using QT = Tile<Tr, 32, D>;
+  using OT = Tile<Tr, 32, DV>;
+  static constexpr int STAT = 2 * QT::BYTES + OT::BYTES;  // lse1, lse2, r1, r2, lambda of the 32 rows
+  static constexpr int STAGE = STAT + 1024;
+  static constexpr int LDS = 2 * STAGE;
+  static_assert(QT::LOADS % 4 == 0 && OT::LOADS % 4 == 0, "loads spread evenly over the waves");
+};
+
+template <class Tr, int D, int DV>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) bwd_keys(BwdParams P) {
+  using T = typename Tr::T;
+  using frag = typename Tr::frag;
+  using S = KeyShape<Tr, D, DV>;
+  using QT = typename S::QT;
+  using OT = typename S::OT;
+  constexpr int NT = D / 16, NV = DV / 16, QL = QT::LOADS / 4, OL = OT::LOADS / 4;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+
+  const int l = lane_id(), n32 = l & 31, g = l >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = P.H / P.Hk, parts = G / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
+  const uint32_t bid = tda::grid_bid<256>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
+  if (bid >= heads * (uint32_t)nkt) return;
+  const Item it = item_of(bid, heads, nkt, false);
+  const int part = it.head % parts, bk = it.head / parts, b = bk / P.Hk, hk = bk % P.Hk;
+  const int h0 = hk * G + part * P.gs;
+  const int k0 = it.tile * kKeyRows, k0w = k0 + 32 * wv, key = k0w + n32;
+  const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
+  const bool live = key < len;
+  const int64_t rows = (int64_t)P.B * P.H * P.Nq;
+
+  // query tiles of 32 rows: from the first that sees the workgroup's first key on
+  const int nqt = (P.Nq + 31) / 32;
+  const int first = P.see.causal ? max(k0 - off, 0) >> 5 : 0;
+  const int per = k0 < len ? max(nqt - first, 0) : 0;
+  const int steps = per * P.gs;
+
+  uint32_t qo[2][QL], oo[OL];
+#pragma unroll
+  for (int u = 0; u < QL; ++u) {
+    qo[0][u] = QT::source(4 * u + wv, (uint32_t)(P.q[0].st * QT::ES));
+    qo[1][u] = QT::source(4 * u + wv, (uint32_t)(P.q[1].st * QT::ES));
+  }
+#pragma unroll
+  for (int u = 0; u < OL; ++u) oo[u] = OT::source(4 * u + wv, (uint32_t)(P.dout.st * OT::ES));
+  auto issue = [&](int j) {
+    const int h = h0 + j / per, i0 = 32 * (first + j % per), n = min(32, P.Nq - i0);
+    char* at = lds + (j & 1) * S::STAGE;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const auto r = rows_rsrc(row_of<T>(P.q[x], b, h, i0), P.q[x].st * QT::ES, n, D * QT::ES);
+#pragma unroll
+      for (int u = 0; u < QL; ++u) QT::load(r, reinterpret_cast<T*>(at + x * QT::BYTES), 4 * u + wv, qo[x][u]);
+    }
+    const auto r = rows_rsrc(row_of<T>(P.dout, b, h, i0), P.dout.st * OT::ES, n, DV * OT::ES);
+#pragma unroll
+    for (int u = 0; u < OL; ++u) OT::load(r, reinterpret_cast<T*>(at + 2 * QT::BYTES), 4 * u + wv, oo[u]);
+    // the rows' statistics: wave w brings lse1, lse2, r1, r2 (w = 0 .. 3), wave 0 lambda too; rows past
+    // Nq read as zeros and meet zero rows of q and dO
+    const int64_t at0 = ((int64_t)b * P.H + h) * P.Nq + i0;
+    const float* src = wv < 2 ? P.lse + wv * rows + at0 : P.stat + (wv - 2) * rows + at0;
+    if (l < 32) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, 4 * n), LDS_PTR(void, at + S::STAT + 128 * wv), 4, 4 * l, 0, 0, 0);
+      if (wv == 0)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(P.stat + 2 * rows + at0, 4 * n), LDS_PTR(void, at + S::STAT + 512), 4, 4 * l, 0, 0, 0);
+    }
+  };
+  if (steps > 0) issue(0);
+
+  frag kf[2][NT], vf[NV];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(live ? row_of<T>(P.k[x], b, hk, key) : nullptr, g, kf[x]);
+  load_frags<Tr, NV>(live ? row_of<T>(P.v, b, hk, key) : nullptr, g, vf);
+  f32x16 dk[2][D / 32] = {}, dv[DV / 32] = {};
+
+  for (int j = 0; j < steps; ++j) {
+    wait_vm<0>();
+    tda::lds_barrier();
+    if (j + 1 < steps) issue(j + 1);
+    const int i0 = 32 * (first + j % per);
+    const bool edge = P.see.causal && off + i0 < k0w + 31;  // some row does not see some key
+    if (P.see.causal && off + min(i0 + 31, P.Nq - 1) < k0w) continue;
+    const char* at = lds + (j & 1) * S::STAGE;
+    const T* ot = reinterpret_cast<const T*>(at + 2 * QT::BYTES);
+    const float* st = reinterpret_cast<const float*>(at + S::STAT);
+    f32x16 dp = {};
+#pragma unroll
+    for (int t = 0; t < NV; ++t) dp = Tr::mma32(OT::row(ot, 0, t), vf[t], dp);
+    f32x16 w;  // P_1 - lambda P_2
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const T* qt = reinterpret_cast<const T*>(at + x * QT::BYTES);
+      f32x16 s = {};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s = Tr::mma32(QT::row(qt, 0, t), kf[x][t], s);
+      f32x16 ds;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = crow(r, g);
+        float p = exp2_(__builtin_fmaf(s[r], P.c, -st[32 * x + i]));
+        float e = p * (dp[r] - st[64 + 32 * x + i]);
+        if (!live || (edge && key > off + i0 + i)) p = e = 0.f;
+        if (x == 0) {
+          w[r] = p;
+          ds[r] = e;
+        } else {
+          const float lam = st[128 + i];
+          w[r] = __builtin_fmaf(-lam, p, w[r]);
+          ds[r] = -lam * e;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const frag f = pack8<Tr>(ds, u);
+#pragma unroll
+        for (int y = 0; y < D / 32; ++y) dk[x][y] = Tr::mma32(QT::col(qt, 0, u, y), f, dk[x][y]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const frag f = pack8<Tr>(w, u);
+#pragma unroll
+      for (int y = 0; y < DV / 32; ++y) dv[y] = Tr::mma32(OT::col(ot, 0, u, y), f, dv[y]);
+    }
+  }
+  wait_vm<0>();
+
+  if (key >= P.Nk) return;
+  if (P.part) {  // dk1, dk2, dv rows of this group, f32
+    constexpr int W = 2 * D + DV;
+    float* to = P.part + (((int64_t)part * P.B * P.Hk + bk) * P.Nk + key) * W + 4 * g;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < D / 32; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store4(to + x * D + 32 * y + 8 * r, f32x4{dk[x][y][4 * r] * P.scale, dk[x][y][4 * r + 1] * P.scale, dk[x][y][4 * r + 2] * P.scale, dk[x][y][4 * r + 3] * P.scale});
+#pragma unroll
+    for (int y = 0; y < DV / 32; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        store4(to + 2 * D + 32 * y + 8 * r, f32x4{dv[y][4 * r], dv[y][4 * r + 1], dv[y][4 * r + 2], dv[y][4 * r + 3]});
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    T* to = row_of<T>(P.dk[x], b, hk, key) + 4 * g;
+#pragma unroll
+    for (int y = 0; y < D / 32; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        store4(to + 32 * y + 8 * r, f32x4{dk[x][y][4 * r] * P.scale, dk[x][y][4 * r + 1] * P.scale, dk[x][y][4 * r + 2] * P.scale, dk[x][y][4 * r + 3] * P.scale});
+  }
+  T* to = row_of<T>(P.dv, b, hk, key) + 4 * g;
+#pragma unroll
+  for (int y = 0; y < DV / 32; ++y)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) store4(to + 32 * y + 8 * r, f32x4{dv[y][4 * r], dv[y][4 * r + 1], dv[y][4 * r + 2], dv[y][4 * r + 3]});
+}
+
+// Sum of the groups' partial rows, in group order.  One thread per 4 values.
+template <class T, int D, int DV>
+__global__ void __launch_bounds__(256) bwd_sum(BwdParams P, int parts) {
+  constexpr int W = 2 * D + DV, C = W / 4;
+  const int64_t rows = (int64_t)P.B * P.Hk * P.Nk, id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
+  const int64_t row = id / C;
+  const int c = 4 * (int)(id % C);
+  if (row >= rows) return;
+  f32x4 a = *reinterpret_cast<const f32x4*>(P.part + row * W + c);
+  for (int x = 1; x < parts; ++x) a += *reinterpret_cast<const f32x4*>(P.part + (x * rows + row) * W + c);
+  const int key = (int)(row % P.Nk), b = (int)(row / P.Nk / P.Hk), h = (int)(row / P.Nk % P.Hk);
+  const Rows& to = c < D ? P.dk[0] : c < 2 * D ? P.dk[1] : P.dv;
+  store4(row_of<T>(to, b, h, key) + (c < D ? c : c < 2 * D ? c - D : c - 2 * D), a);
+}
+
+// ------------------------------------------------------------------ query-major pass
+template <class Tr, int D, int DV>
+struct QueryShape {
+  using KT = Tile<Tr, 32, D>;
+  using VT = Tile<Tr, 32, DV>;
+  static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
+  static constexpr int LDS = 2 * STAGE;
+  static_assert(KT::LOADS % 4 == 0 && VT::LOADS % 4 == 0, "loads spread evenly over the waves");
+};
+
+template <class Tr, int D, int DV>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) bwd_query(BwdParams P) {
+  using T = typename Tr::T;
+  using frag = typename Tr::frag;
+  using S = QueryShape<Tr, D, DV>;
+  using KT = typename S::KT;
+  using VT = typename S::VT;
+  constexpr int NT = D / 16, NV = DV / 16, KL = KT::LOADS / 4, VL = VT::LOADS / 4;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+
+  const int l = lane_id(), n32 = l & 31, g = l >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nqt = (P.Nq + 127) / 128;
+  const uint32_t bid = tda::grid_bid<256>();
+  if (bid >= (uint32_t)(P.B * P.H) * (uint32_t)nqt) return;
+  const Item it = item_of(bid, P.B * P.H, nqt, true);
+  const int b = it.head / P.H, h = it.head % P.H, hk = h / (P.H / P.Hk);
+  const int q0 = it.tile * 128, q0w = q0 + 32 * wv, qi = q0w + n32;
+  const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
+  const int lim = P.see.causal ? min(len, max(off + min(q0 + 128, P.Nq), 0)) : len;
+  const int limw = P.see.causal ? min(len, max(off + min(q0w + 32, P.Nq), 0)) : len;
+  const int clear = P.see.causal ? min(len, max(off + q0w + 1, 0)) : len;
+  const int see = P.see.causal ? min(len, off + qi + 1) : len;
+  const int nst = (lim + 31) / 32;
+  const int64_t rows = (int64_t)P.B * P.H * P.Nq;
+
+  uint32_t ko[2][KL], vo[VL];
+#pragma unroll
+  for (int u = 0; u < KL; ++u) {
+    ko[0][u] = KT::source(4 * u + wv, (uint32_t)(P.k[0].st * KT::ES));
+    ko[1][u] = KT::source(4 * u + wv, (uint32_t)(P.k[1].st * KT::ES));
+  }
+#pragma unroll
+  for (int u = 0; u < VL; ++u) vo[u] = VT::source(4 * u + wv, (uint32_t)(P.v.st * VT::ES));
+  auto issue = [&](int j) {
+    char* at = lds + (j & 1) * S::STAGE;
+    const int n = min(32, lim - 32 * j);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const auto r = rows_rsrc(row_of<T>(P.k[x], b, hk, 32 * (int64_t)j), P.k[x].st * KT::ES, n, D * KT::ES);
+#pragma unroll
+      for (int u = 0; u < KL; ++u) KT::load(r, reinterpret_cast<T*>(at + x * KT::BYTES), 4 * u + wv, ko[x][u]);
+    }
+    const auto r = rows_rsrc(row_of<T>(P.v, b, hk, 32 * (int64_t)j), P.v.st * VT::ES, n, DV * VT::ES);
+#pragma unroll
+    for (int u = 0; u < VL; ++u) VT::load(r, reinterpret_cast<T*>(at + 2 * KT::BYTES), 4 * u + wv, vo[u]);
+  };
+  if (nst > 0) issue(0);
+
+  const bool row = qi < P.Nq;
+  frag qf[2][NT], of[NV];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(row ? row_of<T>(P.q[x], b, h, qi) : nullptr, g, qf[x]);
+  load_frags<Tr, NV>(row ? row_of<T>(P.dout, b, h, qi) : nullptr, g, of);
+  const int64_t at0 = (int64_t)it.head * P.Nq + qi;
+  float lse[2], rs[2], lam = 0.f;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    lse[x] = row ? P.lse[x * rows + at0] : 0.f;
+    rs[x] = row ? P.stat[x * rows + at0] : 0.f;
+  }
+  if (row) lam = P.stat[2 * rows + at0];
+  f32x16 dq[2][D / 32] = {};
+
+  for (int j = 0; j < nst; ++j) {
+    wait_vm<0>();
+    tda::lds_barrier();
+    if (j + 1 < nst) issue(j + 1);
+    const int k0 = 32 * j;
+    if (k0 >= limw) continue;
+    const char* at = lds + (j & 1) * S::STAGE;
+    const T* vt = reinterpret_cast<const T*>(at + 2 * KT::BYTES);
+    f32x16 dp = {};
+#pragma unroll
+    for (int t = 0; t < NV; ++t) dp = Tr::mma32(VT::row(vt, 0, t), of[t], dp);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const T* kt = reinterpret_cast<const T*>(at + x * KT::BYTES);
+      f32x16 s = {};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s = Tr::mma32(KT::row(kt, 0, t), qf[x][t], s);
+      const float f = x ? -lam : 1.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = exp2_(__builtin_fmaf(s[r], P.c, -lse[x]));
+        s[r] = f * (p * (dp[r] - rs[x]));
+      }
+      if (k0 + 32 > clear) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + crow(r, g) >= see) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const frag e = pack8<Tr>(s, u);
+#pragma unroll
+        for (int y = 0; y < D / 32; ++y) dq[x][y] = Tr::mma32(KT::col(kt, 0, u, y), e, dq[x][y]);
+      }
+    }
+  }
+  wait_vm<0>();
+  if (!row) return;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    T* to = row_of<T>(P.dq[x], b, h, qi) + 4 * g;
+#pragma unroll
+    for (int y = 0; y < D / 32; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        store4(to + 32 * y + 8 * r, f32x4{dq[x][y][4 * r] * P.scale, dq[x][y][4 * r + 1] * P.scale, dq[x][y][4 * r + 2] * P.scale, dq[x][y][4 * r + 3] * P.scale});
+  }
+}
+
+// ------------------------------------------------------------------ dlambda
+// One workgroup per distinct element: minus the sum of r_2 over the axes it is broadcast along, each
+// thread's share in order and the threads' by a fixed tree.  `each`: nothing is summed, one thread
+// per element.
+__global__ void __launch_bounds__(256) bwd_lambda(BwdParams P, int each) {
+  const int64_t rows = (int64_t)P.B * P.H * P.Nq;
+  const float* r2 = P.stat + rows;
+  if (each) {
+    const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
+    if (id >= rows) return;
+    if (P.lam.bf16) static_cast<bf16*>(P.dlam)[id] = (bf16)-r2[id];
+    else static_cast<float*>(P.dlam)[id] = -r2[id];
+    return;
+  }
+  __shared__ float part[4];
+  const int64_t e = tda::grid_bid<256>();
+  if (e >= P.dlam_n[0] * P.dlam_n[1] * P.dlam_n[2]) return;
+  const int64_t i0 = e % P.dlam_n[2], h0 = e / P.dlam_n[2] % P.dlam_n[1], b0 = e / P.dlam_n[2] / P.dlam_n[1];
+  const int nb = P.dlam_n[0] == 1 ? P.B : 1, nh = P.dlam_n[1] == 1 ? P.H : 1, ni = P.dlam_n[2] == 1 ? P.Nq : 1;
+  float a = 0.f;
+  for (int b = 0; b < nb; ++b)
+    for (int h = 0; h < nh; ++h) {
+      const float* row = r2 + ((b0 + b) * P.H + h0 + h) * P.Nq + i0;
+      for (int i = threadIdx.x; i < ni; i += 256) a += row[i];
+    }
+  a = tda::wave_sum(a);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
+  __syncthreads();
+  if (threadIdx.x) return;
+  a = -(part[0] + part[1] + part[2] + part[3]);
+  if (P.lam.bf16) static_cast<bf16*>(P.dlam)[e] = (bf16)a;
+  else static_cast<float*>(P.dlam)[e] = a;
+}
+
+// ------------------------------------------------------------------ launches
+template <class F>
+static int big_lds(F* fn, int bytes) {
+  if (bytes <= 65536) return 0;
+  return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+template <class Tr, int D, int DV>
+static int run(const BwdParams& p, hipStream_t st) {
+  using T = typename Tr::T;
+  using KS = KeyShape<Tr, D, DV>;
+  using QS = QueryShape<Tr, D, DV>;
+  const int64_t rows = (int64_t)p.B * p.H * p.Nq;
+  int e = big_lds(&bwd_keys<Tr, D, DV>, KS::LDS);
+  if (!e) e = big_lds(&bwd_query<Tr, D, DV>, QS::LDS);
+  if (e) return e;
+  bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
+  tda::launched(st, "sda_bwd_rows");
+  const int parts = p.H / p.Hk / p.gs;
+  bwd_keys<Tr, D, DV><<<tda::grid_of<256>((int64_t)((p.Nk + kKeyRows - 1) / kKeyRows) * p.B * p.Hk * parts), 256, KS::LDS, st>>>(p);
+  tda::launched(st, "sda_bwd_keys");
+  if (p.part) {
+    const int64_t n = (int64_t)p.B * p.Hk * p.Nk * ((2 * D + DV) / 4);
+    bwd_sum<T, D, DV><<<tda::grid_of<256>((n + 255) / 256), 256, 0, st>>>(p, parts);
+    tda::launched(st, "sda_bwd_sum");
+  }
+  bwd_query<Tr, D, DV><<<tda::grid_of<256>((int64_t)((p.Nq + 127) / 128) * p.B * p.H), 256, QS::LDS, st>>>(p);
+  tda::launched(st, "sda_bwd_query");
+  if (p.dlam) {
+    const int64_t n = p.dlam_n[0] * p.dlam_n[1] * p.dlam_n[2];
+    const int each = n == rows;
+    bwd_lambda<<<tda::grid_of<256>(each ? (n + 255) / 256 : n), 256, 0, st>>>(p, each);
+    tda::launched(st, "sda_bwd_lambda");
+  }
+  return (int)hipGetLastError();
+}
+template <class Tr>
+static int pick(const BwdParams& p, int d, int dv, hipStream_t st) {
+  if (d == 64) return dv == 64 ? run<Tr, 64, 64>(p, st) : run<Tr, 64, 128>(p, st);
+  return dv == 128 ? run<Tr, 128, 128>(p, st) : run<Tr, 128, 256>(p, st);
+}
+int launch_bwd(const BwdParams& p, int dtype, int d, int dv, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == 1 ? pick<TrB>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
+}
+
+}  // namespace sda

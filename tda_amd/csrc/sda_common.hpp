@@ -1,0 +1,195 @@
+// sda_common.hpp -- device building blocks of the softmax differential attention kernels.
+//
+// Matrix-core layouts are those of tda_common.hpp.  A fragment here is always 8 contraction
+// elements per lane (16 per 32x32 product, 32 per 16x16 product); fp32 computes it as 8 steps of one
+// element, so that both types share every index below.
+#pragma once
+
+#include "sda_params.hpp"
+#include "tda_common.hpp"
+
+namespace sda {
+
+using tda::bf16;
+using tda::bf16x2;
+using tda::bf16x4;
+using tda::bf16x8;
+using tda::crow;
+using tda::f32x16;
+using tda::f32x4;
+using tda::lane_id;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Running maxima start here instead of at -inf: a masked score (-inf) then weighs exp2(-inf) = 0
+// before the first visible one too.
+constexpr float kNoMax = -1e37f;
+// A running maximum moves only when a new score passes it by this much (log2): the sums then hold
+// weights up to 2^8 instead of 1, which costs 32-bit sums nothing and saves rescaling them.
+constexpr float kSlack = 8.0f;
+
+struct TrB {
+  using T = bf16;
+  using frag = bf16x8;
+  __device__ __forceinline__ static f32x16 mma32(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 mma16(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+struct TrF {
+  using T = float;
+  using frag = f32x8;
+  __device__ __forceinline__ static f32x16 mma32(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  __device__ __forceinline__ static f32x4 mma16(frag a, frag b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Values 8 s .. 8 s + 7 of a score tile as the B operand of the next product (round to nearest
+// even; bf16 holds a weight to 2^-9, as it would hold the output).
+template <class Tr>
+__device__ __forceinline__ typename Tr::frag pack8(const f32x16& c, int s) {
+  typename Tr::frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (typename Tr::T)c[8 * s + j];
+  return f;
+}
+
+template <class T>
+__device__ __forceinline__ T* row_of(const Rows& r, int b, int h, int64_t i) {
+  return static_cast<T*>(r.p) + (int64_t)b * r.sb + (int64_t)h * r.sh + i * r.st;
+}
+__device__ __forceinline__ float lambda_of(const Lambda& l, int b, int h, int i) {
+  const int64_t at = (int64_t)b * l.sb + (int64_t)h * l.sh + (int64_t)i * l.si;
+  return l.bf16 ? (float)static_cast<const bf16*>(l.p)[at] : static_cast<const float*>(l.p)[at];
+}
+__device__ __forceinline__ int len_of(const Sight& s, int b, int Nk) {
+  return s.lens ? min(max(s.lens[b], 0), Nk) : Nk;
+}
+__device__ __forceinline__ int off_of(const Sight& s, int b) {
+  // a position beyond +-2^30 sees all or nothing already
+  return s.qoffs ? min(max(s.qoffs[b], -(1 << 30)), 1 << 30) : s.qoff;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+// Descriptor over `rows` rows of `width` bytes, `stride` bytes apart: rows past them read as zeros.
+// rows * stride stays below 2^32 (tiles of up to 64 rows, strides of at most 2^25 bytes).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t stride, int rows, int width) {
+  return rsrc_of(base, rows > 0 ? (uint32_t)((int64_t)(rows - 1) * stride + width) : 0u);
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {  // vmcnt(N) with the other counters left alone
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
+
+// ------------------------------------------------------------------ tiles in LDS
+// ROWS x W values, row-major, filled by direct buffer -> LDS loads of 16 bytes a lane: the load of
+// instruction u puts chunk 64 u + lane of the tile in place, so the bank swizzle is applied to the
+// source address: place (row, chunk) holds the row's chunk (chunk ^ swz(row)).
+template <class Tr, int ROWS, int W>
+struct Tile {
+  using T = typename Tr::T;
+  static constexpr int ES = sizeof(T);
+  static constexpr int CPR = W * ES / 16;          // 16-byte chunks of a row
+  static constexpr int BYTES = ROWS * W * ES;
+  static constexpr int LOADS = BYTES / 1024;       // load instructions (64 lanes x 16 bytes)
+  static constexpr int PER = 16 / ES;              // values of a chunk
+
+  __device__ __forceinline__ static int swz(int r) {
+    if constexpr (ES == 2) return tda::bswz<W>(r);
+    else return r & 15;
+  }
+  // Byte offset (from the tile's first row in memory) that this lane loads in instruction u.
+  __device__ __forceinline__ static uint32_t source(int u, uint32_t stride) {
+    const int ci = 64 * u + lane_id(), r = ci / CPR, c = ci % CPR;
+    return (uint32_t)r * stride + 16u * (uint32_t)(c ^ swz(r));
+  }
+  __device__ __forceinline__ static void load(__amdgpu_buffer_rsrc_t r, T* lds, int u, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(void, reinterpret_cast<char*>(lds) + 1024 * u), 16, off, 0, 0, 0);
+  }
+  // Row fragment step t: lane (m, g) gets row r0 + m, values 16 t + 8 g + [0, 8).
+  __device__ __forceinline__ static typename Tr::frag row(const T* lds, int r0, int t) {
+    const int l = lane_id(), r = r0 + (l & 31), g = l >> 5;
+    if constexpr (ES == 2) {
+      return *reinterpret_cast<const bf16x8*>(lds + r * W + 8 * ((2 * t + g) ^ swz(r)));
+    } else {
+      const int c = 4 * t + 2 * g;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * (c ^ swz(r)));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * ((c + 1) ^ swz(r)));
+      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+  // Transposed fragment, step s (16 rows from r0 + 16 s): lane (n, g) gets column 32 cs + n at rows
+  // r0 + crow(8 s + j, g), j = 0 .. 7, which is the order of a score tile's values.
+  __device__ __forceinline__ static typename Tr::frag col(const T* lds, int r0, int s, int cs) {
+    if constexpr (ES == 2) {
+      return tda::tile_tr_frag<W>(lds + r0 * W, s, cs);
+    } else {
+      const int l = lane_id(), g = l >> 5, n = 32 * cs + (l & 31);
+      f32x8 f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = r0 + crow(8 * s + j, g);
+        f[j] = lds[r * W + 4 * ((n >> 2) ^ swz(r)) + (n & 3)];
+      }
+      return f;
+    }
+  }
+};
+
+// Row fragments of one row in memory (null: zeros), lane half g.
+template <class Tr, int NT>
+__device__ __forceinline__ void load_frags(const typename Tr::T* row, int g, typename Tr::frag (&f)[NT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (row) {
+      if constexpr (sizeof(typename Tr::T) == 2) {
+        f[t] = *reinterpret_cast<const bf16x8*>(row + 16 * t + 8 * g);
+      } else {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(row + 16 * t + 8 * g);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(row + 16 * t + 8 * g + 4);
+        f[t] = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      }
+    } else {
+      f[t] = typename Tr::frag{};
+    }
+  }
+}
+
+// Store 4 consecutive values.
+__device__ __forceinline__ void store4(bf16* p, f32x4 v) { tda::store4(p, v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+
+// Workgroup ids over (heads x tiles) with the heaviest tiles first: consecutive ids go to the 8 XCDs
+// in turn, so where the heads divide evenly an XCD keeps to its own heads, whose rows its L2 then
+// serves; `late`: tile 0 is the lightest.
+struct Item { int head, tile; };
+__device__ __forceinline__ Item item_of(uint32_t bid, uint32_t heads, int tiles, bool late) {
+  Item it;
+  uint32_t t;
+  if (heads % 8 == 0) {
+    const uint32_t per = heads / 8, x = bid & 7, i = bid >> 3;
+    it.head = x * per + i % per;
+    t = i / per;
+  } else {
+    it.head = bid % heads;
+    t = bid / heads;
+  }
+  it.tile = late ? tiles - 1 - (int)t : (int)t;
+  return it;
+}
+
+}  // namespace sda

@@ -1,0 +1,449 @@
+// sda_kv4.hip -- a key/value cache held in 4 bits: append, read, and the attention of few query rows.
+//
+// A row in groups of 64 values x: m = bf16(min), s = bf16((max - m) * (1 / 15)) in 32 bits,
+// code = rint((x - m) / s) clamped to 0 .. 15, value m + s code.  4.5 bits a value.
+//
+// Codes lie so that the attention's registers need no exchange between lanes:
+//   keys: word u (32 bits) of a group holds its values 8 u .. 8 u + 7; bits 4 i hold value 2 i and bits
+//   16 + 4 i value 2 i + 1, so (word >> 4 i) & 0x000f000f is a pair of neighbours;
+//   values: 16-bit units of four neighbouring columns, bits 4 j holding column 4 n + j of group gr in
+//   unit (gr, n); a row of 64 columns holds its units in order, a wider one pairs the units (gr, n) and
+//   (gr + 1, n) of two groups in a word, words by n, then by pair.
+// Behind the codes of all rows: (m, s) of each row's groups, s in the high half of a word.
+#include "sda_decode.hpp"
+
+namespace sda {
+
+constexpr float kSmallStep = 0x1p-100f;  // a step below this is zero: all codes 0
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t bf16_bits(float x) {  // round to nearest even
+  const bf16 r = (bf16)x;
+  return __builtin_bit_cast(uint16_t, r);
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {  // 16-byte aligned
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int u = 0; u < 8 / V; ++u) {
+    const vec v = reinterpret_cast<const vec*>(p)[u];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[V * u + e] = (float)v[e];
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int u = 0; u < 8 / V; ++u) {
+    vec v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (T)x[V * u + e];
+    reinterpret_cast<vec*>(p)[u] = v;
+  }
+}
+// rint((x - m) / s) for m + 0.5 s boundaries decided exactly: x - m as an unevaluated sum hi + lo, the
+// nearest boundary p = (q + 1/2) s exact (q < 16, s of 8 bits), hi - p exact wherever its sign is in
+// doubt.  Ties go to the even code.
+__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
+  const float hi = x - m, z = hi - x, lo = (x - (hi - z)) + (-m - z);
+  const float q = floorf(fminf(fmaxf(hi * inv, 0.f), 15.f));
+  const float p = (q + 0.5f) * s, a = hi - p;
+  const int k = (int)q;
+  const bool up = a > -lo || (a == -lo && (k & 1));
+  return (uint32_t)min(k + (up ? 1 : 0), 15);
+}
+
+// ------------------------------------------------------------------ append
+// 8 lanes per group of 64 values, 8 values a lane.
+template <class T>
+__global__ void __launch_bounds__(256) kv4_append(Kv4Params P) {
+  const int z = blockIdx.z, W = z < 2 ? P.D : P.DV, L = W / 8;  // lanes of a row
+  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
+  const int u = (int)(id % L);
+  const int64_t r = id / L;  // (b, hk, i)
+  const int i = (int)(r % P.rows);
+  const int64_t bk = r / P.rows;
+  const bool in = bk < (int64_t)P.B * P.Hk;
+  const int b = in ? (int)(bk / P.Hk) : 0, hk = in ? (int)(bk % P.Hk) : 0;
+  const int start = P.start ? P.start[b] : P.lengths[b];
+  const int count = P.counts ? min(max(P.counts[b], 0), P.rows) : P.rows;
+  const int64_t at = (int64_t)start + i;
+  const bool put = in && i < count && at >= 0 && at < P.cap;
+  float x[8] = {};
+  if (put) load8(row_of<const T>(P.x[z], b, hk, i) + 8 * u, x);
+  float lo = x[0], hi = x[0];
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo = fminf(lo, x[e]);
+    hi = fmaxf(hi, x[e]);
+    bad |= !(fabsf(x[e]) < __builtin_inff());
+  }
+  lo = -tda::group_max<8>(-lo);
+  hi = tda::group_max<8>(hi);
+  bad = tda::group_max<8>(bad ? 1.f : 0.f) > 0.f;
+  const uint32_t mb = bf16_bits(lo);
+  const float m = bf16_lo(mb);
+  uint32_t sb = bf16_bits((hi - m) * (1.0f / 15.0f));
+  float s = bf16_lo(sb);
+  if (!(s >= kSmallStep)) s = 0.f, sb = 0;
+  bad |= !(s < __builtin_inff()) || !(fabsf(m) < __builtin_inff());
+  const float inv = s > 0.f && !bad ? 1.0f / s : 0.f;
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = inv > 0.f ? code_of(x[e], m, s, inv) : 0u;
+  const int64_t row = bk * P.cap + at;
+  uint32_t word;
+  int place;
+  if (z < 2) {
+    word = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) word |= (c[2 * e] << (4 * e)) | (c[2 * e + 1] << (16 + 4 * e));
+    place = u;
+  } else {
+    const uint32_t a = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12, d = c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12;
+    if (W == 64) {
+      word = a | d << 16;
+      place = u;
+    } else {  // lanes u and u + 8 (the same columns of two groups) swap a unit
+      const bool second = u & 8;
+      const uint32_t other = (uint32_t)__shfl_xor((int)(second ? a : d), 8);
+      word = second ? other | d << 16 : a | other << 16;
+      place = 16 * (u >> 4) + 2 * (u & 7) + (second ? 1 : 0);
+    }
+  }
+  if (put) {
+    reinterpret_cast<uint32_t*>(P.codes[z])[row * L + place] = word;
+    if ((u & 7) == 0) P.pars[z][row * (W / 64) + u / 8] = bad ? 0x7fc0u : mb | sb << 16;
+  }
+  if (P.start && z == 0 && in && hk == 0 && i == 0 && u == 0)
+    P.lengths[b] = (int)min(max((int64_t)start + count, (int64_t)0), (int64_t)P.cap);
+}
+__global__ void kv4_lengths(Kv4Params P) {
+  const int b = blockIdx.x * 64 + threadIdx.x;
+  if (b >= P.B) return;
+  const int count = P.counts ? min(max(P.counts[b], 0), P.rows) : P.rows;
+  P.lengths[b] = (int)min((int64_t)max(P.lengths[b], 0) + count, (int64_t)P.cap);
+}
+
+// ------------------------------------------------------------------ read
+template <class T>
+__global__ void __launch_bounds__(256) kv4_read(Kv4Params P) {
+  const int z = blockIdx.z, W = z < 2 ? P.D : P.DV, L = W / 8;
+  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
+  const int u = (int)(id % L);
+  const int64_t r = id / L;
+  const int i = (int)(r % P.rows);
+  const int64_t bk = r / P.rows;
+  if (bk >= (int64_t)P.B * P.Hk) return;
+  const int b = (int)(bk / P.Hk), hk = (int)(bk % P.Hk);
+  float x[8] = {};
+  if (i < min(P.lengths[b], P.cap)) {
+    const int64_t row = bk * P.cap + i;
+    const uint32_t par = P.pars[z][row * (W / 64) + u / 8];
+    const float m = bf16_lo(par), s = bf16_hi(par);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.codes[z]) + row * L;
+    if (z < 2) {
+      const uint32_t w = words[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s, (float)(w >> (4 * (e >> 1) + 16 * (e & 1)) & 15), m);
+    } else {
+      uint32_t a, d;  // units of columns 8 u' .. + 3 and + 4 .. + 7
+      if (W == 64) {
+        const uint32_t w = words[u];
+        a = w & 0xffff;
+        d = w >> 16;
+      } else {
+        const uint32_t w0 = words[16 * (u >> 4) + 2 * (u & 7)], w1 = words[16 * (u >> 4) + 2 * (u & 7) + 1];
+        a = u & 8 ? w0 >> 16 : w0 & 0xffff;
+        d = u & 8 ? w1 >> 16 : w1 & 0xffff;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = __builtin_fmaf(s, (float)(a >> (4 * e) & 15), m);
+        x[4 + e] = __builtin_fmaf(s, (float)(d >> (4 * e) & 15), m);
+      }
+    }
+  }
+  store8(row_of<T>(P.x[z], b, hk, i) + 8 * u, x);
+}
+
+// ------------------------------------------------------------------ attention
+// NP: bf16 parts that a query value and a weight are split into: 1 (bf16 queries), 2 (f16: 16 bits), 3
+// (f32: 24 bits); a product with a code is exact in each.  Codes become bf16 by setting 0x4300 above
+// them (128 + code); the 128 leaves through the sums of the other operand.  f32 and f16 convert the
+// codes themselves: 128 times the sum would cost them bits.  Values are taken around their middle, m + 8 s
+// + s (code - 8): the rounding of weight * s then counts with |s (code - 8)|, about the value itself, and
+// not with s code (bf16 outputs of a short cache: 3.3e-3 off without, 2.3e-3 with).
+template <class T, int NP, int D_, int DV_>
+struct Kv4Src {
+  using Out = T;
+  static constexpr int D = D_, DV = DV_, GK = D / 64, GV = DV / 64, WV = DV / 128 ? DV / 128 : 1;
+  struct Regs {
+    uint32_t k[2][2][GK][2];      // [branch][16 keys][group][word 2 kq + i]
+    uint32_t kp[2][2][4][GK];     // [branch][16 keys][key 4 kq + r][group]
+    uint32_t v[8][WV];            // [key][pair of groups]
+    uint32_t vp[8][GV];
+  };
+  const Kv4Params* C;
+  bf16x8 q[2][NP][GK][2];
+  float qs[2][GK];                // sum of a group's query values
+  float corr[2][GV];              // what every column of a group still gets
+  const uint32_t *kc[2], *kpar[2], *vc, *vpar;
+
+  __device__ __forceinline__ static bf16x8 codes(uint32_t w) {  // 8 codes of a key word, in value order
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = pair(w >> (4 * i));
+    return __builtin_bit_cast(bf16x8, x);
+  }
+  __device__ __forceinline__ static uint32_t pair(uint32_t w) {
+    if constexpr (NP == 1) {
+      return (w & 0x000f000fu) | 0x43004300u;
+    } else {
+      const float a = (float)(w & 15u), b = (float)(w >> 16 & 15u);  // exact: their low halves are zero
+      return __builtin_bit_cast(uint32_t, a) >> 16 | __builtin_bit_cast(uint32_t, b);
+    }
+  }
+  static constexpr float kBias = NP == 1 ? 128.f : 0.f;
+  // x as NP bf16 parts
+  __device__ __forceinline__ static void split(float x, bf16 (&p)[NP]) {
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      p[e] = (bf16)x;
+      x -= (float)p[e];
+    }
+  }
+
+  __device__ __forceinline__ void begin(const DecParams& P, int b, int hk, int h, int i, bool live) {
+    const int kq = lane_id() >> 4;
+    const int64_t row0 = ((int64_t)b * P.Hk + hk) * P.Nk;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      kc[x] = reinterpret_cast<const uint32_t*>(C->codes[x]) + row0 * (D / 8);
+      kpar[x] = C->pars[x] + row0 * GK;
+      const T* r = row_of<const T>(P.q[x], b, h, i);
+#pragma unroll
+      for (int y = 0; y < GK; ++y) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float f[8] = {};
+          if (live) load8(r + 64 * y + 16 * kq + 8 * w, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            a += f[e];
+            bf16 p[NP];
+            split(f[e], p);
+#pragma unroll
+            for (int z = 0; z < NP; ++z) q[x][z][y][w][e] = p[z];
+          }
+        }
+        a += __shfl_xor(a, 16);
+        qs[x][y] = a + __shfl_xor(a, 32);
+      }
+#pragma unroll
+      for (int y = 0; y < GV; ++y) corr[x][y] = 0.f;
+    }
+    vc = reinterpret_cast<const uint32_t*>(C->codes[2]) + row0 * (DV / 8);
+    vpar = C->pars[2] + row0 * GV;
+  }
+  __device__ __forceinline__ void load(Regs& g, int t0, int lim, bool edge) {
+    const int n = lane_id() & 15, kq = lane_id() >> 4;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int64_t key = min(t0 + 16 * y + n, lim - 1);
+#pragma unroll
+        for (int z = 0; z < GK; ++z) {
+          const uint2 w = *reinterpret_cast<const uint2*>(kc[x] + key * (D / 8) + 8 * z + 2 * kq);
+          g.k[x][y][z][0] = w.x;
+          g.k[x][y][z][1] = w.y;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t k = min(t0 + 16 * y + 4 * kq + r, lim - 1);
+#pragma unroll
+          for (int z = 0; z < GK; ++z) g.kp[x][y][r][z] = kpar[x][k * GK + z];
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = t0 + 16 * (j >> 2) + 4 * kq + (j & 3);
+      const int64_t k = min(key, lim - 1);
+      const uint32_t* w = vc + k * (DV / 8);
+#pragma unroll
+      for (int z = 0; z < WV; ++z) g.v[j][z] = DV == 64 ? w[n >> 1] : w[16 * z + n];
+#pragma unroll
+      for (int z = 0; z < GV; ++z) {
+        g.vp[j][z] = vpar[k * GV + z];
+        if (edge && key >= lim) g.vp[j][z] = 0;  // weight 0: nothing, whatever the row holds
+      }
+    }
+  }
+  __device__ __forceinline__ void scores(const Regs& g, int x, f32x4 (&s)[2]) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      s[y] = f32x4{};
+#pragma unroll
+      for (int z = 0; z < GK; ++z) {
+        f32x4 a = {};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const bf16x8 c = codes(g.k[x][y][z][w]);
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) a = TrB::mma16(c, q[x][p][z][w], a);  // small parts first
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float sc = bf16_hi(g.kp[x][y][r][z]), m = bf16_lo(g.kp[x][y][r][z]);
+          s[y][r] = __builtin_fmaf(sc, __builtin_fmaf(-kBias, qs[x][z], a[r]), __builtin_fmaf(m, qs[x][z], s[y][r]));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void rescale(int x, float f) {
+#pragma unroll
+    for (int y = 0; y < GV; ++y) corr[x][y] *= f;
+  }
+  __device__ __forceinline__ void add(const Regs& g, int x, const f32x4 (&s)[2], f32x4 (&o)[DV / 16]) {
+#pragma unroll
+    for (int z = 0; z < GV; ++z) {
+      bf16x8 p[NP];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = s[j >> 2][j & 3];
+        bf16 e[NP];
+        split(w * bf16_hi(g.vp[j][z]), e);
+        float used = 0.f;
+#pragma unroll
+        for (int y = 0; y < NP; ++y) {
+          p[y][j] = e[y];
+          used += (float)e[y];
+        }
+        const float mid = __builtin_fmaf(8.f, bf16_hi(g.vp[j][z]), bf16_lo(g.vp[j][z]));
+        corr[x][z] = __builtin_fmaf(w, mid, __builtin_fmaf(-(kBias + 8.f), used, corr[x][z]));
+      }
+      uint32_t half[4];  // keys 2 i, 2 i + 1: the units of this group, side by side
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = g.v[2 * i][z / 2], b = g.v[2 * i + 1][z / 2];
+        const bool up = DV == 64 ? lane_id() & 1 : z & 1;
+        half[i] = up ? __builtin_amdgcn_perm(b, a, 0x07060302) : __builtin_amdgcn_perm(b, a, 0x05040100);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pair(half[i] >> (4 * c));
+        const bf16x8 a = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+        for (int y = NP - 1; y >= 0; --y) o[4 * z + c] = TrB::mma16(a, p[y], o[4 * z + c]);
+      }
+    }
+  }
+  __device__ __forceinline__ void finish(f32x4 (&o)[2][DV / 16]) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int z = 0; z < GV; ++z) {
+        float a = corr[x][z];
+        a += __shfl_xor(a, 16);
+        a += __shfl_xor(a, 32);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[x][4 * z + c] += a;
+      }
+  }
+  __device__ __forceinline__ static int column(int t, int m) { return 64 * (t / 4) + 4 * m + t % 4; }
+};
+
+template <class T, int NP, int D, int DV>
+__global__ void __launch_bounds__(256) kv4_attend(DecParams P, Kv4Params C) {
+  extern __shared__ float lds[];
+  Kv4Src<T, NP, D, DV> src;
+  src.C = &C;
+  decode_body(P, src, lds);
+}
+
+// ------------------------------------------------------------------ launches
+int launch_kv4_append(const Kv4Params& p, int dtype, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  const int W = p.D > p.DV ? p.D : p.DV;
+  const int64_t n = (int64_t)p.B * p.Hk * p.rows * (W / 8);
+  dim3 grid = tda::grid_of<256>((n + 255) / 256);
+  grid.z = 3;
+  if (dtype == 0) kv4_append<float><<<grid, 256, 0, st>>>(p);
+  else if (dtype == 1) kv4_append<bf16><<<grid, 256, 0, st>>>(p);
+  else kv4_append<_Float16><<<grid, 256, 0, st>>>(p);
+  tda::launched(st, "sda_kv4_append");
+  if (!p.start) {  // every workgroup above reads the lengths
+    kv4_lengths<<<dim3((unsigned)((p.B + 63) / 64)), 64, 0, st>>>(p);
+    tda::launched(st, "sda_kv4_lengths");
+  }
+  return (int)hipGetLastError();
+}
+int launch_kv4_read(const Kv4Params& p, int dtype, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  const int W = p.D > p.DV ? p.D : p.DV;
+  const int64_t n = (int64_t)p.B * p.Hk * p.rows * (W / 8);
+  dim3 grid = tda::grid_of<256>((n + 255) / 256);
+  grid.z = 3;
+  if (dtype == 0) kv4_read<float><<<grid, 256, 0, st>>>(p);
+  else if (dtype == 1) kv4_read<bf16><<<grid, 256, 0, st>>>(p);
+  else kv4_read<_Float16><<<grid, 256, 0, st>>>(p);
+  tda::launched(st, "sda_kv4_read");
+  return (int)hipGetLastError();
+}
+template <class T, int NP, int D, int DV>
+static int run(const DecParams& p, const Kv4Params& c, hipStream_t st) {
+  constexpr int LDS = kDecLds<DV>;
+  if (LDS > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_attend<T, NP, D, DV>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return (int)e;
+  }
+  const int64_t items = (int64_t)p.B * p.Hk * ((p.H / p.Hk * (int64_t)p.Nq + kDecRows - 1) / kDecRows);
+  kv4_attend<T, NP, D, DV><<<tda::grid_of<256>(items * p.nsplit), 256, LDS, st>>>(p, c);
+  tda::launched(st, "sda_kv4_attend");
+  if (p.nsplit > 1) {
+    decode_join<T><<<tda::grid_of<256>(items * (DV / 16)), 256, 0, st>>>(p);
+    tda::launched(st, "sda_decode_join");
+  }
+  return (int)hipGetLastError();
+}
+template <class T, int NP>
+static int pick(const DecParams& p, const Kv4Params& c, hipStream_t st) {
+  if (p.D == 64) return p.DV == 64 ? run<T, NP, 64, 64>(p, c, st) : run<T, NP, 64, 128>(p, c, st);
+  return p.DV == 128 ? run<T, NP, 128, 128>(p, c, st) : run<T, NP, 128, 256>(p, c, st);
+}
+int launch_kv4_attend(const Kv4Params& c, int dtype, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  DecParams p{};
+  p.q[0] = c.q[0];
+  p.q[1] = c.q[1];
+  p.out = c.out;
+  p.lam = c.lam;
+  p.see.lens = c.lengths;
+  p.tail = 1;
+  p.B = c.B;
+  p.H = c.H;
+  p.Hk = c.Hk;
+  p.Nq = c.Nq;
+  p.Nk = c.cap;
+  p.D = c.D;
+  p.DV = c.DV;
+  p.c = c.c;
+  p.part = c.part;
+  p.nsplit = c.nsplit;
+  p.chunk = c.chunk;
+  if (dtype == 0) return pick<float, 3>(p, c, st);
+  return dtype == 1 ? pick<bf16, 1>(p, c, st) : pick<_Float16, 2>(p, c, st);
+}
+
+}  // namespace sda

@@ -1,0 +1,192 @@
+"""A key/value cache of softmax differential attention held in 4 bits, and the attention over it."""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from . import _sda_abi
+from .softmax import (_CODE, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _launch, _new_rows, _scale, _usable,
+                       differential_attention)
+
+_PUT = struct.Struct("<Q").pack_into
+_DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
+_ATTEND_OFF = {n: getattr(_sda_abi.SdaKv4AttendArgs, n).offset for n in ("q1", "q2", "out", "lambda_param", "workspace")}
+_APPEND_OFF = {n: getattr(_sda_abi.SdaKv4AppendArgs, n).offset for n in ("k1", "k2", "v", "start", "counts")}
+_READ_OFF = {n: getattr(_sda_abi.SdaKv4ReadArgs, n).offset for n in ("k1", "k2", "v")}
+_FEW = 32  # query rows that share a key head: up to here attend() reads the codes themselves
+
+
+class Int4KVCache:
+    """The k1, k2 and v rows of up to `capacity` positions for each of `batch` sequences, 4.5 bits a value.
+
+    Every row is held in groups of 64 values x as m = bf16(min x), s = bf16((max x - m) * (1 / 15)) (in 32
+    bits) and codes rint((x - m) / s) in 0 .. 15 (ties to even; all 0 when s < 2^-100); it stands for m + s
+    code.  A group with a NaN or an infinity reads as NaN.  (head_dim, v_head_dim): (64, 64), (64, 128), (128, 128) or (128, 256).
+
+    `lengths` (int32, (batch,), on the device) counts the rows each sequence holds; the calls read and
+    write it on the GPU, without synchronising, so they can be captured into a graph.  A program may set
+    it, to drop rows or to hand a place to another sequence.  The cache carries no gradient."""
+
+    def __init__(self, batch: int, kv_heads: int, capacity: int, head_dim: int, v_head_dim: int | None = None, *,
+                 device="cuda"):
+        v_head_dim = head_dim if v_head_dim is None else v_head_dim
+        for name, n in (("batch", batch), ("kv_heads", kv_heads), ("capacity", capacity)):
+            if n < 1:
+                raise ValueError(f"{name} must be at least 1, got {n}")
+        if (head_dim, v_head_dim) not in _DIMS:
+            raise ValueError(f"(head_dim, v_head_dim) must be one of {_DIMS}, got {(head_dim, v_head_dim)}")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"tda_amd runs on the GPU only (HIP); got {device}")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.batch, self.kv_heads, self.capacity = int(batch), int(kv_heads), int(capacity)
+        self.head_dim, self.v_head_dim, self.device = int(head_dim), int(v_head_dim), device
+        lib = _sda_abi.load()
+        self._held = [torch.empty(lib.sda_kv4_bytes(batch, kv_heads, capacity, w), dtype=torch.uint8, device=device)
+                      for w in (head_dim, head_dim, v_head_dim)]
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._lengths_at = None
+        self._templates: dict = {}
+
+    # -------------------------------------------------------------- calls
+    def _cache(self) -> _sda_abi.SdaKv4:
+        c = _sda_abi.SdaKv4()
+        c.batch, c.kv_heads, c.capacity = self.batch, self.kv_heads, self.capacity
+        c.head_dim, c.v_head_dim = self.head_dim, self.v_head_dim
+        c.k1, c.k2, c.v = (t.data_ptr() for t in self._held)
+        c.lengths = self.lengths.data_ptr()
+        return c
+
+    def _template(self, key, build):
+        """The argument block of a call, cached by its configuration (this cache's own buffers are part
+        of it)."""
+        n = self.lengths
+        if not isinstance(n, torch.Tensor) or n.shape != (self.batch,) or n.dtype != torch.int32 or n.device != self.device \
+                or not n.is_contiguous():
+            raise ValueError(f"lengths must be a contiguous int32 tensor of shape ({self.batch},) on {self.device}")
+        if n.data_ptr() != self._lengths_at or len(self._templates) > 64:
+            self._templates.clear()
+            self._lengths_at = n.data_ptr()
+        got = self._templates.get(key)
+        if got is None:
+            got = self._templates[key] = build()
+        return got
+
+    def _check(self, tensors, names, shapes):
+        _check_rows(tensors, names)
+        for t, n, s in zip(tensors, names, shapes):
+            if t.shape != s:
+                raise ValueError(f"{n} must have shape {tuple(s)}, got {tuple(t.shape)}")
+        if tensors[0].device != self.device:
+            raise ValueError(f"device mismatch: the cache is on {self.device}, {names[0]} on {tensors[0].device}")
+        if tensors[0].dtype not in _CODE:
+            raise ValueError(f"unsupported dtype {tensors[0].dtype}")
+
+    def append(self, k1, k2, v, counts=None, start=None):
+        """Add the rows of new positions: k1, k2 (batch, kv_heads, n, head_dim), v (..., n, v_head_dim),
+        float32, bfloat16 or float16, n <= capacity.
+
+        Row i of sequence b goes to position lengths[b] + i, or start[b] + i where start (int32/int64,
+        (batch,)) is given, for i < counts[b] (all n by default; rows past it are padding and are not
+        read); lengths[b] becomes the position behind the last one.  Positions outside 0 .. capacity - 1
+        are dropped, and lengths stops at the capacity: a caller that must not lose rows keeps count."""
+        n = k1.shape[2] if isinstance(k1, torch.Tensor) and k1.dim() == 4 else 0
+        b, hk = self.batch, self.kv_heads
+        self._check((k1, k2, v), ("k1", "k2", "v"),
+                    ((b, hk, n, self.head_dim), (b, hk, n, self.head_dim), (b, hk, n, self.v_head_dim)))
+        if n > self.capacity:
+            raise ValueError(f"{n} rows do not fit a cache of {self.capacity}")
+        counts = None if counts is None else _ints(counts, b, self.device, "counts")
+        start = None if start is None else _ints(start, b, self.device, "start")
+        if n == 0:
+            if start is not None:
+                self.lengths.copy_(start.clamp(0, self.capacity))
+            return
+        rows = [_usable(t.detach()) for t in (k1, k2, v)]
+
+        def build():
+            a = _sda_abi.SdaKv4AppendArgs()
+            a.abi_version, a.dtype, a.cache, a.rows = _sda_abi.ABI_VERSION, _CODE[rows[0].dtype], self._cache(), n
+            for name, t in zip(("k1", "k2", "v"), rows):
+                getattr(a, name).stride[:] = t.stride()
+            return bytes(a)
+
+        buf = bytearray(self._template(("append", n, rows[0].dtype, tuple(t.stride() for t in rows)), build))
+        for name, t in zip(("k1", "k2", "v", "start", "counts"), (*rows, start, counts)):
+            if t is not None:
+                _PUT(buf, _APPEND_OFF[name], t.data_ptr())
+        _launch(_sda_abi.load().sda_kv4_append, _sda_abi.SdaKv4AppendArgs, buf, self.device, "sda_kv4_append")
+
+    def read(self, rows: int | None = None, dtype=torch.bfloat16):
+        """The first `rows` (default: capacity) positions as tensors k1, k2, v of a dtype; positions a
+        sequence does not hold are zero."""
+        n = self.capacity if rows is None else int(rows)
+        if not 1 <= n <= self.capacity:
+            raise ValueError(f"rows must be 1 to {self.capacity}, got {n}")
+        if dtype not in _CODE:
+            raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+        res = tuple(torch.empty((self.batch, self.kv_heads, n, w), dtype=dtype, device=self.device)
+                    for w in (self.head_dim, self.head_dim, self.v_head_dim))
+
+        def build():
+            a = _sda_abi.SdaKv4ReadArgs()
+            a.abi_version, a.dtype, a.cache, a.rows = _sda_abi.ABI_VERSION, _CODE[dtype], self._cache(), n
+            for name, t in zip(("k1", "k2", "v"), res):
+                getattr(a, name).stride[:] = t.stride()
+            return bytes(a)
+
+        buf = bytearray(self._template(("read", n, dtype), build))
+        for name, t in zip(("k1", "k2", "v"), res):
+            _PUT(buf, _READ_OFF[name], t.data_ptr())
+        _launch(_sda_abi.load().sda_kv4_read, _sda_abi.SdaKv4ReadArgs, buf, self.device, "sda_kv4_read")
+        return res
+
+    def attend(self, q1, q2, lambda_param, scale=None):
+        """Softmax differential attention of q1, q2 (batch, heads, n, head_dim), the last n positions of each
+        sequence, over the cache: row i of sequence b sees the keys up to lengths[b] - n + i (a row before
+        the sequence's first position is zero).  Returns (batch, heads, n, v_head_dim); no gradient.
+
+        Few rows (n heads / kv_heads <= 32, as in decoding) are computed from the codes; more, as a
+        prompt's chunk, from the rows that read() gives in q1's dtype."""
+        b, hk = self.batch, self.kv_heads
+        if isinstance(q1, torch.Tensor) and q1.dim() == 4:
+            h, n = q1.shape[1], q1.shape[2]
+        else:
+            h, n = hk, 0
+        self._check((q1, q2), ("q1", "q2"), ((b, h, n, self.head_dim),) * 2)
+        _check_heads(h, hk)
+        s = _scale(scale, self.head_dim)
+        lam = _lambda(lambda_param, b, h, n, self.device).detach()
+        if n == 0:
+            return torch.zeros((b, h, 0, self.v_head_dim), dtype=q1.dtype, device=self.device)
+        if h // hk * n > _FEW:
+            with torch.no_grad():
+                return differential_attention(q1, q2, *self.read(dtype=q1.dtype), lam, s, q_offset=self.lengths - n,
+                                              kv_lens=self.lengths)
+        q1, q2 = _usable(q1.detach()), _usable(q2.detach())
+        out = _new_rows(q1, self.v_head_dim)
+        ls = _lambda_strides(lam)
+
+        def build():
+            a = _sda_abi.SdaKv4AttendArgs()
+            a.abi_version, a.dtype, a.cache = _sda_abi.ABI_VERSION, _CODE[q1.dtype], self._cache()
+            a.heads, a.seq_len, a.scale = h, n, s
+            for name, t in zip(("q1", "q2", "out"), (q1, q2, out)):
+                getattr(a, name).stride[:] = t.stride()
+            a.lambda_stride[:] = ls
+            a.lambda_dtype = _CODE[lam.dtype]
+            a.workspace_bytes = _sda_abi.load().sda_kv4_attend_workspace_bytes(ctypes.byref(a))
+            return bytes(a), a.workspace_bytes
+
+        key = ("attend", h, n, s, q1.dtype, lam.dtype, ls, q1.stride(), q2.stride())
+        tpl, size = self._template(key, build)
+        buf = bytearray(tpl)
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+        for name, t in zip(("q1", "q2", "out", "lambda_param", "workspace"), (q1, q2, out, lam, ws)):
+            if t is not None:
+                _PUT(buf, _ATTEND_OFF[name], t.data_ptr())
+        _launch(_sda_abi.load().sda_kv4_attend, _sda_abi.SdaKv4AttendArgs, buf, self.device, "sda_kv4_attend")
+        return out

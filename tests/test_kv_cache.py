@@ -1,0 +1,308 @@
+"""The 4-bit cache (tda_amd.Int4KVCache): what it holds against the definition, exactly; the attention over
+it against float64 on the values held, within the bounds of oracle/softmax.py."""
+import math
+
+import pytest
+import torch
+
+import tda_amd
+from oracle import softmax as oracle
+
+BF, F32, F16 = torch.bfloat16, torch.float32, torch.float16
+U = {BF: 2.0 ** -8, F32: 2.0 ** -24, F16: 2.0 ** -11}
+DIMS = [(64, 64), (64, 128), (128, 128), (128, 256)]
+gpu = pytest.mark.gpu
+
+
+def rows(b, h, n, d, seed, dtype, level=0.0):
+    g = torch.Generator("cpu").manual_seed(seed)
+    x = torch.randn(b, n, h, d, generator=g) + level * torch.randn(1, 1, h, d, generator=g)
+    return x.to(dtype).cuda().transpose(1, 2)
+
+
+def context(b, hk, n, d, dv, dtype, seed=0):
+    return rows(b, hk, n, d, seed, dtype, 1.5), rows(b, hk, n, d, seed + 1, dtype, 1.5), rows(b, hk, n, dv, seed + 2, dtype)
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0)) and torch.equal(a.isnan(), b.isnan())
+
+
+def held(x, dtype=F32):
+    return oracle.held4(x).float().to(dtype)  # m + s code has at most 24 bits when their exponents are near
+
+
+# ------------------------------------------------------------------ what it holds
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+@pytest.mark.parametrize("d, dv", DIMS)
+@pytest.mark.parametrize("n", [1, 7, 130])
+def test_append_and_read(dtype, d, dv, n):
+    c = tda_amd.Int4KVCache(2, 3, 131, d, dv)
+    xs = context(2, 3, n, d, dv, dtype)
+    c.append(*xs)
+    assert c.lengths.tolist() == [n, n]
+    for got, x in zip(c.read(n, F32), xs):
+        want = oracle.held4(x)
+        assert ((got.double() - want).abs() <= 2.0 ** -24 * want.abs()).all()  # one rounding of m + s code
+    for got, x, w in zip(c.read(dtype=BF), xs, (d, d, dv)):
+        assert got.shape == (2, 3, 131, w) and not got[:, :, n:].any()
+        assert torch.equal(got[:, :, :n], held(x, BF))
+
+
+@gpu
+def test_values_next_to_borders():
+    """Inputs laid on and one step beside every border between codes, with steps that are no power of two;
+    constant groups, groups of zeros, a step below the smallest, subnormals."""
+    m, s = torch.tensor(-1.0), torch.tensor(0.171875)
+    q = torch.arange(15, dtype=torch.float64)
+    border = (m.double() + (q + 0.5) * s.double()).float()
+    up, down = (torch.nextafter(border, torch.tensor(w)) for w in (math.inf, -math.inf))
+    row = torch.cat((m[None], border, up, down, (m + 15 * s)[None]))
+    row = torch.cat((row, row[:1].expand(64 - row.numel())))
+    lines = [row, torch.zeros(64), torch.full((64,), 3.7), torch.linspace(1, 1 + 1e-6, 64), 1e-33 * torch.arange(64.0),
+             2.0 ** -140 * torch.arange(64.0), torch.cat((torch.full((63,), 1e-20), torch.ones(1))), -row * 1e30]
+    x = torch.stack(lines)[None, None].cuda()  # (1, 1, 8, 64)
+    c = tda_amd.Int4KVCache(1, 1, 8, 64, 64)
+    c.append(x, x, x)
+    for got in c.read(dtype=F32):
+        want = oracle.held4(x)
+        assert ((got.double() - want).abs() <= 2.0 ** -24 * want.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_group_that_is_not_finite(bad):
+    xs = [x.clone() for x in context(1, 2, 5, 128, 128, BF)]
+    for x in xs:
+        x[0, 1, 3, 70] = bad
+    c = tda_amd.Int4KVCache(1, 2, 5, 128)
+    c.append(*xs)
+    for got, x in zip(c.read(dtype=F32), xs):
+        nan = torch.zeros_like(got, dtype=torch.bool)
+        nan[0, 1, 3, 64:] = True
+        assert torch.equal(got.isnan(), nan) and same(got, held(x))
+
+
+@gpu
+def test_ragged_appends_leave_other_rows_alone():
+    c = tda_amd.Int4KVCache(3, 2, 40, 64, 128)
+    first = context(3, 2, 20, 64, 128, BF)
+    c.append(*first, counts=torch.tensor([20, 3, 0]).cuda())
+    assert c.lengths.tolist() == [20, 3, 0]
+    second = context(3, 2, 25, 64, 128, BF, seed=9)
+    c.append(*second, counts=torch.tensor([25, 7, 40], dtype=torch.int32).cuda())  # 45 > 40: dropped; 40 > 25: clamped
+    assert c.lengths.tolist() == [40, 10, 25]
+    for got, a, b in zip(c.read(dtype=F32), first, second):
+        a, b = held(a), held(b)
+        assert torch.equal(got[0], torch.cat((a[0], b[0, :, :20]), 1))
+        assert torch.equal(got[1, :, :10], torch.cat((a[1, :, :3], b[1, :, :7]), 1)) and not got[1, :, 10:].any()
+        assert torch.equal(got[2, :, :25], b[2])
+    # one sequence rewritten from an earlier position; places outside the cache are dropped
+    third = context(3, 2, 2, 64, 128, BF, seed=20)
+    c.append(*third, start=torch.tensor([5, 39, -1]).cuda())
+    assert c.lengths.tolist() == [7, 40, 1]
+    c.lengths.fill_(40)
+    for got, a, b, t in zip(c.read(dtype=F32), first, second, third):
+        a, b, t = held(a), held(b), held(t)
+        assert torch.equal(got[0, :, 5:7], t[0]) and torch.equal(got[0, :, 7:20], a[0, :, 7:])
+        assert torch.equal(got[1, :, 39], t[1, :, 0])
+        assert torch.equal(got[2, :, 0], t[2, :, 1]) and torch.equal(got[2, :, 1:25], b[2, :, 1:])
+
+
+# ------------------------------------------------------------------ attention over it
+def attend(c, q1, q2, lam, scale=None):
+    """The oracle on the values that the cache holds."""
+    n = q1.shape[2]
+    ks = [x.double() for x in c.read(dtype=F32)]
+    lens = c.lengths.clamp(0, c.capacity).cpu()
+    return oracle.attention(q1, q2, *ks, lam, scale, u=U[BF] if q1.dtype == BF else 2.0 ** -16 if q1.dtype == F16 else U[F32],
+                            q_offset=lens - n, kv_lens=lens), ks
+
+
+def close(got, ref, c, ks, q1, q2, dtype):
+    """The oracle's bound counts the sums' magnitudes with the held values; the kernel sums m and s code
+    (bf16: s (128 + code), its 128 taken off) apart: up to 64 times the group's largest value for bf16 and
+    5 times otherwise, in 24 bits.  That enters as a share of the largest magnitudes."""
+    times = 64 if dtype == BF else 6
+    f, d = 2.0 ** -24, c.head_dim
+    big = max(x.abs().max().item() for x in ks[2:])
+    score = max(q.double().abs().sum(-1).max().item() * k.abs().max().item() for q, k in ((q1, ks[0]), (q2, ks[1]))) / math.sqrt(d)
+    extra = 4 * times * f * (score * big + (c.capacity ** 0.5 + 16) * big)
+    off = ref["out_off"] + U[dtype] * ref["out"].abs() + extra
+    if dtype == BF:  # weight times step is rounded, around a group's middle: up to 8 steps of 1/15 of its range
+        off = off + U[BF] * ref["around"]
+    assert ((got.double() - ref["out"]).abs() <= off).all()
+
+
+def around(c, q1, q2, lam):
+    """sum over keys of (P1 + |lambda| P2) times 8 steps of the value's group, per output."""
+    v = c.read(dtype=F32)[2].double().nan_to_num()
+    y = v.unflatten(-1, (-1, 64))
+    reach = ((y.amax(-1, keepdim=True) - y.amin(-1, keepdim=True)).expand_as(y)).flatten(-2)
+    lens = c.lengths.clamp(0, c.capacity).cpu()
+    k1, k2 = (x.double() for x in c.read(dtype=F32)[:2])
+    a = oracle.attention(q1, q2, k1, k2, reach, torch.tensor(0.0), q_offset=lens - q1.shape[2], kv_lens=lens)["out"]
+    b = oracle.attention(q2, q1, k2, k1, reach, torch.tensor(0.0), q_offset=lens - q1.shape[2], kv_lens=lens)["out"]
+    return a + oracle.lambda_rows(lam, *q1.shape[:3], q1.device).abs() * b
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+@pytest.mark.parametrize("d, dv", DIMS)
+@pytest.mark.parametrize("h, hk, n, cap", [(1, 1, 1, 1), (8, 8, 1, 1000), (8, 2, 1, 33), (40, 2, 1, 300), (4, 4, 4, 129),
+                                           (6, 3, 7, 520), (4, 2, 16, 2000), (4, 1, 70, 300)])
+def test_attend(dtype, d, dv, h, hk, n, cap):
+    c = tda_amd.Int4KVCache(3, hk, cap, d, dv)
+    c.append(*context(3, hk, cap, d, dv, dtype))
+    c.lengths.copy_(torch.tensor([cap, (cap + 1) // 2, 0]))
+    q1, q2 = rows(3, h, n, d, 50, dtype), rows(3, h, n, d, 51, dtype)
+    lam = torch.linspace(-0.5, 0.9, h).cuda()
+    got = c.attend(q1, q2, lam)
+    assert got.dtype == dtype and not got[2].any()
+    if h // hk * n > 32:  # by way of read(): the values rounded to the queries' type
+        ks = c.read(dtype=dtype)
+        want = tda_amd.differential_attention(q1, q2, *ks, lam, q_offset=c.lengths - n, kv_lens=c.lengths)
+        assert torch.equal(got, want)
+        return
+    ref, ks = attend(c, q1, q2, lam)
+    ref["around"] = around(c, q1, q2, lam)
+    close(got, ref, c, ks, q1, q2, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_decoding_steps(dtype):
+    """A run of steps as a serving program makes them: a prompt, then token by token."""
+    b, h, hk, d = 2, 8, 2, 64
+    c = tda_amd.Int4KVCache(b, hk, 64, d)
+    prompt = context(b, hk, 30, d, d, dtype)
+    c.append(*prompt, counts=torch.tensor([30, 11]).cuda())
+    for t in range(20):
+        c.append(*context(b, hk, 1, d, d, dtype, seed=100 + 3 * t))
+        q1, q2 = rows(b, h, 1, d, 300 + t, dtype), rows(b, h, 1, d, 400 + t, dtype)
+        got = c.attend(q1, q2, 0.4)
+        ref, ks = attend(c, q1, q2, 0.4)
+        ref["around"] = around(c, q1, q2, 0.4)
+        close(got, ref, c, ks, q1, q2, dtype)
+    assert c.lengths.tolist() == [50, 31]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_nothing_behind_the_length_is_read(dtype):
+    c = tda_amd.Int4KVCache(2, 2, 200, 64, 128)
+    bad = [x.clone() for x in context(2, 2, 200, 64, 128, dtype)]
+    for x in bad:
+        x[0, :, 77:] = math.nan
+        x[1, :, 130:] = math.inf
+    c.append(*bad)
+    lens = torch.tensor([77, 130], dtype=torch.int32)
+    c.lengths.copy_(lens)
+    q1, q2 = rows(2, 4, 2, 64, 50, dtype), rows(2, 4, 2, 64, 51, dtype)
+    got = c.attend(q1, q2, 0.5)
+    ref, ks = attend(c, q1, q2, 0.5)
+    ref["around"] = around(c, q1, q2, 0.5)
+    close(got, ref, c, ks, q1, q2, dtype)
+    # lengths out of range are clamped
+    c.lengths.copy_(torch.tensor([-3, 1000]))
+    got = c.attend(q1, q2, 0.5)
+    assert not got[0].any() and got[1].isnan().any()
+
+
+@gpu
+def test_captured_steps():
+    """Two graphs of append and attend on caches of their own, replayed between eager steps on a third."""
+    b, h, hk, d = 2, 8, 2, 128
+    new = [x.contiguous() for x in context(b, hk, 1, d, d, BF, seed=7)]
+    q1, q2 = rows(b, h, 1, d, 50, BF).contiguous(), rows(b, h, 1, d, 51, BF).contiguous()
+    caches = [tda_amd.Int4KVCache(b, hk, 3000, d) for _ in range(3)]
+    for c in caches:
+        c.append(*context(b, hk, 2500, d, d, BF), counts=torch.tensor([2500, 1200]).cuda())
+        c.append(*new)
+        c.attend(q1, q2, 0.3)
+        c.lengths.sub_(1)
+
+    def step(c):
+        c.append(*new)
+        return c.attend(q1, q2, 0.3)
+
+    graphs, outs = [], []
+    for c in caches[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(c))
+        graphs.append(g)
+    for k in range(3):
+        for x in (*new, q1, q2):
+            x.mul_(1.1 + 0.1 * k)
+        want = step(caches[2])
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for c, got in zip(caches, outs):
+            assert torch.equal(got, want) and torch.equal(c.lengths, caches[2].lengths)
+    assert caches[0].lengths.tolist() == [2503, 1203]
+
+
+@gpu
+def test_other_stream_and_replaced_lengths():
+    c = tda_amd.Int4KVCache(1, 2, 500, 64)
+    c.append(*context(1, 2, 400, 64, 64, BF))
+    q1, q2 = rows(1, 4, 1, 64, 50, BF), rows(1, 4, 1, 64, 51, BF)
+    want = c.attend(q1, q2, 0.5)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = c.attend(q1, q2, 0.5)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    c.lengths = torch.full((1,), 300, dtype=torch.int32, device="cuda")
+    short = c.attend(q1, q2, 0.5)
+    d = tda_amd.Int4KVCache(1, 2, 300, 64)
+    d.append(*(x[:, :, :300] for x in context(1, 2, 400, 64, 64, BF)))
+    assert (short - d.attend(q1, q2, 0.5)).abs().max() <= 2.0 ** -6 * short.abs().max()  # another split of the keys
+    for wrong in (torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros(1, dtype=torch.int32), None):
+        c.lengths = wrong
+        with pytest.raises(ValueError):
+            c.attend(q1, q2, 0.5)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals_without_a_gpu():
+    for args in ((0, 1, 4, 64), (1, 0, 4, 64), (1, 1, 0, 64), (1, 1, 4, 32), (1, 1, 4, 128, 64), (1, 1, 4, 64, 96)):
+        with pytest.raises(ValueError):
+            tda_amd.Int4KVCache(*args)
+    with pytest.raises(ValueError, match="GPU only"):
+        tda_amd.Int4KVCache(1, 1, 4, 64, device="cpu")
+
+
+@gpu
+def test_refusals():
+    c = tda_amd.Int4KVCache(2, 2, 10, 64, 128)
+    k, v = torch.zeros(2, 2, 3, 64, device="cuda"), torch.zeros(2, 2, 3, 128, device="cuda")
+    many = torch.zeros(2, 2, 11, 64, device="cuda"), torch.zeros(2, 2, 11, 64, device="cuda"), torch.zeros(2, 2, 11, 128, device="cuda")
+    for args in ((k, k, k), (k, k[:, :1], v), (k, k[:, :, :2], v), (k[:1], k[:1], v[:1]), (k.double(),) * 2 + (v.double(),),
+                 (k.half(), k, v), (k.cpu(), k.cpu(), v.cpu()), many):
+        with pytest.raises(ValueError):
+            c.append(*args)
+    for kw in (dict(counts=torch.zeros(3, dtype=torch.int32, device="cuda")), dict(start=torch.zeros(2, device="cuda")),
+               dict(counts=torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            c.append(k, k, v, **kw)
+    with pytest.raises(TypeError):
+        c.append(None, k, v)
+    for n in (0, 11, -1):
+        with pytest.raises(ValueError):
+            c.read(n)
+    with pytest.raises(ValueError):
+        c.read(dtype=torch.float64)
+    q = torch.zeros(2, 4, 1, 64, device="cuda")
+    for args in ((q, q[:, :2], 0.5), (q[:, :3], q[:, :3], 0.5), (q[:1], q[:1], 0.5), (q, q, torch.zeros(3)), (q.double(), q.double(), 0.5)):
+        with pytest.raises(ValueError):
+            c.attend(*args)
+    with pytest.raises(ValueError):
+        c.attend(q, q, 0.5, scale=-1.0)
+    assert c.lengths.tolist() == [0, 0]
+    c.append(k[:, :, :0], k[:, :, :0], v[:, :, :0])
+    assert c.attend(q[:, :, :0], q[:, :, :0], 0.5).shape == (2, 4, 0, 128)
