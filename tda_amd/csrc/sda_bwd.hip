@@ -128,6 +128,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(live ? row_of<T>(P.k[x], b, hk, key) : nullptr, g, kf[x]);
   load_frags<Tr, NV>(live ? row_of<T>(P.v, b, hk, key) : nullptr, g, vf);
   f32x16 dk[2][D / 32] = {}, dv[DV / 32] = {};
+  pin(dk[0]);
+  pin(dk[1]);
+  pin(dv);
 
   for (int j = 0; j < steps; ++j) {
     wait_vm<0>();
@@ -139,49 +142,58 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
     const char* at = lds + (j & 1) * S::STAGE;
     const T* ot = reinterpret_cast<const T*>(at + 2 * QT::BYTES);
     const float* st = reinterpret_cast<const float*>(at + S::STAT);
-    f32x16 dp = {};
-#pragma unroll
-    for (int t = 0; t < NV; ++t) dp = Tr::mma32(OT::row(ot, 0, t), vf[t], dp);
+    const f32x16 dp = chain<Tr, NV>([&](int t) { return OT::row(ot, 0, t); }, vf);
     f32x16 w;  // P_1 - lambda P_2
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const T* qt = reinterpret_cast<const T*>(at + x * QT::BYTES);
-      f32x16 s = {};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s = Tr::mma32(QT::row(qt, 0, t), kf[x][t], s);
+      f32x16 s = chain<Tr, NT>([&](int t) { return QT::row(qt, 0, t); }, kf[x]);
       f32x16 ds;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = crow(r, g);
-        float p = exp2_(__builtin_fmaf(s[r], P.c, -st[32 * x + i]));
-        float e = p * (dp[r] - st[64 + 32 * x + i]);
-        if (!live || (edge && key > off + i0 + i)) p = e = 0.f;
-        if (x == 0) {
-          w[r] = p;
-          ds[r] = e;
-        } else {
-          const float lam = st[128 + i];
-          w[r] = __builtin_fmaf(-lam, p, w[r]);
-          ds[r] = -lam * e;
+        s[r] = exp2_(__builtin_fmaf(s[r], P.c, -st[32 * x + i]));
+        ds[r] = s[r] * (dp[r] - st[64 + 32 * x + i]);
+      }
+      if (edge) {
+        asm volatile("");  // a branch: few tiles need this
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool hide = key > off + i0 + crow(r, g);
+          s[r] = hide ? 0.f : s[r];
+          ds[r] = hide ? 0.f : ds[r];
         }
       }
+      if (x == 0) {
+        w = s;
+      } else {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag f = pack8<Tr>(ds, u);
-#pragma unroll
-        for (int y = 0; y < D / 32; ++y) dk[x][y] = Tr::mma32(QT::col(qt, 0, u, y), f, dk[x][y]);
+        for (int r = 0; r < 16; ++r) {
+          const float lam = st[128 + crow(r, g)];
+          w[r] = __builtin_fmaf(-lam, s[r], w[r]);
+          ds[r] *= -lam;
+        }
       }
+      const frag f[2] = {pack8<Tr>(ds, 0), pack8<Tr>(ds, 1)};
+      columns<Tr, D / 32>([&](int u, int y) { return QT::col(qt, 0, u, y); }, f, dk[x]);
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const frag f = pack8<Tr>(w, u);
-#pragma unroll
-      for (int y = 0; y < DV / 32; ++y) dv[y] = Tr::mma32(OT::col(ot, 0, u, y), f, dv[y]);
-    }
+    const frag f[2] = {pack8<Tr>(w, 0), pack8<Tr>(w, 1)};
+    columns<Tr, DV / 32>([&](int u, int y) { return OT::col(ot, 0, u, y); }, f, dv);
   }
   wait_vm<0>();
 
   if (key >= P.Nk) return;
+  // a key past the length met weights of its own making (of a zero row): its column holds nothing else
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < D / 32; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[x][y][r] = live ? dk[x][y][r] * P.scale : 0.f;
+#pragma unroll
+  for (int y = 0; y < DV / 32; ++y)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dv[y][r] = live ? dv[y][r] : 0.f;
   if (P.part) {  // dk1, dk2, dv rows of this group, f32
     constexpr int W = 2 * D + DV;
     float* to = P.part + (((int64_t)part * P.B * P.Hk + bk) * P.Nk + key) * W + 4 * g;
@@ -191,7 +203,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
       for (int y = 0; y < D / 32; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          store4(to + x * D + 32 * y + 8 * r, f32x4{dk[x][y][4 * r] * P.scale, dk[x][y][4 * r + 1] * P.scale, dk[x][y][4 * r + 2] * P.scale, dk[x][y][4 * r + 3] * P.scale});
+          store4(to + x * D + 32 * y + 8 * r, f32x4{dk[x][y][4 * r], dk[x][y][4 * r + 1], dk[x][y][4 * r + 2], dk[x][y][4 * r + 3]});
 #pragma unroll
     for (int y = 0; y < DV / 32; ++y)
 #pragma unroll
@@ -206,7 +218,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
     for (int y = 0; y < D / 32; ++y)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        store4(to + 32 * y + 8 * r, f32x4{dk[x][y][4 * r] * P.scale, dk[x][y][4 * r + 1] * P.scale, dk[x][y][4 * r + 2] * P.scale, dk[x][y][4 * r + 3] * P.scale});
+        store4(to + 32 * y + 8 * r, f32x4{dk[x][y][4 * r], dk[x][y][4 * r + 1], dk[x][y][4 * r + 2], dk[x][y][4 * r + 3]});
   }
   T* to = row_of<T>(P.dv, b, hk, key) + 4 * g;
 #pragma unroll
@@ -303,6 +315,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   }
   if (row) lam = P.stat[2 * rows + at0];
   f32x16 dq[2][D / 32] = {};
+  pin(dq[0]);
+  pin(dq[1]);
 
   for (int j = 0; j < nst; ++j) {
     wait_vm<0>();
@@ -312,15 +326,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
     if (k0 >= limw) continue;
     const char* at = lds + (j & 1) * S::STAGE;
     const T* vt = reinterpret_cast<const T*>(at + 2 * KT::BYTES);
-    f32x16 dp = {};
-#pragma unroll
-    for (int t = 0; t < NV; ++t) dp = Tr::mma32(VT::row(vt, 0, t), of[t], dp);
+    const f32x16 dp = chain<Tr, NV>([&](int t) { return VT::row(vt, 0, t); }, of);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const T* kt = reinterpret_cast<const T*>(at + x * KT::BYTES);
-      f32x16 s = {};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s = Tr::mma32(KT::row(kt, 0, t), qf[x][t], s);
+      f32x16 s = chain<Tr, NT>([&](int t) { return KT::row(kt, 0, t); }, qf[x]);
       const float f = x ? -lam : 1.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -328,16 +338,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
         s[r] = f * (p * (dp[r] - rs[x]));
       }
       if (k0 + 32 > clear) {
+        asm volatile("");  // a branch: few tiles need this
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (k0 + crow(r, g) >= see) s[r] = 0.f;
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag e = pack8<Tr>(s, u);
-#pragma unroll
-        for (int y = 0; y < D / 32; ++y) dq[x][y] = Tr::mma32(KT::col(kt, 0, u, y), e, dq[x][y]);
-      }
+      const frag e[2] = {pack8<Tr>(s, 0), pack8<Tr>(s, 1)};
+      columns<Tr, D / 32>([&](int u, int y) { return KT::col(kt, 0, u, y); }, e, dq[x]);
     }
   }
   wait_vm<0>();

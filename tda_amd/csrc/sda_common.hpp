@@ -169,6 +169,58 @@ __device__ __forceinline__ void load_frags(const typename Tr::T* row, int g, typ
   }
 }
 
+// acc += a(t) b(t) over NT steps, the operands a read from LDS a group of four steps ahead of their use
+// and no further (see tda::mma_chain): left to itself the compiler waits for every read by itself.
+template <class Tr, int NT, class FA>
+__device__ __forceinline__ f32x16 chain(FA&& a, const typename Tr::frag (&b)[NT]) {
+  constexpr int G = sizeof(typename Tr::T) == 2 ? 4 : 2;
+  static_assert(NT % G == 0, "whole groups");
+  typename Tr::frag f[2][G];
+  f32x16 acc = {};
+#pragma unroll
+  for (int t0 = -G; t0 < NT; t0 += G) {
+    if (t0 + G < NT) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) f[(t0 / G + 1) & 1][u] = a(t0 + G + u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 >= 0) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) acc = Tr::mma32(f[(t0 / G) & 1][u], b[t0 + u], acc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return acc;
+}
+// acc[y] += col(u, y) b[u] for a transposed tile of 32 rows and NY blocks of 32 columns, the operands read
+// four ahead in the same way.
+template <class Tr, int NY, class FA>
+__device__ __forceinline__ void columns(FA&& col, const typename Tr::frag (&b)[2], f32x16 (&acc)[NY]) {
+  constexpr int G = sizeof(typename Tr::T) == 2 && NY * 2 % 4 == 0 ? 4 : 2, N = 2 * NY;
+  typename Tr::frag f[2][G];
+#pragma unroll
+  for (int t0 = -G; t0 < N; t0 += G) {
+    if (t0 + G < N) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) f[(t0 / G + 1) & 1][u] = col((t0 + G + u) / NY, (t0 + G + u) % NY);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 >= 0) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) acc[(t0 + u) % NY] = Tr::mma32(f[(t0 / G) & 1][u], b[(t0 + u) / NY], acc[(t0 + u) % NY]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Accumulators that a loop carries stay whole in accumulation registers: known to start at zero, they
+// would be taken apart into 16 floats each, which are moved there and back in every iteration.
+template <int N>
+__device__ __forceinline__ void pin(f32x16 (&acc)[N]) {
+#pragma unroll
+  for (int y = 0; y < N; ++y) asm("" : "+a"(acc[y]));
+}
+
 // Store 4 consecutive values.
 __device__ __forceinline__ void store4(bf16* p, f32x4 v) { tda::store4(p, v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }

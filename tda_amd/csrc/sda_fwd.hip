@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
       for (int t = 0; t < NT; ++t) s[x] = Tr::mma32(KT::row(kt, 32 * x, t), qf[t], s[x]);
     }
     if (k0 + BN > clear) {
+      asm volatile("");  // a branch: few tiles need this
 #pragma unroll
       for (int x = 0; x < NS; ++x)
 #pragma unroll
