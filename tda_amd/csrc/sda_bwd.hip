@@ -16,6 +16,8 @@
 namespace sda {
 
 // ------------------------------------------------------------------ row sums
+// What the passes need of a row, so that it enters their products as a starting value: the log-sums as
+// -lse_b / c (score and weight: P = 2^(c (q k - lse / c))), -r_1, r_1 - r_2, -lambda; and r_2 for dlambda.
 // 16 lanes per row, 16 rows per workgroup.
 template <class T, int DV>
 __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
@@ -42,26 +44,33 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
   rx = tda::group_sum<16>(rx);
   ry = tda::group_sum<16>(ry);
   if (c == 0) {
-    const float lam = lambda_of(P.lam, b, h, i);
-    P.stat[row] = __builtin_fmaf(lam, ry, rx);
-    P.stat[rows + row] = ry;
-    P.stat[2 * rows + row] = lam;
+    const float lam = lambda_of(P.lam, b, h, i), r1 = __builtin_fmaf(lam, ry, rx), inv = 1.0f / P.c;
+    P.stat[row] = -P.lse[row] * inv;
+    P.stat[rows + row] = -P.lse[rows + row] * inv;
+    P.stat[2 * rows + row] = -r1;
+    P.stat[3 * rows + row] = r1 - ry;
+    P.stat[4 * rows + row] = -lam;
+    P.stat[5 * rows + row] = ry;
   }
 }
 
 // ------------------------------------------------------------------ key-major pass
-constexpr int kKeyRows = 128;  // keys of a workgroup: 4 waves of 32
+constexpr int kKeyRows = 128;  // keys of a workgroup: 4 groups of 32
 
 template <class Tr, int D, int DV>
 struct KeyShape {
   using QT = Tile<Tr, 32, D>;
   using OT = Tile<Tr, 32, DV>;
-  static constexpr int STAT = 2 * QT::BYTES + OT::BYTES;  // lse1, lse2, r1, r2, lambda of the 32 rows
+  static constexpr int STAT = 2 * QT::BYTES + OT::BYTES;  // the statistics of the 32 rows
   static constexpr int STAGE = STAT + 1024;
   static constexpr int LDS = 2 * STAGE;
   static_assert(QT::LOADS % 4 == 0 && OT::LOADS % 4 == 0, "loads spread evenly over the waves");
 };
 
+// One wave per SIMD (the three gradients' accumulators and the resident rows fill the registers), so
+// the wave hides its own latencies: the LDS operands of a step are one sequence, read a group ahead of their
+// use, and the first branch's weights are computed between the second's score products, the second's
+// between the first's gradient products.
 template <class Tr, int D, int DV>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) bwd_keys(BwdParams P) {
   using T = typename Tr::T;
@@ -70,16 +79,21 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   using QT = typename S::QT;
   using OT = typename S::OT;
   constexpr int NT = D / 16, NV = DV / 16, QL = QT::LOADS / 4, OL = OT::LOADS / 4;
+  constexpr int G = sizeof(T) == 2 ? 4 : 1;  // an fp32 fragment is eight products itself
+  // The statistics enter the products as their starting values; f32 adds them after, where a sum that starts
+  // far from zero would cost it bits.
+  constexpr bool START = sizeof(T) == 2;
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = P.H / P.Hk, parts = G / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
+  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
   const uint32_t bid = tda::grid_bid<256>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
   if (bid >= heads * (uint32_t)nkt) return;
   const Item it = item_of(bid, heads, nkt, false);
   const int part = it.head % parts, bk = it.head / parts, b = bk / P.Hk, hk = bk % P.Hk;
-  const int h0 = hk * G + part * P.gs;
+  const int h0 = hk * GQ + part * P.gs;
   const int k0 = it.tile * kKeyRows, k0w = k0 + 32 * wv, key = k0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   const bool live = key < len;
@@ -99,8 +113,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   }
 #pragma unroll
   for (int u = 0; u < OL; ++u) oo[u] = OT::source(4 * u + wv, (uint32_t)(P.dout.st * OT::ES));
-  auto issue = [&](int j) {
-    const int h = h0 + j / per, i0 = 32 * (first + j % per), n = min(32, P.Nq - i0);
+  auto issue = [&](int j, int h, int qt) {  // step j: query tile qt of head h
+    const int i0 = 32 * qt, n = min(32, P.Nq - i0);
     char* at = lds + (j & 1) * S::STAGE;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -111,17 +125,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
     const auto r = rows_rsrc(row_of<T>(P.dout, b, h, i0), P.dout.st * OT::ES, n, DV * OT::ES);
 #pragma unroll
     for (int u = 0; u < OL; ++u) OT::load(r, reinterpret_cast<T*>(at + 2 * QT::BYTES), 4 * u + wv, oo[u]);
-    // the rows' statistics: wave w brings lse1, lse2, r1, r2 (w = 0 .. 3), wave 0 lambda too; rows past
-    // Nq read as zeros and meet zero rows of q and dO
-    const int64_t at0 = ((int64_t)b * P.H + h) * P.Nq + i0;
-    const float* src = wv < 2 ? P.lse + wv * rows + at0 : P.stat + (wv - 2) * rows + at0;
+    // the rows' statistics; rows past Nq read as zeros and meet zero rows of q and dO
+    const float* src = P.stat + ((int64_t)b * P.H + h) * P.Nq + i0;
     if (l < 32) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, 4 * n), LDS_PTR(void, at + S::STAT + 128 * wv), 4, 4 * l, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + wv * rows, 4 * n), LDS_PTR(void, at + S::STAT + 128 * wv), 4, 4 * l, 0, 0, 0);
       if (wv == 0)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(P.stat + 2 * rows + at0, 4 * n), LDS_PTR(void, at + S::STAT + 512), 4, 4 * l, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + 4 * rows, 4 * n), LDS_PTR(void, at + S::STAT + 512), 4, 4 * l, 0, 0, 0);
     }
   };
-  if (steps > 0) issue(0);
+  if (steps > 0) issue(0, h0, first);
 
   frag kf[2][NT], vf[NV];
 #pragma unroll
@@ -132,54 +144,107 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   pin(dk[1]);
   pin(dv);
 
-  for (int j = 0; j < steps; ++j) {
-    wait_vm<0>();
-    tda::lds_barrier();
-    if (j + 1 < steps) issue(j + 1);
-    const int i0 = 32 * (first + j % per);
+  auto step = [&](const char* at, int i0) {
     const bool edge = P.see.causal && off + i0 < k0w + 31;  // some row does not see some key
-    if (P.see.causal && off + min(i0 + 31, P.Nq - 1) < k0w) continue;
-    const char* at = lds + (j & 1) * S::STAGE;
+    const T* qt[2] = {reinterpret_cast<const T*>(at), reinterpret_cast<const T*>(at + QT::BYTES)};
     const T* ot = reinterpret_cast<const T*>(at + 2 * QT::BYTES);
     const float* st = reinterpret_cast<const float*>(at + S::STAT);
-    const f32x16 dp = chain<Tr, NV>([&](int t) { return OT::row(ot, 0, t); }, vf);
-    f32x16 w;  // P_1 - lambda P_2
+    // the sequence: dO rows (dP), q1 rows, q2 rows (scores), q1 columns (dk1), q2 columns (dk2), dO columns (dv)
+    constexpr int E1 = NV, E2 = E1 + NT, E3 = E2 + NT, E4 = E3 + D / 16, E5 = E4 + D / 16, E6 = E5 + DV / 16;
+    frag f[AHEAD + 1][G];
+    auto read = [&](auto i) {  // group i of it
+      times<G>([&](auto u) {
+        constexpr int e = i * G + u;
+        frag& to = f[i % (AHEAD + 1)][u];
+        if constexpr (e < E1) to = OT::row(ot, 0, e);
+        else if constexpr (e < E2) to = QT::row(qt[0], 0, e - E1);
+        else if constexpr (e < E3) to = QT::row(qt[1], 0, e - E2);
+        else if constexpr (e < E4) to = QT::col(qt[0], 0, (e - E3) / (D / 32), (e - E3) % (D / 32));
+        else if constexpr (e < E5) to = QT::col(qt[1], 0, (e - E4) / (D / 32), (e - E4) % (D / 32));
+        else to = OT::col(ot, 0, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
+      });
+    };
+    auto rowstat = [&](int z) {  // statistic z of the lane's 16 rows
+      f32x16 x;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const T* qt = reinterpret_cast<const T*>(at + x * QT::BYTES);
-      f32x16 s = chain<Tr, NT>([&](int t) { return QT::row(qt, 0, t); }, kf[x]);
-      f32x16 ds;
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(st + 32 * z + 8 * r + 4 * g);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = crow(r, g);
-        s[r] = exp2_(__builtin_fmaf(s[r], P.c, -st[32 * x + i]));
-        ds[r] = s[r] * (dp[r] - st[64 + 32 * x + i]);
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = w[e];
       }
+      return x;
+    };
+    times<AHEAD>([&](auto i) { read(i); });
+    f32x16 dp = START ? rowstat(2) : f32x16{}, s[2], w, dif, lam;
+    frag ds[2][2], wf[2];
+    auto hide = [&](f32x16& x) {
       if (edge) {
         asm volatile("");  // a branch: few tiles need this
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool hide = key > off + i0 + crow(r, g);
-          s[r] = hide ? 0.f : s[r];
-          ds[r] = hide ? 0.f : ds[r];
-        }
+        for (int r = 0; r < 16; ++r) x[r] = key > off + i0 + crow(r, g) ? -__builtin_inff() : x[r];
       }
-      if (x == 0) {
-        w = s;
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float lam = st[128 + crow(r, g)];
-          w[r] = __builtin_fmaf(-lam, s[r], w[r]);
-          ds[r] *= -lam;
+    };
+    auto weight = [&](int x, int r) {
+      return START ? exp2_(P.c * s[x][r]) : exp2_(__builtin_fmaf(P.c, s[x][r], P.c * st[32 * x + crow(r, g)]));
+    };
+    auto first_branch = [&](int r) {
+      const float p = weight(0, r);
+      w[r] = p;
+      s[0][r] = p * (START ? dp[r] : dp[r] + st[64 + crow(r, g)]);
+    };
+    auto second_branch = [&](int r) {
+      const float p = lam[r] * weight(1, r);
+      w[r] += p;
+      s[1][r] = p * (START ? dp[r] + dif[r] : dp[r] + (dif[r] + st[64 + crow(r, g)]));
+    };
+    constexpr int NG = E6 / G;
+    times<NG>([&](auto i) {
+      if constexpr (i + AHEAD < NG) read(std::integral_constant<int, i + AHEAD>());
+      if constexpr (i * G == E2) hide(s[0]);
+      if constexpr (i * G == E3) hide(s[1]);
+      if constexpr (i * G == E1 - G) s[0] = START ? rowstat(0) : f32x16{};
+      if constexpr (i * G == E2 - G) s[1] = START ? rowstat(1) : f32x16{};
+      if constexpr (i * G == E3 - G) dif = rowstat(3), lam = rowstat(4);
+      __builtin_amdgcn_sched_barrier(0);
+      times<G>([&](auto u) {
+        constexpr int e = i * G + u;
+        const frag& a = f[i % (AHEAD + 1)][u];
+        if constexpr (e < E1) dp = Tr::mma32(a, vf[e], dp);
+        else if constexpr (e < E2) s[0] = Tr::mma32(a, kf[0][e - E1], s[0]);
+        else if constexpr (e < E3) s[1] = Tr::mma32(a, kf[1][e - E2], s[1]);
+        else if constexpr (e < E4) dk[0][(e - E3) % (D / 32)] = Tr::mma32(a, ds[0][(e - E3) / (D / 32)], dk[0][(e - E3) % (D / 32)]);
+        else if constexpr (e < E5) dk[1][(e - E4) % (D / 32)] = Tr::mma32(a, ds[1][(e - E4) / (D / 32)], dk[1][(e - E4) % (D / 32)]);
+        else dv[(e - E5) % (DV / 32)] = Tr::mma32(a, wf[(e - E5) / (DV / 32)], dv[(e - E5) % (DV / 32)]);
+        // between them, the weights: 16 rows over the segment's products
+        if constexpr (e >= E2 && e < E3) {
+          constexpr int n = 16 / NT;
+          times<n>([&](auto r) { first_branch((e - E2) * n + r); });
+          if constexpr (e == E3 - 1) ds[0][0] = pack8<Tr>(s[0], 0), ds[0][1] = pack8<Tr>(s[0], 1);
         }
-      }
-      const frag f[2] = {pack8<Tr>(ds, 0), pack8<Tr>(ds, 1)};
-      columns<Tr, D / 32>([&](int u, int y) { return QT::col(qt, 0, u, y); }, f, dk[x]);
-    }
-    const frag f[2] = {pack8<Tr>(w, 0), pack8<Tr>(w, 1)};
-    columns<Tr, DV / 32>([&](int u, int y) { return OT::col(ot, 0, u, y); }, f, dv);
+        if constexpr (e >= E3 && e < E4) {
+          constexpr int n = 16 / (D / 16);
+          times<n>([&](auto r) { second_branch((e - E3) * n + r); });
+          if constexpr (e == E4 - 1) {
+            ds[1][0] = pack8<Tr>(s[1], 0), ds[1][1] = pack8<Tr>(s[1], 1);
+            wf[0] = pack8<Tr>(w, 0), wf[1] = pack8<Tr>(w, 1);
+          }
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  int h = h0, qt = first, nh = h0, nq = first;  // of this step, and of the one on its way
+  for (int j = 0; j < steps; ++j) {
+    wait_vm<0>();
+    tda::lds_barrier();
+    if (++nq == nqt) nq = first, ++nh;
+    if (j + 1 < steps) issue(j + 1, nh, nq);
+    const int i0 = 32 * qt;
+    const char* at = lds + (j & 1) * S::STAGE;
+    step(at, i0);
+    h = nh, qt = nq;
   }
+  (void)h;
   wait_vm<0>();
 
   if (key >= P.Nk) return;
@@ -194,37 +259,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   for (int y = 0; y < DV / 32; ++y)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dv[y][r] = live ? dv[y][r] : 0.f;
-  if (P.part) {  // dk1, dk2, dv rows of this group, f32
-    constexpr int W = 2 * D + DV;
-    float* to = P.part + (((int64_t)part * P.B * P.Hk + bk) * P.Nk + key) * W + 4 * g;
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < D / 32; ++y)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store4(to + x * D + 32 * y + 8 * r, f32x4{dk[x][y][4 * r], dk[x][y][4 * r + 1], dk[x][y][4 * r + 2], dk[x][y][4 * r + 3]});
-#pragma unroll
-    for (int y = 0; y < DV / 32; ++y)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store4(to + 2 * D + 32 * y + 8 * r, f32x4{dv[y][4 * r], dv[y][4 * r + 1], dv[y][4 * r + 2], dv[y][4 * r + 3]});
-    return;
-  }
+  constexpr int W = 2 * D + DV;
+  float* pt = P.part ? P.part + (((int64_t)part * P.B * P.Hk + bk) * P.Nk + key) * W + 4 * g : nullptr;  // dk1, dk2, dv, f32
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     T* to = row_of<T>(P.dk[x], b, hk, key) + 4 * g;
 #pragma unroll
     for (int y = 0; y < D / 32; ++y)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store4(to + 32 * y + 8 * r, f32x4{dk[x][y][4 * r], dk[x][y][4 * r + 1], dk[x][y][4 * r + 2], dk[x][y][4 * r + 3]});
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 z = {dk[x][y][4 * r], dk[x][y][4 * r + 1], dk[x][y][4 * r + 2], dk[x][y][4 * r + 3]};
+        if (pt) store4(pt + x * D + 32 * y + 8 * r, z);
+        else store4(to + 32 * y + 8 * r, z);
+      }
   }
   T* to = row_of<T>(P.dv, b, hk, key) + 4 * g;
 #pragma unroll
   for (int y = 0; y < DV / 32; ++y)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) store4(to + 32 * y + 8 * r, f32x4{dv[y][4 * r], dv[y][4 * r + 1], dv[y][4 * r + 2], dv[y][4 * r + 3]});
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 z = {dv[y][4 * r], dv[y][4 * r + 1], dv[y][4 * r + 2], dv[y][4 * r + 3]};
+      if (pt) store4(pt + 2 * D + 32 * y + 8 * r, z);
+      else store4(to + 32 * y + 8 * r, z);
+    }
 }
 
 // Sum of the groups' partial rows, in group order.  One thread per 4 values.
@@ -243,33 +300,36 @@ __global__ void __launch_bounds__(256) bwd_sum(BwdParams P, int parts) {
 }
 
 // ------------------------------------------------------------------ query-major pass
-template <class Tr, int D, int DV>
+template <class Tr, int D, int DV, bool SPLIT>
 struct QueryShape {
   using KT = Tile<Tr, 32, D>;
   using VT = Tile<Tr, 32, DV>;
+  static constexpr int WAVES = SPLIT ? 8 : 4;
   static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
-  static constexpr int LDS = 2 * STAGE;
-  static_assert(KT::LOADS % 4 == 0 && VT::LOADS % 4 == 0, "loads spread evenly over the waves");
+  static constexpr int RING = 2;
+  static constexpr int LDS = RING * STAGE;
+  static constexpr int KL = (KT::LOADS + WAVES - 1) / WAVES, VL = (VT::LOADS + WAVES - 1) / WAVES;
+  static constexpr int MIN_LOADS = 2 * (KT::LOADS / WAVES) + VT::LOADS / WAVES;  // of a wave, a stage
 };
 
-template <class Tr, int D, int DV>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) bwd_query(BwdParams P) {
+template <class Tr, int D, int DV, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves_per_eu(SPLIT || (sizeof(typename Tr::T) == 2 && D == 64) ? 2 : 1))) bwd_query(BwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
-  using S = QueryShape<Tr, D, DV>;
+  using S = QueryShape<Tr, D, DV, SPLIT>;
   using KT = typename S::KT;
   using VT = typename S::VT;
-  constexpr int NT = D / 16, NV = DV / 16, KL = KT::LOADS / 4, VL = VT::LOADS / 4;
+  constexpr int NT = D / 16, NV = DV / 16, KL = S::KL, VL = S::VL, NW = S::WAVES, NB = SPLIT ? 1 : 2;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv & 3, br = wv >> 2;
   const int nqt = (P.Nq + 127) / 128;
-  const uint32_t bid = tda::grid_bid<256>();
+  const uint32_t bid = tda::grid_bid<64 * NW>();
   if (bid >= (uint32_t)(P.B * P.H) * (uint32_t)nqt) return;
   const Item it = item_of(bid, P.B * P.H, nqt, true);
   const int b = it.head / P.H, h = it.head % P.H, hk = h / (P.H / P.Hk);
-  const int q0 = it.tile * 128, q0w = q0 + 32 * wv, qi = q0w + n32;
+  const int q0 = it.tile * 128, q0w = q0 + 32 * rg, qi = q0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   const int lim = P.see.causal ? min(len, max(off + min(q0 + 128, P.Nq), 0)) : len;
   const int limw = P.see.causal ? min(len, max(off + min(q0w + 32, P.Nq), 0)) : len;
@@ -281,57 +341,66 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   uint32_t ko[2][KL], vo[VL];
 #pragma unroll
   for (int u = 0; u < KL; ++u) {
-    ko[0][u] = KT::source(4 * u + wv, (uint32_t)(P.k[0].st * KT::ES));
-    ko[1][u] = KT::source(4 * u + wv, (uint32_t)(P.k[1].st * KT::ES));
+    ko[0][u] = KT::source(NW * u + wv, (uint32_t)(P.k[0].st * KT::ES));
+    ko[1][u] = KT::source(NW * u + wv, (uint32_t)(P.k[1].st * KT::ES));
   }
 #pragma unroll
-  for (int u = 0; u < VL; ++u) vo[u] = VT::source(4 * u + wv, (uint32_t)(P.v.st * VT::ES));
+  for (int u = 0; u < VL; ++u) vo[u] = VT::source(NW * u + wv, (uint32_t)(P.v.st * VT::ES));
   auto issue = [&](int j) {
-    char* at = lds + (j & 1) * S::STAGE;
+    char* at = lds + j % S::RING * S::STAGE;
     const int n = min(32, lim - 32 * j);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const auto r = rows_rsrc(row_of<T>(P.k[x], b, hk, 32 * (int64_t)j), P.k[x].st * KT::ES, n, D * KT::ES);
 #pragma unroll
-      for (int u = 0; u < KL; ++u) KT::load(r, reinterpret_cast<T*>(at + x * KT::BYTES), 4 * u + wv, ko[x][u]);
+      for (int u = 0; u < KL; ++u)
+        if (KT::LOADS % NW == 0 || NW * u + wv < KT::LOADS) KT::load(r, reinterpret_cast<T*>(at + x * KT::BYTES), NW * u + wv, ko[x][u]);
     }
     const auto r = rows_rsrc(row_of<T>(P.v, b, hk, 32 * (int64_t)j), P.v.st * VT::ES, n, DV * VT::ES);
 #pragma unroll
-    for (int u = 0; u < VL; ++u) VT::load(r, reinterpret_cast<T*>(at + 2 * KT::BYTES), 4 * u + wv, vo[u]);
+    for (int u = 0; u < VL; ++u)
+      if (VT::LOADS % NW == 0 || NW * u + wv < VT::LOADS) VT::load(r, reinterpret_cast<T*>(at + 2 * KT::BYTES), NW * u + wv, vo[u]);
   };
-  if (nst > 0) issue(0);
+#pragma unroll
+  for (int j = 0; j < S::RING - 1; ++j)
+    if (j < nst) issue(j);
 
   const bool row = qi < P.Nq;
-  frag qf[2][NT], of[NV];
+  frag qf[NB][NT], of[NV];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(row ? row_of<T>(P.q[x], b, h, qi) : nullptr, g, qf[x]);
+  for (int x = 0; x < NB; ++x) load_frags<Tr, NT>(row ? row_of<T>(P.q[SPLIT ? br : x], b, h, qi) : nullptr, g, qf[x]);
   load_frags<Tr, NV>(row ? row_of<T>(P.dout, b, h, qi) : nullptr, g, of);
   const int64_t at0 = (int64_t)it.head * P.Nq + qi;
-  float lse[2], rs[2], lam = 0.f;
+  float lse[NB], rs[NB], lam = 0.f;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    lse[x] = row ? P.lse[x * rows + at0] : 0.f;
-    rs[x] = row ? P.stat[x * rows + at0] : 0.f;
+  for (int x = 0; x < NB; ++x) {
+    const int z = SPLIT ? br : x;
+    lse[x] = row ? -P.c * P.stat[z * rows + at0] : 0.f;
+    rs[x] = row ? -P.stat[2 * rows + at0] - (z ? P.stat[3 * rows + at0] : 0.f) : 0.f;
   }
-  if (row) lam = P.stat[2 * rows + at0];
-  f32x16 dq[2][D / 32] = {};
-  pin(dq[0]);
-  pin(dq[1]);
+  if (row) lam = -P.stat[4 * rows + at0];
+  f32x16 dq[NB][D / 32] = {};
+  if constexpr (!SPLIT) {
+    pin(dq[0]);
+    pin(dq[1]);
+  }
 
   for (int j = 0; j < nst; ++j) {
-    wait_vm<0>();
+    if (j + 1 < nst) wait_vm<(S::RING - 2) * S::MIN_LOADS>();
+    else wait_vm<0>();
     tda::lds_barrier();
-    if (j + 1 < nst) issue(j + 1);
+    if (j + S::RING - 1 < nst) issue(j + S::RING - 1);
     const int k0 = 32 * j;
     if (k0 >= limw) continue;
-    const char* at = lds + (j & 1) * S::STAGE;
+    const char* at = lds + j % S::RING * S::STAGE;
     const T* vt = reinterpret_cast<const T*>(at + 2 * KT::BYTES);
     const f32x16 dp = chain<Tr, NV>([&](int t) { return VT::row(vt, 0, t); }, of);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const T* kt = reinterpret_cast<const T*>(at + x * KT::BYTES);
+    for (int x = 0; x < NB; ++x) {
+      const int z = SPLIT ? br : x;
+      const T* kt = reinterpret_cast<const T*>(at + z * KT::BYTES);
       f32x16 s = chain<Tr, NT>([&](int t) { return KT::row(kt, 0, t); }, qf[x]);
-      const float f = x ? -lam : 1.f;
+      const float f = z ? -lam : 1.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = exp2_(__builtin_fmaf(s[r], P.c, -lse[x]));
@@ -350,8 +419,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   wait_vm<0>();
   if (!row) return;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    T* to = row_of<T>(P.dq[x], b, h, qi) + 4 * g;
+  for (int x = 0; x < NB; ++x) {
+    T* to = row_of<T>(P.dq[SPLIT ? br : x], b, h, qi) + 4 * g;
 #pragma unroll
     for (int y = 0; y < D / 32; ++y)
 #pragma unroll
@@ -366,7 +435,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
 // per element.
 __global__ void __launch_bounds__(256) bwd_lambda(BwdParams P, int each) {
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
-  const float* r2 = P.stat + rows;
+  const float* r2 = P.stat + 5 * rows;
   if (each) {
     const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
     if (id >= rows) return;
@@ -403,11 +472,12 @@ static int big_lds(F* fn, int bytes) {
 template <class Tr, int D, int DV>
 static int run(const BwdParams& p, hipStream_t st) {
   using T = typename Tr::T;
+  constexpr bool QSPLIT = sizeof(T) == 2 ? D == 128 : DV <= 64;
   using KS = KeyShape<Tr, D, DV>;
-  using QS = QueryShape<Tr, D, DV>;
+  using QS = QueryShape<Tr, D, DV, QSPLIT>;
   const int64_t rows = (int64_t)p.B * p.H * p.Nq;
   int e = big_lds(&bwd_keys<Tr, D, DV>, KS::LDS);
-  if (!e) e = big_lds(&bwd_query<Tr, D, DV>, QS::LDS);
+  if (!e) e = big_lds(&bwd_query<Tr, D, DV, QSPLIT>, QS::LDS);
   if (e) return e;
   bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
   tda::launched(st, "sda_bwd_rows");
@@ -419,7 +489,7 @@ static int run(const BwdParams& p, hipStream_t st) {
     bwd_sum<T, D, DV><<<tda::grid_of<256>((n + 255) / 256), 256, 0, st>>>(p, parts);
     tda::launched(st, "sda_bwd_sum");
   }
-  bwd_query<Tr, D, DV><<<tda::grid_of<256>((int64_t)((p.Nq + 127) / 128) * p.B * p.H), 256, QS::LDS, st>>>(p);
+  bwd_query<Tr, D, DV, QSPLIT><<<tda::grid_of<64 * QS::WAVES>((int64_t)((p.Nq + 127) / 128) * p.B * p.H), 64 * QS::WAVES, QS::LDS, st>>>(p);
   tda::launched(st, "sda_bwd_query");
   if (p.dlam) {
     const int64_t n = p.dlam_n[0] * p.dlam_n[1] * p.dlam_n[2];

@@ -5,6 +5,9 @@
 // element, so that both types share every index below.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "sda_params.hpp"
 #include "tda_common.hpp"
 
@@ -27,6 +30,16 @@ constexpr float kNoMax = -1e37f;
 // A running maximum moves only when a new score passes it by this much (log2): the sums then hold
 // weights up to 2^8 instead of 1, which costs 32-bit sums nothing and saves rescaling them.
 constexpr float kSlack = 8.0f;
+
+// f(0), .., f(N - 1) with constant arguments: an unrolled loop of any length.
+template <class F, int... I>
+__device__ __forceinline__ void times_(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void times(F&& f) {
+  times_(f, std::make_integer_sequence<int, N>());
+}
 
 struct TrB {
   using T = bf16;
@@ -150,6 +163,70 @@ struct Tile {
   }
 };
 
+// The same fragments by way of LDS addresses that a lane keeps (bf16): the swizzle makes the address of each
+// step another one, which the compiler would work out again for every read (a third of a pass' vector
+// instructions).  `at` of a read is a constant offset: the tile's place, and rows 32 apart.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+template <class Tr, int W>
+struct RowReader {
+  static constexpr int NT = W / 16;
+  uint32_t a[NT];
+  __device__ __forceinline__ void init(const void* lds) {
+    const int r = lane_id() & 31, g = lane_id() >> 5;
+    const uint32_t base = lds_address(lds);
+    if constexpr (sizeof(typename Tr::T) == 2) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        a[t] = base + r * W * 2 + 16 * ((2 * t + g) ^ Tile<Tr, 32, W>::swz(r));
+        asm volatile("" : "+v"(a[t]));
+      }
+    }
+  }
+  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int t) const {
+    if constexpr (sizeof(typename Tr::T) == 2)
+      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(a[t] + at);
+    else
+      return Tile<Tr, 32, W>::row(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, t);
+  }
+};
+template <class Tr, int W>
+struct ColReader {
+  static constexpr int NY = W / 32;
+  uint32_t a[2][NY];
+  __device__ __forceinline__ void init(const void* lds) {
+    const int l = lane_id(), bk = l >> 4, j = l & 15;
+    const uint32_t base = lds_address(lds);
+    if constexpr (sizeof(typename Tr::T) == 2) {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int y = 0; y < NY; ++y) {
+          const int r = 8 * hh + 4 * (bk >> 1) + (j >> 2), d = 32 * y + 16 * (bk & 1) + 4 * (j & 3);
+          a[hh][y] = base + r * W * 2 + 16 * ((d >> 3) ^ Tile<Tr, 32, W>::swz(r)) + 2 * (d & 7);
+          asm volatile("" : "+v"(a[hh][y]));
+        }
+    }
+  }
+  // Step s (16 rows) of the tile at `at`, column block y.
+  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int s, int y) const {
+    if constexpr (sizeof(typename Tr::T) == 2) {
+      typedef __attribute__((address_space(3))) tda::s16x4 quad;
+      bf16x8 f;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const bf16x4 w = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<quad*>(a[hh][y] + at + 32 * W * s)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * hh + e] = w[e];
+      }
+      return f;
+    } else {
+      return Tile<Tr, 32, W>::col(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, s, y);
+    }
+  }
+};
+
 // Row fragments of one row in memory (null: zeros), lane half g.
 template <class Tr, int NT>
 __device__ __forceinline__ void load_frags(const typename Tr::T* row, int g, typename Tr::frag (&f)[NT]) {
@@ -173,7 +250,7 @@ __device__ __forceinline__ void load_frags(const typename Tr::T* row, int g, typ
 // and no further (see tda::mma_chain): left to itself the compiler waits for every read by itself.
 template <class Tr, int NT, class FA>
 __device__ __forceinline__ f32x16 chain(FA&& a, const typename Tr::frag (&b)[NT]) {
-  constexpr int G = sizeof(typename Tr::T) == 2 ? 4 : 2;
+  constexpr int G = sizeof(typename Tr::T) == 2 ? 4 : 1;  // an fp32 step is eight products itself
   static_assert(NT % G == 0, "whole groups");
   typename Tr::frag f[2][G];
   f32x16 acc = {};
@@ -196,7 +273,7 @@ __device__ __forceinline__ f32x16 chain(FA&& a, const typename Tr::frag (&b)[NT]
 // four ahead in the same way.
 template <class Tr, int NY, class FA>
 __device__ __forceinline__ void columns(FA&& col, const typename Tr::frag (&b)[2], f32x16 (&acc)[NY]) {
-  constexpr int G = sizeof(typename Tr::T) == 2 && NY * 2 % 4 == 0 ? 4 : 2, N = 2 * NY;
+  constexpr int G = sizeof(typename Tr::T) == 2 ? 4 : 1, N = 2 * NY;
   typename Tr::frag f[2][G];
 #pragma unroll
   for (int t0 = -G; t0 < N; t0 += G) {

@@ -16,7 +16,7 @@ namespace sda {
 template <class Tr, int D, int DV>
 struct FwdShape {
   using T = typename Tr::T;
-  static constexpr int BN = sizeof(T) == 2 ? 64 : 32;  // keys of a stage
+  static constexpr int BN = sizeof(T) == 2 && DV <= 128 ? 64 : 32;  // keys of a stage
   using KT = Tile<Tr, BN, D>;
   using VT = Tile<Tr, BN, DV>;
   static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
@@ -34,6 +34,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   using VT = typename S::VT;
   constexpr int BN = S::BN, NS = BN / 32, NT = D / 16, NO = DV / 32;
   constexpr int KL = KT::LOADS / 8, VL = VT::LOADS / 8;
+  constexpr int G = sizeof(T) == 2 ? 4 : 1;  // an fp32 fragment is eight products itself
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
@@ -84,22 +85,40 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   frag qf[NT];
   load_frags<Tr, NT>(qi < P.Nq ? row_of<T>(P.q[br], b, h, qi) : nullptr, g, qf);
   f32x16 o[NO] = {};
-  float m = kNoMax, sum = 0.f;
+  float m = kNoMax, sums[4] = {};
 
-  for (int j = 0; j < nst; ++j) {
+  RowReader<Tr, D> kr;
+  ColReader<Tr, DV> vr;
+  kr.init(lds + br * KT::BYTES);
+  vr.init(lds + 2 * KT::BYTES);
+  auto step = [&](int j, auto half) {  // stage j, in the half of the buffers that its parity names
+    constexpr int AT = half * S::STAGE;
     wait_vm<0>();
     tda::lds_barrier();  // stage j is in place, and every wave is done with stage j - 1
     if (j + 1 < nst) issue(j + 1);
     const int k0 = j * BN;
-    if (k0 >= limw) continue;
-    const T* kt = reinterpret_cast<const T*>(lds + (j & 1) * S::STAGE + br * KT::BYTES);
-    const T* vt = reinterpret_cast<const T*>(lds + (j & 1) * S::STAGE + 2 * KT::BYTES);
-    f32x16 s[NS];
+    if (k0 >= limw) return;
+    // The stage's products take their LDS operands as one sequence, NS NT key fragments then 2 NS NO value
+    // fragments, read a group of G ahead of their use: the first value group is on its way before the softmax.
+    frag f[2][G];
+    auto read = [&](int i) {
 #pragma unroll
-    for (int x = 0; x < NS; ++x) {
-      s[x] = f32x16{};
+      for (int u = 0; u < G; ++u) {
+        const int e = i * G + u, w = e - NS * NT;
+        if (e < NS * NT) f[i & 1][u] = kr.read(lds + br * KT::BYTES, AT + 32 * D * KT::ES * (e % NS), e / NS);
+        else f[i & 1][u] = vr.read(lds + 2 * KT::BYTES, AT + 32 * DV * VT::ES * (w / (2 * NO)), w / NO % 2, w % NO);
+      }
+    };
+    f32x16 s[NS] = {};
+    read(0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[x] = Tr::mma32(KT::row(kt, 32 * x, t), qf[t], s[x]);
+    for (int i = 0; i < NS * NT / G; ++i) {
+      read(i + 1);
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        const int e = i * G + u;
+        s[e % NS] = Tr::mma32(f[i & 1][u], qf[e / NS], s[e % NS]);
+      }
     }
     if (k0 + BN > clear) {
       asm volatile("");  // a branch: few tiles need this
@@ -109,16 +128,19 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
         for (int r = 0; r < 16; ++r)
           if (k0 + 32 * x + crow(r, g) >= see) s[x][r] = -__builtin_inff();
     }
-    float top = s[0][0];
+    // the maximum and the sum in four chains: one of 32 dependent steps takes longer than the products
+    float four[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
     for (int x = 0; x < NS; ++x)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[x][r]);
-    top = fmaxf(top, __shfl_xor(top, 32)) * P.c;
+      for (int r = 0; r < 16; ++r) four[r % 4] = fmaxf(four[r % 4], s[x][r]);
+    float top = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3])) * P.c;
     if (__any(top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
       const float to = fmaxf(m, top), f = exp2_(m - to);
       m = to;
-      sum *= f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[r] *= f;
 #pragma unroll
       for (int x = 0; x < NO; ++x)
 #pragma unroll
@@ -129,18 +151,28 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[x][r] = exp2_(__builtin_fmaf(s[x][r], P.c, -m));
-        sum += s[x][r];
+        sums[r % 4] += s[x][r];
       }
+    frag p[2 * NS];
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+    for (int x = 0; x < 2 * NS; ++x) p[x] = pack8<Tr>(s[x / 2], x % 2);
+    constexpr int first = NS * NT / G, last = first + 2 * NS * NO / G;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag p = pack8<Tr>(s[x], u);
+    for (int i = first; i < last; ++i) {
+      if (i + 1 < last) read(i + 1);
 #pragma unroll
-        for (int y = 0; y < NO; ++y) o[y] = Tr::mma32(VT::col(vt, 32 * x, u, y), p, o[y]);
+      for (int u = 0; u < G; ++u) {
+        const int w = i * G + u - NS * NT;
+        o[w % NO] = Tr::mma32(f[i & 1][u], p[w / NO], o[w % NO]);
       }
+    }
+  };
+  for (int j = 0; j < nst; j += 2) {
+    step(j, std::integral_constant<int, 0>());
+    if (j + 1 < nst) step(j + 1, std::integral_constant<int, 1>());
   }
 
+  float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   sum += __shfl_xor(sum, 32);
   const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;  // no visible key: zeros
   const bool row = qi < P.Nq;

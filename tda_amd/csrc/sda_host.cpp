@@ -104,7 +104,7 @@ int64_t key_group(const sda_bwd_args& a) {
     if (G % gs == 0 && base * (G / gs) >= 1024) return gs;
   return 1;
 }
-int64_t stat_bytes(const sda_bwd_args& a) { return round256(3 * a.batch * a.heads * a.seq_len * 4); }
+int64_t stat_bytes(const sda_bwd_args& a) { return round256(6 * a.batch * a.heads * a.seq_len * 4); }
 int64_t part_bytes(const sda_bwd_args& a) {
   const int64_t G = a.heads / a.kv_heads, gs = key_group(a);
   return gs == G ? 0 : G / gs * a.batch * a.kv_heads * a.seq_len_kv * (2 * a.head_dim + a.v_head_dim) * 4;
