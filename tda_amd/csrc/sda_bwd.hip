@@ -55,7 +55,9 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
 }
 
 // ------------------------------------------------------------------ key-major pass
-constexpr int kKeyRows = 128;  // keys of a workgroup: 4 groups of 32
+// Waves (32 keys each) of a key-pass workgroup.
+template <class Tr, int D, int DV>
+constexpr int kKeyWaves = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64 ? 8 : 4;
 
 template <class Tr, int D, int DV>
 struct KeyShape {
@@ -63,8 +65,11 @@ struct KeyShape {
   using OT = Tile<Tr, 32, DV>;
   static constexpr int STAT = 2 * QT::BYTES + OT::BYTES;  // the statistics of the 32 rows
   static constexpr int STAGE = STAT + 1024;
-  static constexpr int LDS = 2 * STAGE;
-  static_assert(QT::LOADS % 4 == 0 && OT::LOADS % 4 == 0, "loads spread evenly over the waves");
+  static constexpr int RING = 2;  // stages in LDS, all but one of them on their way
+  static constexpr int LDS = RING * STAGE;
+  static constexpr int NW = kKeyWaves<Tr, D, DV>, KEYS = 32 * NW;
+  static constexpr int LOADS = (2 * QT::LOADS + OT::LOADS) / NW + 8 / NW;  // of a wave, a stage
+  static_assert((QT::LOADS % NW == 0 && OT::LOADS % NW == 0) || RING == 2, "loads spread evenly over the waves");
 };
 
 // One wave per SIMD (the three gradients' accumulators and the resident rows fill the registers), so
@@ -72,29 +77,29 @@ struct KeyShape {
 // use, and the first branch's weights are computed between the second's score products, the second's
 // between the first's gradient products.
 template <class Tr, int D, int DV>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) bwd_keys(BwdParams P) {
+__global__ void __launch_bounds__((64 * kKeyWaves<Tr, D, DV>)) __attribute__((amdgpu_waves_per_eu((kKeyWaves<Tr, D, DV> / 4)))) bwd_keys(BwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
   using S = KeyShape<Tr, D, DV>;
   using QT = typename S::QT;
   using OT = typename S::OT;
-  constexpr int NT = D / 16, NV = DV / 16, QL = QT::LOADS / 4, OL = OT::LOADS / 4;
-  constexpr int G = sizeof(T) == 2 ? 4 : 1;  // an fp32 fragment is eight products itself
+  constexpr int NT = D / 16, NV = DV / 16, NW = S::NW, QL = (QT::LOADS + NW - 1) / NW, OL = (OT::LOADS + NW - 1) / NW;
+  constexpr int G = sizeof(T) == 4 ? 1 : NW == 8 ? 2 : 4;  // an fp32 fragment is eight products itself
   // The statistics enter the products as their starting values; f32 adds them after, where a sum that starts
   // far from zero would cost it bits.
   constexpr bool START = sizeof(T) == 2;
-  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
+  constexpr int AHEAD = sizeof(T) == 2 && NW == 4 ? 2 : 1;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
-  const uint32_t bid = tda::grid_bid<256>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
+  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + S::KEYS - 1) / S::KEYS;
+  const uint32_t bid = tda::grid_bid<64 * NW>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
   if (bid >= heads * (uint32_t)nkt) return;
   const Item it = item_of(bid, heads, nkt, false);
   const int part = it.head % parts, bk = it.head / parts, b = bk / P.Hk, hk = bk % P.Hk;
   const int h0 = hk * GQ + part * P.gs;
-  const int k0 = it.tile * kKeyRows, k0w = k0 + 32 * wv, key = k0w + n32;
+  const int k0 = it.tile * S::KEYS, k0w = k0 + 32 * wv, key = k0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   const bool live = key < len;
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
@@ -108,47 +113,65 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
   uint32_t qo[2][QL], oo[OL];
 #pragma unroll
   for (int u = 0; u < QL; ++u) {
-    qo[0][u] = QT::source(4 * u + wv, (uint32_t)(P.q[0].st * QT::ES));
-    qo[1][u] = QT::source(4 * u + wv, (uint32_t)(P.q[1].st * QT::ES));
+    qo[0][u] = QT::source(NW * u + wv, (uint32_t)(P.q[0].st * QT::ES));
+    qo[1][u] = QT::source(NW * u + wv, (uint32_t)(P.q[1].st * QT::ES));
   }
 #pragma unroll
-  for (int u = 0; u < OL; ++u) oo[u] = OT::source(4 * u + wv, (uint32_t)(P.dout.st * OT::ES));
-  auto issue = [&](int j, int h, int qt) {  // step j: query tile qt of head h
+  for (int u = 0; u < OL; ++u) oo[u] = OT::source(NW * u + wv, (uint32_t)(P.dout.st * OT::ES));
+  auto issue = [&](int slot, int h, int qt) {  // query tile qt of head h
     const int i0 = 32 * qt, n = min(32, P.Nq - i0);
-    char* at = lds + (j & 1) * S::STAGE;
+    char* at = lds + slot * S::STAGE;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const auto r = rows_rsrc(row_of<T>(P.q[x], b, h, i0), P.q[x].st * QT::ES, n, D * QT::ES);
 #pragma unroll
-      for (int u = 0; u < QL; ++u) QT::load(r, reinterpret_cast<T*>(at + x * QT::BYTES), 4 * u + wv, qo[x][u]);
+      for (int u = 0; u < QL; ++u)
+        if (QT::LOADS % NW == 0 || NW * u + wv < QT::LOADS) QT::load(r, reinterpret_cast<T*>(at + x * QT::BYTES), NW * u + wv, qo[x][u]);
     }
     const auto r = rows_rsrc(row_of<T>(P.dout, b, h, i0), P.dout.st * OT::ES, n, DV * OT::ES);
 #pragma unroll
-    for (int u = 0; u < OL; ++u) OT::load(r, reinterpret_cast<T*>(at + 2 * QT::BYTES), 4 * u + wv, oo[u]);
-    // the rows' statistics; rows past Nq read as zeros and meet zero rows of q and dO
+    for (int u = 0; u < OL; ++u)
+      if (OT::LOADS % NW == 0 || NW * u + wv < OT::LOADS) OT::load(r, reinterpret_cast<T*>(at + 2 * QT::BYTES), NW * u + wv, oo[u]);
+    // the rows' statistics, two loads a wave (the last three bring the fifth again: every wave's loads of a
+    // stage are as many); rows past Nq read as zeros and meet zero rows of q and dO
     const float* src = P.stat + ((int64_t)b * P.H + h) * P.Nq + i0;
-    if (l < 32) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + wv * rows, 4 * n), LDS_PTR(void, at + S::STAT + 128 * wv), 4, 4 * l, 0, 0, 0);
-      if (wv == 0)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + 4 * rows, 4 * n), LDS_PTR(void, at + S::STAT + 512), 4, 4 * l, 0, 0, 0);
-    }
+#pragma unroll
+    for (int z = 0; z < 8; z += NW)
+      if (l < 32)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + min(z + wv, 4) * rows, 4 * n), LDS_PTR(void, at + S::STAT + 128 * (z + wv)), 4, 4 * l, 0, 0, 0);
   };
-  if (steps > 0) issue(0, h0, first);
+  int nh = h0, nq = first;  // head and query tile of the next stage to send for
+  auto send = [&](int slot) {
+    issue(slot, nh, nq);
+    if (++nq == nqt) nq = first, ++nh;
+  };
+  for (int j = 0; j < S::RING - 1; ++j)
+    if (j < steps) send(j);
 
   frag kf[2][NT], vf[NV];
 #pragma unroll
   for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(live ? row_of<T>(P.k[x], b, hk, key) : nullptr, g, kf[x]);
   load_frags<Tr, NV>(live ? row_of<T>(P.v, b, hk, key) : nullptr, g, vf);
   f32x16 dk[2][D / 32] = {}, dv[DV / 32] = {};
-  pin(dk[0]);
-  pin(dk[1]);
-  pin(dv);
+  if constexpr (NW == 4) {
+    pin(dk[0]);
+    pin(dk[1]);
+    pin(dv);
+  }
 
-  auto step = [&](const char* at, int i0) {
+  RowReader<Tr, D> qr;
+  RowReader<Tr, DV> orow;
+  ColReader<Tr, D> qc;
+  ColReader<Tr, DV> oc;
+  qr.init(lds);
+  qc.init(lds);
+  orow.init(lds + 2 * QT::BYTES);
+  oc.init(lds + 2 * QT::BYTES);
+  auto step = [&](int i0, auto half) {  // the stage in that half of the buffers
+    constexpr int AT = half * S::STAGE;
+    const char* ot = lds + 2 * QT::BYTES;
     const bool edge = P.see.causal && off + i0 < k0w + 31;  // some row does not see some key
-    const T* qt[2] = {reinterpret_cast<const T*>(at), reinterpret_cast<const T*>(at + QT::BYTES)};
-    const T* ot = reinterpret_cast<const T*>(at + 2 * QT::BYTES);
-    const float* st = reinterpret_cast<const float*>(at + S::STAT);
+    const float* st = reinterpret_cast<const float*>(lds + AT + S::STAT);
     // the sequence: dO rows (dP), q1 rows, q2 rows (scores), q1 columns (dk1), q2 columns (dk2), dO columns (dv)
     constexpr int E1 = NV, E2 = E1 + NT, E3 = E2 + NT, E4 = E3 + D / 16, E5 = E4 + D / 16, E6 = E5 + DV / 16;
     frag f[AHEAD + 1][G];
@@ -156,12 +179,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
       times<G>([&](auto u) {
         constexpr int e = i * G + u;
         frag& to = f[i % (AHEAD + 1)][u];
-        if constexpr (e < E1) to = OT::row(ot, 0, e);
-        else if constexpr (e < E2) to = QT::row(qt[0], 0, e - E1);
-        else if constexpr (e < E3) to = QT::row(qt[1], 0, e - E2);
-        else if constexpr (e < E4) to = QT::col(qt[0], 0, (e - E3) / (D / 32), (e - E3) % (D / 32));
-        else if constexpr (e < E5) to = QT::col(qt[1], 0, (e - E4) / (D / 32), (e - E4) % (D / 32));
-        else to = OT::col(ot, 0, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
+        if constexpr (e < E1) to = orow.read(ot, AT, e);
+        else if constexpr (e < E2) to = qr.read(lds, AT, e - E1);
+        else if constexpr (e < E3) to = qr.read(lds, AT + QT::BYTES, e - E2);
+        else if constexpr (e < E4) to = qc.read(lds, AT, (e - E3) / (D / 32), (e - E3) % (D / 32));
+        else if constexpr (e < E5) to = qc.read(lds, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
+        else to = oc.read(ot, AT, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
       });
     };
     auto rowstat = [&](int z) {  // statistic z of the lane's 16 rows
@@ -233,18 +256,107 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) b
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  int h = h0, qt = first, nh = h0, nq = first;  // of this step, and of the one on its way
-  for (int j = 0; j < steps; ++j) {
-    wait_vm<0>();
+  // The same for two waves a SIMD, which cover each other: fewer registers, the branches one after the other.
+  auto lean = [&](int i0, auto half) {
+    constexpr int AT = half * S::STAGE;
+    const char* ot = lds + 2 * QT::BYTES;
+    const bool edge = P.see.causal && off + i0 < k0w + 31;
+    const float* st = reinterpret_cast<const float*>(lds + AT + S::STAT) + 4 * g;
+    constexpr int E1 = NV, E2 = E1 + NT, E3 = E2 + D / 16, E4 = E3 + NT, E5 = E4 + D / 16, E6 = E5 + DV / 16;
+    frag f[2][G];
+    auto read = [&](auto i) {
+      times<G>([&](auto u) {
+        constexpr int e = i * G + u;
+        frag& to = f[i % 2][u];
+        if constexpr (e < E1) to = orow.read(ot, AT, e);
+        else if constexpr (e < E2) to = qr.read(lds, AT, e - E1);
+        else if constexpr (e < E3) to = qc.read(lds, AT, (e - E2) / (D / 32), (e - E2) % (D / 32));
+        else if constexpr (e < E4) to = qr.read(lds, AT + QT::BYTES, e - E3);
+        else if constexpr (e < E5) to = qc.read(lds, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
+        else to = oc.read(ot, AT, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
+      });
+    };
+    auto rowstat = [&](int z) {
+      f32x16 x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(st + 32 * z + 8 * r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = y[e];
+      }
+      return x;
+    };
+    auto hide = [&](f32x16& x) {
+      if (edge) {
+        asm volatile("");  // a branch: few tiles need this
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = key > off + i0 + crow(r, g) ? -__builtin_inff() : x[r];
+      }
+    };
+    read(std::integral_constant<int, 0>());
+    f32x16 dp = rowstat(2), sc, w;
+    frag ds[2];
+    constexpr int NG = E6 / G;
+    times<NG>([&](auto i) {
+      if constexpr (i + 1 < NG) read(std::integral_constant<int, i + 1>());
+      if constexpr (i * G == E1) sc = rowstat(0);
+      if constexpr (i * G == E3) sc = rowstat(1);
+      if constexpr (i * G == E2) {  // the first branch's weights
+        hide(sc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          w[r] = exp2_(P.c * sc[r]);
+          sc[r] = w[r] * dp[r];
+        }
+        ds[0] = pack8<Tr>(sc, 0), ds[1] = pack8<Tr>(sc, 1);
+      }
+      if constexpr (i * G == E4) {  // the second's
+        hide(sc);
+        dp += rowstat(3);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 lam = *reinterpret_cast<const f32x4*>(st + 128 + 8 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * q + e;
+            const float p = lam[e] * exp2_(P.c * sc[r]);
+            w[r] += p;
+            sc[r] = p * dp[r];
+          }
+        }
+        ds[0] = pack8<Tr>(sc, 0), ds[1] = pack8<Tr>(sc, 1);
+      }
+      if constexpr (i * G == E5) ds[0] = pack8<Tr>(w, 0), ds[1] = pack8<Tr>(w, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      times<G>([&](auto u) {
+        constexpr int e = i * G + u;
+        const frag& a = f[i % 2][u];
+        if constexpr (e < E1) dp = Tr::mma32(a, vf[e], dp);
+        else if constexpr (e < E2) sc = Tr::mma32(a, kf[0][e - E1], sc);
+        else if constexpr (e < E3) dk[0][(e - E2) % (D / 32)] = Tr::mma32(a, ds[(e - E2) / (D / 32)], dk[0][(e - E2) % (D / 32)]);
+        else if constexpr (e < E4) sc = Tr::mma32(a, kf[1][e - E3], sc);
+        else if constexpr (e < E5) dk[1][(e - E4) % (D / 32)] = Tr::mma32(a, ds[(e - E4) / (D / 32)], dk[1][(e - E4) % (D / 32)]);
+        else dv[(e - E5) % (DV / 32)] = Tr::mma32(a, ds[(e - E5) / (DV / 32)], dv[(e - E5) % (DV / 32)]);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  int qt = first;  // of this step
+  auto one = [&](int j, auto slot) {
+    if (j + 1 < steps) wait_vm<(S::RING - 2) * S::LOADS>();  // the later stages may stay on their way
+    else wait_vm<0>();
     tda::lds_barrier();
-    if (++nq == nqt) nq = first, ++nh;
-    if (j + 1 < steps) issue(j + 1, nh, nq);
-    const int i0 = 32 * qt;
-    const char* at = lds + (j & 1) * S::STAGE;
-    step(at, i0);
-    h = nh, qt = nq;
-  }
-  (void)h;
+    if (j + S::RING - 1 < steps) send((slot + S::RING - 1) % S::RING);
+    if (!P.see.causal || off + min(32 * qt + 31, P.Nq - 1) >= k0w) {
+      if constexpr (NW == 8) lean(32 * qt, slot);
+      else step(32 * qt, slot);
+    }
+    if (++qt == nqt) qt = first;
+  };
+  for (int j = 0; j < steps; j += S::RING)
+    times<S::RING>([&](auto x) {
+      if (j + x < steps) one(j + x, x);
+    });
   wait_vm<0>();
 
   if (key >= P.Nk) return;
@@ -482,7 +594,7 @@ static int run(const BwdParams& p, hipStream_t st) {
   bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
   tda::launched(st, "sda_bwd_rows");
   const int parts = p.H / p.Hk / p.gs;
-  bwd_keys<Tr, D, DV><<<tda::grid_of<256>((int64_t)((p.Nk + kKeyRows - 1) / kKeyRows) * p.B * p.Hk * parts), 256, KS::LDS, st>>>(p);
+  bwd_keys<Tr, D, DV><<<tda::grid_of<64 * KS::NW>((int64_t)((p.Nk + KS::KEYS - 1) / KS::KEYS) * p.B * p.Hk * parts), 64 * KS::NW, KS::LDS, st>>>(p);
   tda::launched(st, "sda_bwd_keys");
   if (p.part) {
     const int64_t n = (int64_t)p.B * p.Hk * p.Nk * ((2 * D + DV) / 4);
