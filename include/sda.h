@@ -44,8 +44,11 @@ typedef struct sda_fwd_args {
   int64_t head_dim, v_head_dim;     /* (64, 64), (64, 128), (128, 128) or (128, 256) */
   tda_tensor q1, k1, q2, k2, v;     /* (B, H, Nq, d), (B, Hk, Nk, d), ..., (B, Hk, Nk, dv) */
   tda_tensor out;                   /* (B, H, Nq, dv) */
-  tda_tensor out2;          /* optional (data may be NULL): softmax(s q2 k2^T + M) v, which the
-                               backward reads */
+  tda_tensor out2;          /* optional (data may be NULL), f32 rows: softmax(s q2 k2^T + M) v, and */
+  tda_tensor out_low;       /* with it for bf16, bf16 rows: what out's rounding left out.  The
+                               backward's row sums of the outputs keep 16 bits with them: from the
+                               rounded outputs alone they would cost its gradients half again the error
+                               that their own rounding has */
   const void* lambda_param; /* element (b, h, i) at b ls[0] + h ls[1] + i ls[2] */
   int64_t lambda_stride[3]; /* 0: the same along that axis */
   int32_t lambda_dtype;     /* TDA_DTYPE_F32 or TDA_DTYPE_BF16 */
@@ -64,7 +67,7 @@ typedef struct sda_bwd_args {
   float   scale;
   int64_t batch, heads, kv_heads, seq_len, seq_len_kv, head_dim, v_head_dim;
   tda_tensor q1, k1, q2, k2, v;     /* the forward's */
-  tda_tensor out, out2, dout;       /* the forward's outputs and the upstream gradient */
+  tda_tensor out, out2, out_low, dout;  /* the forward's outputs and the upstream gradient */
   tda_tensor dq1, dk1, dq2, dk2, dv;
   const void* lambda_param;
   int64_t lambda_stride[3];

@@ -30,11 +30,11 @@ _WORK = [("workspace", _p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class SdaFwdArgs(ctypes.Structure):
-    _fields_ = _HEAD + _ROWS + [("out", TdaTensor), ("out2", TdaTensor)] + _SIGHT + _WORK
+    _fields_ = _HEAD + _ROWS + [("out", TdaTensor), ("out2", TdaTensor), ("out_low", TdaTensor)] + _SIGHT + _WORK
 
 
 class SdaBwdArgs(ctypes.Structure):
-    _fields_ = (_HEAD + _ROWS + [(n, TdaTensor) for n in ("out", "out2", "dout", "dq1", "dk1", "dq2", "dk2", "dv")]
+    _fields_ = (_HEAD + _ROWS + [(n, TdaTensor) for n in ("out", "out2", "out_low", "dout", "dq1", "dk1", "dq2", "dk2", "dv")]
                 + _SIGHT + [("dlambda", _p)] + _WORK)
 
 

@@ -30,11 +30,14 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
   const int b = (int)(bh / P.H), h = (int)(bh % P.H);
   const T* d = row_of<T>(P.dout, b, h, i);
   const T* x = row_of<T>(P.out, b, h, i);
-  const T* y = row_of<T>(P.out2, b, h, i);
+  const float* y = row_of<float>(P.out2, b, h, i);
+  const T* z = sizeof(T) == 2 ? row_of<T>(P.low, b, h, i) : nullptr;
   float rx = 0.f, ry = 0.f;
 #pragma unroll
   for (int u = 0; u < DV / 64; ++u) {
-    const f32x4 dd = tda::load4(d + 64 * u + 4 * c), xx = tda::load4(x + 64 * u + 4 * c), yy = tda::load4(y + 64 * u + 4 * c);
+    const f32x4 dd = tda::load4(d + 64 * u + 4 * c), yy = tda::load4(y + 64 * u + 4 * c);
+    f32x4 xx = tda::load4(x + 64 * u + 4 * c);
+    if constexpr (sizeof(T) == 2) xx += tda::load4(z + 64 * u + 4 * c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       rx = __builtin_fmaf(dd[e], xx[e], rx);
@@ -55,9 +58,10 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
 }
 
 // ------------------------------------------------------------------ key-major pass
-// Waves (32 keys each) of a key-pass workgroup.
+// Whether two workgroups of the key pass fit a CU (two waves a SIMD).
 template <class Tr, int D, int DV>
-constexpr int kKeyWaves = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64 ? 8 : 4;
+constexpr bool kKeyLean = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64;
+constexpr int kKeyRows = 128;  // keys of a workgroup: 4 waves of 32
 
 template <class Tr, int D, int DV>
 struct KeyShape {
@@ -67,7 +71,7 @@ struct KeyShape {
   static constexpr int STAGE = STAT + 1024;
   static constexpr int RING = 2;  // stages in LDS, all but one of them on their way
   static constexpr int LDS = RING * STAGE;
-  static constexpr int NW = kKeyWaves<Tr, D, DV>, KEYS = 32 * NW;
+  static constexpr int NW = 4;
   static constexpr int LOADS = (2 * QT::LOADS + OT::LOADS) / NW + 8 / NW;  // of a wave, a stage
   static_assert((QT::LOADS % NW == 0 && OT::LOADS % NW == 0) || RING == 2, "loads spread evenly over the waves");
 };
@@ -77,29 +81,30 @@ struct KeyShape {
 // use, and the first branch's weights are computed between the second's score products, the second's
 // between the first's gradient products.
 template <class Tr, int D, int DV>
-__global__ void __launch_bounds__((64 * kKeyWaves<Tr, D, DV>)) __attribute__((amdgpu_waves_per_eu((kKeyWaves<Tr, D, DV> / 4)))) bwd_keys(BwdParams P) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyLean<Tr, D, DV> ? 2 : 1)))) bwd_keys(BwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
   using S = KeyShape<Tr, D, DV>;
   using QT = typename S::QT;
   using OT = typename S::OT;
+  constexpr bool LEAN = kKeyLean<Tr, D, DV>;
   constexpr int NT = D / 16, NV = DV / 16, NW = S::NW, QL = (QT::LOADS + NW - 1) / NW, OL = (OT::LOADS + NW - 1) / NW;
-  constexpr int G = sizeof(T) == 4 ? 1 : NW == 8 ? 2 : 4;  // an fp32 fragment is eight products itself
+  constexpr int G = sizeof(T) == 4 ? 1 : LEAN ? 2 : 4;  // an fp32 fragment is eight products itself
   // The statistics enter the products as their starting values; f32 adds them after, where a sum that starts
   // far from zero would cost it bits.
   constexpr bool START = sizeof(T) == 2;
-  constexpr int AHEAD = sizeof(T) == 2 && NW == 4 ? 2 : 1;
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + S::KEYS - 1) / S::KEYS;
+  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
   const uint32_t bid = tda::grid_bid<64 * NW>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
   if (bid >= heads * (uint32_t)nkt) return;
   const Item it = item_of(bid, heads, nkt, false);
   const int part = it.head % parts, bk = it.head / parts, b = bk / P.Hk, hk = bk % P.Hk;
   const int h0 = hk * GQ + part * P.gs;
-  const int k0 = it.tile * S::KEYS, k0w = k0 + 32 * wv, key = k0w + n32;
+  const int k0 = it.tile * kKeyRows, k0w = k0 + 32 * wv, key = k0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   const bool live = key < len;
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
@@ -153,11 +158,9 @@ __global__ void __launch_bounds__((64 * kKeyWaves<Tr, D, DV>)) __attribute__((am
   for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(live ? row_of<T>(P.k[x], b, hk, key) : nullptr, g, kf[x]);
   load_frags<Tr, NV>(live ? row_of<T>(P.v, b, hk, key) : nullptr, g, vf);
   f32x16 dk[2][D / 32] = {}, dv[DV / 32] = {};
-  if constexpr (NW == 4) {
-    pin(dk[0]);
-    pin(dk[1]);
-    pin(dv);
-  }
+  pin(dk[0]);
+  pin(dk[1]);
+  pin(dv);
 
   RowReader<Tr, D> qr;
   RowReader<Tr, DV> orow;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__((64 * kKeyWaves<Tr, D, DV>)) __attribute__((am
     tda::lds_barrier();
     if (j + S::RING - 1 < steps) send((slot + S::RING - 1) % S::RING);
     if (!P.see.causal || off + min(32 * qt + 31, P.Nq - 1) >= k0w) {
-      if constexpr (NW == 8) lean(32 * qt, slot);
+      if constexpr (LEAN) lean(32 * qt, slot);
       else step(32 * qt, slot);
     }
     if (++qt == nqt) qt = first;
@@ -418,10 +421,8 @@ struct QueryShape {
   using VT = Tile<Tr, 32, DV>;
   static constexpr int WAVES = SPLIT ? 8 : 4;
   static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
-  static constexpr int RING = 2;
-  static constexpr int LDS = RING * STAGE;
+  static constexpr int LDS = 2 * STAGE;
   static constexpr int KL = (KT::LOADS + WAVES - 1) / WAVES, VL = (VT::LOADS + WAVES - 1) / WAVES;
-  static constexpr int MIN_LOADS = 2 * (KT::LOADS / WAVES) + VT::LOADS / WAVES;  // of a wave, a stage
 };
 
 template <class Tr, int D, int DV, bool SPLIT>
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
 #pragma unroll
   for (int u = 0; u < VL; ++u) vo[u] = VT::source(NW * u + wv, (uint32_t)(P.v.st * VT::ES));
   auto issue = [&](int j) {
-    char* at = lds + j % S::RING * S::STAGE;
+    char* at = lds + (j & 1) * S::STAGE;
     const int n = min(32, lim - 32 * j);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -473,9 +474,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     for (int u = 0; u < VL; ++u)
       if (VT::LOADS % NW == 0 || NW * u + wv < VT::LOADS) VT::load(r, reinterpret_cast<T*>(at + 2 * KT::BYTES), NW * u + wv, vo[u]);
   };
-#pragma unroll
-  for (int j = 0; j < S::RING - 1; ++j)
-    if (j < nst) issue(j);
+  if (nst > 0) issue(0);
 
   const bool row = qi < P.Nq;
   frag qf[NB][NT], of[NV];
@@ -497,21 +496,25 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     pin(dq[1]);
   }
 
-  for (int j = 0; j < nst; ++j) {
-    if (j + 1 < nst) wait_vm<(S::RING - 2) * S::MIN_LOADS>();
-    else wait_vm<0>();
+  RowReader<Tr, D> kr;
+  RowReader<Tr, DV> vr;
+  ColReader<Tr, D> kc;
+  const char* kbuf = lds + (SPLIT ? br * KT::BYTES : 0);  // the wave's own branch of the keys
+  kr.init(kbuf);
+  kc.init(kbuf);
+  vr.init(lds + 2 * KT::BYTES);
+  auto step = [&](int j, auto half) {  // stage j, in that half of the buffers
+    constexpr int AT = half * S::STAGE;
+    wait_vm<0>();
     tda::lds_barrier();
-    if (j + S::RING - 1 < nst) issue(j + S::RING - 1);
+    if (j + 1 < nst) issue(j + 1);
     const int k0 = 32 * j;
-    if (k0 >= limw) continue;
-    const char* at = lds + j % S::RING * S::STAGE;
-    const T* vt = reinterpret_cast<const T*>(at + 2 * KT::BYTES);
-    const f32x16 dp = chain<Tr, NV>([&](int t) { return VT::row(vt, 0, t); }, of);
+    if (k0 >= limw) return;
+    const f32x16 dp = chain<Tr, NV>([&](int t) { return vr.read(lds + 2 * KT::BYTES, AT, t); }, of);
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
-      const int z = SPLIT ? br : x;
-      const T* kt = reinterpret_cast<const T*>(at + z * KT::BYTES);
-      f32x16 s = chain<Tr, NT>([&](int t) { return KT::row(kt, 0, t); }, qf[x]);
+      const int z = SPLIT ? br : x, kt = AT + x * KT::BYTES;
+      f32x16 s = chain<Tr, NT>([&](int t) { return kr.read(kbuf, kt, t); }, qf[x]);
       const float f = z ? -lam : 1.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -525,8 +528,12 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
           if (k0 + crow(r, g) >= see) s[r] = 0.f;
       }
       const frag e[2] = {pack8<Tr>(s, 0), pack8<Tr>(s, 1)};
-      columns<Tr, D / 32>([&](int u, int y) { return KT::col(kt, 0, u, y); }, e, dq[x]);
+      columns<Tr, D / 32>([&](int u, int y) { return kc.read(kbuf, kt, u, y); }, e, dq[x]);
     }
+  };
+  for (int j = 0; j < nst; j += 2) {
+    step(j, std::integral_constant<int, 0>());
+    if (j + 1 < nst) step(j + 1, std::integral_constant<int, 1>());
   }
   wait_vm<0>();
   if (!row) return;
@@ -594,7 +601,7 @@ static int run(const BwdParams& p, hipStream_t st) {
   bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
   tda::launched(st, "sda_bwd_rows");
   const int parts = p.H / p.Hk / p.gs;
-  bwd_keys<Tr, D, DV><<<tda::grid_of<64 * KS::NW>((int64_t)((p.Nk + KS::KEYS - 1) / KS::KEYS) * p.B * p.Hk * parts), 64 * KS::NW, KS::LDS, st>>>(p);
+  bwd_keys<Tr, D, DV><<<tda::grid_of<64 * KS::NW>((int64_t)((p.Nk + kKeyRows - 1) / kKeyRows) * p.B * p.Hk * parts), 64 * KS::NW, KS::LDS, st>>>(p);
   tda::launched(st, "sda_bwd_keys");
   if (p.part) {
     const int64_t n = (int64_t)p.B * p.Hk * p.Nk * ((2 * D + DV) / 4);

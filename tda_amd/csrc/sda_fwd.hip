@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   __syncthreads();  // the stages are read: their place carries branch 2's result
   f32x4* xch = reinterpret_cast<f32x4*>(lds) + rg * (NO * 4 * 64) + l;
   if (br) {
-    T* to = P.out2.p && row ? row_of<T>(P.out2, b, h, qi) : nullptr;
+    float* to = P.out2.p && row ? row_of<float>(P.out2, b, h, qi) : nullptr;
 #pragma unroll
     for (int y = 0; y < NO; ++y)
 #pragma unroll
@@ -195,6 +195,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   if (!br && row) {
     const float lam = lambda_of(P.lam, b, h, qi);
     T* to = row_of<T>(P.out, b, h, qi);
+    T* low = P.out2.p ? row_of<T>(P.low, b, h, qi) : nullptr;  // what rounding leaves out, for the backward's row sums
 #pragma unroll
     for (int y = 0; y < NO; ++y)
 #pragma unroll
@@ -204,6 +205,14 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, w[e], o[y][4 * r + e] * inv);
         store4(to + 32 * y + 8 * r + 4 * g, z);
+        if constexpr (sizeof(T) == 2) {
+          if (low) {
+            f32x4 rest;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rest[e] = z[e] - (float)(T)z[e];
+            store4(low + 32 * y + 8 * r + 4 * g, rest);
+          }
+        }
       }
   }
 }

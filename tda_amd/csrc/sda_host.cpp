@@ -67,6 +67,13 @@ int32_t check_common(const A& a) {
   return check_lambda(a.lambda_param, a.lambda_stride, a.lambda_dtype);
 }
 
+// What a training forward keeps for the backward.
+template <class A>
+int32_t check_kept(const A& a) {
+  if (int32_t rc = check_rows(a.out2, 4)) return rc;
+  return a.dtype == TDA_DTYPE_BF16 ? check_rows(a.out_low, 2) : TDA_OK;
+}
+
 sda::Rows rows_of(const tda_tensor& t) { return {t.data, t.stride[0], t.stride[1], t.stride[2]}; }
 sda::Lambda lambda_of(const void* p, const int64_t (&s)[3], int32_t dtype) {
   return {p, s[0], s[1], s[2], dtype == TDA_DTYPE_BF16 ? 1 : 0};
@@ -120,6 +127,7 @@ void fill(P& p, const A& a) {
   p.v = rows_of(a.v);
   p.out = rows_of(a.out);
   p.out2 = rows_of(a.out2);
+  p.low = rows_of(a.out_low);
   p.lam = lambda_of(a.lambda_param, a.lambda_stride, a.lambda_dtype);
   p.see = {a.causal, (int)(a.q_offsets ? 0 : a.q_offset), a.q_offsets, a.kv_lens};
   p.B = (int)a.batch;
@@ -201,7 +209,7 @@ int32_t sda_validate_fwd(const sda_fwd_args* a) {
   for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out})
     if (int32_t rc = check_rows(*t, es)) return rc;
   if (a->out2.data)
-    if (int32_t rc = check_rows(a->out2, es)) return rc;
+    if (int32_t rc = check_kept(*a)) return rc;
   return check_workspace(a->workspace, a->workspace_bytes, sda_fwd_workspace_bytes(a));
 }
 
@@ -232,9 +240,10 @@ int32_t sda_validate_bwd(const sda_bwd_args* a) {
   if (!a) return TDA_ERR_NULL_POINTER;
   if (int32_t rc = check_common(*a)) return rc;
   const int64_t es = bytes_of(a->dtype);
-  for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out, &a->out2, &a->dout, &a->dq1, &a->dk1,
-                              &a->dq2, &a->dk2, &a->dv})
+  for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out, &a->dout, &a->dq1, &a->dk1, &a->dq2,
+                              &a->dk2, &a->dv})
     if (int32_t rc = check_rows(*t, es)) return rc;
+  if (int32_t rc = check_kept(*a)) return rc;
   if (!a->lse) return TDA_ERR_NULL_POINTER;
   return check_workspace(a->workspace, a->workspace_bytes, sda_bwd_workspace_bytes(a));
 }

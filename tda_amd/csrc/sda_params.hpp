@@ -26,7 +26,7 @@ struct Sight {
 };
 
 struct FwdParams {
-  Rows q[2], k[2], v, out, out2;  // out2.p may be null
+  Rows q[2], k[2], v, out, out2, low;  // out2.p (f32) may be null; low: bf16 alone
   Lambda lam;
   Sight see;
   int B, H, Hk, Nq, Nk, nqt;      // nqt: query tiles of kBlockRows
@@ -38,7 +38,7 @@ struct FwdParams {
 };
 
 struct BwdParams {
-  Rows q[2], k[2], v, out, out2, dout, dq[2], dk[2], dv;
+  Rows q[2], k[2], v, out, out2, low, dout, dq[2], dk[2], dv;
   Lambda lam;
   Sight see;
   int B, H, Hk, Nq, Nk;

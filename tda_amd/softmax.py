@@ -25,8 +25,8 @@ _COMPUTE = {torch.float32: torch.float32, torch.bfloat16: torch.bfloat16,
 _CODE = {torch.float32: _abi.DTYPE_F32, torch.bfloat16: _abi.DTYPE_BF16, torch.float16: _sda_abi.DTYPE_F16}
 _ROW_BYTES = 1 << 25  # the largest distance between rows that the kernels take
 
-_FWD_ROWS = ("q1", "k1", "q2", "k2", "v", "out", "out2")
-_BWD_ROWS = ("q1", "k1", "q2", "k2", "v", "out", "out2", "dout", "dq1", "dk1", "dq2", "dk2", "dv")
+_FWD_ROWS = ("q1", "k1", "q2", "k2", "v", "out", "out2", "out_low")
+_BWD_ROWS = ("q1", "k1", "q2", "k2", "v", "out", "out2", "out_low", "dout", "dq1", "dk1", "dq2", "dk2", "dv")
 
 
 def _offsets(args, names):
@@ -129,12 +129,12 @@ def _pad(t: torch.Tensor, d: int) -> torch.Tensor:
     return t if t.shape[-1] == d else F.pad(t, (0, d - t.shape[-1]))
 
 
-def _new_rows(like: torch.Tensor, width: int) -> torch.Tensor:
+def _new_rows(like: torch.Tensor, width: int, dtype=None) -> torch.Tensor:
     """Uninitialised (B, H, N, width) rows in like's memory order."""
     b, h, n, _ = like.shape
     if h > 1 and n > 1 and like.stride(1) < like.stride(2):
-        return torch.empty((b, n, h, width), dtype=like.dtype, device=like.device).transpose(1, 2)
-    return torch.empty((b, h, n, width), dtype=like.dtype, device=like.device)
+        return torch.empty((b, n, h, width), dtype=dtype or like.dtype, device=like.device).transpose(1, 2)
+    return torch.empty((b, h, n, width), dtype=dtype or like.dtype, device=like.device)
 
 
 # ------------------------------------------------------------------ calls
@@ -183,14 +183,15 @@ def _fill(buf, off, names, tensors):
 
 
 def _forward(q1, q2, k1, k2, v, lam, scale, causal, q_offset, q_offsets, kv_lens, saving):
-    """One sda_fwd call on usable tensors: out, and (saving) out2 and lse for the backward."""
+    """One sda_fwd call on usable tensors: out, and (saving) out2, out_low and lse for the backward."""
     lib = _sda_abi.load()
     out = _new_rows(q1, v.shape[3])
-    out2 = lse = None
+    out2 = low = lse = None
     if saving:
-        out2 = _new_rows(q1, v.shape[3])
+        out2 = _new_rows(q1, v.shape[3], torch.float32)
+        low = _new_rows(q1, v.shape[3]) if q1.dtype == torch.bfloat16 else None
         lse = torch.empty((2,) + q1.shape[:3], dtype=torch.float32, device=q1.device)
-    rows = (q1, k1, q2, k2, v, out, out2)
+    rows = (q1, k1, q2, k2, v, out, out2, low)
     tpl, size = _template("sda_fwd", rows, _FWD_ROWS, _sda_abi.SdaFwdArgs, "sda_fwd_workspace_bytes", lam, scale,
                           causal, q_offset, (saving,))
     buf = bytearray(tpl)
@@ -198,7 +199,7 @@ def _forward(q1, q2, k1, k2, v, lam, scale, causal, q_offset, q_offsets, kv_lens
     ws = torch.empty(size, dtype=torch.uint8, device=q1.device) if size else None
     _fill(buf, _FWD_OFF, ("lambda_param", "q_offsets", "kv_lens", "lse", "workspace"), (lam, q_offsets, kv_lens, lse, ws))
     _launch(lib.sda_fwd, _sda_abi.SdaFwdArgs, buf, q1.device, "sda_fwd")
-    return out, out2, lse
+    return out, out2, low, lse
 
 
 class _DifferentialAttention(torch.autograd.Function):
@@ -206,23 +207,23 @@ class _DifferentialAttention(torch.autograd.Function):
     def forward(ctx, q1, q2, k1, k2, v, lam, scale, causal, q_offset, q_offsets, kv_lens):
         saving = any(ctx.needs_input_grad[:6])
         rows = [_usable(t) for t in (q1, q2, k1, k2, v)]
-        out, out2, lse = _forward(*rows, lam, scale, causal, q_offset, q_offsets, kv_lens, saving)
+        out, out2, low, lse = _forward(*rows, lam, scale, causal, q_offset, q_offsets, kv_lens, saving)
         if saving:
-            ctx.save_for_backward(*rows, lam, out, out2, lse, q_offsets, kv_lens)
+            ctx.save_for_backward(*rows, lam, out, out2, low, lse, q_offsets, kv_lens)
             ctx.cfg = (scale, causal, q_offset)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q1, q2, k1, k2, v, lam, out, out2, lse, q_offsets, kv_lens = ctx.saved_tensors
+        q1, q2, k1, k2, v, lam, out, out2, low, lse, q_offsets, kv_lens = ctx.saved_tensors
         scale, causal, q_offset = ctx.cfg
         lib = _sda_abi.load()
         dout = _usable(dout if dout.dtype == q1.dtype else dout.to(q1.dtype))
         dq1, dq2 = _new_rows(q1, q1.shape[3]), _new_rows(q2, q2.shape[3])
         dk1, dk2, dv = (_new_rows(t, t.shape[3]) for t in (k1, k2, v))
         dlam = torch.empty(lam.shape, dtype=lam.dtype, device=lam.device) if ctx.needs_input_grad[5] else None
-        rows = (q1, k1, q2, k2, v, out, out2, dout, dq1, dk1, dq2, dk2, dv)
+        rows = (q1, k1, q2, k2, v, out, out2, low, dout, dq1, dk1, dq2, dk2, dv)
         tpl, size = _template("sda_bwd", rows, _BWD_ROWS, _sda_abi.SdaBwdArgs, "sda_bwd_workspace_bytes", lam, scale,
                               causal, q_offset)
         buf = bytearray(tpl)

@@ -75,7 +75,8 @@ def fwd(**kw):
 
 def bwd(**kw):
     a = _common(_sda_abi.SdaBwdArgs(), **kw)
-    for n, like in (("out2", "out"), ("dout", "out"), ("dq1", "q1"), ("dq2", "q2"), ("dk1", "k1"), ("dk2", "k2"), ("dv", "v")):
+    a.out2 = _rows((a.batch, a.heads, a.seq_len, a.v_head_dim))
+    for n, like in (("out_low", "out"), ("dout", "out"), ("dq1", "q1"), ("dq2", "q2"), ("dk1", "k1"), ("dk2", "k2"), ("dv", "v")):
         setattr(a, n, getattr(a, like))
     a.lse = a.workspace = FAKE
     a.workspace_bytes = lib().sda_bwd_workspace_bytes(ctypes.byref(a))
@@ -141,6 +142,12 @@ def test_attention_workspaces():
     b = bwd()
     b.lse = None
     assert so.sda_validate_bwd(ctypes.byref(b)) == _abi.ERR_NULL_POINTER
+    for name in ("out2", "out_low"):  # what the forward keeps; f32 needs no low part
+        b = bwd()
+        getattr(b, name).data = None
+        assert so.sda_validate_bwd(ctypes.byref(b)) == _abi.ERR_NULL_POINTER
+        b.dtype = _abi.DTYPE_F32
+        assert so.sda_validate_bwd(ctypes.byref(b)) == (_abi.OK if name == "out_low" else _abi.ERR_NULL_POINTER)
     assert so.sda_fwd_workspace_bytes(None) == so.sda_bwd_workspace_bytes(None) == so.sda_kv4_attend_workspace_bytes(None) == 0
 
 
