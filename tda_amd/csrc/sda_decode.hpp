@@ -190,19 +190,42 @@ __global__ void __launch_bounds__(256) decode_join(DecParams P) {
   const int n = threadIdx.x & 15, y = 16 * cb + (threadIdx.x >> 4);
   const int64_t step = dec_part_floats(DV);
   const float* base = P.part + (int64_t)item * P.nsplit * step;
+  // eight parts at a time: their loads are on their way together
   float res[2];
+  float all[2] = {kNoMax, kNoMax}, l[2] = {}, a[2] = {};
+  for (int s0 = 0; s0 < P.nsplit; s0 += 8) {
+    float mm[2][8], ll[2][8], aa[2][8];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    float all = kNoMax, l = 0.f, a = 0.f;
-    for (int s = 0; s < P.nsplit; ++s) all = fmaxf(all, base[s * step + 32 * x + n]);
-    for (int s = 0; s < P.nsplit; ++s) {
-      const float w = exp2_(base[s * step + 32 * x + n] - all), ls = base[s * step + 32 * x + 16 + n];
-      if (ls == 0.f) continue;  // no key of this part: its sums are not written
-      l = __builtin_fmaf(ls, w, l);
-      a = __builtin_fmaf(base[s * step + 64 + (x * DV + y) * 16 + n], w, a);
+    for (int u = 0; u < 8; ++u) {
+      const float* part = base + min(s0 + u, P.nsplit - 1) * step;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mm[x][u] = part[32 * x + n];
+        ll[x][u] = s0 + u < P.nsplit ? part[32 * x + 16 + n] : 0.f;
+        aa[x][u] = part[64 + (x * DV + y) * 16 + n];
+      }
     }
-    res[x] = l > 0.f || l != l ? a / l : 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float top = all[x];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, mm[x][u]);
+      const float f = exp2_(all[x] - top);
+      l[x] *= f;
+      a[x] *= f;
+      all[x] = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = exp2_(mm[x][u] - top);
+        if (ll[x][u] != 0.f) {  // else no key of this part: its sums are not written
+          l[x] = __builtin_fmaf(ll[x][u], w, l[x]);
+          a[x] = __builtin_fmaf(aa[x][u], w, a[x]);
+        }
+      }
+    }
   }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) res[x] = l[x] > 0.f || l[x] != l[x] ? a[x] / l[x] : 0.f;
   __shared__ float turned[16][17];
   const int row = rt * kDecRows + n;
   const bool live = row < R;

@@ -119,5 +119,9 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
             raise ValueError("a tensor of xs has no heads")
         res = tuple(t.clone() for t in ts)
         return res[0] if one else res
-    res = _Rotary.apply(positions, inv_freq.contiguous(), sections, bool(interleaved), *ts)
+    inv_freq = inv_freq.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        res = _Rotary.apply(positions, inv_freq, sections, bool(interleaved), *ts)
+    else:
+        res = _turn(ts, positions, inv_freq, sections, bool(interleaved), False)
     return res[0] if one else res

@@ -23,6 +23,8 @@ _PUT = struct.Struct("<Q").pack_into
 _COMPUTE = {torch.float32: torch.float32, torch.bfloat16: torch.bfloat16,
             torch.float16: torch.float32, torch.float64: torch.float32}
 _CODE = {torch.float32: _abi.DTYPE_F32, torch.bfloat16: _abi.DTYPE_BF16, torch.float16: _sda_abi.DTYPE_F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)  # the current stream's handle
 _ROW_BYTES = 1 << 25  # the largest distance between rows that the kernels take
 
 _FWD_ROWS = ("q1", "k1", "q2", "k2", "v", "out", "out2", "out_low")
@@ -38,24 +40,34 @@ _BWD_OFF = _offsets(_sda_abi.SdaBwdArgs, _BWD_ROWS + ("lambda_param", "q_offsets
 
 
 # ------------------------------------------------------------------ arguments
+_stride_ok: dict = {}  # (strides, element size): whether rows laid out so can be read in place
+
+
 def _usable(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it in place, else a contiguous copy."""
-    u = ops._usable(t)
-    return u if u.stride(2) * u.element_size() <= _ROW_BYTES else u.contiguous()
+    st, es = t.stride(), t.element_size()
+    ok = _stride_ok.get((st, es))
+    if ok is None:
+        if len(_stride_ok) > 4096:
+            _stride_ok.clear()
+        ok = _stride_ok[st, es] = (st[3] == 1 and all(s >= 0 and s * es % 16 == 0 for s in st[:3])
+                                   and st[2] * es <= _ROW_BYTES)
+    return t if ok and t.data_ptr() % 16 == 0 else t.contiguous()
 
 
 def _check_rows(tensors, names, shapes=None):
     """4-D floating tensors of one dtype on one GPU, the batch the same."""
     ref = tensors[0]
+    dtype, device = getattr(ref, "dtype", None), getattr(ref, "device", None)
     for t, n in zip(tensors, names):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{n} must be a torch.Tensor")
         if t.dim() != 4:
             raise ValueError(f"{n} must have shape (batch, heads, seq_len, head_dim), got {tuple(t.shape)}")
-        if t.dtype != ref.dtype:
-            raise ValueError(f"dtype mismatch: {names[0]} {ref.dtype} vs {n} {t.dtype}")
-        if t.device != ref.device:
-            raise ValueError(f"device mismatch: {names[0]} {ref.device} vs {n} {t.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"dtype mismatch: {names[0]} {dtype} vs {n} {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"device mismatch: {names[0]} {device} vs {n} {t.device}")
     if ref.device.type != "cuda":
         raise ValueError(f"tda_amd runs on the GPU only (HIP); got tensors on {ref.device}")
     if not ref.dtype.is_floating_point:
@@ -170,10 +182,12 @@ def _template(kind, rows, names, args_type, size_fn, lam, scale, causal, q_offse
 def _launch(fn, args_type, buf, device, what):
     a = args_type.from_buffer(buf)
     if torch.cuda.current_device() == device.index:
-        _sda_abi.check(fn(ctypes.byref(a), ops._stream(device)), what)
+        rc = fn(ctypes.byref(a), _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            _sda_abi.check(fn(ctypes.byref(a), ops._stream(device)), what)
+            rc = fn(ctypes.byref(a), _raw_stream(device.index))
+    if rc:
+        _sda_abi.check(rc, what)
 
 
 def _fill(buf, off, names, tensors):
@@ -283,7 +297,10 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
         return torch.zeros((b, h, n, dv), dtype=q1.dtype, device=dev) + zero
     rows = [t if t.dtype == cdt else t.to(cdt) for t in tensors]
     rows = [_pad(t, kd) for t in rows[:4]] + [_pad(rows[4], kv)]
-    out = _DifferentialAttention.apply(*rows, lam, s, bool(causal), off, q_offsets, lens)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*rows, lam)):
+        out = _DifferentialAttention.apply(*rows, lam, s, bool(causal), off, q_offsets, lens)
+    else:
+        out = _forward(*(_usable(t) for t in rows), lam, s, bool(causal), off, q_offsets, lens, False)[0]
     if kv != dv:
         out = out[..., :dv]
     return out if out.dtype == q1.dtype else out.to(q1.dtype)
