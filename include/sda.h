@@ -112,8 +112,9 @@ typedef struct sda_rotary_args {
  * values x: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) in 32 bits, code =
  * min(max(rint((x - m) / s), 0), 15) (ties to even, 0 when s < 2^-100), value m + s code; a group with a NaN or an infinity, or whose
  * s is not finite, reads as NaN.  Three buffers of
- * sda_kv4_bytes() bytes each: for (b, head) capacity rows of codes (d / 2 bytes each), then behind all
- * codes the groups' (m, s). */
+ * sda_kv4_bytes() bytes each: for (b, head) the codes of capacity rows (rounded up to four; d / 2
+ * bytes a row), then behind all codes the groups' (m, s); their order within is the kernels' own.
+ * capacity is at most 2^24. */
 typedef struct sda_kv4 {
   int64_t batch, kv_heads, capacity, head_dim, v_head_dim;
   void*    k1;

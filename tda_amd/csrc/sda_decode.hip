@@ -11,6 +11,7 @@ struct DenseSrc {
   static constexpr int D = D_, DV = DV_, NT = D / 32;
   static constexpr int CW = DV / 16 < 8 ? DV / 16 : 8, NB = DV / (16 * CW);  // columns of a lane, blocks of them
   typedef T row __attribute__((ext_vector_type(CW)));
+  static constexpr int NBUF = sizeof(T) == 2 && DV <= 128 ? 2 : 1;
   struct Regs {
     frag k[2][2][NT];
     row v[8][NB];
@@ -42,40 +43,54 @@ struct DenseSrc {
     vp = row_of<T>(F->v, b, hk, 0);
     vs = F->v.st;
   }
-  __device__ __forceinline__ void load(Regs& g, int t0, int lim, bool edge) {
-    const int n = lane_id() & 15, kq = lane_id() >> 4;
+  __device__ __forceinline__ static frag load8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(bf16x8, a);
+    } else {
+      const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
+      return f32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
+  }
+  __device__ __forceinline__ void load(Regs& g, int t0, int lim) {
+    const int n = lane_id() & 15, kq = lane_id() >> 4, rows = min(32, lim - t0);
+    constexpr int ES = sizeof(T);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const auto r = rows_rsrc(kp[x] + (int64_t)t0 * ks[x], ks[x] * ES, rows, D * ES);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) g.k[x][y][t] = load8(r, (uint32_t)(16 * y + n) * (uint32_t)(ks[x] * ES) + (32 * t + 8 * kq) * ES);
+    }
+    const auto r = rows_rsrc(vp + (int64_t)t0 * vs, vs * ES, rows, DV * ES);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int y = 0; y < NB; ++y) {
+        const uint32_t off = (uint32_t)(16 * (j >> 2) + 4 * kq + (j & 3)) * (uint32_t)(vs * ES) + (CW * n + 16 * CW * y) * ES;
+        if constexpr (CW * ES == 8) g.v[j][y] = __builtin_bit_cast(row, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+        else if constexpr (CW * ES == 16) g.v[j][y] = __builtin_bit_cast(row, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+        else g.v[j][y] = load8(r, off);
+      }
+  }
+  __device__ __forceinline__ void scores(const Regs& g, f32x4 (&s)[2][2]) {
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const T* r = kp[x] + (int64_t)min(t0 + 16 * y + n, lim - 1) * ks[x] + 8 * kq;  // a row past the keys: masked
+        s[x][y] = f32x4{};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) g.k[x][y][t] = load8(r + 32 * t);
+        for (int t = 0; t < NT; ++t) s[x][y] = Tr::mma16(g.k[x][y][t], q[x][t], s[x][y]);
       }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = t0 + 16 * (j >> 2) + 4 * kq + (j & 3);
-      const T* r = vp + (int64_t)min(key, lim - 1) * vs + CW * n;
-#pragma unroll
-      for (int y = 0; y < NB; ++y) g.v[j][y] = *reinterpret_cast<const row*>(r + 16 * CW * y);
-      if (edge && key >= lim)
-#pragma unroll
-        for (int y = 0; y < NB; ++y) g.v[j][y] = row{};  // weight 0: nothing, whatever the row holds
-    }
-  }
-  __device__ __forceinline__ void scores(const Regs& g, int x, f32x4 (&s)[2]) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      s[y] = f32x4{};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s[y] = Tr::mma16(g.k[x][y][t], q[x][t], s[y]);
-    }
   }
   __device__ __forceinline__ void rescale(int, float) {}
-  __device__ __forceinline__ void add(const Regs& g, int, const f32x4 (&s)[2], f32x4 (&o)[DV / 16]) {
-    frag p;
+  __device__ __forceinline__ void add(const Regs& g, const f32x4 (&s)[2][2], f32x4 (&o)[2][DV / 16]) {
+    frag p[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = (T)s[j >> 2][j & 3];
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[x][j] = (T)s[x][j >> 2][j & 3];
 #pragma unroll
     for (int y = 0; y < NB; ++y)
 #pragma unroll
@@ -83,7 +98,8 @@ struct DenseSrc {
         frag a;
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = g.v[j][y][c];
-        o[CW * y + c] = Tr::mma16(a, p, o[CW * y + c]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) o[x][CW * y + c] = Tr::mma16(a, p[x], o[x][CW * y + c]);
       }
   }
   __device__ __forceinline__ void finish(f32x4 (&)[2][DV / 16]) {}

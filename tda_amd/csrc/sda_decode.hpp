@@ -8,8 +8,8 @@
 // every key and value byte is used by one wave alone and goes straight to its registers.  Bound by
 // reading the cache.  The waves' sums meet in LDS, the parts' in a second launch.
 //
-// A source (Src) brings: D, DV, `Regs` (a tile's loads), load, scores, add (O += V^T P^T), finish
-// and column (the output column of value r of tile t in lane quarter kq).
+// A source (Src) brings: D, DV, `Regs` (a tile's loads) and NBUF, load, scores, add (O += V^T P^T), finish and column (the output column of value r of tile t in lane
+// quarter kq).
 #pragma once
 
 #include "sda_common.hpp"
@@ -55,27 +55,29 @@ __device__ __forceinline__ void decode_body(const DecParams& P, Src& src, float*
   float m[2] = {kNoMax, kNoMax}, sum[2] = {0.f, 0.f};
   if (k0 < k1) {
     src.begin(P, b, hk, h, i, live);
-    typename Src::Regs regs;
-    for (int t0 = k0 + 32 * wv; t0 < k1; t0 += 128) {
-      const bool edge = t0 + 32 > k1;
-      src.load(regs, t0, k1, edge);
+    // NBUF tiles' registers: one in use, the others' loads on their way.  Rows past the part's end, and
+    // whole tiles, read as zeros by the buffer descriptors' range check: a weight of zero times whatever lies
+    // there must stay zero.  (Skipping such loads would keep the compiler from counting the loads behind
+    // the one it waits for.)
+    constexpr int NBUF = Src::NBUF;
+    typename Src::Regs regs[NBUF];
+    const int t1 = k0 + 32 * wv;
+    times<NBUF - 1>([&](auto u) { src.load(regs[u], t1 + 128 * u, k1); });
+    auto tile = [&](typename Src::Regs& r, int t0) {
+      f32x4 w[2][2];
+      src.scores(r, w);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        f32x4 s[2];
-        src.scores(regs, x, s);
+        f32x4(&s)[2] = w[x];
         if (__any(t0 + 31 >= see)) {
 #pragma unroll
           for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (t0 + 16 * y + 4 * kq + r >= min(see, k1)) s[y][r] = -__builtin_inff();
+            for (int e = 0; e < 4; ++e)
+              if (t0 + 16 * y + 4 * kq + e >= min(see, k1)) s[y][e] = -__builtin_inff();
         }
-        float top = s[0][0];
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[y][r]);
-        top *= P.c;
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * P.c;
         if (__any(top > m[x] + kSlack)) {
           top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32));
@@ -87,15 +89,20 @@ __device__ __forceinline__ void decode_body(const DecParams& P, Src& src, float*
           for (int y = 0; y < NO; ++y) o[x][y] *= f;
         }
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < 2; ++y) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[y][r] = exp2_(__builtin_fmaf(s[y][r], P.c, -m[x]));
-            sum[x] += s[y][r];
-          }
-        src.add(regs, x, s, o[x]);
+          for (int e = 0; e < 4; ++e) s[y][e] = exp2_(__builtin_fmaf(s[y][e], P.c, -m[x]));
+          sum[x] += (s[y][0] + s[y][1]) + (s[y][2] + s[y][3]);
+        }
       }
-    }
+      src.add(r, w, o);
+    };
+    for (int t0 = t1; t0 < k1; t0 += 128 * NBUF)
+      times<NBUF>([&](auto u) {
+        const int t = t0 + 128 * u;
+        src.load(regs[(u + NBUF - 1) % NBUF], t + 128 * (NBUF - 1), k1);
+        if (t < k1) tile(regs[u], t);
+      });
     src.finish(o);
   }
 #pragma unroll

@@ -13,6 +13,7 @@ namespace {
 
 constexpr int64_t kMaxPos = (int64_t(1) << 30) - 64;      // positions and row counts stay in int32
 constexpr int64_t kMaxRowBytes = int64_t(1) << 25;        // a tile of 64 rows spans at most 2^31 bytes
+constexpr int64_t kMaxCapacity = int64_t(1) << 24;        // a head's codes stay within 32-bit offsets
 constexpr double kLog2e = 1.4426950408889634074;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -141,7 +142,7 @@ void fill(P& p, const A& a) {
 int32_t check_cache(const sda_kv4& c) {
   if (c.batch < 1 || c.kv_heads < 1 || c.capacity < 1) return TDA_ERR_SHAPE;
   if (!head_dims(c.head_dim, c.v_head_dim)) return TDA_ERR_HEAD_DIM;
-  if (c.capacity > kMaxPos || c.batch > kMaxPos || c.kv_heads > kMaxPos || c.batch * c.kv_heads > kMaxPos) return SDA_ERR_CACHE;
+  if (c.capacity > kMaxCapacity || c.batch > kMaxPos || c.kv_heads > kMaxPos || c.batch * c.kv_heads > kMaxPos) return SDA_ERR_CACHE;
   if (!fits_grid((double)c.batch * c.kv_heads * c.capacity * c.v_head_dim / 2048.0)) return SDA_ERR_CACHE;
   if (!c.k1 || !c.k2 || !c.v || !c.lengths) return TDA_ERR_NULL_POINTER;
   for (const void* p : {c.k1, c.k2, c.v})
@@ -154,12 +155,13 @@ void fill_cache(sda::Kv4Params& p, const sda_kv4& c) {
   for (int z = 0; z < 3; ++z) {
     const int64_t w = z < 2 ? c.head_dim : c.v_head_dim;
     p.codes[z] = static_cast<uint8_t*>(at[z]);
-    p.pars[z] = reinterpret_cast<uint32_t*>(p.codes[z] + c.batch * c.kv_heads * c.capacity * (w / 2));
+    p.pars[z] = reinterpret_cast<uint32_t*>(p.codes[z] + c.batch * c.kv_heads * ceil_div(c.capacity, 4) * 4 * (w / 2));
   }
   p.lengths = c.lengths;
   p.B = (int)c.batch;
   p.Hk = (int)c.kv_heads;
   p.cap = (int)c.capacity;
+  p.cap4 = ceil_div(c.capacity, 4) * 4;
   p.D = (int)c.head_dim;
   p.DV = (int)c.v_head_dim;
 }
@@ -329,7 +331,7 @@ int32_t sda_rotary(const sda_rotary_args* a, void* stream) {
 
 size_t sda_kv4_bytes(int64_t batch, int64_t kv_heads, int64_t capacity, int64_t width) {
   if (batch < 1 || kv_heads < 1 || capacity < 1 || (width != 64 && width != 128 && width != 256)) return 0;
-  return (size_t)(batch * kv_heads * capacity * (width / 2 + width / 64 * 4));
+  return (size_t)(batch * kv_heads * (ceil_div(capacity, 4) * 4) * (width / 2 + width / 64 * 4));
 }
 
 int32_t sda_validate_kv4_append(const sda_kv4_append_args* a) {

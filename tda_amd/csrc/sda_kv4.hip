@@ -3,13 +3,16 @@
 // A row in groups of 64 values x: m = bf16(min), s = bf16((max - m) * (1 / 15)) in 32 bits,
 // code = rint((x - m) / s) clamped to 0 .. 15, value m + s code.  4.5 bits a value.
 //
-// Codes lie so that the attention's registers need no exchange between lanes:
+// Codes lie so that the attention's registers need no exchange between lanes and its loads are wide (the
+// loads' number is what bounds it next to the memory's rate):
 //   keys: word u (32 bits) of a group holds its values 8 u .. 8 u + 7; bits 4 i hold value 2 i and bits
-//   16 + 4 i value 2 i + 1, so (word >> 4 i) & 0x000f000f is a pair of neighbours;
+//   16 + 4 i value 2 i + 1, so (word >> 4 i) & 0x000f000f is a pair of neighbours; a row of two groups
+//   has words 2 q and 2 q + 1 of both side by side;
 //   values: 16-bit units of four neighbouring columns, bits 4 j holding column 4 n + j of group gr in
-//   unit (gr, n); a row of 64 columns holds its units in order, a wider one pairs the units (gr, n) and
-//   (gr + 1, n) of two groups in a word, words by n, then by pair.
-// Behind the codes of all rows: (m, s) of each row's groups, s in the high half of a word.
+//   unit (gr, n); the words of a row are its units in order (64 columns), or pair the units (gr, n) and
+//   (gr + 1, n) of two groups, by n, then by pair.  Four rows lie together, word by word.
+// Behind the codes of all rows: (m, s) of each row's groups, s in the high half of a word.  A head has
+// rows for its capacity rounded up to four.
 #include "sda_decode.hpp"
 
 namespace sda {
@@ -58,6 +61,13 @@ __device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv
   return (uint32_t)min(k + (up ? 1 : 0), 15);
 }
 
+// Place of key word u (of W / 8) in its row, and of word w of value row i (L words) of the head whose rows
+// start at row0.
+__device__ __forceinline__ int key_place(int W, int u) { return W == 64 ? u : 4 * ((u & 7) >> 1) + 2 * (u >> 3) + (u & 1); }
+__device__ __forceinline__ int64_t value_word(int64_t row0, int64_t i, int L, int w) {
+  return row0 * L + (i >> 2) * (4 * L) + 4 * w + (i & 3);
+}
+
 // ------------------------------------------------------------------ append
 // 8 lanes per group of 64 values, 8 values a lane.
 template <class T>
@@ -97,14 +107,14 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P) {
   uint32_t c[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) c[e] = inv > 0.f ? code_of(x[e], m, s, inv) : 0u;
-  const int64_t row = bk * P.cap + at;
+  const int64_t row = bk * P.cap4 + at;
   uint32_t word;
   int place;
   if (z < 2) {
     word = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) word |= (c[2 * e] << (4 * e)) | (c[2 * e + 1] << (16 + 4 * e));
-    place = u;
+    place = key_place(W, u);
   } else {
     const uint32_t a = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12, d = c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12;
     if (W == 64) {
@@ -118,7 +128,7 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P) {
     }
   }
   if (put) {
-    reinterpret_cast<uint32_t*>(P.codes[z])[row * L + place] = word;
+    reinterpret_cast<uint32_t*>(P.codes[z])[z < 2 ? row * L + place : value_word(bk * P.cap4, at, L, place)] = word;
     if ((u & 7) == 0) P.pars[z][row * (W / 64) + u / 8] = bad ? 0x7fc0u : mb | sb << 16;
   }
   if (P.start && z == 0 && in && hk == 0 && i == 0 && u == 0)
@@ -144,22 +154,23 @@ __global__ void __launch_bounds__(256) kv4_read(Kv4Params P) {
   const int b = (int)(bk / P.Hk), hk = (int)(bk % P.Hk);
   float x[8] = {};
   if (i < min(P.lengths[b], P.cap)) {
-    const int64_t row = bk * P.cap + i;
+    const int64_t row = bk * P.cap4 + i;
     const uint32_t par = P.pars[z][row * (W / 64) + u / 8];
     const float m = bf16_lo(par), s = bf16_hi(par);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.codes[z]) + row * L;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.codes[z]);
     if (z < 2) {
-      const uint32_t w = words[u];
+      const uint32_t w = words[row * L + key_place(W, u)];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s, (float)(w >> (4 * (e >> 1) + 16 * (e & 1)) & 15), m);
     } else {
       uint32_t a, d;  // units of columns 8 u' .. + 3 and + 4 .. + 7
       if (W == 64) {
-        const uint32_t w = words[u];
+        const uint32_t w = words[value_word(bk * P.cap4, i, L, u)];
         a = w & 0xffff;
         d = w >> 16;
       } else {
-        const uint32_t w0 = words[16 * (u >> 4) + 2 * (u & 7)], w1 = words[16 * (u >> 4) + 2 * (u & 7) + 1];
+        const int place = 16 * (u >> 4) + 2 * (u & 7);
+        const uint32_t w0 = words[value_word(bk * P.cap4, i, L, place)], w1 = words[value_word(bk * P.cap4, i, L, place + 1)];
         a = u & 8 ? w0 >> 16 : w0 & 0xffff;
         d = u & 8 ? w1 >> 16 : w1 & 0xffff;
       }
@@ -187,14 +198,16 @@ struct Kv4Src {
   struct Regs {
     uint32_t k[2][2][GK][2];      // [branch][16 keys][group][word 2 kq + i]
     uint32_t kp[2][2][4][GK];     // [branch][16 keys][key 4 kq + r][group]
-    uint32_t v[8][WV];            // [key][pair of groups]
+    uint32_t v[2][WV][4];         // [16 keys][pair of groups][key 4 kq + r]
     uint32_t vp[8][GV];
   };
   const Kv4Params* C;
   bf16x8 q[2][NP][GK][2];
   float qs[2][GK];                // sum of a group's query values
-  float corr[2][GV];              // what every column of a group still gets
-  const uint32_t *kc[2], *kpar[2], *vc, *vpar;
+  float corr[2][GV];              // sum of weight * middle, which every column of a group still gets
+  f32x4 used[2][GV];              // sum of the rounded weight * step
+  static constexpr int NBUF = 1;
+  const uint32_t *kc[2], *kpar[2], *vc, *vpar;  // the head's rows: within them offsets are 32-bit
 
   __device__ __forceinline__ static bf16x8 codes(uint32_t w) {  // 8 codes of a key word, in value order
     u32x4 x;
@@ -222,7 +235,7 @@ struct Kv4Src {
 
   __device__ __forceinline__ void begin(const DecParams& P, int b, int hk, int h, int i, bool live) {
     const int kq = lane_id() >> 4;
-    const int64_t row0 = ((int64_t)b * P.Hk + hk) * P.Nk;
+    const int64_t row0 = ((int64_t)b * P.Hk + hk) * C->cap4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       kc[x] = reinterpret_cast<const uint32_t*>(C->codes[x]) + row0 * (D / 8);
@@ -248,92 +261,109 @@ struct Kv4Src {
         qs[x][y] = a + __shfl_xor(a, 32);
       }
 #pragma unroll
-      for (int y = 0; y < GV; ++y) corr[x][y] = 0.f;
+      for (int y = 0; y < GV; ++y) corr[x][y] = 0.f, used[x][y] = f32x4{};
     }
     vc = reinterpret_cast<const uint32_t*>(C->codes[2]) + row0 * (DV / 8);
     vpar = C->pars[2] + row0 * GV;
   }
-  __device__ __forceinline__ void load(Regs& g, int t0, int lim, bool edge) {
-    const int n = lane_id() & 15, kq = lane_id() >> 4;
+  // N words from word `at` on (rows past the descriptor's: zeros).
+  template <int N>
+  __device__ __forceinline__ static void words(uint32_t* to, __amdgpu_buffer_rsrc_t r, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      if constexpr (N % 4 == 0) {
+        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, 4 * (at + i), 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[i + e] = w[e];
+      } else {
+        static_assert(N == 2, "2 or a multiple of 4 words");
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, 4 * at, 0, 0);
+        to[0] = w[0], to[1] = w[1];
+      }
+    }
+  }
+  __device__ __forceinline__ void load(Regs& g, int t0, int lim) {
+    const int n = lane_id() & 15, kq = lane_id() >> 4, t = t0 + 4 * kq;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const auto c = rsrc_of(kc[x], (uint32_t)lim * (D / 2)), p = rsrc_of(kpar[x], (uint32_t)lim * (4 * GK));
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        words<2 * GK>(&g.k[x][y][0][0], c, (uint32_t)(t0 + 16 * y + n) * (D / 8) + 2 * GK * kq);
+        words<4 * GK>(&g.kp[x][y][0][0], p, (uint32_t)(t + 16 * y) * GK);
+      }
+    }
+    // codes of rows past the keys may be anything: their steps and minima are zeros
+    const auto c = rsrc_of(vc, (uint32_t)((lim + 3) & ~3) * (DV / 2)), p = rsrc_of(vpar, (uint32_t)lim * (4 * GV));
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      words<4 * GV>(&g.vp[4 * y][0], p, (uint32_t)(t + 16 * y) * GV);
+#pragma unroll
+      for (int z = 0; z < WV; ++z)
+        words<4>(&g.v[y][z][0], c, (uint32_t)(t + 16 * y) * (DV / 8) + 4 * (DV == 64 ? n >> 1 : 16 * z + n));
+    }
+  }
+  __device__ __forceinline__ void scores(const Regs& g, f32x4 (&s)[2][2]) {
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int64_t key = min(t0 + 16 * y + n, lim - 1);
+        s[x][y] = f32x4{};
 #pragma unroll
         for (int z = 0; z < GK; ++z) {
-          const uint2 w = *reinterpret_cast<const uint2*>(kc[x] + key * (D / 8) + 8 * z + 2 * kq);
-          g.k[x][y][z][0] = w.x;
-          g.k[x][y][z][1] = w.y;
-        }
+          f32x4 a = {};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int64_t k = min(t0 + 16 * y + 4 * kq + r, lim - 1);
+          for (int w = 0; w < 2; ++w) {
+            const bf16x8 c = codes(g.k[x][y][z][w]);
 #pragma unroll
-          for (int z = 0; z < GK; ++z) g.kp[x][y][r][z] = kpar[x][k * GK + z];
-        }
-      }
+            for (int p = NP - 1; p >= 0; --p) a = TrB::mma16(c, q[x][p][z][w], a);  // small parts first
+          }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = t0 + 16 * (j >> 2) + 4 * kq + (j & 3);
-      const int64_t k = min(key, lim - 1);
-      const uint32_t* w = vc + k * (DV / 8);
-#pragma unroll
-      for (int z = 0; z < WV; ++z) g.v[j][z] = DV == 64 ? w[n >> 1] : w[16 * z + n];
-#pragma unroll
-      for (int z = 0; z < GV; ++z) {
-        g.vp[j][z] = vpar[k * GV + z];
-        if (edge && key >= lim) g.vp[j][z] = 0;  // weight 0: nothing, whatever the row holds
-      }
-    }
-  }
-  __device__ __forceinline__ void scores(const Regs& g, int x, f32x4 (&s)[2]) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      s[y] = f32x4{};
-#pragma unroll
-      for (int z = 0; z < GK; ++z) {
-        f32x4 a = {};
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const bf16x8 c = codes(g.k[x][y][z][w]);
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p) a = TrB::mma16(c, q[x][p][z][w], a);  // small parts first
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float sc = bf16_hi(g.kp[x][y][r][z]), m = bf16_lo(g.kp[x][y][r][z]);
-          s[y][r] = __builtin_fmaf(sc, __builtin_fmaf(-kBias, qs[x][z], a[r]), __builtin_fmaf(m, qs[x][z], s[y][r]));
+          for (int r = 0; r < 4; ++r) {
+            const float sc = bf16_hi(g.kp[x][y][r][z]), m = bf16_lo(g.kp[x][y][r][z]);
+            s[x][y][r] = __builtin_fmaf(sc, __builtin_fmaf(-kBias, qs[x][z], a[r]), __builtin_fmaf(m, qs[x][z], s[x][y][r]));
+          }
         }
       }
-    }
   }
   __device__ __forceinline__ void rescale(int x, float f) {
 #pragma unroll
-    for (int y = 0; y < GV; ++y) corr[x][y] *= f;
+    for (int y = 0; y < GV; ++y) {
+      corr[x][y] *= f;
+      used[x][y] *= f;
+    }
   }
-  __device__ __forceinline__ void add(const Regs& g, int x, const f32x4 (&s)[2], f32x4 (&o)[DV / 16]) {
+  __device__ __forceinline__ void add(const Regs& g, const f32x4 (&s)[2][2], f32x4 (&o)[2][DV / 16]) {
+    u32x4 ones;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ones[i] = 0x3f803f80u;
 #pragma unroll
     for (int z = 0; z < GV; ++z) {
-      bf16x8 p[NP];
+      float step[8], mid[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float w = s[j >> 2][j & 3];
-        bf16 e[NP];
-        split(w * bf16_hi(g.vp[j][z]), e);
-        float used = 0.f;
+        step[j] = bf16_hi(g.vp[j][z]);
+        mid[j] = __builtin_fmaf(8.f, step[j], bf16_lo(g.vp[j][z]));
+      }
+      bf16x8 p[2][NP];
 #pragma unroll
-        for (int y = 0; y < NP; ++y) {
-          p[y][j] = e[y];
-          used += (float)e[y];
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = s[x][j >> 2][j & 3];
+          bf16 e[NP];
+          split(w * step[j], e);
+#pragma unroll
+          for (int y = 0; y < NP; ++y) p[x][y][j] = e[y];
+          corr[x][z] = __builtin_fmaf(w, mid[j], corr[x][z]);
         }
-        const float mid = __builtin_fmaf(8.f, bf16_hi(g.vp[j][z]), bf16_lo(g.vp[j][z]));
-        corr[x][z] = __builtin_fmaf(w, mid, __builtin_fmaf(-(kBias + 8.f), used, corr[x][z]));
+#pragma unroll
+        for (int y = NP - 1; y >= 0; --y) used[x][z] = TrB::mma16(__builtin_bit_cast(bf16x8, ones), p[x][y], used[x][z]);
       }
       uint32_t half[4];  // keys 2 i, 2 i + 1: the units of this group, side by side
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a = g.v[2 * i][z / 2], b = g.v[2 * i + 1][z / 2];
+        const uint32_t a = g.v[i / 2][z / 2][2 * i % 4], b = g.v[i / 2][z / 2][2 * i % 4 + 1];
         const bool up = DV == 64 ? lane_id() & 1 : z & 1;
         half[i] = up ? __builtin_amdgcn_perm(b, a, 0x07060302) : __builtin_amdgcn_perm(b, a, 0x05040100);
       }
@@ -344,7 +374,9 @@ struct Kv4Src {
         for (int i = 0; i < 4; ++i) w[i] = pair(half[i] >> (4 * c));
         const bf16x8 a = __builtin_bit_cast(bf16x8, w);
 #pragma unroll
-        for (int y = NP - 1; y >= 0; --y) o[4 * z + c] = TrB::mma16(a, p[y], o[4 * z + c]);
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = NP - 1; y >= 0; --y) o[x][4 * z + c] = TrB::mma16(a, p[x][y], o[x][4 * z + c]);
       }
     }
   }
@@ -356,6 +388,7 @@ struct Kv4Src {
         float a = corr[x][z];
         a += __shfl_xor(a, 16);
         a += __shfl_xor(a, 32);
+        a = __builtin_fmaf(-(kBias + 8.f), used[x][z][0], a);  // every value of the tile is the lane's query's sum
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[x][4 * z + c] += a;
       }
@@ -364,7 +397,7 @@ struct Kv4Src {
 };
 
 template <class T, int NP, int D, int DV>
-__global__ void __launch_bounds__(256) kv4_attend(DecParams P, Kv4Params C) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((DV <= 128 ? 2 : 1)))) kv4_attend(DecParams P, Kv4Params C) {
   extern __shared__ float lds[];
   Kv4Src<T, NP, D, DV> src;
   src.C = &C;

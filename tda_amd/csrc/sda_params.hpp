@@ -71,6 +71,7 @@ struct Kv4Params {
   uint32_t* pars[3];               // (m, s) bf16 pairs: s in the high half
   int32_t* lengths;
   int B, Hk, cap, D, DV;
+  int64_t cap4;                    // rows of a head: cap rounded up to four
   // append / read
   Rows x[3];
   int rows;

@@ -212,7 +212,7 @@ KINDS = {"append": _sda_abi.SdaKv4AppendArgs, "read": _sda_abi.SdaKv4ReadArgs, "
 @pytest.mark.parametrize("mutate, code", [
     (lambda a: setattr(a, "abi_version", 0), _abi.ERR_ABI), (lambda a: setattr(a, "dtype", 3), _abi.ERR_DTYPE),
     (lambda a: setattr(a.cache, "batch", 0), _abi.ERR_SHAPE), (lambda a: setattr(a.cache, "head_dim", 96), _abi.ERR_HEAD_DIM),
-    (lambda a: setattr(a.cache, "capacity", 1 << 30), _sda_abi.ERR_CACHE),
+    (lambda a: setattr(a.cache, "capacity", (1 << 24) + 1), _sda_abi.ERR_CACHE),
     (lambda a: setattr(a.cache, "k2", None), _abi.ERR_NULL_POINTER), (lambda a: setattr(a.cache, "lengths", None), _abi.ERR_NULL_POINTER),
     (lambda a: setattr(a.cache, "v", FAKE + 8), _abi.ERR_LAYOUT), (lambda a: setattr(a.cache, "lengths", FAKE + 2), _abi.ERR_LAYOUT)])
 def test_cache_refuses(kind, mutate, code):
@@ -242,7 +242,7 @@ def test_cache_refuses_its_own(kind, mutate, code):
 
 def test_cache_sizes_and_error_strings():
     so = lib()
-    assert so.sda_kv4_bytes(2, 3, 10, 128) == 2 * 3 * 10 * (64 + 8)
+    assert so.sda_kv4_bytes(2, 3, 10, 128) == 2 * 3 * 12 * (64 + 8)  # rows in fours
     assert so.sda_kv4_bytes(2, 3, 10, 96) == so.sda_kv4_bytes(0, 3, 10, 64) == 0
     texts = [so.sda_error_string(c).decode() for c in (*range(-13, 0), *range(-23, -19), -100)]
     assert all(texts) and len(set(texts[-5:])) == 5
