@@ -143,7 +143,7 @@ static int run(const FwdParams& f, hipStream_t st) {
   decode<Tr, D, DV><<<tda::grid_of<256>(items * f.nsplit), 256, LDS, st>>>(p, f);
   tda::launched(st, "sda_decode");
   if (f.nsplit > 1) {
-    decode_join<typename Tr::T><<<tda::grid_of<256>(items * (DV / 16)), 256, 0, st>>>(p);
+    decode_join<typename Tr::T><<<tda::grid_of<256>(((int64_t)f.B * f.H * f.Nq * DV + 255) / 256), 256, 0, st>>>(p);
     tda::launched(st, "sda_decode_join");
   }
   return (int)hipGetLastError();

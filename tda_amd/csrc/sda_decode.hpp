@@ -27,6 +27,8 @@ struct DecParams {
   int nsplit, chunk;
 };
 constexpr int kDecRows = 16;
+template <int DV>
+constexpr int kDecRow = DV + 4;  // LDS row stride of a wave's sums: rows start in different banks
 __host__ __device__ constexpr int64_t dec_part_floats(int dv) { return 64 + 2 * 16 * (int64_t)dv; }
 
 template <class Src>
@@ -110,8 +112,9 @@ __device__ __forceinline__ void decode_body(const DecParams& P, Src& src, float*
     sum[x] += __shfl_xor(sum[x], 16);
     sum[x] += __shfl_xor(sum[x], 32);
   }
-  // the waves' maxima and sums, then their outputs under the common maximum
-  float* ml = lds + 4 * 2 * DV * 16;  // [wave][branch][m, l][16]
+  // the waves' maxima and sums, then their outputs under the common maximum, a branch at a time
+  float* ml = lds + 4 * 16 * kDecRow<DV>;  // [wave][branch][m, l][16]
+  float* scale = ml + 256;                 // [branch][16]: 1 / l, times -lambda for branch 2
   if (kq == 0) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -119,86 +122,68 @@ __device__ __forceinline__ void decode_body(const DecParams& P, Src& src, float*
       ml[((wv * 2 + x) * 2 + 1) * 16 + n] = sum[x];
     }
   }
-  __syncthreads();
-  float all[2], tot[2];
+  const int tid = threadIdx.x, rows = min(kDecRows, R - rt * kDecRows);
+  float* part = P.nsplit > 1 ? P.part + ((int64_t)item * P.nsplit + split) * dec_part_floats(DV) : nullptr;
+  float fin[2][DV / 16];  // this thread's values: tid + 256 k, by row, then column
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    all[x] = kNoMax;
-    tot[x] = 0.f;
+    __syncthreads();
+    float all = kNoMax, tot = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) all[x] = fmaxf(all[x], ml[((w * 2 + x) * 2) * 16 + n]);
+    for (int w = 0; w < 4; ++w) all = fmaxf(all, ml[((w * 2 + x) * 2) * 16 + n]);
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      tot[x] = __builtin_fmaf(ml[((w * 2 + x) * 2 + 1) * 16 + n], exp2_(ml[((w * 2 + x) * 2) * 16 + n] - all[x]), tot[x]);
-    const float f = exp2_(m[x] - all[x]);
+      tot = __builtin_fmaf(ml[((w * 2 + x) * 2 + 1) * 16 + n], exp2_(ml[((w * 2 + x) * 2) * 16 + n] - all), tot);
+    const float f = exp2_(m[x] - all);
 #pragma unroll
     for (int y = 0; y < NO; ++y)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        lds[((wv * 2 + x) * DV + Src::column(y, 4 * kq + r)) * 16 + n] = o[x][y][r] * f;
-  }
-  __syncthreads();
-  // thread t: row t % 16, columns t / 16, + 16, ...
-  const int tid = threadIdx.x, c0 = tid >> 4;
-  if (P.nsplit > 1) {
-    float* to = P.part + ((int64_t)item * P.nsplit + split) * dec_part_floats(DV);
+      for (int r = 0; r < 4; ++r) lds[(wv * 16 + n) * kDecRow<DV> + Src::column(y, 4 * kq + r)] = o[x][y][r] * f;
     if (tid < 16) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        to[32 * x + n] = all[x];
-        to[32 * x + 16 + n] = tot[x];
+      const float inv = tot > 0.f || tot != tot ? 1.0f / tot : 0.f;
+      scale[16 * x + n] = x && live ? -lambda_of(P.lam, b, h, i) * inv : inv;
+      if (part) {
+        part[32 * x + n] = all;
+        part[32 * x + 16 + n] = tot;
       }
     }
-    if (k0 >= k1) return;  // no sums: the joining launch skips a part without weight
+    __syncthreads();
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      for (int y = c0; y < DV; y += 16) {
-        float a = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) a += lds[((w * 2 + x) * DV + y) * 16 + n];
-        to[64 + (x * DV + y) * 16 + n] = a;
+    for (int k = 0; k < DV / 16; ++k) {
+      const int e = tid + 256 * k, r = e / DV, c = e % DV;
+      if (r < rows) {
+        fin[x][k] = (lds[r * kDecRow<DV> + c] + lds[(16 + r) * kDecRow<DV> + c]) +
+                    (lds[(32 + r) * kDecRow<DV> + c] + lds[(48 + r) * kDecRow<DV> + c]);
+        if (part && k0 < k1) part[64 + (x * 16 + r) * DV + c] = fin[x][k];  // a part without keys: not read
       }
-    return;
+    }
   }
-  const float lam = live ? lambda_of(P.lam, b, h, i) : 0.f;
-  float inv[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) inv[x] = tot[x] > 0.f || tot[x] != tot[x] ? 1.0f / tot[x] : 0.f;
-  // the rows' outputs turned in LDS so that a thread stores along a row
-  float* turned = lds + 4 * 2 * DV * 16 + 256;  // [16][DV + 1]
-  for (int y = c0; y < DV; y += 16) {
-    float a[2] = {0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) a[x] += lds[((w * 2 + x) * DV + y) * 16 + n];
-    turned[n * (DV + 1) + y] = __builtin_fmaf(-lam * inv[1], a[1], a[0] * inv[0]);
-  }
-  __syncthreads();
+  if (part) return;
   using T = typename Src::Out;
-  for (int e = tid; e < 16 * DV; e += 256) {
-    const int r = rt * kDecRows + e / DV;
-    if (r >= R) break;
-    row_of<T>(P.out, b, hk * G + r / P.Nq, r % P.Nq)[e % DV] = (T)turned[(e / DV) * (DV + 1) + e % DV];
+#pragma unroll
+  for (int k = 0; k < DV / 16; ++k) {
+    const int e = tid + 256 * k, r = e / DV, c = e % DV;
+    if (r >= rows) break;
+    const int q = rt * kDecRows + r;
+    row_of<T>(P.out, b, hk * G + q / P.Nq, q % P.Nq)[c] = (T)__builtin_fmaf(scale[16 + r], fin[1][k], scale[r] * fin[0][k]);
   }
 }
 template <int DV>
-constexpr int kDecLds = (4 * 2 * DV * 16 + 256 + 16 * (DV + 1)) * 4;
+constexpr int kDecLds = (4 * 16 * kDecRow<DV> + 256 + 32) * 4;
 
-// Joins the parts of 16 rows: thread per (row, column of a group of 16), parts in order.
+// Joins the parts: a thread per value, the parts in order, eight at a time (their loads are on their way
+// together).
 template <class T>
 __global__ void __launch_bounds__(256) decode_join(DecParams P) {
   const int G = P.H / P.Hk, R = G * P.Nq, tiles = (R + kDecRows - 1) / kDecRows, DV = P.DV;
-  const int cols = DV / 16;
-  const uint32_t bid = tda::grid_bid<256>();
-  const int cb = (int)(bid % (uint32_t)cols), item = (int)(bid / (uint32_t)cols);
-  if (item >= P.B * P.Hk * tiles) return;
-  const int rt = item % tiles, bk = item / tiles, b = bk / P.Hk, hk = bk % P.Hk;
-  const int n = threadIdx.x & 15, y = 16 * cb + (threadIdx.x >> 4);
+  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
+  const int c = (int)(id % DV);
+  const int64_t at = id / DV;  // (b, hk, row)
+  if (at >= (int64_t)P.B * P.Hk * R) return;
+  const int row = (int)(at % R), bk = (int)(at / R), b = bk / P.Hk, hk = bk % P.Hk;
+  const int n = row % kDecRows;
   const int64_t step = dec_part_floats(DV);
-  const float* base = P.part + (int64_t)item * P.nsplit * step;
-  // eight parts at a time: their loads are on their way together
-  float res[2];
+  const float* base = P.part + ((int64_t)bk * tiles + row / kDecRows) * P.nsplit * step;
   float all[2] = {kNoMax, kNoMax}, l[2] = {}, a[2] = {};
   for (int s0 = 0; s0 < P.nsplit; s0 += 8) {
     float mm[2][8], ll[2][8], aa[2][8];
@@ -209,7 +194,7 @@ __global__ void __launch_bounds__(256) decode_join(DecParams P) {
       for (int x = 0; x < 2; ++x) {
         mm[x][u] = part[32 * x + n];
         ll[x][u] = s0 + u < P.nsplit ? part[32 * x + 16 + n] : 0.f;
-        aa[x][u] = part[64 + (x * DV + y) * 16 + n];
+        aa[x][u] = part[64 + (x * 16 + n) * DV + c];
       }
     }
 #pragma unroll
@@ -231,16 +216,11 @@ __global__ void __launch_bounds__(256) decode_join(DecParams P) {
       }
     }
   }
+  float res[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) res[x] = l[x] > 0.f || l[x] != l[x] ? a[x] / l[x] : 0.f;
-  __shared__ float turned[16][17];
-  const int row = rt * kDecRows + n;
-  const bool live = row < R;
-  const float lam = live ? lambda_of(P.lam, b, hk * G + row / P.Nq, row % P.Nq) : 0.f;
-  turned[n][threadIdx.x >> 4] = __builtin_fmaf(-lam, res[1], res[0]);
-  __syncthreads();
-  const int r = rt * kDecRows + (threadIdx.x >> 4);
-  if (r < R) row_of<T>(P.out, b, hk * G + r / P.Nq, r % P.Nq)[16 * cb + n] = (T)turned[threadIdx.x >> 4][n];
+  const int h = hk * G + row / P.Nq, i = row % P.Nq;
+  row_of<T>(P.out, b, h, i)[c] = (T)__builtin_fmaf(-lambda_of(P.lam, b, h, i), res[1], res[0]);
 }
 
 }  // namespace sda

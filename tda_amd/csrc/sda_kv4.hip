@@ -445,7 +445,7 @@ static int run(const DecParams& p, const Kv4Params& c, hipStream_t st) {
   kv4_attend<T, NP, D, DV><<<tda::grid_of<256>(items * p.nsplit), 256, LDS, st>>>(p, c);
   tda::launched(st, "sda_kv4_attend");
   if (p.nsplit > 1) {
-    decode_join<T><<<tda::grid_of<256>(items * (DV / 16)), 256, 0, st>>>(p);
+    decode_join<T><<<tda::grid_of<256>(((int64_t)p.B * p.H * p.Nq * DV + 255) / 256), 256, 0, st>>>(p);
     tda::launched(st, "sda_decode_join");
   }
   return (int)hipGetLastError();
