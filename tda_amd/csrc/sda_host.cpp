@@ -87,15 +87,19 @@ bool few_rows(int64_t heads, int64_t kv_heads, int64_t seq_len) { return heads /
 int64_t dec_items(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len) {
   return batch * kv_heads * ceil_div(heads / kv_heads * seq_len, 16);
 }
-// Parts of the key axis: whole tiles of the four waves (128 keys) each; about 1024 workgroups in all
-// (four a CU: enough loads in flight), no part shorter than 128 keys.
-void dec_split(int64_t items, int64_t nk, int* nsplit, int* chunk) {
-  int64_t want = ceil_div(1024, items);
+// Parts of the key axis: whole tiles of the four waves (128 keys) each, about `target` workgroups in all,
+// no part shorter than 128 keys.
+void dec_split(int64_t items, int64_t nk, int64_t target, int* nsplit, int* chunk) {
+  int64_t want = ceil_div(target, items);
   const int64_t most = ceil_div(nk, 128);
   if (want > most) want = most;
   *chunk = (int)(ceil_div(ceil_div(nk, want), 128) * 128);
   *nsplit = (int)ceil_div(nk, *chunk);
 }
+// 1024 workgroups over a bf16 or f32 cache, 512 over the 4-bit one, whose kernel holds two to a CU: one
+// token over (32, 32 over 8, 8192, 128) of unequal lengths takes 256 us (2048: 274, 4096: 275) and 103 us
+// (768: 118, 1024: 112, 2048: 124).
+constexpr int64_t kDecTarget = 1024, kKv4Target = 512;
 int64_t dec_bytes(int64_t items, int nsplit, int64_t dv) {
   return nsplit > 1 ? items * nsplit * (64 + 32 * dv) * 4 : 0;
 }
@@ -200,7 +204,7 @@ size_t sda_fwd_workspace_bytes(const sda_fwd_args* a) {
     return 0;
   int nsplit, chunk;
   const int64_t items = dec_items(a->batch, a->heads, a->kv_heads, a->seq_len);
-  dec_split(items, a->seq_len_kv, &nsplit, &chunk);
+  dec_split(items, a->seq_len_kv, kDecTarget, &nsplit, &chunk);
   return (size_t)dec_bytes(items, nsplit, a->v_head_dim);
 }
 
@@ -224,7 +228,7 @@ int32_t sda_fwd(const sda_fwd_args* a, void* stream) {
   p.lse = a->lse;
   tda::timing_begin(stream);
   if (decodes(*a)) {
-    dec_split(dec_items(a->batch, a->heads, a->kv_heads, a->seq_len), a->seq_len_kv, &p.nsplit, &p.chunk);
+    dec_split(dec_items(a->batch, a->heads, a->kv_heads, a->seq_len), a->seq_len_kv, kDecTarget, &p.nsplit, &p.chunk);
     p.part = static_cast<float*>(a->workspace);
     return done(sda::launch_decode(p, a->dtype, (int)a->head_dim, (int)a->v_head_dim, stream));
   }
@@ -388,7 +392,7 @@ size_t sda_kv4_attend_workspace_bytes(const sda_kv4_attend_args* a) {
     return 0;
   int nsplit, chunk;
   const int64_t items = dec_items(a->cache.batch, a->heads, a->cache.kv_heads, a->seq_len);
-  dec_split(items, a->cache.capacity, &nsplit, &chunk);
+  dec_split(items, a->cache.capacity, kKv4Target, &nsplit, &chunk);
   return (size_t)dec_bytes(items, nsplit, a->cache.v_head_dim);
 }
 int32_t sda_validate_kv4_attend(const sda_kv4_attend_args* a) {
@@ -420,7 +424,7 @@ int32_t sda_kv4_attend(const sda_kv4_attend_args* a, void* stream) {
   p.Nq = (int)a->seq_len;
   p.c = (float)(a->scale * kLog2e);
   p.part = static_cast<float*>(a->workspace);
-  dec_split(dec_items(a->cache.batch, a->heads, a->cache.kv_heads, a->seq_len), a->cache.capacity, &p.nsplit, &p.chunk);
+  dec_split(dec_items(a->cache.batch, a->heads, a->cache.kv_heads, a->seq_len), a->cache.capacity, kKv4Target, &p.nsplit, &p.chunk);
   tda::timing_begin(stream);
   return done(sda::launch_kv4_attend(p, a->dtype, stream));
 }

@@ -209,15 +209,17 @@ struct Kv4Src {
   static constexpr int NBUF = 1;
   const uint32_t *kc[2], *kpar[2], *vc, *vpar;  // the head's rows: within them offsets are 32-bit
 
-  __device__ __forceinline__ static bf16x8 codes(uint32_t w) {  // 8 codes of a key word, in value order
+  uint32_t high;  // 0x43004300 in a vector register: and + or are then one instruction
+
+  __device__ __forceinline__ bf16x8 codes(uint32_t w) const {  // 8 codes of a key word, in value order
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = pair(w >> (4 * i));
     return __builtin_bit_cast(bf16x8, x);
   }
-  __device__ __forceinline__ static uint32_t pair(uint32_t w) {
+  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
     if constexpr (NP == 1) {
-      return (w & 0x000f000fu) | 0x43004300u;
+      return (w & 0x000f000fu) | high;
     } else {
       const float a = (float)(w & 15u), b = (float)(w >> 16 & 15u);  // exact: their low halves are zero
       return __builtin_bit_cast(uint32_t, a) >> 16 | __builtin_bit_cast(uint32_t, b);
@@ -263,6 +265,8 @@ struct Kv4Src {
 #pragma unroll
       for (int y = 0; y < GV; ++y) corr[x][y] = 0.f, used[x][y] = f32x4{};
     }
+    high = 0x43004300u;
+    asm volatile("" : "+v"(high));
     vc = reinterpret_cast<const uint32_t*>(C->codes[2]) + row0 * (DV / 8);
     vpar = C->pars[2] + row0 * GV;
   }
@@ -311,7 +315,8 @@ struct Kv4Src {
         s[x][y] = f32x4{};
 #pragma unroll
         for (int z = 0; z < GK; ++z) {
-          f32x4 a = {};
+          const float start = -kBias * qs[x][z];
+          f32x4 a = {start, start, start, start};
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const bf16x8 c = codes(g.k[x][y][z][w]);
@@ -321,7 +326,7 @@ struct Kv4Src {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float sc = bf16_hi(g.kp[x][y][r][z]), m = bf16_lo(g.kp[x][y][r][z]);
-            s[x][y][r] = __builtin_fmaf(sc, __builtin_fmaf(-kBias, qs[x][z], a[r]), __builtin_fmaf(m, qs[x][z], s[x][y][r]));
+            s[x][y][r] = __builtin_fmaf(sc, a[r], __builtin_fmaf(m, qs[x][z], s[x][y][r]));
           }
         }
       }
