@@ -9,9 +9,17 @@
 // weights feed the second product (O^T = V^T P^T) from the registers that hold them, and rescaling is
 // one factor per lane.  Keys arrive by direct loads to LDS, one stage (64 keys bf16, 32 fp32) ahead.
 // Branch 2's normalised result meets branch 1's through LDS at the end.
+//
+// Grids that would leave CUs idle take 64 query rows a workgroup (RG = 2 row groups): the other four waves
+// take the second half of each stage's keys, and the halves' maxima, sums and outputs meet in LDS first.
 #include "sda_common.hpp"
 
 namespace sda {
+
+// Up to this many workgroups of 128 rows, half of the 256 CUs, the launch takes 64 rows a workgroup: bf16
+// (2, 16 over 4 heads, 500 rows of 4355 keys, 128) 127 -> 103 us, (1, 16, 500 of 4355, 128) 114 -> 87 us,
+// (1, 16, 1024, 64/128) 31 -> 26 us; with 240 (1, 24, 1280 of 4096, 128) it would be 128 -> 151 us.
+constexpr int64_t kFewTiles = 128;
 
 template <class Tr, int D, int DV>
 struct FwdShape {
@@ -21,32 +29,33 @@ struct FwdShape {
   using VT = Tile<Tr, BN, DV>;
   static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
   static constexpr int XCH = 4 * 32 * DV * 4;          // branch 2's result, f32
-  static constexpr int LDS = 2 * STAGE > XCH ? 2 * STAGE : XCH;
+  static constexpr int LDS = 2 * STAGE > XCH + 2048 ? 2 * STAGE : XCH + 2048;
   static_assert(KT::LOADS % 8 == 0 && VT::LOADS % 8 == 0, "loads spread evenly over the waves");
 };
 
-template <class Tr, int D, int DV>
+template <class Tr, int D, int DV, int RG>
 __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
   using S = FwdShape<Tr, D, DV>;
   using KT = typename S::KT;
   using VT = typename S::VT;
-  constexpr int BN = S::BN, NS = BN / 32, NT = D / 16, NO = DV / 32;
-  constexpr int KL = KT::LOADS / 8, VL = VT::LOADS / 8;
+  constexpr int BN = S::BN, NS = BN / 32 * RG / 4, NT = D / 16, NO = DV / 32;
+  static_assert(NS >= 1, "a wave has whole key tiles");
+  constexpr int KL = KT::LOADS / 8, VL = VT::LOADS / 8, ROWS = 32 * RG;
   constexpr int G = sizeof(T) == 2 ? 4 : 1;  // an fp32 fragment is eight products itself
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv & 3, br = wv >> 2;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv % RG, br = wv / RG & 1, kh = wv / (2 * RG);  // kh: which half of a stage's keys
   const uint32_t bid = tda::grid_bid<512>();
   if (bid >= (uint32_t)(P.B * P.H) * (uint32_t)P.nqt) return;
   const Item it = item_of(bid, P.B * P.H, P.nqt, true);
   const int b = it.head / P.H, h = it.head % P.H, hk = h / (P.H / P.Hk);
-  const int q0 = it.tile * kBlockRows, q0w = q0 + 32 * rg;
+  const int q0 = it.tile * ROWS, q0w = q0 + 32 * rg;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   // keys the workgroup / the wave sees at most
-  const int qlast = min(q0 + kBlockRows, P.Nq) - 1;
+  const int qlast = min(q0 + ROWS, P.Nq) - 1;
   const int lim = P.see.causal ? min(len, max(off + qlast + 1, 0)) : len;
   const int limw = P.see.causal ? min(len, max(off + min(q0w + 31, P.Nq - 1) + 1, 0)) : len;
   const int clear = P.see.causal ? min(len, max(off + q0w + 1, 0)) : len;  // every row of the wave sees these
@@ -89,14 +98,16 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 
   RowReader<Tr, D> kr;
   ColReader<Tr, DV> vr;
-  kr.init(lds + br * KT::BYTES);
-  vr.init(lds + 2 * KT::BYTES);
+  const char* kbuf = lds + br * KT::BYTES + 32 * kh * D * KT::ES;
+  const char* vbuf = lds + 2 * KT::BYTES + 32 * kh * DV * VT::ES;
+  kr.init(kbuf);
+  vr.init(vbuf);
   auto step = [&](int j, auto half) {  // stage j, in the half of the buffers that its parity names
     constexpr int AT = half * S::STAGE;
     wait_vm<0>();
     tda::lds_barrier();  // stage j is in place, and every wave is done with stage j - 1
     if (j + 1 < nst) issue(j + 1);
-    const int k0 = j * BN;
+    const int k0 = j * BN + 32 * kh;
     if (k0 >= limw) return;
     // The stage's products take their LDS operands as one sequence, NS NT key fragments then 2 NS NO value
     // fragments, read a group of G ahead of their use: the first value group is on its way before the softmax.
@@ -105,8 +116,8 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 #pragma unroll
       for (int u = 0; u < G; ++u) {
         const int e = i * G + u, w = e - NS * NT;
-        if (e < NS * NT) f[i & 1][u] = kr.read(lds + br * KT::BYTES, AT + 32 * D * KT::ES * (e % NS), e / NS);
-        else f[i & 1][u] = vr.read(lds + 2 * KT::BYTES, AT + 32 * DV * VT::ES * (w / (2 * NO)), w / NO % 2, w % NO);
+        if (e < NS * NT) f[i & 1][u] = kr.read(kbuf, AT + 32 * D * KT::ES * (e % NS), e / NS);
+        else f[i & 1][u] = vr.read(vbuf, AT + 32 * DV * VT::ES * (w / (2 * NO)), w / NO % 2, w % NO);
       }
     };
     f32x16 s[NS] = {};
@@ -120,7 +131,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
         s[e % NS] = Tr::mma32(f[i & 1][u], qf[e / NS], s[e % NS]);
       }
     }
-    if (k0 + BN > clear) {
+    if (k0 + 32 * NS > clear) {
       asm volatile("");  // a branch: few tiles need this
 #pragma unroll
       for (int x = 0; x < NS; ++x)
@@ -174,13 +185,40 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 
   float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   sum += __shfl_xor(sum, 32);
+  if constexpr (RG == 2) {  // the second half's sums join the first's
+    __syncthreads();
+    float* stat = reinterpret_cast<float*>(lds + 4 * 32 * DV * 4);  // behind the outputs: m, sum by pair and lane
+    f32x4* half = reinterpret_cast<f32x4*>(lds) + (wv & 3) * (NO * 4 * 64) + l;
+    if (kh) {
+      stat[128 * (wv & 3) + l] = m;
+      stat[128 * (wv & 3) + 64 + l] = sum;
+#pragma unroll
+      for (int y = 0; y < NO; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) half[(4 * y + r) * 64] = f32x4{o[y][4 * r], o[y][4 * r + 1], o[y][4 * r + 2], o[y][4 * r + 3]};
+    }
+    __syncthreads();
+    if (!kh) {
+      const float m2 = stat[128 * wv + l], all = fmaxf(m, m2), f1 = exp2_(m - all), f2 = exp2_(m2 - all);
+      sum = __builtin_fmaf(stat[128 * wv + 64 + l], f2, sum * f1);
+      m = all;
+#pragma unroll
+      for (int y = 0; y < NO; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 w = half[(4 * y + r) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[y][4 * r + e] = __builtin_fmaf(w[e], f2, o[y][4 * r + e] * f1);
+        }
+    }
+  }
   const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;  // no visible key: zeros
   const bool row = qi < P.Nq;
-  if (P.lse && row && g == 0)  // a row without keys: +inf, which weighs everything 0
+  if (P.lse && row && g == 0 && !kh)  // a row without keys: +inf, which weighs everything 0
     P.lse[((int64_t)br * P.B * P.H + it.head) * P.Nq + qi] = sum > 0.f || sum != sum ? m + __builtin_amdgcn_logf(sum) : __builtin_inff();
   __syncthreads();  // the stages are read: their place carries branch 2's result
   f32x4* xch = reinterpret_cast<f32x4*>(lds) + rg * (NO * 4 * 64) + l;
-  if (br) {
+  if (br && !kh) {
     float* to = P.out2.p && row ? row_of<float>(P.out2, b, h, qi) : nullptr;
 #pragma unroll
     for (int y = 0; y < NO; ++y)
@@ -192,7 +230,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
       }
   }
   __syncthreads();
-  if (!br && row) {
+  if (!br && !kh && row) {
     const float lam = lambda_of(P.lam, b, h, qi);
     T* to = row_of<T>(P.out, b, h, qi);
     T* low = P.out2.p ? row_of<T>(P.low, b, h, qi) : nullptr;  // what rounding leaves out, for the backward's row sums
@@ -217,18 +255,26 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   }
 }
 
-template <class Tr, int D, int DV>
-static int run(const FwdParams& p, hipStream_t st) {
+template <class Tr, int D, int DV, int RG>
+static int launch(FwdParams p, hipStream_t st) {
   using S = FwdShape<Tr, D, DV>;
-  const void* fn = reinterpret_cast<const void*>(&fwd_tiles<Tr, D, DV>);
+  const void* fn = reinterpret_cast<const void*>(&fwd_tiles<Tr, D, DV, RG>);
   if (S::LDS > 65536) {
     const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
     if (e != hipSuccess) return (int)e;
   }
-  fwd_tiles<Tr, D, DV><<<tda::grid_of<512>((int64_t)p.nqt * p.B * p.H), 512, S::LDS, st>>>(p);
+  p.nqt = (p.Nq + 32 * RG - 1) / (32 * RG);
+  fwd_tiles<Tr, D, DV, RG><<<tda::grid_of<512>((int64_t)p.nqt * p.B * p.H), 512, S::LDS, st>>>(p);
   const hipError_t e = hipGetLastError();
   tda::launched(st, "sda_fwd_tiles");
   return (int)e;
+}
+template <class Tr, int D, int DV>
+static int run(const FwdParams& p, hipStream_t st) {
+  if constexpr (FwdShape<Tr, D, DV>::BN == 64) {
+    if ((int64_t)((p.Nq + 127) / 128) * p.B * p.H <= kFewTiles) return launch<Tr, D, DV, 2>(p, st);
+  }
+  return launch<Tr, D, DV, 4>(p, st);
 }
 template <class Tr>
 static int pick(const FwdParams& p, int d, int dv, hipStream_t st) {

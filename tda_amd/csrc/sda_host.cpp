@@ -224,7 +224,6 @@ int32_t sda_fwd(const sda_fwd_args* a, void* stream) {
   sda::FwdParams p;
   std::memset(&p, 0, sizeof(p));
   fill(p, *a);
-  p.nqt = (int)ceil_div(a->seq_len, sda::kBlockRows);
   p.lse = a->lse;
   tda::timing_begin(stream);
   if (decodes(*a)) {

@@ -29,7 +29,7 @@ struct FwdParams {
   Rows q[2], k[2], v, out, out2, low;  // out2.p (f32) may be null; low: bf16 alone
   Lambda lam;
   Sight see;
-  int B, H, Hk, Nq, Nk, nqt;      // nqt: query tiles of kBlockRows
+  int B, H, Hk, Nq, Nk, nqt;      // nqt: query tiles (set by launch_fwd)
   float c;                        // scale * log2(e)
   float* lse;                     // may be null
   // decode kernels: the keys cut into nsplit parts of `chunk` keys; per (row, part) the partial sums
@@ -50,8 +50,6 @@ struct BwdParams {
   void* dlam;        // may be null
   int64_t dlam_n[3]; // extents of the distinct elements (1 along a broadcast axis)
 };
-
-constexpr int kBlockRows = 128;  // query rows of a forward workgroup
 
 struct RotaryParams {
   Rows x[4], y[4];
