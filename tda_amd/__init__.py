@@ -9,7 +9,7 @@ from .api import (  # noqa: F401
     threshold_rela_triton,
 )
 from .kv_cache import Int4KVCache  # noqa: F401
-from .layer import ThresholdDifferentialAttention  # noqa: F401
+from .layer import DifferentialAttention, ThresholdDifferentialAttention  # noqa: F401
 from .ops import grad_prealloc, grad_prealloc_enabled, set_grad_prealloc  # noqa: F401
 from .rotary import rotary_axes  # noqa: F401
 from .softmax import differential_attention  # noqa: F401
@@ -17,4 +17,4 @@ from .stats import TileStats, tile_sparsity  # noqa: F401
 
 __all__ = ["threshold_rela_triton", "differential_threshold_rela_triton", "ThresholdRelaFunction",
            "ThresholdDifferentialAttention", "tile_sparsity", "TileStats", "set_grad_prealloc",
-           "grad_prealloc", "grad_prealloc_enabled", "differential_attention", "rotary_axes", "Int4KVCache"]
+           "grad_prealloc", "grad_prealloc_enabled", "differential_attention", "rotary_axes", "Int4KVCache", "DifferentialAttention"]

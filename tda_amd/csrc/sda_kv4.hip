@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P) {
   const int64_t bk = r / P.rows;
   const bool in = bk < (int64_t)P.B * P.Hk;
   const int b = in ? (int)(bk / P.Hk) : 0, hk = in ? (int)(bk % P.Hk) : 0;
-  const int start = P.start ? P.start[b] : P.lengths[b];
+  const int start = P.start ? P.start[b] : max(P.lengths[b], 0);
   const int count = P.counts ? min(max(P.counts[b], 0), P.rows) : P.rows;
   const int64_t at = (int64_t)start + i;
   const bool put = in && i < count && at >= 0 && at < P.cap;

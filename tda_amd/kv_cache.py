@@ -12,6 +12,7 @@ from .softmax import (_CODE, _check_heads, _check_rows, _ints, _lambda, _lambda_
 
 _PUT = struct.Struct("<Q").pack_into
 _DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
+_LENGTHS = _sda_abi.SdaKv4AttendArgs.cache.offset + _sda_abi.SdaKv4.lengths.offset  # the same in all three calls
 _ATTEND_OFF = {n: getattr(_sda_abi.SdaKv4AttendArgs, n).offset for n in ("q1", "q2", "out", "lambda_param", "workspace")}
 _APPEND_OFF = {n: getattr(_sda_abi.SdaKv4AppendArgs, n).offset for n in ("k1", "k2", "v", "start", "counts")}
 _READ_OFF = {n: getattr(_sda_abi.SdaKv4ReadArgs, n).offset for n in ("k1", "k2", "v")}
@@ -48,7 +49,6 @@ class Int4KVCache:
         self._held = [torch.empty(lib.sda_kv4_bytes(batch, kv_heads, capacity, w), dtype=torch.uint8, device=device)
                       for w in (head_dim, head_dim, v_head_dim)]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
-        self._lengths_at = None
         self._templates: dict = {}
 
     # -------------------------------------------------------------- calls
@@ -57,23 +57,24 @@ class Int4KVCache:
         c.batch, c.kv_heads, c.capacity = self.batch, self.kv_heads, self.capacity
         c.head_dim, c.v_head_dim = self.head_dim, self.v_head_dim
         c.k1, c.k2, c.v = (t.data_ptr() for t in self._held)
-        c.lengths = self.lengths.data_ptr()
         return c
 
     def _template(self, key, build):
-        """The argument block of a call, cached by its configuration (this cache's own buffers are part
-        of it)."""
+        """The argument block of a call but for the call's own pointers, cached by its configuration (this
+        cache's buffers are part of it)."""
         n = self.lengths
         if not isinstance(n, torch.Tensor) or n.shape != (self.batch,) or n.dtype != torch.int32 or n.device != self.device \
                 or not n.is_contiguous():
             raise ValueError(f"lengths must be a contiguous int32 tensor of shape ({self.batch},) on {self.device}")
-        if n.data_ptr() != self._lengths_at or len(self._templates) > 64:
-            self._templates.clear()
-            self._lengths_at = n.data_ptr()
         got = self._templates.get(key)
         if got is None:
-            got = self._templates[key] = build()
-        return got
+            if len(self._templates) > 64:
+                self._templates.clear()
+            block = build()
+            got = self._templates[key] = bytes(block), getattr(block, "workspace_bytes", 0)
+        buf = bytearray(got[0])
+        _PUT(buf, _LENGTHS, n.data_ptr())
+        return buf, got[1]
 
     def _check(self, tensors, names, shapes):
         _check_rows(tensors, names)
@@ -112,9 +113,9 @@ class Int4KVCache:
             a.abi_version, a.dtype, a.cache, a.rows = _sda_abi.ABI_VERSION, _CODE[rows[0].dtype], self._cache(), n
             for name, t in zip(("k1", "k2", "v"), rows):
                 getattr(a, name).stride[:] = t.stride()
-            return bytes(a)
+            return a
 
-        buf = bytearray(self._template(("append", n, rows[0].dtype, tuple(t.stride() for t in rows)), build))
+        buf, _ = self._template(("append", n, rows[0].dtype, tuple(t.stride() for t in rows)), build)
         for name, t in zip(("k1", "k2", "v", "start", "counts"), (*rows, start, counts)):
             if t is not None:
                 _PUT(buf, _APPEND_OFF[name], t.data_ptr())
@@ -136,9 +137,9 @@ class Int4KVCache:
             a.abi_version, a.dtype, a.cache, a.rows = _sda_abi.ABI_VERSION, _CODE[dtype], self._cache(), n
             for name, t in zip(("k1", "k2", "v"), res):
                 getattr(a, name).stride[:] = t.stride()
-            return bytes(a)
+            return a
 
-        buf = bytearray(self._template(("read", n, dtype), build))
+        buf, _ = self._template(("read", n, dtype), build)
         for name, t in zip(("k1", "k2", "v"), res):
             _PUT(buf, _READ_OFF[name], t.data_ptr())
         _launch(_sda_abi.load().sda_kv4_read, _sda_abi.SdaKv4ReadArgs, buf, self.device, "sda_kv4_read")
@@ -148,6 +149,8 @@ class Int4KVCache:
         """Softmax differential attention of q1, q2 (batch, heads, n, head_dim), the last n positions of each
         sequence, over the cache: row i of sequence b sees the keys up to lengths[b] - n + i (a row before
         the sequence's first position is zero).  Returns (batch, heads, n, v_head_dim); no gradient.
+        (A group of values that is not finite reaches the rows that see it, and may reach other rows of
+        the same call that stand before it.)
 
         Few rows (n heads / kv_heads <= 32, as in decoding) are computed from the codes; more, as a
         prompt's chunk, from the rows that read() gives in q1's dtype."""
@@ -164,8 +167,9 @@ class Int4KVCache:
             return torch.zeros((b, h, 0, self.v_head_dim), dtype=q1.dtype, device=self.device)
         if h // hk * n > _FEW:
             with torch.no_grad():
-                return differential_attention(q1, q2, *self.read(dtype=q1.dtype), lam, s, q_offset=self.lengths - n,
-                                              kv_lens=self.lengths)
+                rows = self.read(dtype=q1.dtype)  # checks lengths
+                lens = self.lengths.clamp(0, self.capacity)
+                return differential_attention(q1, q2, *rows, lam, s, q_offset=lens - n, kv_lens=lens)
         q1, q2 = _usable(q1.detach()), _usable(q2.detach())
         out = _new_rows(q1, self.v_head_dim)
         ls = _lambda_strides(lam)
@@ -179,11 +183,10 @@ class Int4KVCache:
             a.lambda_stride[:] = ls
             a.lambda_dtype = _CODE[lam.dtype]
             a.workspace_bytes = _sda_abi.load().sda_kv4_attend_workspace_bytes(ctypes.byref(a))
-            return bytes(a), a.workspace_bytes
+            return a
 
         key = ("attend", h, n, s, q1.dtype, lam.dtype, ls, q1.stride(), q2.stride())
-        tpl, size = self._template(key, build)
-        buf = bytearray(tpl)
+        buf, size = self._template(key, build)
         ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         for name, t in zip(("q1", "q2", "out", "lambda_param", "workspace"), (q1, q2, out, lam, ws)):
             if t is not None:

@@ -293,8 +293,8 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
         off = _offset(q_offset, n, nk)
     lens = None if kv_lens is None else _ints(kv_lens, b, dev, "kv_lens")
     if any(t.numel() == 0 for t in tensors):  # no rows or no keys: zeros, connected to the inputs
-        zero = sum(t.sum() for t in tensors) * 0.0 + lam.sum().to(q1.dtype) * 0.0
-        return torch.zeros((b, h, n, dv), dtype=q1.dtype, device=dev) + zero
+        none = sum(t[:0].sum() for t in tensors) + lam.reshape(-1)[:0].sum().to(q1.dtype)
+        return torch.zeros((b, h, n, dv), dtype=q1.dtype, device=dev) + none
     rows = [t if t.dtype == cdt else t.to(cdt) for t in tensors]
     rows = [_pad(t, kd) for t in rows[:4]] + [_pad(rows[4], kv)]
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*rows, lam)):

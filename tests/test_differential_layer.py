@@ -1,0 +1,222 @@
+"""The softmax attention, the rotary positions and the 4-bit cache run together, as the layer
+tda_amd.DifferentialAttention runs them: a training step with every gradient, and a prompt with decoding
+steps, against the same layer in float64 on the CPU."""
+import math
+
+import pytest
+import torch
+
+import tda_amd
+from oracle import softmax as oracle
+
+gpu = pytest.mark.gpu
+F32, BF = torch.float32, torch.bfloat16
+U = 2.0 ** -24
+
+
+def layer(device="cuda", **kw):
+    torch.manual_seed(3)
+    return tda_amd.DifferentialAttention(**{"embed_dim": 96, "num_heads": 4, "kv_heads": 2, "head_dim": 64, "device": device, **kw})
+
+
+class Plain:
+    """The layer's formula in float64, differentiable, on copies of its weights."""
+
+    def __init__(self, m):
+        self.m = m
+        self.w = {n: p.detach().double().cpu().requires_grad_() for n, p in m.named_parameters()}
+
+    def project(self, x):
+        m = self.m
+        y = x @ self.w["in_proj.weight"].T + self.w.get("in_proj.bias", 0.0)
+        heads = (m.num_heads,) * 2 + (m.kv_heads,) * 3
+        dims = (m.head_dim,) * 4 + (m.v_head_dim,)
+        parts = y.split([h * w for h, w in zip(heads, dims)], -1)
+        return [p.unflatten(-1, (h, w)).transpose(1, 2) for p, h, w in zip(parts, heads, dims)]
+
+    def turn(self, x, positions):
+        m = self.m
+        pairs = sum(m.rotary_sections)
+        freq = m._inv_freq.float().double().cpu()
+        axis = [a for a, k in enumerate(m.rotary_sections) for _ in range(k)]
+        ang = positions.double()[axis].permute(1, 2, 0)[:, None] * freq
+        a, b, rest = x[..., :pairs], x[..., pairs:2 * pairs], x[..., 2 * pairs:]
+        return torch.cat((a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin(), rest), -1)
+
+    def attend(self, q1, q2, k1, k2, v, **kw):
+        g = self.m.num_heads // self.m.kv_heads
+        hide = oracle.hidden(q1.shape[0], q1.shape[2], v.shape[2], **kw)
+        w = [oracle.weights(q, k.repeat_interleave(g, 1), 1 / math.sqrt(self.m.head_dim), hide) for q, k in ((q1, k1), (q2, k2))]
+        return (w[0] - self.w["lambda_param"][:, None, None] * w[1]) @ v.repeat_interleave(g, 1)
+
+    def out(self, o):
+        return o.transpose(1, 2).flatten(2) @ self.w["out_proj.weight"].T + self.w.get("out_proj.bias", 0.0)
+
+    def __call__(self, x, positions, **kw):
+        q1, q2, k1, k2, v = self.project(x)
+        q1, q2, k1, k2 = (self.turn(t, positions) for t in (q1, q2, k1, k2))
+        return self.out(self.attend(q1, q2, k1, k2, v, **kw))
+
+
+def off(got, want):
+    return ((got.double().cpu() - want).norm() / want.norm()).item()
+
+
+def test_parameters():
+    m = layer("cpu", v_head_dim=128, bias=True)
+    shapes = {n: tuple(p.shape) for n, p in m.named_parameters()}
+    width = 2 * 4 * 64 + 2 * 2 * 64 + 2 * 128
+    assert shapes == {"lambda_param": (4,), "in_proj.weight": (width, 96), "in_proj.bias": (width,),
+                      "out_proj.weight": (96, 4 * 128), "out_proj.bias": (96,)}
+    assert m.rotary_sections == (32,) and m.lambda_param.tolist() == [0.5] * 4
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="head_dim"):
+        layer("cpu", head_dim=32)
+    with pytest.raises(ValueError, match="multiple"):
+        layer("cpu", kv_heads=3)
+    for sections in ((), (33,), (-1, 3), (1, 1, 1, 1, 1), (0, 0)):
+        with pytest.raises(ValueError, match="rotary_sections"):
+            layer("cpu", rotary_sections=sections)
+    m = layer("cpu")
+    with pytest.raises(ValueError, match="shape"):
+        m(torch.zeros(1, 3, 95))
+    with pytest.raises(ValueError, match="GPU"):
+        m(torch.zeros(1, 3, 96))
+
+
+@gpu
+@pytest.mark.parametrize("kw, n", [({}, 70), ({"v_head_dim": 128, "bias": True, "rotary_sections": (8, 12, 12)}, 133),
+                                   ({"kv_heads": 4, "rotary_sections": (20,)}, 1)])
+@pytest.mark.parametrize("padded", [False, True])
+def test_training_step(kw, n, padded):
+    """fp32.  The longest chain has the sums of two projections (96 and 4 dv terms), a score (64), a
+    softmax and a row of weights (n each), and the gradient passes each of them twice more: a relative
+    norm error of 3 (96 + 4 dv + 64 + 2 n) 2^-24 times 1 + the largest score, by which the softmax
+    enlarges a score's error, and 4 for the signs in the difference of the branches."""
+    m = layer(**kw)
+    axes = len(m.rotary_sections)
+    x = torch.randn(2, n, 96, generator=torch.Generator().manual_seed(5))
+    pos = torch.randint(0, 900, (axes, 2, n), generator=torch.Generator().manual_seed(6)) if axes > 1 else None
+    lens = torch.tensor([n, (n + 1) // 2]) if padded else None
+    up = torch.randn(2, n, 96, generator=torch.Generator().manual_seed(7))
+    plain, xd = Plain(m), x.double().requires_grad_()
+    kv = {} if lens is None else {"kv_lens": lens}
+    want = plain(xd, torch.arange(n).expand(axes, 2, n) if pos is None else pos, **kv)
+    want.backward(up.double())
+    xg = x.cuda().requires_grad_()
+    got = m(xg, None if pos is None else pos.cuda(), None if lens is None else lens.cuda())
+    got.backward(up.cuda())
+    with torch.no_grad():
+        q1, _, k1, _, _ = plain.project(xd)
+        score = (q1.norm(dim=-1).max() * k1.norm(dim=-1).max() / 8).item()
+    tol = 4 * 3 * (96 + 4 * m.v_head_dim + 64 + 2 * n) * U * (1 + score)
+    assert tol < 2e-2
+    assert off(got, want.detach()) < tol and off(xg.grad, xd.grad) < tol
+    for name, p in m.named_parameters():
+        assert p.grad is not None and off(p.grad, plain.w[name].grad) < tol, name
+
+
+@gpu
+def test_training_step_bf16_runs():
+    m = layer(dtype=BF)
+    x = torch.randn(2, 200, 96, device="cuda", dtype=BF, requires_grad=True)
+    m(x).square().mean().backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in (x, *m.parameters()))
+
+
+@gpu
+@pytest.mark.parametrize("kw", [{}, {"v_head_dim": 128}, {"num_heads": 20, "kv_heads": 1, "head_dim": 128, "v_head_dim": 256}])
+@pytest.mark.parametrize("prompt", [1, 5, 90])
+def test_prompt_and_decoding(kw, prompt):
+    """fp32: the rows that the cache holds, read back, lie within a quantisation step of the float64
+    layer's (group range / 15 / 2, its scale rounded to 8 bits: 15 steps of 2^-9 of one; and the group's
+    smallest value to 8 bits), and each step's outputs are the float64 attention over the rows read back.
+    The tolerance is the training step's without its gradients; the cache's kernel adds up m and code
+    parts of a value apart, each up to 16 times the difference that they stand for."""
+    m = layer(**kw)
+    plain = Plain(m)
+    steps, cap = 3, prompt + 3
+    x = torch.randn(2, cap, 96, generator=torch.Generator().manual_seed(8))
+    cache = m.new_cache(2, cap)
+    outs = [m(x[:, :prompt].cuda(), cache=cache)]
+    outs += [m(x[:, i:i + 1].cuda(), cache=cache) for i in range(prompt, cap)]
+    assert cache.lengths.tolist() == [cap, cap] and len(outs) == 1 + steps and not outs[0].requires_grad
+    got = torch.cat(outs, 1)
+    held = [t.double().cpu() for t in cache.read(dtype=F32)]
+    with torch.no_grad():
+        pos = torch.arange(cap).expand(1, 2, cap)
+        q1, q2, k1, k2, v = plain.project(x.double())
+        q1, q2, k1, k2 = (plain.turn(t, pos) for t in (q1, q2, k1, k2))
+        want = plain.out(plain.attend(q1, q2, *held))
+        score = (q1.norm(dim=-1).max() * k1.norm(dim=-1).max() / math.sqrt(m.head_dim)).item()
+    for row, t in zip(held, (k1, k2, v)):
+        y = t.unflatten(-1, (-1, 64))
+        step = (y.amax(-1, keepdim=True) - y.amin(-1, keepdim=True)) / 15
+        room = step / 2 + 16 * step * 2.0 ** -9 + y.abs().amax(-1, keepdim=True) * (2.0 ** -8 + 1e-5)
+        assert ((row.unflatten(-1, (-1, 64)) - y).abs() <= room).all()
+    tol = 4 * 16 * (96 + m.num_heads * m.v_head_dim + m.head_dim + 2 * cap) * U * (1 + score)
+    assert tol < 0.2  # says something: another row's or head's output is off by more than its norm
+    assert off(got, want) < tol
+
+
+@gpu
+def test_padded_prompt_is_decoded_on_from_its_own_length():
+    m = layer()
+    x = torch.randn(2, 40, 96, generator=torch.Generator().manual_seed(9)).cuda()
+    both = m.new_cache(2, 64)
+    first = m(x, cache=both)
+    both.lengths.copy_(torch.tensor([40, 13]))
+    step = torch.randn(2, 1, 96, generator=torch.Generator().manual_seed(10)).cuda()
+    out = m(step, cache=both)
+    alone = m.new_cache(1, 64)
+    own = m(x[1:, :13], cache=alone)
+    # the projections of other row counts round otherwise: within an output's own tolerance of above,
+    # but a key that rounds to the other side moves a code by one step
+    assert off(first[1:, :13], own.double().cpu()) < 0.05
+    assert off(out[1:], m(step[1:], cache=alone).double().cpu()) < 0.05
+    assert both.lengths.tolist() == [41, 14] and alone.lengths.tolist() == [14]
+
+
+@gpu
+def test_cache_refusals():
+    m = layer()
+    x = torch.zeros(2, 1, 96, device="cuda")
+    with pytest.raises(ValueError, match="sequences"):
+        m(x, cache=m.new_cache(3, 8))
+    with pytest.raises(ValueError, match="exclude"):
+        m(x, kv_lens=torch.ones(2, device="cuda", dtype=torch.int32), cache=m.new_cache(2, 8))
+    with pytest.raises(ValueError, match="do not fit"):
+        m(torch.zeros(2, 9, 96, device="cuda"), cache=m.new_cache(2, 8))
+    with pytest.raises(ValueError, match="shape"):
+        m(x, cache=layer(v_head_dim=128).new_cache(2, 8))
+
+
+@gpu
+def test_captured_decoding():
+    """A graph of one decoding step, replayed over a growing cache with other work between."""
+    m = layer(dtype=BF)
+    with torch.no_grad():
+        x = torch.randn(2, 12, 96, device="cuda", dtype=BF)
+        own, eager = m.new_cache(2, 32), m.new_cache(2, 32)
+        m(x[:, :6], cache=own)
+        m(x[:, :6], cache=eager)
+        now = x[:, 6:7].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m(now, cache=own)
+        torch.cuda.current_stream().wait_stream(side)
+        own.lengths.fill_(6)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m(now, cache=own)
+        own.lengths.fill_(6)
+        for i in range(6, 12):
+            now.copy_(x[:, i:i + 1])
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, m(now, cache=eager))
+    assert own.lengths.tolist() == eager.lengths.tolist() == [12, 12]
+    assert all(torch.equal(a, b) for a, b in zip(own.read(), eager.read()))

@@ -306,3 +306,24 @@ def test_refusals():
     assert c.lengths.tolist() == [0, 0]
     c.append(k[:, :, :0], k[:, :, :0], v[:, :, :0])
     assert c.attend(q[:, :, :0], q[:, :, :0], 0.5).shape == (2, 4, 0, 128)
+
+
+@gpu
+def test_lengths_below_zero_count_from_the_start():
+    c = tda_amd.Int4KVCache(2, 1, 8, 64, 64)
+    c.lengths.copy_(torch.tensor([-3, 0]))
+    xs = context(2, 1, 4, 64, 64, BF)
+    c.append(*xs)
+    assert c.lengths.tolist() == [4, 4]
+    assert all(torch.equal(got[:, :, :4], held(x)) for got, x in zip(c.read(dtype=F32), xs))
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 40])
+def test_lengths_beyond_the_capacity(n):
+    c = tda_amd.Int4KVCache(1, 1, 50, 64, 64)
+    c.append(*context(1, 1, 50, 64, 64, BF))
+    q = rows(1, 1, n, 64, 3, BF)
+    want = c.attend(q, q * 0.5, 0.5)
+    c.lengths.fill_(1 << 30)
+    assert torch.equal(c.attend(q, q * 0.5, 0.5), want)

@@ -406,3 +406,14 @@ def test_rows_far_into_memory():
     # weights and output rounded to bf16; the sum of 2^20 terms in 1024 parts of 32-bit adds, the
     # scores' 32-bit sums: under 2^-12 of the magnitudes together
     assert ((out[-1:].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * big).all()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_no_keys_and_rows_that_are_not_finite(bad):
+    q = rows((1, 2, 3, 64), 1, F32).fill_(bad).requires_grad_()
+    none = torch.empty(1, 2, 0, 64, device="cuda", requires_grad=True)
+    out = tda_amd.differential_attention(q, q, none, none, none, 0.5)
+    assert out.shape == (1, 2, 3, 64) and not out.any()
+    out.sum().backward()
+    assert not q.grad.any() and none.grad.shape == none.shape
