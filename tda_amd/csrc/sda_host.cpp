@@ -14,6 +14,7 @@ namespace {
 constexpr int64_t kMaxPos = (int64_t(1) << 30) - 64;      // positions and row counts stay in int32
 constexpr int64_t kMaxRowBytes = int64_t(1) << 25;        // a tile of 64 rows spans at most 2^31 bytes
 constexpr int64_t kMaxCapacity = int64_t(1) << 24;        // a head's codes stay within 32-bit offsets
+constexpr int64_t kMaxStride = int64_t(1) << 50;          // elements: offsets of whole tensors stay in int64
 constexpr double kLog2e = 1.4426950408889634074;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -28,7 +29,7 @@ int32_t check_rows(const tda_tensor& t, int64_t es, bool fine = false) {
   const int64_t unit = fine ? es : 16;
   if (reinterpret_cast<uintptr_t>(t.data) % unit != 0) return TDA_ERR_LAYOUT;
   for (int k = 0; k < 3; ++k) {
-    if (t.stride[k] < 0) return TDA_ERR_LAYOUT;
+    if (t.stride[k] < 0 || t.stride[k] > kMaxStride) return TDA_ERR_LAYOUT;
     if ((t.stride[k] * es) % unit != 0) return TDA_ERR_LAYOUT;
   }
   return t.stride[2] * es > kMaxRowBytes ? TDA_ERR_LAYOUT : TDA_OK;
@@ -40,8 +41,14 @@ int32_t check_lambda(const void* p, const int64_t (&s)[3], int32_t dtype) {
   if (!p) return TDA_ERR_NULL_POINTER;
   if (dtype != TDA_DTYPE_F32 && dtype != TDA_DTYPE_BF16) return TDA_ERR_DTYPE;
   for (int64_t x : s)
-    if (x < 0) return TDA_ERR_LAYOUT;
+    if (x < 0 || x > kMaxStride) return TDA_ERR_LAYOUT;
   return reinterpret_cast<uintptr_t>(p) % bytes_of(dtype) ? TDA_ERR_LAYOUT : TDA_OK;
+}
+// Optional arrays of 4-byte elements.
+int32_t check_words(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return TDA_ERR_LAYOUT;
+  return TDA_OK;
 }
 int32_t check_workspace(const void* p, size_t have, size_t need) {
   if (!need) return TDA_OK;
@@ -50,21 +57,28 @@ int32_t check_workspace(const void* p, size_t have, size_t need) {
 // A launch lays its workgroups out over two grid axes of at most 2^32 work-items each.
 bool fits_grid(double blocks) { return blocks < 4294967295.0; }
 
+// What the buffer sizes depend on.
+template <class A>
+int32_t check_sizes(const A& a) {
+  if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.seq_len < 1 || a.seq_len_kv < 1) return TDA_ERR_SHAPE;
+  if (a.heads % a.kv_heads) return SDA_ERR_HEADS;
+  if (!head_dims(a.head_dim, a.v_head_dim)) return TDA_ERR_HEAD_DIM;
+  if (a.batch > kMaxPos || a.heads > kMaxPos || a.batch * a.heads > kMaxPos) return TDA_ERR_SHAPE;
+  if (a.seq_len > kMaxPos || a.seq_len_kv > kMaxPos) return TDA_ERR_OFFSET;
+  // the most workgroups that any launch of the operator takes: one per 16 rows or keys and column group
+  return fits_grid((double)a.batch * a.heads * ((double)a.seq_len + a.seq_len_kv + 32) / 16.0 * (a.v_head_dim / 16.0))
+             ? TDA_OK
+             : TDA_ERR_SHAPE;
+}
 template <class A>
 int32_t check_common(const A& a) {
   if (a.abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
   if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16) return TDA_ERR_DTYPE;
   if (a.causal != 0 && a.causal != 1) return TDA_ERR_CAUSAL;
   if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return SDA_ERR_SCALE;
-  if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.seq_len < 1 || a.seq_len_kv < 1) return TDA_ERR_SHAPE;
-  if (a.heads % a.kv_heads) return SDA_ERR_HEADS;
-  if (!head_dims(a.head_dim, a.v_head_dim)) return TDA_ERR_HEAD_DIM;
-  if (a.batch > kMaxPos || a.heads > kMaxPos || a.batch * a.heads > kMaxPos) return TDA_ERR_SHAPE;
-  if (a.seq_len > kMaxPos || a.seq_len_kv > kMaxPos) return TDA_ERR_OFFSET;
-  if (!a.q_offsets && (a.q_offset < -kMaxPos || a.q_offset + a.seq_len > kMaxPos)) return TDA_ERR_OFFSET;
-  // the most workgroups that any launch of the operator takes: one per 16 rows or keys and column group
-  if (!fits_grid((double)a.batch * a.heads * ((double)a.seq_len + a.seq_len_kv + 32) / 16.0 * (a.v_head_dim / 16.0)))
-    return TDA_ERR_SHAPE;
+  if (int32_t rc = check_sizes(a)) return rc;
+  if (!a.q_offsets && (a.q_offset < -kMaxPos || a.q_offset > kMaxPos - a.seq_len)) return TDA_ERR_OFFSET;
+  if (int32_t rc = check_words({a.q_offsets, a.kv_lens, a.lse})) return rc;
   return check_lambda(a.lambda_param, a.lambda_stride, a.lambda_dtype);
 }
 
@@ -143,11 +157,15 @@ void fill(P& p, const A& a) {
   p.c = (float)(a.scale * kLog2e);
 }
 
-int32_t check_cache(const sda_kv4& c) {
+int32_t check_cache_sizes(const sda_kv4& c) {
   if (c.batch < 1 || c.kv_heads < 1 || c.capacity < 1) return TDA_ERR_SHAPE;
   if (!head_dims(c.head_dim, c.v_head_dim)) return TDA_ERR_HEAD_DIM;
   if (c.capacity > kMaxCapacity || c.batch > kMaxPos || c.kv_heads > kMaxPos || c.batch * c.kv_heads > kMaxPos) return SDA_ERR_CACHE;
   if (!fits_grid((double)c.batch * c.kv_heads * c.capacity * c.v_head_dim / 2048.0)) return SDA_ERR_CACHE;
+  return TDA_OK;
+}
+int32_t check_cache(const sda_kv4& c) {
+  if (int32_t rc = check_cache_sizes(c)) return rc;
   if (!c.k1 || !c.k2 || !c.v || !c.lengths) return TDA_ERR_NULL_POINTER;
   for (const void* p : {c.k1, c.k2, c.v})
     if (reinterpret_cast<uintptr_t>(p) % 16) return TDA_ERR_LAYOUT;
@@ -199,9 +217,7 @@ const char* sda_error_string(int32_t code) {
 }
 
 size_t sda_fwd_workspace_bytes(const sda_fwd_args* a) {
-  if (!a || a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->seq_len < 1 ||
-      a->seq_len_kv < 1 || !head_dims(a->head_dim, a->v_head_dim) || !decodes(*a))
-    return 0;
+  if (!a || check_sizes(*a) || !decodes(*a)) return 0;
   int nsplit, chunk;
   const int64_t items = dec_items(a->batch, a->heads, a->kv_heads, a->seq_len);
   dec_split(items, a->seq_len_kv, kDecTarget, &nsplit, &chunk);
@@ -235,9 +251,7 @@ int32_t sda_fwd(const sda_fwd_args* a, void* stream) {
 }
 
 size_t sda_bwd_workspace_bytes(const sda_bwd_args* a) {
-  if (!a || a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->seq_len < 1 ||
-      a->seq_len_kv < 1 || !head_dims(a->head_dim, a->v_head_dim))
-    return 0;
+  if (!a || check_sizes(*a)) return 0;
   return (size_t)(stat_bytes(*a) + part_bytes(*a));
 }
 
@@ -250,6 +264,7 @@ int32_t sda_validate_bwd(const sda_bwd_args* a) {
     if (int32_t rc = check_rows(*t, es)) return rc;
   if (int32_t rc = check_kept(*a)) return rc;
   if (!a->lse) return TDA_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(a->dlambda) % bytes_of(a->lambda_dtype)) return TDA_ERR_LAYOUT;
   return check_workspace(a->workspace, a->workspace_bytes, sda_bwd_workspace_bytes(a));
 }
 
@@ -296,7 +311,7 @@ int32_t sda_validate_rotary(const sda_rotary_args* a) {
   if (reinterpret_cast<uintptr_t>(a->positions) % a->position_dtype || reinterpret_cast<uintptr_t>(a->inv_freq) % 4)
     return TDA_ERR_LAYOUT;
   for (int64_t s : a->position_stride)
-    if (s < 0) return TDA_ERR_LAYOUT;
+    if (s < 0 || s > kMaxStride) return TDA_ERR_LAYOUT;
   for (int z = 0; z < a->count; ++z) {
     if (a->heads[z] < 1 || a->heads[z] > (1 << 20)) return TDA_ERR_SHAPE;
     if (int32_t rc = check_rows(a->x[z], bytes_of(a->dtype), true)) return rc;
@@ -333,7 +348,8 @@ int32_t sda_rotary(const sda_rotary_args* a, void* stream) {
 }
 
 size_t sda_kv4_bytes(int64_t batch, int64_t kv_heads, int64_t capacity, int64_t width) {
-  if (batch < 1 || kv_heads < 1 || capacity < 1 || (width != 64 && width != 128 && width != 256)) return 0;
+  if (batch < 1 || kv_heads < 1 || capacity < 1 || batch > kMaxPos || kv_heads > kMaxPos || batch * kv_heads > kMaxPos ||
+      capacity > kMaxCapacity || (width != 64 && width != 128 && width != 256)) return 0;
   return (size_t)(batch * kv_heads * (ceil_div(capacity, 4) * 4) * (width / 2 + width / 64 * 4));
 }
 
@@ -345,7 +361,7 @@ int32_t sda_validate_kv4_append(const sda_kv4_append_args* a) {
   if (a->rows < 1 || a->rows > a->cache.capacity) return SDA_ERR_CACHE;
   for (const tda_tensor* t : {&a->k1, &a->k2, &a->v})
     if (int32_t rc = check_rows(*t, bytes_of(a->dtype))) return rc;
-  return TDA_OK;
+  return check_words({a->start, a->counts});
 }
 int32_t sda_kv4_append(const sda_kv4_append_args* a, void* stream) {
   if (int32_t rc = sda_validate_kv4_append(a)) return rc;
@@ -385,10 +401,17 @@ int32_t sda_kv4_read(const sda_kv4_read_args* a, void* stream) {
   return done(sda::launch_kv4_read(p, a->dtype, stream));
 }
 
+static int32_t check_attend_sizes(const sda_kv4_attend_args& a) {
+  if (int32_t rc = check_cache_sizes(a.cache)) return rc;
+  if (a.heads < 1 || a.seq_len < 1) return TDA_ERR_SHAPE;
+  if (a.heads % a.cache.kv_heads) return SDA_ERR_HEADS;
+  return a.heads <= kMaxPos && a.seq_len <= kMaxPos &&
+                 fits_grid((double)a.cache.batch * a.heads * a.seq_len * ((double)a.cache.capacity + 256) / 128.0)
+             ? TDA_OK
+             : TDA_ERR_SHAPE;
+}
 size_t sda_kv4_attend_workspace_bytes(const sda_kv4_attend_args* a) {
-  if (!a || a->cache.batch < 1 || a->cache.kv_heads < 1 || a->heads < 1 || a->heads % a->cache.kv_heads ||
-      a->seq_len < 1 || a->cache.capacity < 1 || !head_dims(a->cache.head_dim, a->cache.v_head_dim))
-    return 0;
+  if (!a || check_attend_sizes(*a)) return 0;
   int nsplit, chunk;
   const int64_t items = dec_items(a->cache.batch, a->heads, a->cache.kv_heads, a->seq_len);
   dec_split(items, a->cache.capacity, kKv4Target, &nsplit, &chunk);
@@ -400,11 +423,7 @@ int32_t sda_validate_kv4_attend(const sda_kv4_attend_args* a) {
   if (!any_dtype(a->dtype)) return TDA_ERR_DTYPE;
   if (int32_t rc = check_cache(a->cache)) return rc;
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return SDA_ERR_SCALE;
-  if (a->heads < 1 || a->seq_len < 1) return TDA_ERR_SHAPE;
-  if (a->heads % a->cache.kv_heads) return SDA_ERR_HEADS;
-  if (a->heads > kMaxPos || a->seq_len > kMaxPos ||
-      !fits_grid((double)a->cache.batch * a->heads * a->seq_len * ((double)a->cache.capacity + 256) / 128.0))
-    return TDA_ERR_SHAPE;
+  if (int32_t rc = check_attend_sizes(*a)) return rc;
   if (int32_t rc = check_lambda(a->lambda_param, a->lambda_stride, a->lambda_dtype)) return rc;
   for (const tda_tensor* t : {&a->q1, &a->q2, &a->out})
     if (int32_t rc = check_rows(*t, bytes_of(a->dtype))) return rc;
