@@ -60,31 +60,31 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
 // ------------------------------------------------------------------ key-major pass
 // Whether two workgroups of the key pass fit a CU (two waves a SIMD).
 template <class Tr, int D, int DV>
-constexpr bool kKeyLean = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64;
-constexpr int kKeyRows = 128;  // keys of a workgroup: 4 waves of 32
-
+constexpr bool kKeyTwo = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64;
 template <class Tr, int D, int DV>
+constexpr bool kKeyLean = kKeyTwo<Tr, D, DV> || (sizeof(typename Tr::T) == 2 ? DV == 256 : DV >= 128);
+
+template <class Tr, int D, int DV, int RH>
 struct KeyShape {
   using QT = Tile<Tr, 32, D>;
   using OT = Tile<Tr, 32, DV>;
   static constexpr int STAT = 2 * QT::BYTES + OT::BYTES;  // the statistics of the 32 rows
-  static constexpr int STAGE = STAT + 1024;
-  static constexpr int RING = 2;  // stages in LDS, all but one of them on their way
-  static constexpr int LDS = RING * STAGE;
-  static constexpr int NW = 4;
-  static constexpr int LOADS = (2 * QT::LOADS + OT::LOADS) / NW + 8 / NW;  // of a wave, a stage
-  static_assert((QT::LOADS % NW == 0 && OT::LOADS % NW == 0) || RING == 2, "loads spread evenly over the waves");
+  static constexpr int TILE = STAT + 1024;
+  static constexpr int STAGE = RH * TILE;               // of two, one on its way
+  static constexpr int XCH = (RH - 1) * 2 * 32 * (2 * D + DV) * 4;  // the second half's sums
+  static constexpr int LDS = 2 * STAGE > XCH ? 2 * STAGE : XCH;
+  static constexpr int NW = 4, KEYS = 32 * NW / RH;
 };
 
 // One wave per SIMD (the three gradients' accumulators and the resident rows fill the registers), so
 // the wave hides its own latencies: the LDS operands of a step are one sequence, read a group ahead of their
 // use, and the first branch's weights are computed between the second's score products, the second's
 // between the first's gradient products.
-template <class Tr, int D, int DV>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyLean<Tr, D, DV> ? 2 : 1)))) bwd_keys(BwdParams P) {
+template <class Tr, int D, int DV, int RH>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyTwo<Tr, D, DV> ? 2 : 1)))) bwd_keys(BwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
-  using S = KeyShape<Tr, D, DV>;
+  using S = KeyShape<Tr, D, DV, RH>;
   using QT = typename S::QT;
   using OT = typename S::OT;
   constexpr bool LEAN = kKeyLean<Tr, D, DV>;
@@ -97,22 +97,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + kKeyRows - 1) / kKeyRows;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rh = RH == 1 ? 0 : wv / (NW / RH);
+  const int GQ = P.H / P.Hk, parts = GQ / P.gs, nkt = (P.Nk + S::KEYS - 1) / S::KEYS;
   const uint32_t bid = tda::grid_bid<64 * NW>(), heads = (uint32_t)(P.B * P.Hk) * (uint32_t)parts;
   if (bid >= heads * (uint32_t)nkt) return;
   const Item it = item_of(bid, heads, nkt, false);
   const int part = it.head % parts, bk = it.head / parts, b = bk / P.Hk, hk = bk % P.Hk;
   const int h0 = hk * GQ + part * P.gs;
-  const int k0 = it.tile * kKeyRows, k0w = k0 + 32 * wv, key = k0w + n32;
+  const int k0 = it.tile * S::KEYS, k0w = k0 + 32 * (wv % (NW / RH)), key = k0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
   const bool live = key < len;
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
 
-  // query tiles of 32 rows: from the first that sees the workgroup's first key on
+  // query tiles of 32 rows, RH a step: from the first that sees the workgroup's first key on
   const int nqt = (P.Nq + 31) / 32;
   const int first = P.see.causal ? max(k0 - off, 0) >> 5 : 0;
-  const int per = k0 < len ? max(nqt - first, 0) : 0;
+  const int per = k0 < len ? max(nqt - first + RH - 1, 0) / RH : 0;
   const int steps = per * P.gs;
 
   uint32_t qo[2][QL], oo[OL];
@@ -123,9 +123,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   }
 #pragma unroll
   for (int u = 0; u < OL; ++u) oo[u] = OT::source(NW * u + wv, (uint32_t)(P.dout.st * OT::ES));
-  auto issue = [&](int slot, int h, int qt) {  // query tile qt of head h
-    const int i0 = 32 * qt, n = min(32, P.Nq - i0);
-    char* at = lds + slot * S::STAGE;
+  auto issue = [&](char* at, int h, int qt) {  // query tile qt of head h
+    const int i0 = 32 * qt, n = max(min(32, P.Nq - i0), 0);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const auto r = rows_rsrc(row_of<T>(P.q[x], b, h, i0), P.q[x].st * QT::ES, n, D * QT::ES);
@@ -147,11 +146,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   };
   int nh = h0, nq = first;  // head and query tile of the next stage to send for
   auto send = [&](int slot) {
-    issue(slot, nh, nq);
-    if (++nq == nqt) nq = first, ++nh;
+#pragma unroll
+    for (int s = 0; s < RH; ++s) issue(lds + slot * S::STAGE + s * S::TILE, nh, nq + s);
+    nq += RH;
+    if (nq >= nqt) nq = first, ++nh;
   };
-  for (int j = 0; j < S::RING - 1; ++j)
-    if (j < steps) send(j);
+  if (steps > 0) send(0);
 
   frag kf[2][NT], vf[NV];
 #pragma unroll
@@ -166,15 +166,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   RowReader<Tr, DV> orow;
   ColReader<Tr, D> qc;
   ColReader<Tr, DV> oc;
-  qr.init(lds);
-  qc.init(lds);
-  orow.init(lds + 2 * QT::BYTES);
-  oc.init(lds + 2 * QT::BYTES);
+  char* qb = lds + rh * S::TILE;
+  char* ot = qb + 2 * QT::BYTES;
+  qr.init(qb);
+  qc.init(qb);
+  orow.init(ot);
+  oc.init(ot);
   auto step = [&](int i0, auto half) {  // the stage in that half of the buffers
     constexpr int AT = half * S::STAGE;
-    const char* ot = lds + 2 * QT::BYTES;
     const bool edge = P.see.causal && off + i0 < k0w + 31;  // some row does not see some key
-    const float* st = reinterpret_cast<const float*>(lds + AT + S::STAT);
+    const float* st = reinterpret_cast<const float*>(qb + AT + S::STAT);
     // the sequence: dO rows (dP), q1 rows, q2 rows (scores), q1 columns (dk1), q2 columns (dk2), dO columns (dv)
     constexpr int E1 = NV, E2 = E1 + NT, E3 = E2 + NT, E4 = E3 + D / 16, E5 = E4 + D / 16, E6 = E5 + DV / 16;
     frag f[AHEAD + 1][G];
@@ -183,10 +184,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
         constexpr int e = i * G + u;
         frag& to = f[i % (AHEAD + 1)][u];
         if constexpr (e < E1) to = orow.read(ot, AT, e);
-        else if constexpr (e < E2) to = qr.read(lds, AT, e - E1);
-        else if constexpr (e < E3) to = qr.read(lds, AT + QT::BYTES, e - E2);
-        else if constexpr (e < E4) to = qc.read(lds, AT, (e - E3) / (D / 32), (e - E3) % (D / 32));
-        else if constexpr (e < E5) to = qc.read(lds, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
+        else if constexpr (e < E2) to = qr.read(qb, AT, e - E1);
+        else if constexpr (e < E3) to = qr.read(qb, AT + QT::BYTES, e - E2);
+        else if constexpr (e < E4) to = qc.read(qb, AT, (e - E3) / (D / 32), (e - E3) % (D / 32));
+        else if constexpr (e < E5) to = qc.read(qb, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
         else to = oc.read(ot, AT, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
       });
     };
@@ -262,9 +263,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   // The same for two waves a SIMD, which cover each other: fewer registers, the branches one after the other.
   auto lean = [&](int i0, auto half) {
     constexpr int AT = half * S::STAGE;
-    const char* ot = lds + 2 * QT::BYTES;
     const bool edge = P.see.causal && off + i0 < k0w + 31;
-    const float* st = reinterpret_cast<const float*>(lds + AT + S::STAT) + 4 * g;
+    const float* st = reinterpret_cast<const float*>(qb + AT + S::STAT) + 4 * g;
     constexpr int E1 = NV, E2 = E1 + NT, E3 = E2 + D / 16, E4 = E3 + NT, E5 = E4 + D / 16, E6 = E5 + DV / 16;
     frag f[2][G];
     auto read = [&](auto i) {
@@ -272,10 +272,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
         constexpr int e = i * G + u;
         frag& to = f[i % 2][u];
         if constexpr (e < E1) to = orow.read(ot, AT, e);
-        else if constexpr (e < E2) to = qr.read(lds, AT, e - E1);
-        else if constexpr (e < E3) to = qc.read(lds, AT, (e - E2) / (D / 32), (e - E2) % (D / 32));
-        else if constexpr (e < E4) to = qr.read(lds, AT + QT::BYTES, e - E3);
-        else if constexpr (e < E5) to = qc.read(lds, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
+        else if constexpr (e < E2) to = qr.read(qb, AT, e - E1);
+        else if constexpr (e < E3) to = qc.read(qb, AT, (e - E2) / (D / 32), (e - E2) % (D / 32));
+        else if constexpr (e < E4) to = qr.read(qb, AT + QT::BYTES, e - E3);
+        else if constexpr (e < E5) to = qc.read(qb, AT + QT::BYTES, (e - E4) / (D / 32), (e - E4) % (D / 32));
         else to = oc.read(ot, AT, (e - E5) / (DV / 32), (e - E5) % (DV / 32));
       });
     };
@@ -297,15 +297,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
       }
     };
     read(std::integral_constant<int, 0>());
-    f32x16 dp = rowstat(2), sc, w;
+    f32x16 dp = START ? rowstat(2) : f32x16{}, sc, w;
     frag ds[2];
     constexpr int NG = E6 / G;
     times<NG>([&](auto i) {
       if constexpr (i + 1 < NG) read(std::integral_constant<int, i + 1>());
-      if constexpr (i * G == E1) sc = rowstat(0);
-      if constexpr (i * G == E3) sc = rowstat(1);
+      if constexpr (i * G == E1) sc = START ? rowstat(0) : f32x16{};
+      if constexpr (i * G == E3) sc = START ? rowstat(1) : f32x16{};
       if constexpr (i * G == E2) {  // the first branch's weights
         hide(sc);
+        if constexpr (!START) dp += rowstat(2), sc += rowstat(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           w[r] = exp2_(P.c * sc[r]);
@@ -315,6 +316,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
       }
       if constexpr (i * G == E4) {  // the second's
         hide(sc);
+        if constexpr (!START) sc += rowstat(1);
         dp += rowstat(3);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -346,22 +348,43 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyL
   };
   int qt = first;  // of this step
   auto one = [&](int j, auto slot) {
-    if (j + 1 < steps) wait_vm<(S::RING - 2) * S::LOADS>();  // the later stages may stay on their way
-    else wait_vm<0>();
+    wait_vm<0>();
     tda::lds_barrier();
-    if (j + S::RING - 1 < steps) send((slot + S::RING - 1) % S::RING);
-    if (!P.see.causal || off + min(32 * qt + 31, P.Nq - 1) >= k0w) {
-      if constexpr (LEAN) lean(32 * qt, slot);
-      else step(32 * qt, slot);
+    if (j + 1 < steps) send(1 - slot);
+    const int i0 = 32 * (qt + rh);
+    if (i0 < P.Nq && (!P.see.causal || off + min(i0 + 31, P.Nq - 1) >= k0w)) {
+      if constexpr (LEAN) lean(i0, slot);
+      else step(i0, slot);
     }
-    if (++qt == nqt) qt = first;
+    qt += RH;
+    if (qt >= nqt) qt = first;
   };
-  for (int j = 0; j < steps; j += S::RING)
-    times<S::RING>([&](auto x) {
-      if (j + x < steps) one(j + x, x);
-    });
+  for (int j = 0; j < steps; j += 2) {
+    one(j, std::integral_constant<int, 0>());
+    if (j + 1 < steps) one(j + 1, std::integral_constant<int, 1>());
+  }
   wait_vm<0>();
 
+  if constexpr (RH == 2) {  // the second half's sums join the first's
+    constexpr int N = (2 * D + DV) / 32 * 4;  // pieces of four values a lane
+    f32x4* x4 = reinterpret_cast<f32x4*>(lds) + (wv & 1) * (N * 64) + l;
+    __syncthreads();
+    if (rh)
+      times<N>([&](auto i) {
+        constexpr int y = i / 4, r = 4 * (i % 4), W = D / 32;
+        const f32x16& a = y < W ? dk[0][y % W] : y < 2 * W ? dk[1][y % W] : dv[y < 2 * W ? 0 : y - 2 * W];
+        x4[i * 64] = f32x4{a[r], a[r + 1], a[r + 2], a[r + 3]};
+      });
+    __syncthreads();
+    if (rh) return;
+    times<N>([&](auto i) {
+      constexpr int y = i / 4, r = 4 * (i % 4), W = D / 32;
+      f32x16& a = y < W ? dk[0][y % W] : y < 2 * W ? dk[1][y % W] : dv[y < 2 * W ? 0 : y - 2 * W];
+      const f32x4 w = x4[i * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[r + e] += w[e];
+    });
+  }
   if (key >= P.Nk) return;
   // a key past the length met weights of its own making (of a zero row): its column holds nothing else
 #pragma unroll
@@ -415,40 +438,41 @@ __global__ void __launch_bounds__(256) bwd_sum(BwdParams P, int parts) {
 }
 
 // ------------------------------------------------------------------ query-major pass
-template <class Tr, int D, int DV, bool SPLIT>
+template <class Tr, int D, int DV, bool SPLIT, int RG>
 struct QueryShape {
   using KT = Tile<Tr, 32, D>;
   using VT = Tile<Tr, 32, DV>;
   static constexpr int WAVES = SPLIT ? 8 : 4;
-  static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
-  static constexpr int LDS = 2 * STAGE;
+  static constexpr int KH = 4 / RG, TILE = 2 * KT::BYTES + VT::BYTES, STAGE = KH * TILE;
+  static constexpr int LDS = 2 * STAGE;  // a half's sums need less
   static constexpr int KL = (KT::LOADS + WAVES - 1) / WAVES, VL = (VT::LOADS + WAVES - 1) / WAVES;
 };
 
-template <class Tr, int D, int DV, bool SPLIT>
+template <class Tr, int D, int DV, bool SPLIT, int RG>
 __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves_per_eu(SPLIT || (sizeof(typename Tr::T) == 2 && D == 64) ? 2 : 1))) bwd_query(BwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
-  using S = QueryShape<Tr, D, DV, SPLIT>;
+  using S = QueryShape<Tr, D, DV, SPLIT, RG>;
   using KT = typename S::KT;
   using VT = typename S::VT;
-  constexpr int NT = D / 16, NV = DV / 16, KL = S::KL, VL = S::VL, NW = S::WAVES, NB = SPLIT ? 1 : 2;
+  constexpr int NT = D / 16, NV = DV / 16, KL = S::KL, VL = S::VL, NW = S::WAVES, NB = SPLIT ? 1 : 2, KH = S::KH, ROWS = 32 * RG;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv & 3, br = wv >> 2;
-  const int nqt = (P.Nq + 127) / 128;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv % RG;
+  const int br = SPLIT ? wv / RG & 1 : 0, kh = RG == 4 ? 0 : wv / (NW / KH);  // kh: which of a stage's key tiles
+  const int nqt = (P.Nq + ROWS - 1) / ROWS;
   const uint32_t bid = tda::grid_bid<64 * NW>();
   if (bid >= (uint32_t)(P.B * P.H) * (uint32_t)nqt) return;
   const Item it = item_of(bid, P.B * P.H, nqt, true);
   const int b = it.head / P.H, h = it.head % P.H, hk = h / (P.H / P.Hk);
-  const int q0 = it.tile * 128, q0w = q0 + 32 * rg, qi = q0w + n32;
+  const int q0 = it.tile * ROWS, q0w = q0 + 32 * rg, qi = q0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
-  const int lim = P.see.causal ? min(len, max(off + min(q0 + 128, P.Nq), 0)) : len;
+  const int lim = P.see.causal ? min(len, max(off + min(q0 + ROWS, P.Nq), 0)) : len;
   const int limw = P.see.causal ? min(len, max(off + min(q0w + 32, P.Nq), 0)) : len;
   const int clear = P.see.causal ? min(len, max(off + q0w + 1, 0)) : len;
   const int see = P.see.causal ? min(len, off + qi + 1) : len;
-  const int nst = (lim + 31) / 32;
+  const int nst = (lim + 32 * KH - 1) / (32 * KH);
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
 
   uint32_t ko[2][KL], vo[VL];
@@ -459,8 +483,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
   }
 #pragma unroll
   for (int u = 0; u < VL; ++u) vo[u] = VT::source(NW * u + wv, (uint32_t)(P.v.st * VT::ES));
-  auto issue = [&](int j) {
-    char* at = lds + (j & 1) * S::STAGE;
+  auto tile = [&](char* at, int j) {  // key tile j
     const int n = min(32, lim - 32 * j);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -473,6 +496,10 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
 #pragma unroll
     for (int u = 0; u < VL; ++u)
       if (VT::LOADS % NW == 0 || NW * u + wv < VT::LOADS) VT::load(r, reinterpret_cast<T*>(at + 2 * KT::BYTES), NW * u + wv, vo[u]);
+  };
+  auto issue = [&](int j) {
+#pragma unroll
+    for (int s = 0; s < KH; ++s) tile(lds + (j & 1) * S::STAGE + s * S::TILE, KH * j + s);
   };
   if (nst > 0) issue(0);
 
@@ -499,18 +526,19 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
   RowReader<Tr, D> kr;
   RowReader<Tr, DV> vr;
   ColReader<Tr, D> kc;
-  const char* kbuf = lds + (SPLIT ? br * KT::BYTES : 0);  // the wave's own branch of the keys
+  const char* kbuf = lds + kh * S::TILE + (SPLIT ? br * KT::BYTES : 0);  // the wave's own branch of the keys
+  const char* vbuf = lds + kh * S::TILE + 2 * KT::BYTES;
   kr.init(kbuf);
   kc.init(kbuf);
-  vr.init(lds + 2 * KT::BYTES);
+  vr.init(vbuf);
   auto step = [&](int j, auto half) {  // stage j, in that half of the buffers
     constexpr int AT = half * S::STAGE;
     wait_vm<0>();
     tda::lds_barrier();
     if (j + 1 < nst) issue(j + 1);
-    const int k0 = 32 * j;
+    const int k0 = 32 * (KH * j + kh);
     if (k0 >= limw) return;
-    const f32x16 dp = chain<Tr, NV>([&](int t) { return vr.read(lds + 2 * KT::BYTES, AT, t); }, of);
+    const f32x16 dp = chain<Tr, NV>([&](int t) { return vr.read(vbuf, AT, t); }, of);
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
       const int z = SPLIT ? br : x, kt = AT + x * KT::BYTES;
@@ -536,6 +564,24 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     if (j + 1 < nst) step(j + 1, std::integral_constant<int, 1>());
   }
   wait_vm<0>();
+  if constexpr (KH == 2) {  // the second half's sums join the first's
+    constexpr int N = NB * D / 32 * 4;
+    f32x4* x4 = reinterpret_cast<f32x4*>(lds) + wv % (NW / KH) * (N * 64) + l;
+    __syncthreads();
+    if (kh)
+      times<N>([&](auto i) {
+        constexpr int x = i / 4 / (D / 32), y = i / 4 % (D / 32), r = 4 * (i % 4);
+        x4[i * 64] = f32x4{dq[x][y][r], dq[x][y][r + 1], dq[x][y][r + 2], dq[x][y][r + 3]};
+      });
+    __syncthreads();
+    if (kh) return;
+    times<N>([&](auto i) {
+      constexpr int x = i / 4 / (D / 32), y = i / 4 % (D / 32), r = 4 * (i % 4);
+      const f32x4 w = x4[i * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dq[x][y][r + e] += w[e];
+    });
+  }
   if (!row) return;
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
@@ -549,35 +595,46 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
 }
 
 // ------------------------------------------------------------------ dlambda
-// One workgroup per distinct element: minus the sum of r_2 over the axes it is broadcast along, each
-// thread's share in order and the threads' by a fixed tree.  `each`: nothing is summed, one thread
-// per element.
-__global__ void __launch_bounds__(256) bwd_lambda(BwdParams P, int each) {
-  const int64_t rows = (int64_t)P.B * P.H * P.Nq;
-  const float* r2 = P.stat + 5 * rows;
-  if (each) {
-    const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
-    if (id >= rows) return;
-    if (P.lam.bf16) static_cast<bf16*>(P.dlam)[id] = (bf16)-r2[id];
-    else static_cast<float*>(P.dlam)[id] = -r2[id];
-    return;
+// Minus the sums of r_2 over the axes lambda is broadcast along, each thread's share in order and the
+// threads' by a fixed tree.  Where that takes in the rows of a head, each head's are summed first (over
+// the first of the row statistics, which no pass reads any more): one workgroup a head.
+__global__ void __launch_bounds__(1024) bwd_lambda_heads(BwdParams P) {
+  const int64_t bh = tda::grid_bid<1024>(), rows = (int64_t)P.B * P.H * P.Nq;
+  if (bh >= (int64_t)P.B * P.H) return;
+  const float* r2 = P.stat + 5 * rows + bh * P.Nq;
+  __shared__ float part[16];
+  float a[4] = {};
+  for (int i = threadIdx.x; i < P.Nq; i += 4096) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a[u] += i + 1024 * u < P.Nq ? r2[i + 1024 * u] : 0.f;
   }
-  __shared__ float part[4];
-  const int64_t e = tda::grid_bid<256>();
-  if (e >= P.dlam_n[0] * P.dlam_n[1] * P.dlam_n[2]) return;
-  const int64_t i0 = e % P.dlam_n[2], h0 = e / P.dlam_n[2] % P.dlam_n[1], b0 = e / P.dlam_n[2] / P.dlam_n[1];
-  const int nb = P.dlam_n[0] == 1 ? P.B : 1, nh = P.dlam_n[1] == 1 ? P.H : 1, ni = P.dlam_n[2] == 1 ? P.Nq : 1;
-  float a = 0.f;
-  for (int b = 0; b < nb; ++b)
-    for (int h = 0; h < nh; ++h) {
-      const float* row = r2 + ((b0 + b) * P.H + h0 + h) * P.Nq + i0;
-      for (int i = threadIdx.x; i < ni; i += 256) a += row[i];
-    }
-  a = tda::wave_sum(a);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
+  const float w = tda::wave_sum((a[0] + a[1]) + (a[2] + a[3]));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = w;
   __syncthreads();
   if (threadIdx.x) return;
-  a = -(part[0] + part[1] + part[2] + part[3]);
+  float sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 16; ++u) sum += part[u];
+  P.stat[bh] = sum;
+}
+// One thread an element (b, h, i), or a wave where an element has whole heads (HEADS: r_2 is summed by
+// head).
+template <bool HEADS>
+__global__ void __launch_bounds__(256) bwd_lambda(BwdParams P) {
+  const int64_t rows = (int64_t)P.B * P.H * P.Nq, all = P.dlam_n[0] * P.dlam_n[1] * P.dlam_n[2];
+  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x, e = HEADS ? id >> 6 : id;
+  if (e >= all) return;
+  const float* from = HEADS ? P.stat : P.stat + 5 * rows;
+  const int64_t N = HEADS ? 1 : P.Nq;
+  const int64_t i0 = HEADS ? 0 : e % P.dlam_n[2], h0 = e / P.dlam_n[2] % P.dlam_n[1], b0 = e / P.dlam_n[2] / P.dlam_n[1];
+  const int nb = P.dlam_n[0] == 1 ? P.B : 1, nh = P.dlam_n[1] == 1 ? P.H : 1;
+  float a = 0.f;
+  for (int x = HEADS ? (int)(id & 63) : 0; x < nb * nh; x += HEADS ? 64 : 1)
+    a -= from[((b0 + x / nh) * P.H + h0 + x % nh) * N + i0];
+  if constexpr (HEADS) {
+    a = tda::wave_sum(a);
+    if (id & 63) return;
+  }
   if (P.lam.bf16) static_cast<bf16*>(P.dlam)[e] = (bf16)a;
   else static_cast<float*>(P.dlam)[e] = a;
 }
@@ -588,32 +645,57 @@ static int big_lds(F* fn, int bytes) {
   if (bytes <= 65536) return 0;
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
+
+template <class Tr, int D, int DV, int RH>
+static int keys(const BwdParams& p, int parts, hipStream_t st) {
+  using S = KeyShape<Tr, D, DV, RH>;
+  if (const int e = big_lds(&bwd_keys<Tr, D, DV, RH>, S::LDS)) return e;
+  bwd_keys<Tr, D, DV, RH><<<tda::grid_of<64 * S::NW>((int64_t)((p.Nk + S::KEYS - 1) / S::KEYS) * p.B * p.Hk * parts), 64 * S::NW, S::LDS, st>>>(p);
+  tda::launched(st, "sda_bwd_keys");
+  return 0;
+}
+template <class Tr, int D, int DV, int RG>
+static int queries(const BwdParams& p, hipStream_t st) {
+  constexpr bool SPLIT = sizeof(typename Tr::T) == 2 ? D == 128 : DV <= 64;
+  using S = QueryShape<Tr, D, DV, SPLIT, RG>;
+  if (const int e = big_lds(&bwd_query<Tr, D, DV, SPLIT, RG>, S::LDS)) return e;
+  bwd_query<Tr, D, DV, SPLIT, RG><<<tda::grid_of<64 * S::WAVES>((int64_t)((p.Nq + 32 * RG - 1) / (32 * RG)) * p.B * p.H), 64 * S::WAVES, S::LDS, st>>>(p);
+  tda::launched(st, "sda_bwd_query");
+  return 0;
+}
 template <class Tr, int D, int DV>
 static int run(const BwdParams& p, hipStream_t st) {
   using T = typename Tr::T;
-  constexpr bool QSPLIT = sizeof(T) == 2 ? D == 128 : DV <= 64;
-  using KS = KeyShape<Tr, D, DV>;
-  using QS = QueryShape<Tr, D, DV, QSPLIT>;
   const int64_t rows = (int64_t)p.B * p.H * p.Nq;
-  int e = big_lds(&bwd_keys<Tr, D, DV>, KS::LDS);
-  if (!e) e = big_lds(&bwd_query<Tr, D, DV, QSPLIT>, QS::LDS);
-  if (e) return e;
   bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
   tda::launched(st, "sda_bwd_rows");
   const int parts = p.H / p.Hk / p.gs;
-  bwd_keys<Tr, D, DV><<<tda::grid_of<64 * KS::NW>((int64_t)((p.Nk + kKeyRows - 1) / kKeyRows) * p.B * p.Hk * parts), 64 * KS::NW, KS::LDS, st>>>(p);
-  tda::launched(st, "sda_bwd_keys");
+  int e = -1;
+  if constexpr (KeyShape<Tr, D, DV, 2>::LDS <= kLds) {
+    if (halve<Tr, D, DV>(p.see, (int64_t)((p.Nk + 127) / 128) * p.B * p.Hk * parts, p.Nq)) e = keys<Tr, D, DV, 2>(p, parts, st);
+  }
+  if (e < 0) e = keys<Tr, D, DV, 1>(p, parts, st);
+  if (e) return e;
   if (p.part) {
     const int64_t n = (int64_t)p.B * p.Hk * p.Nk * ((2 * D + DV) / 4);
     bwd_sum<T, D, DV><<<tda::grid_of<256>((n + 255) / 256), 256, 0, st>>>(p, parts);
     tda::launched(st, "sda_bwd_sum");
   }
-  bwd_query<Tr, D, DV, QSPLIT><<<tda::grid_of<64 * QS::WAVES>((int64_t)((p.Nq + 127) / 128) * p.B * p.H), 64 * QS::WAVES, QS::LDS, st>>>(p);
-  tda::launched(st, "sda_bwd_query");
+  e = -1;
+  if constexpr (QueryShape<Tr, D, DV, false, 2>::LDS <= kLds) {
+    if (halve<Tr, D, DV>(p.see, (int64_t)((p.Nq + 127) / 128) * p.B * p.H, p.Nq)) e = queries<Tr, D, DV, 2>(p, st);
+  }
+  if (e < 0) e = queries<Tr, D, DV, 4>(p, st);
+  if (e) return e;
   if (p.dlam) {
     const int64_t n = p.dlam_n[0] * p.dlam_n[1] * p.dlam_n[2];
-    const int each = n == rows;
-    bwd_lambda<<<tda::grid_of<256>(each ? (n + 255) / 256 : n), 256, 0, st>>>(p, each);
+    if (p.dlam_n[2] == 1) {
+      bwd_lambda_heads<<<tda::grid_of<1024>((int64_t)p.B * p.H), 1024, 0, st>>>(p);
+      tda::launched(st, "sda_bwd_lambda_heads");
+      bwd_lambda<true><<<tda::grid_of<256>((n + 3) / 4), 256, 0, st>>>(p);
+    } else {
+      bwd_lambda<false><<<tda::grid_of<256>((n + 255) / 256), 256, 0, st>>>(p);
+    }
     tda::launched(st, "sda_bwd_lambda");
   }
   return (int)hipGetLastError();

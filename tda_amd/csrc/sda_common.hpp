@@ -321,4 +321,24 @@ __device__ __forceinline__ Item item_of(uint32_t bid, uint32_t heads, int tiles,
   return it;
 }
 
+constexpr int kLds = 160 * 1024;  // of a CU
+
+// Whether a launch of n workgroups of 128 rows (or keys) takes workgroups of 64 instead, whose waves share
+// the other axis out: where the 128s leave half of the 256 CUs' places idle, or, under a causal mask that
+// gives some of them far more work than others, where all of them are placed at once and the longest decides.
+// A CU holds one workgroup, two of bf16 (64, 64).  Forward and backward, us, whole : halved:
+//   bf16 (128, 128), 500 rows of 4355 keys, 128 workgroups   127 : 103
+//   bf16 (64, 128), (1, 8, 1024) causal, 64                   33 : 25 and 98 : 64
+//   bf16 (64, 128), (2, 16, 1024) causal, 256                 40 : 37 and 109 : 88;  all seen 43 : 50, 113 : 122
+//   bf16 (64, 128), (2, 16, 1500) causal, 384                 54 : 63 and 155 : 157
+//   bf16 (64, 64), (2, 16, 2048) causal, 512                  62 : 59 and 236 : 212;  1024: 95 : 109, 339 : 379
+//   f32 (64, 64), (2, 12, 1111) causal, 216                  157 : 94 and 455 : 274;  all seen 156 : 159, 453 : 480
+//   f32 (64, 64), (2, 16, 2048) causal, 512                  291 : 296 and 876 : 903
+template <class Tr, int D, int DV>
+inline bool halve(const Sight& see, int64_t n, int Nq) {
+  const int64_t places = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64 ? 512 : 256;
+  const bool unequal = see.causal && !see.qoffs && see.qoff < Nq / 2;
+  return n <= (unequal ? places : places / 2);
+}
+
 }  // namespace sda

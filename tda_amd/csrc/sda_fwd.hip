@@ -16,15 +16,10 @@
 
 namespace sda {
 
-// Up to this many workgroups of 128 rows, half of the 256 CUs, the launch takes 64 rows a workgroup: bf16
-// (2, 16 over 4 heads, 500 rows of 4355 keys, 128) 127 -> 103 us, (1, 16, 500 of 4355, 128) 114 -> 87 us,
-// (1, 16, 1024, 64/128) 31 -> 26 us; with 240 (1, 24, 1280 of 4096, 128) it would be 128 -> 151 us.
-constexpr int64_t kFewTiles = 128;
-
-template <class Tr, int D, int DV>
+template <class Tr, int D, int DV, int RG>
 struct FwdShape {
   using T = typename Tr::T;
-  static constexpr int BN = sizeof(T) == 2 && DV <= 128 ? 64 : 32;  // keys of a stage
+  static constexpr int BN = (sizeof(T) == 2 && DV <= 128) || RG == 2 ? 64 : 32;  // keys of a stage
   using KT = Tile<Tr, BN, D>;
   using VT = Tile<Tr, BN, DV>;
   static constexpr int STAGE = 2 * KT::BYTES + VT::BYTES;
@@ -37,7 +32,7 @@ template <class Tr, int D, int DV, int RG>
 __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
   using T = typename Tr::T;
   using frag = typename Tr::frag;
-  using S = FwdShape<Tr, D, DV>;
+  using S = FwdShape<Tr, D, DV, RG>;
   using KT = typename S::KT;
   using VT = typename S::VT;
   constexpr int BN = S::BN, NS = BN / 32 * RG / 4, NT = D / 16, NO = DV / 32;
@@ -257,7 +252,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 
 template <class Tr, int D, int DV, int RG>
 static int launch(FwdParams p, hipStream_t st) {
-  using S = FwdShape<Tr, D, DV>;
+  using S = FwdShape<Tr, D, DV, RG>;
   const void* fn = reinterpret_cast<const void*>(&fwd_tiles<Tr, D, DV, RG>);
   if (S::LDS > 65536) {
     const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
@@ -271,8 +266,8 @@ static int launch(FwdParams p, hipStream_t st) {
 }
 template <class Tr, int D, int DV>
 static int run(const FwdParams& p, hipStream_t st) {
-  if constexpr (FwdShape<Tr, D, DV>::BN == 64) {
-    if ((int64_t)((p.Nq + 127) / 128) * p.B * p.H <= kFewTiles) return launch<Tr, D, DV, 2>(p, st);
+  if constexpr (FwdShape<Tr, D, DV, 2>::LDS <= kLds) {
+    if (halve<Tr, D, DV>(p.see, (int64_t)((p.Nq + 127) / 128) * p.B * p.H, p.Nq)) return launch<Tr, D, DV, 2>(p, st);
   }
   return launch<Tr, D, DV, 4>(p, st);
 }
