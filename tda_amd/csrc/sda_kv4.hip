@@ -49,16 +49,38 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     reinterpret_cast<vec*>(p)[u] = v;
   }
 }
-// rint((x - m) / s) for m + 0.5 s boundaries decided exactly: x - m as an unevaluated sum hi + lo, the
-// nearest boundary p = (q + 1/2) s exact (q < 16, s of 8 bits), hi - p exact wherever its sign is in
-// doubt.  Ties go to the even code.
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
+// rint((x - m) / s) with ties to the even code, decided exactly: x - m as an unevaluated sum hi + lo, the
+// nearest boundary p = (q + 1/2) s exact (q < 16, s of 8 bits), hi - p exact wherever its sign is in doubt.
+__device__ __forceinline__ float exact_code(float x, float m, float s, float inv) {
   const float hi = x - m, z = hi - x, lo = (x - (hi - z)) + (-m - z);
   const float q = floorf(fminf(fmaxf(hi * inv, 0.f), 15.f));
   const float p = (q + 0.5f) * s, a = hi - p;
-  const int k = (int)q;
-  const bool up = a > -lo || (a == -lo && (k & 1));
-  return (uint32_t)min(k + (up ? 1 : 0), 15);
+  const bool up = a > -lo || (a == -lo && ((int)q & 1));
+  return fminf(q + (up ? 1.f : 0.f), 15.f);
+}
+// The same for 8 values: t = (x - m) rcp(s), the reciprocal 2^-23 off, is at most 16 * 4 * 2^-24 = 2^-18 off,
+// so its nearest integer is the code unless it lies within 2^-17 of the middle between two; 64 lanes decide
+// a value exactly where one of them does (about every seventh for bf16 rows, whose differences often are
+// odd multiples of s / 2).
+__device__ __forceinline__ void codes_of(const float (&x)[8], float m, float s, bool any, float (&c)[8]) {
+  float inv = any ? __builtin_amdgcn_rcpf(s) : 0.f, sure = 0.5f - 0x1p-17f;
+  if (__any(any && s > 0x1p120f)) {
+    asm volatile("");  // a branch: the reciprocal may have fewer bits
+    if (any && s > 0x1p120f) inv = 1.0f / s, sure = -1.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = fminf(fmaxf((x[e] - m) * inv, 0.f), 15.f);
+    c[e] = __builtin_rintf(t);
+    if (__any(fabsf(t - c[e]) > sure)) {
+      asm volatile("");
+      c[e] = any ? exact_code(x[e], m, s, inv) : 0.f;
+    }
+  }
+}
+// Four codes in 16 bits, the first lowest.
+__device__ __forceinline__ uint32_t unit(float a, float b, float c, float d) {
+  return (uint32_t)__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(d, 16.f, c), 16.f, b), 16.f, a);
 }
 
 // Place of key word u (of W / 8) in its row, and of word w of value row i (L words) of the head whose rows
@@ -69,69 +91,77 @@ __device__ __forceinline__ int64_t value_word(int64_t row0, int64_t i, int L, in
 }
 
 // ------------------------------------------------------------------ append
-// 8 lanes per group of 64 values, 8 values a lane.
-template <class T>
-__global__ void __launch_bounds__(256) kv4_append(Kv4Params P) {
+// 8 lanes per group of 64 values, 8 values a lane; a workgroup has R times 256 / (W / 8) rows of one head,
+// `blocks` workgroups the head's.  Bound by the roundings' arithmetic and the memory's rate: bf16 (4, 8, 2048,
+// 128) 21 us for 64 MB, (32, 8, 8192, 128) 441 us for 2.06 GB (4.7 TB/s).
+template <class T, int R>
+__global__ void __launch_bounds__(256) kv4_append(Kv4Params P, int blocks) {
   const int z = blockIdx.z, W = z < 2 ? P.D : P.DV, L = W / 8;  // lanes of a row
-  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
-  const int u = (int)(id % L);
-  const int64_t r = id / L;  // (b, hk, i)
-  const int i = (int)(r % P.rows);
-  const int64_t bk = r / P.rows;
-  const bool in = bk < (int64_t)P.B * P.Hk;
-  const int b = in ? (int)(bk / P.Hk) : 0, hk = in ? (int)(bk % P.Hk) : 0;
+  const int shift = W == 64 ? 3 : W == 128 ? 4 : 5;
+  const uint32_t wg = tda::grid_bid<256>(), bk = wg / (uint32_t)blocks;
+  if (bk >= (uint32_t)P.B * (uint32_t)P.Hk) return;
+  const int b = (int)(bk / (uint32_t)P.Hk), hk = (int)(bk % (uint32_t)P.Hk);
+  const int u = threadIdx.x & (L - 1), i0 = (int)(wg % (uint32_t)blocks) * R * (256 >> shift) + (threadIdx.x >> shift);
   const int start = P.start ? P.start[b] : max(P.lengths[b], 0);
   const int count = P.counts ? min(max(P.counts[b], 0), P.rows) : P.rows;
-  const int64_t at = (int64_t)start + i;
-  const bool put = in && i < count && at >= 0 && at < P.cap;
-  float x[8] = {};
-  if (put) load8(row_of<const T>(P.x[z], b, hk, i) + 8 * u, x);
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+  float xs[R][8] = {};
+  const int step = 256 >> shift;
+  const T* from = row_of<const T>(P.x[z], b, hk, i0) + 8 * u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    bad |= !(fabsf(x[e]) < __builtin_inff());
+  for (int y = 0; y < R; ++y) {
+    const int i = i0 + y * step;
+    const int64_t at = (int64_t)start + i;
+    if (i < count && at >= 0 && at < P.cap) load8(from + y * step * P.x[z].st, xs[y]);
   }
-  lo = -tda::group_max<8>(-lo);
-  hi = tda::group_max<8>(hi);
-  bad = tda::group_max<8>(bad ? 1.f : 0.f) > 0.f;
-  const uint32_t mb = bf16_bits(lo);
-  const float m = bf16_lo(mb);
-  uint32_t sb = bf16_bits((hi - m) * (1.0f / 15.0f));
-  float s = bf16_lo(sb);
-  if (!(s >= kSmallStep)) s = 0.f, sb = 0;
-  bad |= !(s < __builtin_inff()) || !(fabsf(m) < __builtin_inff());
-  const float inv = s > 0.f && !bad ? 1.0f / s : 0.f;
-  uint32_t c[8];
+  // the head's rows: within them offsets stay in 32 bits; step rows, whole fours, lie between a thread's
+  uint32_t* words = reinterpret_cast<uint32_t*>(P.codes[z]) + bk * P.cap4 * L;
+  uint32_t* pars = P.pars[z] + bk * P.cap4 * (W / 64);
+  const bool second = u & 8;
+  const uint32_t at0 = (uint32_t)(start + i0);
+  const uint32_t to = z < 2 ? at0 * L + key_place(W, u)
+                            : value_word(0, at0, L, W == 64 ? u : 16 * (u >> 4) + 2 * (u & 7) + (second ? 1 : 0));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) c[e] = inv > 0.f ? code_of(x[e], m, s, inv) : 0u;
-  const int64_t row = bk * P.cap4 + at;
-  uint32_t word;
-  int place;
-  if (z < 2) {
-    word = 0;
+  for (int y = 0; y < R; ++y) {
+    const int i = i0 + y * step;
+    const int64_t at = (int64_t)start + i;
+    const bool put = i < count && at >= 0 && at < P.cap;
+    const float (&x)[8] = xs[y];
+    float lo = x[0], hi = x[0], zero = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) word |= (c[2 * e] << (4 * e)) | (c[2 * e + 1] << (16 + 4 * e));
-    place = key_place(W, u);
-  } else {
-    const uint32_t a = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12, d = c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12;
-    if (W == 64) {
-      word = a | d << 16;
-      place = u;
-    } else {  // lanes u and u + 8 (the same columns of two groups) swap a unit
-      const bool second = u & 8;
-      const uint32_t other = (uint32_t)__shfl_xor((int)(second ? a : d), 8);
-      word = second ? other | d << 16 : a | other << 16;
-      place = 16 * (u >> 4) + 2 * (u & 7) + (second ? 1 : 0);
+    for (int e = 0; e < 8; ++e) {
+      lo = fminf(lo, x[e]);
+      hi = fmaxf(hi, x[e]);
+      zero = __builtin_fmaf(x[e], 0.f, zero);  // NaN where a value is not finite
+    }
+    if (!(zero == 0.f)) hi = __builtin_inff();  // then s is not finite either
+    lo = -tda::group_max<8>(-lo);
+    hi = tda::group_max<8>(hi);
+    const uint32_t mb = bf16_bits(lo);
+    const float m = bf16_lo(mb);
+    uint32_t sb = bf16_bits((hi - m) * (1.0f / 15.0f));
+    float s = bf16_lo(sb);
+    if (!(s >= kSmallStep)) s = 0.f, sb = 0;
+    const bool bad = !(s < __builtin_inff()) || !(fabsf(m) < __builtin_inff());
+    float c[8];
+    codes_of(x, bad ? 0.f : m, s, s > 0.f && !bad, c);
+    uint32_t word;
+    if (z < 2) {
+      word = unit(c[0], c[2], c[4], c[6]) | unit(c[1], c[3], c[5], c[7]) << 16;
+    } else {
+      const uint32_t a = unit(c[0], c[1], c[2], c[3]), d = unit(c[4], c[5], c[6], c[7]);
+      if (W == 64) {
+        word = a | d << 16;
+      } else {  // lanes u and u + 8 (the same columns of two groups) swap a unit
+        const uint32_t other = (uint32_t)__shfl_xor((int)(second ? a : d), 8);
+        word = second ? other | d << 16 : a | other << 16;
+      }
+    }
+    if (put) {
+      words[to + y * step * L] = word;
+      if ((u & 7) == 0) pars[((uint32_t)at << (shift - 3)) + (u >> 3)] = bad ? 0x7fc0u : mb | sb << 16;
     }
   }
-  if (put) {
-    reinterpret_cast<uint32_t*>(P.codes[z])[z < 2 ? row * L + place : value_word(bk * P.cap4, at, L, place)] = word;
-    if ((u & 7) == 0) P.pars[z][row * (W / 64) + u / 8] = bad ? 0x7fc0u : mb | sb << 16;
-  }
-  if (P.start && z == 0 && in && hk == 0 && i == 0 && u == 0)
+  if (P.start && z == 0 && hk == 0 && i0 == 0 && u == 0)
     P.lengths[b] = (int)min(max((int64_t)start + count, (int64_t)0), (int64_t)P.cap);
 }
 __global__ void kv4_lengths(Kv4Params P) {
@@ -142,46 +172,56 @@ __global__ void kv4_lengths(Kv4Params P) {
 }
 
 // ------------------------------------------------------------------ read
-template <class T>
-__global__ void __launch_bounds__(256) kv4_read(Kv4Params P) {
+// Lanes and workgroups as above.  bf16 (4, 8, 2048, 128): 13.5 us for 64 MB, the memory's rate.
+template <class T, int R>
+__global__ void __launch_bounds__(256) kv4_read(Kv4Params P, int blocks) {
   const int z = blockIdx.z, W = z < 2 ? P.D : P.DV, L = W / 8;
-  const int64_t id = (int64_t)tda::grid_bid<256>() * 256 + threadIdx.x;
-  const int u = (int)(id % L);
-  const int64_t r = id / L;
-  const int i = (int)(r % P.rows);
-  const int64_t bk = r / P.rows;
-  if (bk >= (int64_t)P.B * P.Hk) return;
-  const int b = (int)(bk / P.Hk), hk = (int)(bk % P.Hk);
-  float x[8] = {};
-  if (i < min(P.lengths[b], P.cap)) {
-    const int64_t row = bk * P.cap4 + i;
-    const uint32_t par = P.pars[z][row * (W / 64) + u / 8];
-    const float m = bf16_lo(par), s = bf16_hi(par);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.codes[z]);
-    if (z < 2) {
-      const uint32_t w = words[row * L + key_place(W, u)];
+  const int shift = W == 64 ? 3 : W == 128 ? 4 : 5;
+  const uint32_t wg = tda::grid_bid<256>(), bk = wg / (uint32_t)blocks;
+  if (bk >= (uint32_t)P.B * (uint32_t)P.Hk) return;
+  const int b = (int)(bk / (uint32_t)P.Hk), hk = (int)(bk % (uint32_t)P.Hk);
+  const int u = threadIdx.x & (L - 1), i0 = (int)(wg % (uint32_t)blocks) * R * (256 >> shift) + (threadIdx.x >> shift);
+  const int64_t row0 = bk * P.cap4;
+  const int held = min(min(P.lengths[b], P.cap), P.rows);
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(P.codes[z]);
+  uint32_t w0[R] = {}, w1[R] = {}, par[R] = {};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s, (float)(w >> (4 * (e >> 1) + 16 * (e & 1)) & 15), m);
+  for (int y = 0; y < R; ++y) {
+    const int i = i0 + y * (256 >> shift);
+    if (i >= held) continue;
+    const int64_t row = row0 + i;
+    par[y] = P.pars[z][row * (W / 64) + u / 8];
+    if (z < 2) {
+      w0[y] = words[row * L + key_place(W, u)];
+    } else if (W == 64) {
+      w0[y] = words[value_word(row0, i, L, u)];
     } else {
-      uint32_t a, d;  // units of columns 8 u' .. + 3 and + 4 .. + 7
-      if (W == 64) {
-        const uint32_t w = words[value_word(bk * P.cap4, i, L, u)];
-        a = w & 0xffff;
-        d = w >> 16;
-      } else {
-        const int place = 16 * (u >> 4) + 2 * (u & 7);
-        const uint32_t w0 = words[value_word(bk * P.cap4, i, L, place)], w1 = words[value_word(bk * P.cap4, i, L, place + 1)];
-        a = u & 8 ? w0 >> 16 : w0 & 0xffff;
-        d = u & 8 ? w1 >> 16 : w1 & 0xffff;
-      }
+      const int place = 16 * (u >> 4) + 2 * (u & 7);
+      w0[y] = words[value_word(row0, i, L, place)];
+      w1[y] = words[value_word(row0, i, L, place + 1)];
+    }
+  }
+#pragma unroll
+  for (int y = 0; y < R; ++y) {
+    const int i = i0 + y * (256 >> shift);
+    if (i >= P.rows) return;
+    const float m = bf16_lo(par[y]), s = bf16_hi(par[y]);  // all zero for a row that is not held
+    float x[8];
+    if (z < 2) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s, (float)(w0[y] >> (4 * (e >> 1) + 16 * (e & 1)) & 15), m);
+    } else {
+      // units of columns 8 u' .. + 3 and + 4 .. + 7
+      const uint32_t a = W > 64 && (u & 8) ? w0[y] >> 16 : w0[y] & 0xffff;
+      const uint32_t d = W == 64 ? w0[y] >> 16 : u & 8 ? w1[y] >> 16 : w1[y] & 0xffff;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[e] = __builtin_fmaf(s, (float)(a >> (4 * e) & 15), m);
         x[4 + e] = __builtin_fmaf(s, (float)(d >> (4 * e) & 15), m);
       }
     }
+    store8(row_of<T>(P.x[z], b, hk, i) + 8 * u, x);
   }
-  store8(row_of<T>(P.x[z], b, hk, i) + 8 * u, x);
 }
 
 // ------------------------------------------------------------------ attention
@@ -410,15 +450,34 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((DV <=
 }
 
 // ------------------------------------------------------------------ launches
+// Rows a thread: four where that leaves enough workgroups (bf16 (4, 8, 2048, 128) read 15.7 -> 13.5 us), one for
+// the few rows of a decoding step.
+template <class F>
+static void by_rows(const Kv4Params& p, F&& launch) {
+  const int per = 2048 / (p.D > p.DV ? p.D : p.DV);  // rows of the widest a workgroup
+  const int64_t heads = (int64_t)p.B * p.Hk;
+  const auto go = [&](auto r) {
+    const int blocks = (p.rows + per * r - 1) / (per * r);
+    dim3 grid = tda::grid_of<256>(heads * blocks);
+    grid.z = 3;
+    launch(r, grid, blocks);
+  };
+  if (heads * p.rows >= 4096 * per) go(std::integral_constant<int, 4>());
+  else go(std::integral_constant<int, 1>());
+}
+template <class T>
+static void append(const Kv4Params& p, hipStream_t st) {
+  by_rows(p, [&](auto r, dim3 grid, int blocks) { kv4_append<T, r><<<grid, 256, 0, st>>>(p, blocks); });
+}
+template <class T>
+static void read(const Kv4Params& p, hipStream_t st) {
+  by_rows(p, [&](auto r, dim3 grid, int blocks) { kv4_read<T, r><<<grid, 256, 0, st>>>(p, blocks); });
+}
 int launch_kv4_append(const Kv4Params& p, int dtype, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const int W = p.D > p.DV ? p.D : p.DV;
-  const int64_t n = (int64_t)p.B * p.Hk * p.rows * (W / 8);
-  dim3 grid = tda::grid_of<256>((n + 255) / 256);
-  grid.z = 3;
-  if (dtype == 0) kv4_append<float><<<grid, 256, 0, st>>>(p);
-  else if (dtype == 1) kv4_append<bf16><<<grid, 256, 0, st>>>(p);
-  else kv4_append<_Float16><<<grid, 256, 0, st>>>(p);
+  if (dtype == 0) append<float>(p, st);
+  else if (dtype == 1) append<bf16>(p, st);
+  else append<_Float16>(p, st);
   tda::launched(st, "sda_kv4_append");
   if (!p.start) {  // every workgroup above reads the lengths
     kv4_lengths<<<dim3((unsigned)((p.B + 63) / 64)), 64, 0, st>>>(p);
@@ -428,13 +487,9 @@ int launch_kv4_append(const Kv4Params& p, int dtype, void* stream) {
 }
 int launch_kv4_read(const Kv4Params& p, int dtype, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const int W = p.D > p.DV ? p.D : p.DV;
-  const int64_t n = (int64_t)p.B * p.Hk * p.rows * (W / 8);
-  dim3 grid = tda::grid_of<256>((n + 255) / 256);
-  grid.z = 3;
-  if (dtype == 0) kv4_read<float><<<grid, 256, 0, st>>>(p);
-  else if (dtype == 1) kv4_read<bf16><<<grid, 256, 0, st>>>(p);
-  else kv4_read<_Float16><<<grid, 256, 0, st>>>(p);
+  if (dtype == 0) read<float>(p, st);
+  else if (dtype == 1) read<bf16>(p, st);
+  else read<_Float16>(p, st);
   tda::launched(st, "sda_kv4_read");
   return (int)hipGetLastError();
 }
