@@ -2,6 +2,9 @@
 // dP = dO v^T, r_b = rowsum(dO O_b) and lambda per row:
 //   dS_1 = P_1 (dP - r_1),  dS_2 = -lambda P_2 (dP - r_2),  dq_b = s dS_b k_b,  dk_b = s dS_b^T q_b,
 //   dv = (P_1 - lambda P_2)^T dO,  dlambda_i = -r_2.
+// The outputs' weights were rounded to bf16, so r_b is off by as much; dlambda gets its r_2 from the query pass,
+// r_2 + rowsum(P_2 (dP - r_2)) of weights in f32 (bf16 (2, 16 over 4, 4096, 128): 2.4e-3 -> 1.7e-3 off, its
+// own rounding).
 // One dP and one dv product serve both branches.  r_1 comes from the outputs: dO O = r_1 - lambda r_2.
 //
 //   bwd_rows   r_1, r_2 and lambda of every row (f32)
@@ -17,7 +20,7 @@ namespace sda {
 
 // ------------------------------------------------------------------ row sums
 // What the passes need of a row, so that it enters their products as a starting value: the log-sums as
-// -lse_b / c (score and weight: P = 2^(c (q k - lse / c))), -r_1, r_1 - r_2, -lambda; and r_2 for dlambda.
+// -lse_b / c (score and weight: P = 2^(c (q k - lse / c))), -r_1, r_1 - r_2, -lambda.
 // 16 lanes per row, 16 rows per workgroup.
 template <class T, int DV>
 __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
@@ -53,7 +56,6 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
     P.stat[2 * rows + row] = -r1;
     P.stat[3 * rows + row] = r1 - ry;
     P.stat[4 * rows + row] = -lam;
-    P.stat[5 * rows + row] = ry;
   }
 }
 
@@ -517,6 +519,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     rs[x] = row ? -P.stat[2 * rows + at0] - (z ? P.stat[3 * rows + at0] : 0.f) : 0.f;
   }
   if (row) lam = -P.stat[4 * rows + at0];
+  float more = 0.f;  // rowsum(P_2 (dP - r_2))
   f32x16 dq[NB][D / 32] = {};
   if constexpr (!SPLIT) {
     pin(dq[0]);
@@ -543,17 +546,24 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     for (int x = 0; x < NB; ++x) {
       const int z = SPLIT ? br : x, kt = AT + x * KT::BYTES;
       f32x16 s = chain<Tr, NT>([&](int t) { return kr.read(kbuf, kt, t); }, qf[x]);
-      const float f = z ? -lam : 1.f;
+      const float f = -lam;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = exp2_(__builtin_fmaf(s[r], P.c, -lse[x]));
-        s[r] = f * (p * (dp[r] - rs[x]));
+        s[r] = p * (dp[r] - rs[x]);
       }
       if (k0 + 32 > clear) {
         asm volatile("");  // a branch: few tiles need this
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (k0 + crow(r, g) >= see) s[r] = 0.f;
+      }
+      if (z) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          more += s[r];
+          s[r] *= f;
+        }
       }
       const frag e[2] = {pack8<Tr>(s, 0), pack8<Tr>(s, 1)};
       columns<Tr, D / 32>([&](int u, int y) { return kc.read(kbuf, kt, u, y); }, e, dq[x]);
@@ -567,14 +577,19 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
   if constexpr (KH == 2) {  // the second half's sums join the first's
     constexpr int N = NB * D / 32 * 4;
     f32x4* x4 = reinterpret_cast<f32x4*>(lds) + wv % (NW / KH) * (N * 64) + l;
+    float* xm = reinterpret_cast<float*>(lds + NW / KH * N * 1024) + wv % (NW / KH) * 64 + l;
+    static_assert(NW / KH * (N * 1024 + 256) <= S::LDS, "the second half's sums fit");
     __syncthreads();
-    if (kh)
+    if (kh) {
+      *xm = more;
       times<N>([&](auto i) {
         constexpr int x = i / 4 / (D / 32), y = i / 4 % (D / 32), r = 4 * (i % 4);
         x4[i * 64] = f32x4{dq[x][y][r], dq[x][y][r + 1], dq[x][y][r + 2], dq[x][y][r + 3]};
       });
+    }
     __syncthreads();
     if (kh) return;
+    more += *xm;
     times<N>([&](auto i) {
       constexpr int x = i / 4 / (D / 32), y = i / 4 % (D / 32), r = 4 * (i % 4);
       const f32x4 w = x4[i * 64];
@@ -582,7 +597,9 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
       for (int e = 0; e < 4; ++e) dq[x][y][r + e] += w[e];
     });
   }
+  more += __shfl_xor(more, 32);
   if (!row) return;
+  if ((!SPLIT || br) && g == 0) P.stat[5 * rows + at0] = rs[NB - 1] + more;
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
     T* to = row_of<T>(P.dq[SPLIT ? br : x], b, h, qi) + 4 * g;
@@ -656,7 +673,9 @@ static int keys(const BwdParams& p, int parts, hipStream_t st) {
 }
 template <class Tr, int D, int DV, int RG>
 static int queries(const BwdParams& p, hipStream_t st) {
-  constexpr bool SPLIT = sizeof(typename Tr::T) == 2 ? D == 128 : DV <= 64;
+  // A wave for each branch where both branches' registers leave no room for the rest: bf16 (128, 128) 297 us
+  // against 314 for the whole backward of (2, 16, 2048); (128, 256) 505 against 473, f32 (64, 64) 946 against 880.
+  constexpr bool SPLIT = sizeof(typename Tr::T) == 2 && D == 128 && DV == 128;
   using S = QueryShape<Tr, D, DV, SPLIT, RG>;
   if (const int e = big_lds(&bwd_query<Tr, D, DV, SPLIT, RG>, S::LDS)) return e;
   bwd_query<Tr, D, DV, SPLIT, RG><<<tda::grid_of<64 * S::WAVES>((int64_t)((p.Nq + 32 * RG - 1) / (32 * RG)) * p.B * p.H), 64 * S::WAVES, S::LDS, st>>>(p);

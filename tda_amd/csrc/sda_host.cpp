@@ -94,9 +94,18 @@ sda::Lambda lambda_of(const void* p, const int64_t (&s)[3], int32_t dtype) {
   return {p, s[0], s[1], s[2], dtype == TDA_DTYPE_BF16 ? 1 : 0};
 }
 
-// Few query rows go to the kernels that cut the key axis: a 128-row workgroup would be mostly empty.
-// They read the cache once per 16 rows.
-bool few_rows(int64_t heads, int64_t kv_heads, int64_t seq_len) { return heads / kv_heads * seq_len <= 32 || seq_len <= 4; }
+// Few query rows go to the kernels that cut the key axis and read it once per 16 rows of the heads that share
+// a key head (a tile): where one tile holds them all, where 64 tiles are all there is, or where the other
+// form would read the keys twice as often, once per 128 rows of each query head.  bf16, widths of 128, us, these
+// kernels : the others, (batch, heads, kv_heads, rows, keys):
+//   (16, 32, 32, 16, 4096) 316 : 352    (16, 32, 32, 32, 4096) 469 : 338    (1, 32, 32, 32, 4096) 52 : 87
+//   (1, 16, 4, 8, 4096) 20 : 67         (1, 16, 4, 64, 4096) 52 : 68        (1, 16, 4, 256, 4096) 103 : 69
+//   (32, 32, 8, 8, 8192) 495 : 1040     (32, 32, 8, 16, 8192) 938 : 1028    (4, 32, 8, 16, 1024) 44 : 25
+//   (64, 64, 1, 4, 8192) 548 : 3390     (4, 16, 4, 64, 2048) 69 : 40        (1, 8, 8, 64, 512) 15 : 17
+bool few_rows(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len) {
+  const int64_t g = heads / kv_heads, tiles = ceil_div(g * seq_len, 16);
+  return tiles == 1 || batch * kv_heads * tiles <= 64 || 2 * tiles <= g * ceil_div(seq_len, 128);
+}
 
 int64_t dec_items(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len) {
   return batch * kv_heads * ceil_div(heads / kv_heads * seq_len, 16);
@@ -119,15 +128,17 @@ int64_t dec_bytes(int64_t items, int nsplit, int64_t dv) {
 }
 
 bool decodes(const sda_fwd_args& a) {
-  return !a.out2.data && !a.lse && few_rows(a.heads, a.kv_heads, a.seq_len);
+  return !a.out2.data && !a.lse && few_rows(a.batch, a.heads, a.kv_heads, a.seq_len);
 }
 
 // Query heads that a workgroup of the key pass sums over: all that share a key head, or fewer where
-// that leaves under 1024 workgroups (four a CU; causal ones are of unequal length).
+// that leaves under 512 workgroups (two a CU; causal ones are of unequal length).  Backward of bf16 (B, 16 over
+// 4, 4096, 128): B = 2 1031 us (all four 1017, one 1033), B = 4 1923 (one 2001), B = 1 552 (all 760); (1, 32 over
+// 1, 4096, 128) 957 us (at least 1024 workgroups 993, all 4468).
 int64_t key_group(const sda_bwd_args& a) {
   const int64_t G = a.heads / a.kv_heads, base = a.batch * a.kv_heads * ceil_div(a.seq_len_kv, 128);
   for (int64_t gs = G; gs > 1; --gs)
-    if (G % gs == 0 && base * (G / gs) >= 1024) return gs;
+    if (G % gs == 0 && base * (G / gs) >= 512) return gs;
   return 1;
 }
 int64_t stat_bytes(const sda_bwd_args& a) { return round256(6 * a.batch * a.heads * a.seq_len * 4); }

@@ -44,7 +44,7 @@ struct BwdParams {
   int B, H, Hk, Nq, Nk;
   float c, scale;
   const float* lse;  // [2][B*H*Nq]
-  float* stat;       // [6][B*H*Nq]: what the passes need of a row (bwd_rows)
+  float* stat;       // [6][B*H*Nq]: what the passes need of a row (bwd_rows), and r_2 (bwd_query)
   float* part;       // may be null: dk1, dk2, dv of each group of gs query heads, f32
   int gs;            // query heads a workgroup of the key pass sums over
   void* dlam;        // may be null

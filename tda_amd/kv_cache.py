@@ -16,7 +16,16 @@ _LENGTHS = _sda_abi.SdaKv4AttendArgs.cache.offset + _sda_abi.SdaKv4.lengths.offs
 _ATTEND_OFF = {n: getattr(_sda_abi.SdaKv4AttendArgs, n).offset for n in ("q1", "q2", "out", "lambda_param", "workspace")}
 _APPEND_OFF = {n: getattr(_sda_abi.SdaKv4AppendArgs, n).offset for n in ("k1", "k2", "v", "start", "counts")}
 _READ_OFF = {n: getattr(_sda_abi.SdaKv4ReadArgs, n).offset for n in ("k1", "k2", "v")}
-_FEW = 32  # query rows that share a key head: up to here attend() reads the codes themselves
+
+
+def _from_codes(batch: int, kv_heads: int, rows: int, dtype) -> bool:
+    """Whether attend() computes `rows` query rows for each key head from the codes, 16 rows a pass over them, or
+    reads the rows out first, for the attention that passes over them once per 128 (in float32 for a
+    float16 or float32 query).  us, codes : rows, (batch, heads, kv_heads, n, keys) of width 128, bf16:
+    (8, 16, 4, 16, 4096) 38 : 108, (32, 32, 8, 32, 4096) 344 : 767, (16, 8, 8, 128, 4096) 178 : 238,
+    (16, 8, 8, 256, 4096) 331 : 261, (1, 16, 4, 256, 4096) 60 : 94, (1, 16, 4, 512, 4096) 92 : 96; float32:
+    (8, 8, 8, 128, 4096) 255 : 1257."""
+    return rows <= (128 if dtype == torch.bfloat16 else 512) or batch * kv_heads * -(-rows // 16) <= 256
 
 
 class Int4KVCache:
@@ -152,8 +161,8 @@ class Int4KVCache:
         (A group of values that is not finite reaches the rows that see it, and may reach other rows of
         the same call that stand before it.)
 
-        Few rows (n heads / kv_heads <= 32, as in decoding) are computed from the codes; more, as a
-        prompt's chunk, from the rows that read() gives in q1's dtype."""
+        The rows of a decoding step or of a short chunk are computed from the codes; those of a long
+        one from the rows that read() gives in q1's dtype."""
         b, hk = self.batch, self.kv_heads
         if isinstance(q1, torch.Tensor) and q1.dim() == 4:
             h, n = q1.shape[1], q1.shape[2]
@@ -165,7 +174,7 @@ class Int4KVCache:
         lam = _lambda(lambda_param, b, h, n, self.device).detach()
         if n == 0:
             return torch.zeros((b, h, 0, self.v_head_dim), dtype=q1.dtype, device=self.device)
-        if h // hk * n > _FEW:
+        if not _from_codes(b, hk, h // hk * n, q1.dtype):
             with torch.no_grad():
                 rows = self.read(dtype=q1.dtype)  # checks lengths
                 lens = self.lengths.clamp(0, self.capacity)

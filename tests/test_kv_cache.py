@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import tda_amd
+from tda_amd.kv_cache import _from_codes
 from oracle import softmax as oracle
 
 BF, F32, F16 = torch.bfloat16, torch.float32, torch.float16
@@ -151,7 +152,7 @@ def around(c, q1, q2, lam):
 @pytest.mark.parametrize("dtype", [BF, F32, F16])
 @pytest.mark.parametrize("d, dv", DIMS)
 @pytest.mark.parametrize("h, hk, n, cap", [(1, 1, 1, 1), (8, 8, 1, 1000), (8, 2, 1, 33), (40, 2, 1, 300), (4, 4, 4, 129),
-                                           (6, 3, 7, 520), (4, 2, 16, 2000), (4, 1, 70, 300)])
+                                           (6, 3, 7, 520), (4, 2, 16, 2000), (4, 1, 70, 300), (16, 1, 300, 300)])
 def test_attend(dtype, d, dv, h, hk, n, cap):
     c = tda_amd.Int4KVCache(3, hk, cap, d, dv)
     c.append(*context(3, hk, cap, d, dv, dtype))
@@ -160,7 +161,7 @@ def test_attend(dtype, d, dv, h, hk, n, cap):
     lam = torch.linspace(-0.5, 0.9, h).cuda()
     got = c.attend(q1, q2, lam)
     assert got.dtype == dtype and not got[2].any()
-    if h // hk * n > 32:  # by way of read(): the values rounded to the queries' type
+    if not _from_codes(3, hk, h // hk * n, dtype):  # by way of read(): the values rounded to the queries' type
         ks = c.read(dtype=dtype)
         want = tda_amd.differential_attention(q1, q2, *ks, lam, q_offset=c.lengths - n, kv_lens=c.lengths)
         assert torch.equal(got, want)
