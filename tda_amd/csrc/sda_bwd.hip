@@ -13,7 +13,10 @@
 //   bwd_sum    adds the key pass' partial sums where several workgroups share a key head
 //   bwd_lambda sums dlambda over the axes lambda is broadcast along
 // Both passes recompute the weights from the forward's log-sums: no atomics, so results do not depend
-// on the order of execution.
+// on the order of execution.  Bound by the matrix cores and, for narrow keys, the vector work between the
+// products.  bf16: (4, 16, 2048, 64/128) keys 267 us (0.51 PFLOP/s), queries 147 (0.70), rows 29, lambda 9;
+// (2, 16 over 4, 4096, 128) keys 577 (0.71), sum 21, queries 416 (0.83), rows 33.  f32 (2, 12, 1111, 64) keys
+// 141, queries 116 (0.08 PFLOP/s of 0.15).
 #include "sda_common.hpp"
 
 namespace sda {
@@ -60,9 +63,15 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
 }
 
 // ------------------------------------------------------------------ key-major pass
-// Whether two workgroups of the key pass fit a CU (two waves a SIMD).
+// A workgroup has 4 waves: RH = 1 of 32 keys each, which walk the query rows that see them 32 at a time, or
+// RH = 2 (few workgroups) pairs of waves on 32 keys, one on every other 32 rows, whose sums meet in LDS.
+//
+// Two workgroups of the narrowest key pass fit a CU (two waves a SIMD): the whole backward of bf16 (4, 16, 2048,
+// 64) 374 -> 343 us.
 template <class Tr, int D, int DV>
 constexpr bool kKeyTwo = sizeof(typename Tr::T) == 2 && D == 64 && DV == 64;
+// The branches one after the other with fewer registers: for two waves a SIMD, and where the sequence of both
+// would spill (backward of bf16 (4, 16, 2048, 128/256) 1556 -> 958 us, f32 (2, 16, 2048, 64/128) 1104 -> 1033).
 template <class Tr, int D, int DV>
 constexpr bool kKeyLean = kKeyTwo<Tr, D, DV> || (sizeof(typename Tr::T) == 2 ? DV == 256 : DV >= 128);
 
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // The same for two waves a SIMD, which cover each other: fewer registers, the branches one after the other.
+  // The same with fewer registers: the branches one after the other.
   auto lean = [&](int i0, auto half) {
     constexpr int AT = half * S::STAGE;
     const bool edge = P.see.causal && off + i0 < k0w + 31;
@@ -440,6 +449,8 @@ __global__ void __launch_bounds__(256) bwd_sum(BwdParams P, int parts) {
 }
 
 // ------------------------------------------------------------------ query-major pass
+// A workgroup has RG groups of 32 query rows, a wave for each (SPLIT: and for each branch); with RG = 2 (few
+// workgroups) two such sets take alternate tiles of 32 keys, and their sums meet in LDS.
 template <class Tr, int D, int DV, bool SPLIT, int RG>
 struct QueryShape {
   using KT = Tile<Tr, 32, D>;

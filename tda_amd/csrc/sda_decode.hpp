@@ -6,10 +6,12 @@
 // that hold them: of a tile of 32 keys the second product takes, from lane quarter kq, keys 4 kq + j
 // and 16 + 4 kq + j (j = 0 .. 3), and the value fragments are read in that order.  Nothing is staged:
 // every key and value byte is used by one wave alone and goes straight to its registers.  Bound by
-// reading the cache.  The waves' sums meet in LDS, the parts' in a second launch.
+// reading the cache: one token over bf16 (32, 32 over 8, 8192, 128) of unequal lengths, 1.22 GB, 253 us and
+// 4.5 us for the join (4.8 TB/s; a copy reaches 5.2).  The waves' sums meet in LDS, the parts' in a second
+// launch.
 //
-// A source (Src) brings: D, DV, `Regs` (a tile's loads) and NBUF, load, scores, add (O += V^T P^T), finish and column (the output column of value r of tile t in lane
-// quarter kq).
+// A source (Src) brings: D, DV, `Regs` (a tile's loads) and NBUF, load, scores, rescale (a branch's running
+// maximum moved), add (O += V^T P^T), finish and column (the output column of value m of tile t).
 #pragma once
 
 #include "sda_common.hpp"
@@ -23,7 +25,7 @@ struct DecParams {
   int tail;      // 1: the rows are the last Nq positions before len (off = len - Nq)
   int B, H, Hk, Nq, Nk, D, DV;
   float c;
-  float* part;   // per (b, hk, row tile, split): m, l of 2 branches x 16 rows, then 2 x DV x 16 sums
+  float* part;   // per (b, hk, row tile, split): [branch][m, l][16 rows], then sums [branch][row][DV]
   int nsplit, chunk;
 };
 constexpr int kDecRows = 16;
@@ -172,7 +174,7 @@ template <int DV>
 constexpr int kDecLds = (4 * 16 * kDecRow<DV> + 256 + 32) * 4;
 
 // Joins the parts: a thread per value, the parts in order, eight at a time (their loads are on their way
-// together).
+// together: eight parts of (32, 32, 1, 128) 4.5 us, 11.4 us one at a time).
 template <class T>
 __global__ void __launch_bounds__(256) decode_join(DecParams P) {
   const int G = P.H / P.Hk, R = G * P.Nq, tiles = (R + kDecRows - 1) / kDecRows, DV = P.DV;
