@@ -27,7 +27,7 @@ extern "C" {
 
 /* error codes beyond those of tda.h */
 #define SDA_ERR_HEADS   -20  /* heads not a multiple of kv_heads */
-#define SDA_ERR_SCALE   -21  /* scale not finite and positive */
+#define SDA_ERR_SCALE   -21  /* scale not in 1e-30 .. 1e30 */
 #define SDA_ERR_AXES    -22  /* axes, sections or rotated width out of range */
 #define SDA_ERR_CACHE   -23  /* 4-bit cache: capacity, lengths or row count out of range */
 
@@ -38,7 +38,7 @@ typedef struct sda_fwd_args {
   int32_t abi_version;      /* SDA_ABI_VERSION */
   int32_t dtype;            /* TDA_DTYPE_F32 or TDA_DTYPE_BF16: q, k, v, out */
   int32_t causal;           /* 1: keys behind the row's own position are hidden */
-  float   scale;            /* s > 0 */
+  float   scale;            /* s, 1e-30 .. 1e30 */
   int64_t batch, heads, kv_heads;   /* query head h reads key head h / (heads / kv_heads) */
   int64_t seq_len, seq_len_kv;      /* query rows, key rows */
   int64_t head_dim, v_head_dim;     /* (64, 64), (64, 128), (128, 128) or (128, 256) */

@@ -1,7 +1,6 @@
 // sda_host.cpp -- C ABI of the softmax differential attention operators (include/sda.h): argument
 // validation, buffer sizing and dispatch.  Every argument that lies in host memory is checked here
 // before any launch; lengths and offsets in device memory are clamped by the kernels.
-#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <initializer_list>
@@ -44,6 +43,8 @@ int32_t check_lambda(const void* p, const int64_t (&s)[3], int32_t dtype) {
     if (x < 0 || x > kMaxStride) return TDA_ERR_LAYOUT;
   return reinterpret_cast<uintptr_t>(p) % bytes_of(dtype) ? TDA_ERR_LAYOUT : TDA_OK;
 }
+// The kernels take scale log2(e) and its reciprocal in 32 bits.
+bool check_scale(float s) { return s >= 1e-30f && s <= 1e30f; }
 // Optional arrays of 4-byte elements.
 int32_t check_words(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
@@ -75,7 +76,7 @@ int32_t check_common(const A& a) {
   if (a.abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
   if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16) return TDA_ERR_DTYPE;
   if (a.causal != 0 && a.causal != 1) return TDA_ERR_CAUSAL;
-  if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return SDA_ERR_SCALE;
+  if (!check_scale(a.scale)) return SDA_ERR_SCALE;
   if (int32_t rc = check_sizes(a)) return rc;
   if (!a.q_offsets && (a.q_offset < -kMaxPos || a.q_offset > kMaxPos - a.seq_len)) return TDA_ERR_OFFSET;
   if (int32_t rc = check_words({a.q_offsets, a.kv_lens, a.lse})) return rc;
@@ -215,7 +216,7 @@ int32_t sda_abi_version(void) { return SDA_ABI_VERSION; }
 const char* sda_error_string(int32_t code) {
   switch (code) {
     case SDA_ERR_HEADS: return "heads must be a multiple of kv_heads";
-    case SDA_ERR_SCALE: return "scale must be finite and positive";
+    case SDA_ERR_SCALE: return "scale must be finite and positive (1e-30 to 1e30)";
     case SDA_ERR_AXES: return "axes, sections or rotated width out of range";
     case SDA_ERR_CACHE: return "4-bit cache: capacity, lengths or row count out of range";
     case TDA_ERR_HEAD_DIM: return "(head_dim, v_head_dim) must be (64, 64), (64, 128), (128, 128) or (128, 256)";
@@ -433,7 +434,7 @@ int32_t sda_validate_kv4_attend(const sda_kv4_attend_args* a) {
   if (a->abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
   if (!any_dtype(a->dtype)) return TDA_ERR_DTYPE;
   if (int32_t rc = check_cache(a->cache)) return rc;
-  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return SDA_ERR_SCALE;
+  if (!check_scale(a->scale)) return SDA_ERR_SCALE;
   if (int32_t rc = check_attend_sizes(*a)) return rc;
   if (int32_t rc = check_lambda(a->lambda_param, a->lambda_stride, a->lambda_dtype)) return rc;
   for (const tda_tensor* t : {&a->q1, &a->q2, &a->out})

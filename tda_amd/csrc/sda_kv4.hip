@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P, int blocks) {
   uint32_t* words = reinterpret_cast<uint32_t*>(P.codes[z]) + bk * P.cap4 * L;
   uint32_t* pars = P.pars[z] + bk * P.cap4 * (W / 64);
   const bool second = u & 8;
-  const uint32_t at0 = (uint32_t)(start + i0);
+  const uint32_t at0 = (uint32_t)start + (uint32_t)i0;
   const uint32_t to = z < 2 ? at0 * L + key_place(W, u)
                             : value_word(0, at0, L, W == 64 ? u : 16 * (u >> 4) + 2 * (u & 7) + (second ? 1 : 0));
 #pragma unroll

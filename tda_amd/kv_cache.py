@@ -33,7 +33,7 @@ class Int4KVCache:
 
     Every row is held in groups of 64 values x as m = bf16(min x), s = bf16((max x - m) * (1 / 15)) (in 32
     bits) and codes rint((x - m) / s) in 0 .. 15 (ties to even; all 0 when s < 2^-100); it stands for m + s
-    code.  A group with a NaN or an infinity reads as NaN.  (head_dim, v_head_dim): (64, 64), (64, 128), (128, 128) or (128, 256).
+    code.  A group with a NaN or an infinity reads as NaN.  (head_dim, v_head_dim): (64, 64), (64, 128), (128, 128) or (128, 256).  capacity is at most 2^24.
 
     `lengths` (int32, (batch,), on the device) counts the rows each sequence holds; the calls read and
     write it on the GPU, without synchronising, so they can be captured into a graph.  A program may set
@@ -55,8 +55,10 @@ class Int4KVCache:
         self.batch, self.kv_heads, self.capacity = int(batch), int(kv_heads), int(capacity)
         self.head_dim, self.v_head_dim, self.device = int(head_dim), int(v_head_dim), device
         lib = _sda_abi.load()
-        self._held = [torch.empty(lib.sda_kv4_bytes(batch, kv_heads, capacity, w), dtype=torch.uint8, device=device)
-                      for w in (head_dim, head_dim, v_head_dim)]
+        sizes = [lib.sda_kv4_bytes(batch, kv_heads, capacity, w) for w in (head_dim, head_dim, v_head_dim)]
+        if not all(sizes):
+            raise ValueError(f"capacity must be at most 2^24 and batch kv_heads below 2^30, got {batch}, {kv_heads}, {capacity}")
+        self._held = [torch.empty(n, dtype=torch.uint8, device=device) for n in sizes]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self._templates: dict = {}
 

@@ -187,7 +187,8 @@ class DifferentialAttention(nn.Module):
 
         With a cache, x are the next seq_len positions of each sequence: their keys and values are appended
         and the attention runs over all that the cache holds, without gradients; positions count from
-        the cache's lengths by default.  A prompt padded at its end is decoded on from after cache.lengths
+        the cache's lengths by default.  Rows past the cache's capacity are dropped, as append() drops them: a
+        caller keeps count.  A prompt padded at its end is decoded on from after cache.lengths
         is set to the sequences' own lengths."""
         if x.dim() != 3 or x.shape[-1] != self.embed_dim:
             raise ValueError(f"x must have shape (batch, seq_len, {self.embed_dim}), got {tuple(x.shape)}")

@@ -81,8 +81,8 @@ def _check_heads(heads: int, kv_heads: int):
 
 def _scale(scale, d: int) -> float:
     s = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < s < float("inf"):
-        raise ValueError(f"scale must be finite and positive, got {s}")
+    if not 1e-30 <= s <= 1e30:  # s log2(e) and its reciprocal stay in 32 bits
+        raise ValueError(f"scale must be finite and positive (1e-30 to 1e30), got {s}")
     return s
 
 
@@ -260,7 +260,7 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     place, others are padded with zeros.
 
     lambda_param: a float, or a tensor that is a scalar, (heads,) or broadcasts to (batch, heads,
-    seq_len); unclamped, differentiable.  scale: default 1 / sqrt(head_dim).
+    seq_len); unclamped, differentiable.  scale: default 1 / sqrt(head_dim); 1e-30 to 1e30.
 
     M: row i of sequence b stands at position q_offset + i (q_offset an int, by default
     max(seq_len_kv - seq_len, 0), or an int32/int64 tensor (batch,), which may be negative).  With

@@ -133,7 +133,7 @@ static void attention() {
   REFUSES(fwd_args(), sda_validate_fwd, a.abi_version = 7, TDA_ERR_ABI);
   REFUSES(fwd_args(), sda_validate_fwd, a.dtype = SDA_DTYPE_F16, TDA_ERR_DTYPE);
   REFUSES(fwd_args(), sda_validate_fwd, a.causal = 2, TDA_ERR_CAUSAL);
-  for (float s : {0.f, -1.f, std::nanf(""), std::numeric_limits<float>::infinity()})
+  for (float s : {0.f, -1.f, std::nanf(""), std::numeric_limits<float>::infinity(), 1e-31f, 1e31f})
     REFUSES(fwd_args(), sda_validate_fwd, a.scale = s, SDA_ERR_SCALE);
   REFUSES(fwd_args(), sda_validate_fwd, a.kv_heads = 3, SDA_ERR_HEADS);
   REFUSES(fwd_args(), sda_validate_fwd, a.v_head_dim = 96, TDA_ERR_HEAD_DIM);

@@ -328,3 +328,17 @@ def test_lengths_beyond_the_capacity(n):
     want = c.attend(q, q * 0.5, 0.5)
     c.lengths.fill_(1 << 30)
     assert torch.equal(c.attend(q, q * 0.5, 0.5), want)
+
+
+@gpu
+def test_capacity_and_starts_out_of_range():
+    with pytest.raises(ValueError, match="capacity"):
+        tda_amd.Int4KVCache(1, 1, (1 << 24) + 1, 64)
+    c = tda_amd.Int4KVCache(2, 1, 8, 64, 64)
+    xs = context(2, 1, 5, 64, 64, BF)
+    c.append(*xs)
+    want = c.read()
+    c.append(*xs, start=torch.tensor([2 ** 31 - 1, -2 ** 31]).cuda())  # nothing to write, beyond either end
+    assert c.lengths.tolist() == [8, 0]
+    c.lengths.fill_(5)
+    assert all(torch.equal(a, b) for a, b in zip(c.read(), want))

@@ -346,7 +346,7 @@ def test_captured(n, nk):
 
     def step():
         out = tda_amd.differential_attention(*xs, lam, kv_lens=lens)
-        return [out, *torch.autograd.grad(out, [*xs, lam], dout)] if n > 1 else [out]
+        return [out.detach(), *torch.autograd.grad(out, [*xs, lam], dout)] if n > 1 else [out]  # no graph outlives a step
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -417,3 +417,57 @@ def test_no_keys_and_rows_that_are_not_finite(bad):
     assert out.shape == (1, 2, 3, 64) and not out.any()
     out.sum().backward()
     assert not q.grad.any() and none.grad.shape == none.shape
+
+
+@gpu
+def test_two_threads_on_two_streams():
+    """Training steps of two threads at once, each on a stream of its own, give what they give alone."""
+    import threading
+    sets = [inputs(2, 4, 2, 300, 300, 64, 128, BF), inputs(1, 8, 8, 500, 500, 128, 128, BF)]
+    sets = [[x.detach().clone().requires_grad_() for x in xs] for xs in sets]
+
+    def step(xs):
+        out = tda_amd.differential_attention(*xs, 0.5)
+        return [out, *torch.autograd.grad(out, xs, out.detach())]
+
+    want = [step(xs) for xs in sets]
+    got, failed = [None, None], []
+    torch.cuda.synchronize()
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[k] = [step(sets[k]) for _ in range(5)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for k in range(2):
+        assert all(torch.equal(a, b) for res in got[k] for a, b in zip(res, want[k]))
+
+
+@gpu
+def test_the_same_tensors_twice():
+    """q1 = q2, k1 = k2 and lambda 1: nothing is left, and each gradient is the two branches' together."""
+    q, k, v = inputs(1, 2, 2, 200, 200, 64, 64, F32)[::2]
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    out = tda_amd.differential_attention(q, q, k, k, v, 1.0)
+    # each branch is off by its own bound: 200 terms in 24 bits
+    assert out.abs().max().item() <= 4 * 200 * 2.0 ** -24 * v.abs().max().item()
+    out.sum().backward()
+    lim = 4 * 200 * 64 * 2.0 ** -24 * v.abs().max().item() * 3
+    assert q.grad.abs().max().item() <= lim * k.abs().max().item() and k.grad.abs().max().item() <= lim * 200 * q.abs().max().item()
+
+
+@gpu
+@pytest.mark.parametrize("scale", [0.0, -1.0, math.nan, math.inf, 1e-31, 1e31])
+def test_scale_out_of_range(scale):
+    xs = inputs(1, 2, 2, 5, 5, 64, 64, BF)
+    with pytest.raises(ValueError, match="scale"):
+        tda_amd.differential_attention(*xs, 0.5, scale=scale)
