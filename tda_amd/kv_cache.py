@@ -7,8 +7,8 @@ import struct
 import torch
 
 from . import _sda_abi
-from .softmax import (_CODE, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _launch, _new_rows, _scale, _usable,
-                       differential_attention)
+from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _launch, _new_rows, _scale, _sig,
+                       _usable, differential_attention)
 
 _PUT = struct.Struct("<Q").pack_into
 _DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
@@ -60,7 +60,8 @@ class Int4KVCache:
             raise ValueError(f"capacity must be at most 2^24 and batch kv_heads below 2^30, got {batch}, {kv_heads}, {capacity}")
         self._held = [torch.empty(n, dtype=torch.uint8, device=device) for n in sizes]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
-        self._templates: dict = {}
+        self._templates: dict = {}  # argument blocks by configuration
+        self._plans: dict = {}      # of calls whose tensors need no copy, by their signature: no checks again
 
     # -------------------------------------------------------------- calls
     def _cache(self) -> _sda_abi.SdaKv4:
@@ -87,6 +88,32 @@ class Int4KVCache:
         _PUT(buf, _LENGTHS, n.data_ptr())
         return buf, got[1]
 
+    def _signature(self, *tensors):
+        """What a call's plan goes by (the lengths' form among it), or None."""
+        for t in tensors:
+            if t is not None and type(t) not in _TENSORS:
+                return None
+        return _sig(self.lengths), *[None if t is None else _sig(t) for t in tensors]
+
+    def _planned(self, key, rows):
+        """(argument block, ...) that _plan kept for calls of this signature; None where there is none, or
+        where an address does not suit the kernels."""
+        got = self._plans.get(key)
+        if got is None:
+            return None
+        for t in rows:
+            if t.data_ptr() % 16:
+                return None
+        buf = bytearray(got[0])
+        _PUT(buf, _LENGTHS, self.lengths.data_ptr())
+        return buf, *got[1:]
+
+    def _plan(self, key, *plan):
+        if key is not None:
+            if len(self._plans) > 64:
+                self._plans.clear()
+            self._plans[key] = plan
+
     def _check(self, tensors, names, shapes):
         _check_rows(tensors, names)
         for t, n, s in zip(tensors, names, shapes):
@@ -105,8 +132,14 @@ class Int4KVCache:
         (batch,)) is given, for i < counts[b] (all n by default; rows past it are padding and are not
         read); lengths[b] becomes the position behind the last one.  Positions outside 0 .. capacity - 1
         are dropped, and lengths stops at the capacity: a caller that must not lose rows keeps count."""
+        key = self._signature(k1, k2, v, start, counts)
+        plan = self._planned(key, (k1, k2, v)) if key is not None else None
+        if plan is not None:
+            self._append(plan[0], k1, k2, v, start, counts)
+            return
         n = k1.shape[2] if isinstance(k1, torch.Tensor) and k1.dim() == 4 else 0
         b, hk = self.batch, self.kv_heads
+        given = k1, k2, v, start, counts
         self._check((k1, k2, v), ("k1", "k2", "v"),
                     ((b, hk, n, self.head_dim), (b, hk, n, self.head_dim), (b, hk, n, self.v_head_dim)))
         if n > self.capacity:
@@ -117,7 +150,7 @@ class Int4KVCache:
             if start is not None:
                 self.lengths.copy_(start.clamp(0, self.capacity))
             return
-        rows = [_usable(t.detach()) for t in (k1, k2, v)]
+        rows = [_usable(t) for t in (k1, k2, v)]
 
         def build():
             a = _sda_abi.SdaKv4AppendArgs()
@@ -127,7 +160,12 @@ class Int4KVCache:
             return a
 
         buf, _ = self._template(("append", n, rows[0].dtype, tuple(t.stride() for t in rows)), build)
-        for name, t in zip(("k1", "k2", "v", "start", "counts"), (*rows, start, counts)):
+        if all(a is b for a, b in zip((*rows, start, counts), given)):
+            self._plan(key, bytes(buf))
+        self._append(buf, *rows, start, counts)
+
+    def _append(self, buf, *tensors):
+        for name, t in zip(("k1", "k2", "v", "start", "counts"), tensors):
             if t is not None:
                 _PUT(buf, _APPEND_OFF[name], t.data_ptr())
         _launch(_sda_abi.load().sda_kv4_append, _sda_abi.SdaKv4AppendArgs, buf, self.device, "sda_kv4_append")
@@ -165,6 +203,15 @@ class Int4KVCache:
 
         The rows of a decoding step or of a short chunk are computed from the codes; those of a long
         one from the rows that read() gives in q1's dtype."""
+        key = self._signature(q1, q2, lambda_param) if scale is None or type(scale) is float else None
+        if key is not None:
+            key = *key, scale
+            plan = self._planned(key, (q1, q2))
+            if plan is not None:
+                buf, size, shape, strides = plan
+                return self._attend(buf, size, q1, q2, lambda_param,
+                                    torch.empty_strided(shape, strides, dtype=q1.dtype, device=self.device))
+        given = q1, q2, lambda_param
         b, hk = self.batch, self.kv_heads
         if isinstance(q1, torch.Tensor) and q1.dim() == 4:
             h, n = q1.shape[1], q1.shape[2]
@@ -173,7 +220,7 @@ class Int4KVCache:
         self._check((q1, q2), ("q1", "q2"), ((b, h, n, self.head_dim),) * 2)
         _check_heads(h, hk)
         s = _scale(scale, self.head_dim)
-        lam = _lambda(lambda_param, b, h, n, self.device).detach()
+        lam = _lambda(lambda_param, b, h, n, self.device)
         if n == 0:
             return torch.zeros((b, h, 0, self.v_head_dim), dtype=q1.dtype, device=self.device)
         if not _from_codes(b, hk, h // hk * n, q1.dtype):
@@ -181,7 +228,7 @@ class Int4KVCache:
                 rows = self.read(dtype=q1.dtype)  # checks lengths
                 lens = self.lengths.clamp(0, self.capacity)
                 return differential_attention(q1, q2, *rows, lam, s, q_offset=lens - n, kv_lens=lens)
-        q1, q2 = _usable(q1.detach()), _usable(q2.detach())
+        q1, q2 = _usable(q1), _usable(q2)
         out = _new_rows(q1, self.v_head_dim)
         ls = _lambda_strides(lam)
 
@@ -196,8 +243,12 @@ class Int4KVCache:
             a.workspace_bytes = _sda_abi.load().sda_kv4_attend_workspace_bytes(ctypes.byref(a))
             return a
 
-        key = ("attend", h, n, s, q1.dtype, lam.dtype, ls, q1.stride(), q2.stride())
-        buf, size = self._template(key, build)
+        buf, size = self._template(("attend", h, n, s, q1.dtype, lam.dtype, ls, q1.stride(), q2.stride()), build)
+        if all(a is b for a, b in zip((q1, q2, lam), given)):
+            self._plan(key, bytes(buf), size, out.shape, out.stride())
+        return self._attend(buf, size, q1, q2, lam, out)
+
+    def _attend(self, buf, size, q1, q2, lam, out):
         ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         for name, t in zip(("q1", "q2", "out", "lambda_param", "workspace"), (q1, q2, out, lam, ws)):
             if t is not None:

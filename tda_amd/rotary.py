@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _sda_abi, ops
-from .softmax import _CODE, _launch, _new_rows
+from .softmax import _CODE, _TENSORS, _free_of_grad, _launch, _new_rows, _sig
 
 _PUT = struct.Struct("<Q").pack_into
 _OFF = {n: getattr(_sda_abi.SdaRotaryArgs, n).offset for n in ("x", "y", "positions", "inv_freq")}
@@ -21,6 +21,37 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 and t.stride(2) * t.element_size() <= 1 << 25 else t.contiguous()
 
 
+# Calls without gradients whose tensors are read in place, by signature: their argument block and the outputs'
+# strides; such a call takes fresh pointers alone.
+_plans: dict = {}
+
+
+def _block(xs, ys, positions, sections, interleaved: bool, inverse: bool) -> bytes:
+    a = _sda_abi.SdaRotaryArgs()
+    a.abi_version, a.dtype = _sda_abi.ABI_VERSION, _CODE[xs[0].dtype]
+    a.interleaved, a.inverse = int(interleaved), int(inverse)
+    a.batch, _, a.seq_len, a.head_dim = xs[0].shape
+    a.rot, a.axes, a.count = 2 * sum(sections), len(sections), len(xs)
+    a.sections[:len(sections)] = sections
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        a.heads[i] = x.shape[1]
+        a.x[i].stride[:] = x.stride()
+        a.y[i].stride[:] = y.stride()
+    a.position_stride[:] = positions.stride()
+    a.position_dtype = positions.element_size()
+    return bytes(a)
+
+
+def _run(block, xs, ys, positions, inv_freq):
+    buf = bytearray(block)
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        _PUT(buf, _OFF["x"] + i * _TENSOR, x.data_ptr())
+        _PUT(buf, _OFF["y"] + i * _TENSOR, y.data_ptr())
+    _PUT(buf, _OFF["positions"], positions.data_ptr())
+    _PUT(buf, _OFF["inv_freq"], inv_freq.data_ptr())
+    _launch(_sda_abi.load().sda_rotary, _sda_abi.SdaRotaryArgs, buf, xs[0].device, "sda_rotary")
+
+
 def _turn(xs, positions, inv_freq, sections, interleaved: bool, inverse: bool):
     """One sda_rotary launch: new tensors with xs turned (inverse: turned back)."""
     xs = [_readable(x) for x in xs]
@@ -28,28 +59,8 @@ def _turn(xs, positions, inv_freq, sections, interleaved: bool, inverse: bool):
     key = ("sda_rotary", xs[0].dtype, tuple(x.shape for x in xs), tuple(x.stride() for x in xs), positions.dtype,
            positions.stride(), sections, interleaved, inverse)
 
-    def build():
-        a = _sda_abi.SdaRotaryArgs()
-        a.abi_version, a.dtype = _sda_abi.ABI_VERSION, _CODE[xs[0].dtype]
-        a.interleaved, a.inverse = int(interleaved), int(inverse)
-        a.batch, _, a.seq_len, a.head_dim = xs[0].shape
-        a.rot, a.axes, a.count = 2 * sum(sections), len(sections), len(xs)
-        a.sections[:len(sections)] = sections
-        for i, (x, y) in enumerate(zip(xs, ys)):
-            a.heads[i] = x.shape[1]
-            a.x[i].stride[:] = x.stride()
-            a.y[i].stride[:] = y.stride()
-        a.position_stride[:] = positions.stride()
-        a.position_dtype = positions.element_size()
-        return bytes(a)
-
-    buf = bytearray(ops._cached(key, build))
-    for i, (x, y) in enumerate(zip(xs, ys)):
-        _PUT(buf, _OFF["x"] + i * _TENSOR, x.data_ptr())
-        _PUT(buf, _OFF["y"] + i * _TENSOR, y.data_ptr())
-    _PUT(buf, _OFF["positions"], positions.data_ptr())
-    _PUT(buf, _OFF["inv_freq"], inv_freq.data_ptr())
-    _launch(_sda_abi.load().sda_rotary, _sda_abi.SdaRotaryArgs, buf, xs[0].device, "sda_rotary")
+    block = ops._cached(key, lambda: _block(xs, ys, positions, sections, interleaved, inverse))
+    _run(block, xs, ys, positions, inv_freq)
     return tuple(ys)
 
 
@@ -81,6 +92,14 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
     bits.  Gradients flow to xs."""
     one = isinstance(xs, torch.Tensor)
     ts = (xs,) if one else tuple(xs)
+    key = None
+    if type(positions) is torch.Tensor and type(inv_freq) is torch.Tensor and all(type(t) in _TENSORS for t in ts):
+        key = (tuple([_sig(t) for t in ts]), _sig(positions), _sig(inv_freq), tuple(sections), bool(interleaved))
+        plan = _plans.get(key)
+        if plan is not None and _free_of_grad(inv_freq, *ts):
+            ys = tuple([torch.empty_strided(t.shape, st, dtype=t.dtype, device=t.device) for t, st in zip(ts, plan[1])])
+            _run(plan[0], ts, ys, positions, inv_freq)
+            return ys[0] if one else ys
     if not 1 <= len(ts) <= _sda_abi.MAX_ROTARY:
         raise ValueError(f"rotary_axes takes 1 to {_sda_abi.MAX_ROTARY} tensors, got {len(ts)}")
     ref = ts[0]
@@ -119,9 +138,13 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
             raise ValueError("a tensor of xs has no heads")
         res = tuple(t.clone() for t in ts)
         return res[0] if one else res
-    inv_freq = inv_freq.contiguous()
+    frequencies, inv_freq = inv_freq, inv_freq.contiguous()
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
         res = _Rotary.apply(positions, inv_freq, sections, bool(interleaved), *ts)
     else:
         res = _turn(ts, positions, inv_freq, sections, bool(interleaved), False)
+        if key is not None and inv_freq is frequencies and all(_readable(t) is t for t in ts):
+            if len(_plans) > 4096:
+                _plans.clear()
+            _plans[key] = _block(ts, res, positions, sections, bool(interleaved), False), [y.stride() for y in res]
     return res[0] if one else res

@@ -35,7 +35,9 @@ def _offsets(args, names):
     return {n: getattr(args, n).offset for n in names}
 
 
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
 _FWD_OFF = _offsets(_sda_abi.SdaFwdArgs, _FWD_ROWS + ("lambda_param", "q_offsets", "kv_lens", "lse", "workspace"))
+_PLAN_OFF = [_FWD_OFF[n] for n in ("q1", "q2", "k1", "k2", "v")]
 _BWD_OFF = _offsets(_sda_abi.SdaBwdArgs, _BWD_ROWS + ("lambda_param", "q_offsets", "kv_lens", "lse", "dlambda", "workspace"))
 
 
@@ -52,7 +54,7 @@ def _usable(t: torch.Tensor) -> torch.Tensor:
             _stride_ok.clear()
         ok = _stride_ok[st, es] = (st[3] == 1 and all(s >= 0 and s * es % 16 == 0 for s in st[:3])
                                    and st[2] * es <= _ROW_BYTES)
-    return t if ok and t.data_ptr() % 16 == 0 else t.contiguous()
+    return t if ok and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_rows(tensors, names, shapes=None):
@@ -179,6 +181,56 @@ def _template(kind, rows, names, args_type, size_fn, lam, scale, causal, q_offse
     return ops._cached(key, build)
 
 
+# A call whose tensors need no copy and no gradient depends on nothing but their layouts: once such a call
+# has passed the checks below, calls of the same signature reuse its argument block and take fresh pointers alone.
+_plans: dict = {}
+
+
+def _sig(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype, t.device
+
+
+def _free_of_grad(*tensors) -> bool:
+    return not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors)
+
+
+def _plan_key(rows, lam, scale, causal, q_offset, kv_lens):
+    """The signature of a forward call that may have a plan, or None."""
+    if type(lam) not in _TENSORS or not (q_offset is None or type(q_offset) is int) or not (scale is None or type(scale) is float):
+        return None
+    for t in rows:
+        if type(t) not in _TENSORS:
+            return None
+    if kv_lens is not None and type(kv_lens) is not torch.Tensor:
+        return None
+    q1, q2, k1, k2, v = rows
+    return (_sig(q1), _sig(q2), _sig(k1), _sig(k2), _sig(v), _sig(lam), scale, bool(causal), q_offset,
+            None if kv_lens is None else _sig(kv_lens))
+
+
+def _run_plan(plan, rows, lam, kv_lens):
+    """The planned call's output, or None where a tensor's address does not suit the kernels."""
+    tpl, size, shape, strides = plan
+    ptrs = [t.data_ptr() for t in rows]
+    for p in ptrs:
+        if p % 16:
+            return None
+    q1 = rows[0]
+    buf = bytearray(tpl)
+    out = torch.empty_strided(shape, strides, dtype=q1.dtype, device=q1.device)
+    for at, p in zip(_PLAN_OFF, ptrs):
+        _PUT(buf, at, p)
+    _PUT(buf, _FWD_OFF["out"], out.data_ptr())
+    _PUT(buf, _FWD_OFF["lambda_param"], lam.data_ptr())
+    if kv_lens is not None:
+        _PUT(buf, _FWD_OFF["kv_lens"], kv_lens.data_ptr())
+    if size:
+        ws = torch.empty(size, dtype=torch.uint8, device=q1.device)
+        _PUT(buf, _FWD_OFF["workspace"], ws.data_ptr())
+    _launch(_sda_abi.load().sda_fwd, _sda_abi.SdaFwdArgs, buf, q1.device, "sda_fwd")
+    return out
+
+
 def _launch(fn, args_type, buf, device, what):
     a = args_type.from_buffer(buf)
     if torch.cuda.current_device() == device.index:
@@ -269,6 +321,12 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     keys that no row of the call sees may hold anything.  (A NaN or infinite value row reaches the rows
     that see it, and may reach other rows of the same call that stand before it.)"""
     tensors, names = (q1, q2, k1, k2, v), ("q1", "q2", "k1", "k2", "v")
+    key = _plan_key(tensors, lambda_param, scale, causal, q_offset, kv_lens)
+    plan = _plans.get(key) if key is not None else None
+    if plan is not None and _free_of_grad(*tensors, lambda_param):
+        out = _run_plan(plan, tensors, lambda_param, kv_lens)
+        if out is not None:
+            return out
     _check_rows(tensors, names)
     if q2.shape != q1.shape:
         raise ValueError(f"shape mismatch: q1 {tuple(q1.shape)} vs q2 {tuple(q2.shape)}")
@@ -300,7 +358,16 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*rows, lam)):
         out = _DifferentialAttention.apply(*rows, lam, s, bool(causal), off, q_offsets, lens)
     else:
-        out = _forward(*(_usable(t) for t in rows), lam, s, bool(causal), off, q_offsets, lens, False)[0]
+        given = rows
+        rows = [_usable(t) for t in rows]
+        out = _forward(*rows, lam, s, bool(causal), off, q_offsets, lens, False)[0]
+        if key is not None and lam is lambda_param and lens is kv_lens and all(
+                a is b is c for a, b, c in zip(rows, given, tensors)):
+            if len(_plans) > 4096:
+                _plans.clear()
+            tpl, size = _template("sda_fwd", (q1, k1, q2, k2, v, out, None, None), _FWD_ROWS, _sda_abi.SdaFwdArgs,
+                                  "sda_fwd_workspace_bytes", lam, s, bool(causal), off, (False,))
+            _plans[key] = tpl, size, out.shape, out.stride()
     if kv != dv:
         out = out[..., :dv]
     return out if out.dtype == q1.dtype else out.to(q1.dtype)

@@ -342,3 +342,30 @@ def test_capacity_and_starts_out_of_range():
     assert c.lengths.tolist() == [8, 0]
     c.lengths.fill_(5)
     assert all(torch.equal(a, b) for a, b in zip(c.read(), want))
+
+
+@gpu
+def test_calls_of_one_signature_take_their_own_tensors():
+    c, d = (tda_amd.Int4KVCache(2, 1, 64, 64, 64) for _ in range(2))
+    for k in range(3):
+        xs = context(2, 1, 3, 64, 64, BF, seed=10 * k)
+        starts = torch.tensor([3 * k, 2 * k], dtype=torch.int32).cuda()  # no row is left unwritten
+        c.append(*xs, start=starts)
+        d.append(*xs, start=starts.long())  # another signature
+        assert all(torch.equal(a, b) for a, b in zip(c.read(), d.read())) and torch.equal(c.lengths, d.lengths)
+        q1, q2 = rows(2, 2, 1, 64, 40 + k, BF), rows(2, 2, 1, 64, 50 + k, BF)
+        lam = torch.tensor([0.3, 0.1 * k]).cuda()
+        assert torch.equal(c.attend(q1, q2, lam), d.attend(q1, q2, lam.double()))
+    off = torch.empty(q1.numel() + 1, dtype=BF, device="cuda")[1:].view_as(q1).copy_(q1)
+    assert torch.equal(c.attend(off, q2, lam), c.attend(q1, q2, lam))
+    c.lengths = d.lengths.clone()
+    c.lengths.fill_(4)
+    d.lengths.fill_(4)
+    assert torch.equal(c.attend(q1, q2, lam), d.attend(q1, q2, lam))
+    c.lengths = c.lengths.long()
+    with pytest.raises(ValueError, match="lengths"):
+        c.attend(q1, q2, lam)
+    with pytest.raises(ValueError):
+        d.attend(q1, q2, lam[:1].expand(3))
+    with pytest.raises(ValueError):
+        d.append(xs[0], xs[1].cpu(), xs[2])

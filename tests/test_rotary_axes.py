@@ -135,3 +135,23 @@ def test_refusals(change):
         freq = freq.detach().requires_grad_(True)
     with pytest.raises(ValueError):
         tda_amd.rotary_axes(x, pos, freq, change.get("sections", (32,)))
+
+
+@gpu
+def test_calls_of_one_signature_take_their_own_tensors():
+    for k in range(3):
+        g = torch.Generator().manual_seed(k)
+        xs = [torch.randn(2, h, 5, 64, generator=g).cuda() for h in (4, 2)]
+        pos, freq = torch.randint(0, 99, (1, 2, 5), generator=g).cuda(), torch.rand(32, generator=g).cuda()
+        got = tda_amd.rotary_axes(xs, pos, freq, (32,))
+        want = tda_amd.rotary_axes(xs, pos.int(), freq, (32,))  # another signature
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(tda_amd.rotary_axes(xs[0], pos, freq, (32,)), got[0])
+    xs[0].requires_grad_()
+    assert tda_amd.rotary_axes(xs, pos, freq, (32,))[0].requires_grad
+    with torch.no_grad():
+        assert not tda_amd.rotary_axes(xs, pos, freq, (32,))[0].requires_grad
+    with pytest.raises(ValueError):
+        tda_amd.rotary_axes([xs[0], xs[1].half()], pos, freq, (32,))
+    with pytest.raises(ValueError):
+        tda_amd.rotary_axes(xs, pos, freq, (31,))

@@ -428,7 +428,7 @@ def test_two_threads_on_two_streams():
 
     def step(xs):
         out = tda_amd.differential_attention(*xs, 0.5)
-        return [out, *torch.autograd.grad(out, xs, out.detach())]
+        return [out.detach(), *torch.autograd.grad(out, xs, out.detach())]
 
     want = [step(xs) for xs in sets]
     got, failed = [None, None], []
@@ -471,3 +471,34 @@ def test_scale_out_of_range(scale):
     xs = inputs(1, 2, 2, 5, 5, 64, 64, BF)
     with pytest.raises(ValueError, match="scale"):
         tda_amd.differential_attention(*xs, 0.5, scale=scale)
+
+
+@gpu
+def test_calls_of_one_signature_take_their_own_tensors():
+    """A repeated call is the first one's with other addresses, lambdas and lengths; what differs is checked."""
+    for n, nk in ((1, 700), (40, 300)):
+        lam = torch.tensor([0.2, 0.5, 0.7, 0.9]).cuda()
+        want = []
+        for fresh in (False, True):
+            for k in range(3):
+                xs = [rows((2, h, m, 64), 10 * k + j, BF) for j, (h, m) in enumerate(((4, n), (4, n), (2, nk), (2, nk), (2, nk)))]
+                lens = torch.tensor([nk - k, nk // (k + 2)], dtype=torch.int32).cuda()
+                if fresh:  # another signature: the lengths in 64 bits
+                    assert torch.equal(tda_amd.differential_attention(*xs, lam * k, kv_lens=lens.long()), want[k])
+                else:
+                    want.append(tda_amd.differential_attention(*xs, lam * k, kv_lens=lens))
+        xs = [rows((2, h, m, 64), 70 + j, BF) for j, (h, m) in enumerate(((4, n), (4, n), (2, nk), (2, nk), (2, nk)))]
+        ref = tda_amd.differential_attention(*xs, lam)
+        assert torch.equal(tda_amd.differential_attention(*xs, lam), ref)
+        off = torch.empty(xs[0].numel() + 1, dtype=BF, device="cuda")[1:].view_as(xs[0]).copy_(xs[0])  # 2 bytes past a line
+        assert torch.equal(tda_amd.differential_attention(off, *xs[1:], lam), ref)
+        xs[4].requires_grad_()
+        assert tda_amd.differential_attention(*xs, lam).requires_grad  # and under no_grad it has none
+        with torch.no_grad():
+            assert not tda_amd.differential_attention(*xs, lam).requires_grad
+        with pytest.raises(ValueError):
+            tda_amd.differential_attention(xs[0], xs[1].cpu(), *xs[2:], lam)
+        with pytest.raises(ValueError):
+            tda_amd.differential_attention(xs[0], xs[1].float(), *xs[2:], lam)
+        with pytest.raises(ValueError):
+            tda_amd.differential_attention(*xs, lam[:3])
