@@ -22,7 +22,7 @@ extern "C" {
 
 #define SDA_ABI_VERSION 1
 
-/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 (sda_rotary, sda_kv4_*) */
+/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 (sda_fwd, sda_rotary, sda_kv4_*) */
 #define SDA_DTYPE_F16 2
 
 /* error codes beyond those of tda.h */
@@ -36,7 +36,7 @@ extern "C" {
  * behind every row's sight may hold anything. */
 typedef struct sda_fwd_args {
   int32_t abi_version;      /* SDA_ABI_VERSION */
-  int32_t dtype;            /* TDA_DTYPE_F32 or TDA_DTYPE_BF16: q, k, v, out */
+  int32_t dtype;            /* q, k, v, out: TDA_DTYPE_F32, TDA_DTYPE_BF16, or without out2 SDA_DTYPE_F16 */
   int32_t causal;           /* 1: keys behind the row's own position are hidden */
   float   scale;            /* s, 1e-30 .. 1e30 */
   int64_t batch, heads, kv_heads;   /* query head h reads key head h / (heads / kv_heads) */

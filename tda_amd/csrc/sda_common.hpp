@@ -51,6 +51,17 @@ struct TrB {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+struct TrH {
+  using T = _Float16;
+  using frag = f16x8;
+  __device__ __forceinline__ static f32x16 mma32(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 mma16(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
 struct TrF {
   using T = float;
   using frag = f32x8;
@@ -69,7 +80,8 @@ struct TrF {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Values 8 s .. 8 s + 7 of a score tile as the B operand of the next product (round to nearest
-// even; bf16 holds a weight to 2^-9, as it would hold the output).
+// even; bf16 holds a weight to 2^-9, as it would hold the output, f16 one of a running maximum's part to 2^-12,
+// and to 2^-25 of the maximum's below 2^-14).
 template <class Tr>
 __device__ __forceinline__ typename Tr::frag pack8(const f32x16& c, int s) {
   typename Tr::frag f;
@@ -136,34 +148,28 @@ struct Tile {
   // Row fragment step t: lane (m, g) gets row r0 + m, values 16 t + 8 g + [0, 8).
   __device__ __forceinline__ static typename Tr::frag row(const T* lds, int r0, int t) {
     const int l = lane_id(), r = r0 + (l & 31), g = l >> 5;
-    if constexpr (ES == 2) {
-      return *reinterpret_cast<const bf16x8*>(lds + r * W + 8 * ((2 * t + g) ^ swz(r)));
-    } else {
-      const int c = 4 * t + 2 * g;
-      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * (c ^ swz(r)));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * ((c + 1) ^ swz(r)));
-      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    }
+    static_assert(ES == 4, "16-bit types: RowReader");
+    const int c = 4 * t + 2 * g;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * (c ^ swz(r)));
+    const f32x4 b = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * ((c + 1) ^ swz(r)));
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
   // Transposed fragment, step s (16 rows from r0 + 16 s): lane (n, g) gets column 32 cs + n at rows
   // r0 + crow(8 s + j, g), j = 0 .. 7, which is the order of a score tile's values.
   __device__ __forceinline__ static typename Tr::frag col(const T* lds, int r0, int s, int cs) {
-    if constexpr (ES == 2) {
-      return tda::tile_tr_frag<W>(lds + r0 * W, s, cs);
-    } else {
-      const int l = lane_id(), g = l >> 5, n = 32 * cs + (l & 31);
-      f32x8 f;
+    static_assert(ES == 4, "16-bit types: ColReader");
+    const int l = lane_id(), g = l >> 5, n = 32 * cs + (l & 31);
+    f32x8 f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = r0 + crow(8 * s + j, g);
-        f[j] = lds[r * W + 4 * ((n >> 2) ^ swz(r)) + (n & 3)];
-      }
-      return f;
+    for (int j = 0; j < 8; ++j) {
+      const int r = r0 + crow(8 * s + j, g);
+      f[j] = lds[r * W + 4 * ((n >> 2) ^ swz(r)) + (n & 3)];
     }
+    return f;
   }
 };
 
-// The same fragments by way of LDS addresses that a lane keeps (bf16): the swizzle makes the address of each
+// The same fragments by way of LDS addresses that a lane keeps (16-bit types): the swizzle makes the address of each
 // step another one, which the compiler would work out again for every read (a third of a pass' vector
 // instructions).  `at` of a read is a constant offset: the tile's place, and rows 32 apart.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
@@ -186,7 +192,7 @@ struct RowReader {
   }
   __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int t) const {
     if constexpr (sizeof(typename Tr::T) == 2)
-      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(a[t] + at);
+      return *reinterpret_cast<const __attribute__((address_space(3))) typename Tr::frag*>(a[t] + at);
     else
       return Tile<Tr, 32, W>::row(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, t);
   }
@@ -213,10 +219,11 @@ struct ColReader {
   __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int s, int y) const {
     if constexpr (sizeof(typename Tr::T) == 2) {
       typedef __attribute__((address_space(3))) tda::s16x4 quad;
-      bf16x8 f;
+      typedef typename Tr::T half4 __attribute__((ext_vector_type(4)));
+      typename Tr::frag f;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        const bf16x4 w = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<quad*>(a[hh][y] + at + 32 * W * s)));
+        const half4 w = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<quad*>(a[hh][y] + at + 32 * W * s)));
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[4 * hh + e] = w[e];
       }
@@ -234,7 +241,7 @@ __device__ __forceinline__ void load_frags(const typename Tr::T* row, int g, typ
   for (int t = 0; t < NT; ++t) {
     if (row) {
       if constexpr (sizeof(typename Tr::T) == 2) {
-        f[t] = *reinterpret_cast<const bf16x8*>(row + 16 * t + 8 * g);
+        f[t] = *reinterpret_cast<const typename Tr::frag*>(row + 16 * t + 8 * g);
       } else {
         const f32x4 a = *reinterpret_cast<const f32x4*>(row + 16 * t + 8 * g);
         const f32x4 b = *reinterpret_cast<const f32x4*>(row + 16 * t + 8 * g + 4);
@@ -300,6 +307,10 @@ __device__ __forceinline__ void pin(f32x16 (&acc)[N]) {
 
 // Store 4 consecutive values.
 __device__ __forceinline__ void store4(bf16* p, f32x4 v) { tda::store4(p, v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(_Float16* p, f32x4 v) {
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<half4*>(p) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+}
 __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
 
 // Workgroup ids over (heads x tiles) with the heaviest tiles first: consecutive ids go to the 8 XCDs
@@ -326,7 +337,7 @@ constexpr int kLds = 160 * 1024;  // of a CU
 // Whether a launch of n workgroups of 128 rows (or keys) takes workgroups of 64 instead, whose waves share
 // the other axis out: where the 128s leave half of the 256 CUs' places idle, or, under a causal mask that
 // gives some of them far more work than others, where all of them are placed at once and the longest decides.
-// A CU holds one workgroup, two of bf16 (64, 64).  Forward and backward, us, whole : halved:
+// A CU holds one workgroup, two of 16-bit (64, 64).  Forward and backward, us, whole : halved:
 //   bf16 (128, 128), 500 rows of 4355 keys, 128 workgroups   127 : 103
 //   bf16 (64, 128), (1, 8, 1024) causal, 64                   33 : 25 and 98 : 64
 //   bf16 (64, 128), (2, 16, 1024) causal, 256                 40 : 37 and 109 : 88;  all seen 43 : 50, 113 : 122

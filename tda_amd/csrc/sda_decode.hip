@@ -23,7 +23,7 @@ struct DenseSrc {
 
   __device__ __forceinline__ static frag load8(const T* p) {
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const bf16x8*>(p);
+      return *reinterpret_cast<const frag*>(p);
     } else {
       const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
       return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -46,7 +46,7 @@ struct DenseSrc {
   __device__ __forceinline__ static frag load8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
     if constexpr (sizeof(T) == 2) {
-      return __builtin_bit_cast(bf16x8, a);
+      return __builtin_bit_cast(frag, a);
     } else {
       const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
       return f32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -155,7 +155,7 @@ static int pick(const FwdParams& p, int d, int dv, hipStream_t st) {
 }
 int launch_decode(const FwdParams& p, int dtype, int d, int dv, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  return dtype == 1 ? pick<TrB>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
+  return dtype == 1 ? pick<TrB>(p, d, dv, st) : dtype == 2 ? pick<TrH>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
 }
 
 }  // namespace sda

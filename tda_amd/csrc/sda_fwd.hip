@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, w[e], o[y][4 * r + e] * inv);
         store4(to + 32 * y + 8 * r + 4 * g, z);
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (std::is_same_v<Tr, TrB>) {
           if (low) {
             f32x4 rest;
 #pragma unroll
@@ -283,7 +283,7 @@ static int pick(const FwdParams& p, int d, int dv, hipStream_t st) {
 }
 int launch_fwd(const FwdParams& p, int dtype, int d, int dv, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  return dtype == 1 ? pick<TrB>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
+  return dtype == 1 ? pick<TrB>(p, d, dv, st) : dtype == 2 ? pick<TrH>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
 }
 
 }  // namespace sda

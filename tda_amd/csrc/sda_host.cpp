@@ -72,9 +72,9 @@ int32_t check_sizes(const A& a) {
              : TDA_ERR_SHAPE;
 }
 template <class A>
-int32_t check_common(const A& a) {
+int32_t check_common(const A& a, bool f16) {
   if (a.abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
-  if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16) return TDA_ERR_DTYPE;
+  if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16 && !(f16 && a.dtype == SDA_DTYPE_F16)) return TDA_ERR_DTYPE;
   if (a.causal != 0 && a.causal != 1) return TDA_ERR_CAUSAL;
   if (!check_scale(a.scale)) return SDA_ERR_SCALE;
   if (int32_t rc = check_sizes(a)) return rc;
@@ -238,7 +238,7 @@ size_t sda_fwd_workspace_bytes(const sda_fwd_args* a) {
 
 int32_t sda_validate_fwd(const sda_fwd_args* a) {
   if (!a) return TDA_ERR_NULL_POINTER;
-  if (int32_t rc = check_common(*a)) return rc;
+  if (int32_t rc = check_common(*a, !a->out2.data)) return rc;
   const int64_t es = bytes_of(a->dtype);
   for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out})
     if (int32_t rc = check_rows(*t, es)) return rc;
@@ -269,7 +269,7 @@ size_t sda_bwd_workspace_bytes(const sda_bwd_args* a) {
 
 int32_t sda_validate_bwd(const sda_bwd_args* a) {
   if (!a) return TDA_ERR_NULL_POINTER;
-  if (int32_t rc = check_common(*a)) return rc;
+  if (int32_t rc = check_common(*a, false)) return rc;
   const int64_t es = bytes_of(a->dtype);
   for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out, &a->dout, &a->dq1, &a->dk1, &a->dq2,
                               &a->dk2, &a->dv})

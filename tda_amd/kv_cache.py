@@ -20,12 +20,11 @@ _READ_OFF = {n: getattr(_sda_abi.SdaKv4ReadArgs, n).offset for n in ("k1", "k2",
 
 def _from_codes(batch: int, kv_heads: int, rows: int, dtype) -> bool:
     """Whether attend() computes `rows` query rows for each key head from the codes, 16 rows a pass over them, or
-    reads the rows out first, for the attention that passes over them once per 128 (in float32 for a
-    float16 or float32 query).  us, codes : rows, (batch, heads, kv_heads, n, keys) of width 128, bf16:
+    reads the rows out first, for the attention that passes over them once per 128.  us, codes : rows, (batch, heads, kv_heads, n, keys) of width 128, bf16:
     (8, 16, 4, 16, 4096) 38 : 108, (32, 32, 8, 32, 4096) 344 : 767, (16, 8, 8, 128, 4096) 178 : 238,
     (16, 8, 8, 256, 4096) 331 : 261, (1, 16, 4, 256, 4096) 60 : 94, (1, 16, 4, 512, 4096) 92 : 96; float32:
     (8, 8, 8, 128, 4096) 255 : 1257."""
-    return rows <= (128 if dtype == torch.bfloat16 else 512) or batch * kv_heads * -(-rows // 16) <= 256
+    return rows <= (512 if dtype == torch.float32 else 128) or batch * kv_heads * -(-rows // 16) <= 256
 
 
 class Int4KVCache:

@@ -3,8 +3,8 @@
     out = (softmax(s q1 k1^T + M) - lambda softmax(s q2 k2^T + M)) v
 
 beside the threshold form of api.py.  Forward and backward run in hand-written kernels behind
-include/sda.h (float32, bfloat16; float16 and float64 are computed in float32, as by the
-threshold operators); a call of few query rows, such as a decoding step, takes kernels that split the
+include/sda.h (float32, bfloat16, and float16 without gradients; float16 with gradients, whose range would
+not hold them, and float64 are computed in float32, as by the threshold operators); a call of few query rows, such as a decoding step, takes kernels that split the
 key axis.  There is no CPU fallback.
 """
 from __future__ import annotations
@@ -353,9 +353,12 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     if any(t.numel() == 0 for t in tensors):  # no rows or no keys: zeros, connected to the inputs
         none = sum(t[:0].sum() for t in tensors) + lam.reshape(-1)[:0].sum().to(q1.dtype)
         return torch.zeros((b, h, n, dv), dtype=q1.dtype, device=dev) + none
+    train = torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors, lam))
+    if q1.dtype == torch.float16 and not train:
+        cdt = torch.float16
     rows = [t if t.dtype == cdt else t.to(cdt) for t in tensors]
     rows = [_pad(t, kd) for t in rows[:4]] + [_pad(rows[4], kv)]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (*rows, lam)):
+    if train:
         out = _DifferentialAttention.apply(*rows, lam, s, bool(causal), off, q_offsets, lens)
     else:
         given = rows

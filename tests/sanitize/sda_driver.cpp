@@ -131,7 +131,10 @@ static void attention() {
   CHECK(sda_bwd(&b, nullptr) == TDA_OK && got::bwd.dlam_n[0] == 1 && got::bwd.dlam_n[1] == 8 && got::bwd.dlam_n[2] == 1);
 
   REFUSES(fwd_args(), sda_validate_fwd, a.abi_version = 7, TDA_ERR_ABI);
-  REFUSES(fwd_args(), sda_validate_fwd, a.dtype = SDA_DTYPE_F16, TDA_ERR_DTYPE);
+  REFUSES(fwd_args(), sda_validate_fwd, a.dtype = 3, TDA_ERR_DTYPE);
+  REFUSES(fwd_args(), sda_validate_fwd, a.dtype = SDA_DTYPE_F16, TDA_OK);
+  REFUSES(fwd_args(), sda_validate_fwd, (a.dtype = SDA_DTYPE_F16, a.out2 = a.out), TDA_ERR_DTYPE);  // no training form
+  REFUSES(bwd_args(), sda_validate_bwd, a.dtype = SDA_DTYPE_F16, TDA_ERR_DTYPE);
   REFUSES(fwd_args(), sda_validate_fwd, a.causal = 2, TDA_ERR_CAUSAL);
   for (float s : {0.f, -1.f, std::nanf(""), std::numeric_limits<float>::infinity(), 1e-31f, 1e31f})
     REFUSES(fwd_args(), sda_validate_fwd, a.scale = s, SDA_ERR_SCALE);

@@ -85,7 +85,7 @@ def bwd(**kw):
 
 BAD_ROWS = [
     (lambda a: setattr(a, "abi_version", 7), _abi.ERR_ABI),
-    (lambda a: setattr(a, "dtype", 2), _abi.ERR_DTYPE),
+    (lambda a: setattr(a, "dtype", 3), _abi.ERR_DTYPE),
     (lambda a: setattr(a, "causal", 2), _abi.ERR_CAUSAL),
     (lambda a: setattr(a, "scale", 0.0), _sda_abi.ERR_SCALE),
     (lambda a: setattr(a, "scale", float("nan")), _sda_abi.ERR_SCALE),

@@ -41,9 +41,11 @@ def check(b, h, hk, n, nk, d, dv, dtype, lam, train=True, seq_major=False, **kw)
     u = U[dtype] if dtype != F16 else U[F32]
     lam = lam if not isinstance(lam, torch.Tensor) else lam.cuda()
     ref_kw = {k: (v.cpu() if isinstance(v, torch.Tensor) else v) for k, v in kw.items()}
-    if not train:
-        ref = oracle.attention(*xs, lam, u=u, **ref_kw)
-        within(tda_amd.differential_attention(*xs, lam, **kw), ref, "out", U[dtype])
+    if not train:  # float16 in its own type: weights round to it, those below 2^-14 of a row's largest to 2^-25 of that
+        ref = oracle.attention(*xs, lam, u=U[dtype], **ref_kw)
+        most = float(torch.as_tensor(lam).abs().max())
+        tiny = nk * 2.0 ** -25 * (1 + most) * xs[4].abs().max().item() if dtype == F16 else 0.0
+        within(tda_amd.differential_attention(*xs, lam, **kw), ref, "out", U[dtype], 1e-30 + tiny)
         return
     dout = rows((b, h, n, dv), 6, dtype)
     leaves = [x.requires_grad_(True) for x in xs]
@@ -502,3 +504,27 @@ def test_calls_of_one_signature_take_their_own_tensors():
             tda_amd.differential_attention(xs[0], xs[1].float(), *xs[2:], lam)
         with pytest.raises(ValueError):
             tda_amd.differential_attention(*xs, lam[:3])
+
+
+@gpu
+@pytest.mark.parametrize("d, dv", DIMS + [(80, 72)])
+@pytest.mark.parametrize("h, hk, n, nk, off", [(6, 2, 70, 200, None), (4, 1, 129, 129, None), (3, 3, 300, 1300, 17), (16, 16, 700, 700, None)])
+def test_float16_without_gradients(d, dv, h, hk, n, nk, off):
+    check(3, h, hk, n, nk, d, dv, F16, torch.linspace(-0.3, 0.9, h), train=False, q_offset=off,
+          kv_lens=torch.tensor([nk, nk // 2, 0], dtype=torch.int32).cuda())
+
+
+@gpu
+def test_float16_under_no_grad_and_with_gradients():
+    """Without gradients in float16's own kernels, with them in float32's: both within float16's rounding."""
+    xs = [x.requires_grad_() for x in inputs(1, 4, 2, 150, 150, 64, 64, F16)]
+    with torch.no_grad():
+        alone = tda_amd.differential_attention(*xs, 0.5)
+    out = tda_amd.differential_attention(*xs, 0.5)
+    assert out.requires_grad and not alone.requires_grad and out.dtype == alone.dtype == F16
+    ref = oracle.attention(*xs, 0.5, u=U[F16])
+    tiny = 150 * 2.0 ** -25 * 1.5 * xs[4].abs().max().item()
+    within(alone, ref, "out", U[F16], tiny)
+    within(out, ref, "out", U[F16], tiny)
+    out.sum().backward()
+    assert all(x.grad.dtype == F16 and x.grad.isfinite().all() for x in xs)
