@@ -22,7 +22,7 @@ extern "C" {
 
 #define SDA_ABI_VERSION 1
 
-/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 (sda_fwd, sda_rotary, sda_kv4_*) */
+/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 (not as lambda_dtype) */
 #define SDA_DTYPE_F16 2
 
 /* error codes beyond those of tda.h */
@@ -36,7 +36,7 @@ extern "C" {
  * behind every row's sight may hold anything. */
 typedef struct sda_fwd_args {
   int32_t abi_version;      /* SDA_ABI_VERSION */
-  int32_t dtype;            /* q, k, v, out: TDA_DTYPE_F32, TDA_DTYPE_BF16, or without out2 SDA_DTYPE_F16 */
+  int32_t dtype;            /* TDA_DTYPE_F32, TDA_DTYPE_BF16 or SDA_DTYPE_F16: q, k, v, out */
   int32_t causal;           /* 1: keys behind the row's own position are hidden */
   float   scale;            /* s, 1e-30 .. 1e30 */
   int64_t batch, heads, kv_heads;   /* query head h reads key head h / (heads / kv_heads) */
@@ -45,7 +45,7 @@ typedef struct sda_fwd_args {
   tda_tensor q1, k1, q2, k2, v;     /* (B, H, Nq, d), (B, Hk, Nk, d), ..., (B, Hk, Nk, dv) */
   tda_tensor out;                   /* (B, H, Nq, dv) */
   tda_tensor out2;          /* optional (data may be NULL), f32 rows: softmax(s q2 k2^T + M) v, and */
-  tda_tensor out_low;       /* with it for bf16, bf16 rows: what out's rounding left out.  The
+  tda_tensor out_low;       /* with it but for f32, rows of dtype: what out's rounding left out.  The
                                backward's row sums of the outputs keep 16 bits with them: from the
                                rounded outputs alone they would cost its gradients half again the error
                                that their own rounding has */

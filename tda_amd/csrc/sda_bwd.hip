@@ -21,6 +21,69 @@
 
 namespace sda {
 
+__device__ __forceinline__ f32x4 load4h(const _Float16* p) {
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  const half4 v = *reinterpret_cast<const half4*>(p);
+  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+template <class T>
+__device__ __forceinline__ f32x4 load4_(const T* p) {
+  if constexpr (std::is_same_v<T, _Float16>) return load4h(p);
+  else return tda::load4(p);
+}
+
+// ------------------------------------------------------------------ f16's range
+// A weight or score gradient in f16 keeps its 11 bits only between 2^-14 and 2^16, so the f16 passes scale
+// them by powers of two: score gradients so that the largest possible, |dS| <= 2 max|dO_i| max(1, |lambda_i|)
+// max|v_j|, comes to 2^13 .. 2^14, weights by up to 2^8 (1 + max |lambda| leaves room).  peak holds the three
+// maxima; bits of floats that are not negative order as integers do, so an atomic maximum has one result.
+struct Scales {
+  float ds, w;  // score gradients by ds, weights by 2^w
+};
+template <class Tr>
+__device__ __forceinline__ Scales scales(const BwdParams& P) {
+  if constexpr (std::is_same_v<Tr, TrH>) {
+    const float a = P.peak[0] * P.peak[1], l = 1.f + P.peak[2];
+    const bool fits = a > 0x1p-100f && a < 0x1p100f;  // else nothing to scale by (zeros, NaN)
+    return {fits ? exp2_(floorf(13.f - __builtin_amdgcn_logf(a))) : 1.f,
+            l < 0x1p100f ? fminf(8.f, floorf(14.f - __builtin_amdgcn_logf(l))) : 0.f};
+  } else {
+    return {1.f, 0.f};
+  }
+}
+__device__ __forceinline__ void raise(float* to, float x) { atomicMax(reinterpret_cast<unsigned*>(to), __builtin_bit_cast(unsigned, x)); }
+__global__ void bwd_clear(BwdParams P) {
+  if (threadIdx.x < 3) P.peak[threadIdx.x] = 0.f;
+}
+// max|v_j| over the rows that some row sees.  16 lanes per row, rows in strides of the grid.
+template <int DV>
+__global__ void __launch_bounds__(256) bwd_peak(BwdParams P) {
+  const int64_t rows = (int64_t)P.B * P.Hk * P.Nk;
+  const int c = threadIdx.x & 15;
+  float top = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.x * 16) {
+    const int j = (int)(row % P.Nk), b = (int)(row / P.Nk / P.Hk), h = (int)(row / P.Nk % P.Hk);
+    const int len = len_of(P.see, b, P.Nk), lim = P.see.causal ? min(len, off_of(P.see, b) + P.Nq) : len;
+    if (j >= lim) continue;  // whole rows: 16 lanes together
+    const _Float16* v = row_of<_Float16>(P.v, b, h, j);
+    float n = 0.f;
+#pragma unroll
+    for (int u = 0; u < DV / 64; ++u) {
+      const f32x4 x = load4h(v + 64 * u + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n = __builtin_fmaf(x[e], x[e], n);
+    }
+    n = tda::group_sum<16>(n);
+    top = n != n ? n : top != top ? top : fmaxf(top, n);
+  }
+  __shared__ float all[16];
+  if (c == 0) all[threadIdx.x >> 4] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int x = 1; x < 16; ++x) top = all[x] != all[x] ? all[x] : top != top ? top : fmaxf(top, all[x]);
+  raise(P.peak + 1, sqrtf(top));
+}
+
 // ------------------------------------------------------------------ row sums
 // What the passes need of a row, so that it enters their products as a starting value: the log-sums as
 // -lse_b / c (score and weight: P = 2^(c (q k - lse / c))), -r_1, r_1 - r_2, -lambda.
@@ -30,35 +93,59 @@ __global__ void __launch_bounds__(256) bwd_rows(BwdParams P) {
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
   const int64_t row = (int64_t)tda::grid_bid<256>() * 16 + (threadIdx.x >> 4);
   const int c = threadIdx.x & 15;
-  if (row >= rows) return;
-  const int i = (int)(row % P.Nq);
-  const int64_t bh = row / P.Nq;
-  const int b = (int)(bh / P.H), h = (int)(bh % P.H);
-  const T* d = row_of<T>(P.dout, b, h, i);
-  const T* x = row_of<T>(P.out, b, h, i);
-  const float* y = row_of<float>(P.out2, b, h, i);
-  const T* z = sizeof(T) == 2 ? row_of<T>(P.low, b, h, i) : nullptr;
-  float rx = 0.f, ry = 0.f;
+  constexpr bool HALF = std::is_same_v<T, _Float16>;
+  __shared__ float peak[2][16];
+  if (HALF && c == 0) peak[0][threadIdx.x >> 4] = peak[1][threadIdx.x >> 4] = 0.f;
+  if (row < rows) {
+    const int i = (int)(row % P.Nq);
+    const int64_t bh = row / P.Nq;
+    const int b = (int)(bh / P.H), h = (int)(bh % P.H);
+    const T* d = row_of<T>(P.dout, b, h, i);
+    const T* x = row_of<T>(P.out, b, h, i);
+    const float* y = row_of<float>(P.out2, b, h, i);
+    const T* z = sizeof(T) == 2 ? row_of<T>(P.low, b, h, i) : nullptr;
+    float rx = 0.f, ry = 0.f, n2 = 0.f;
 #pragma unroll
-  for (int u = 0; u < DV / 64; ++u) {
-    const f32x4 dd = tda::load4(d + 64 * u + 4 * c), yy = tda::load4(y + 64 * u + 4 * c);
-    f32x4 xx = tda::load4(x + 64 * u + 4 * c);
-    if constexpr (sizeof(T) == 2) xx += tda::load4(z + 64 * u + 4 * c);
+    for (int u = 0; u < DV / 64; ++u) {
+      const f32x4 dd = load4_(d + 64 * u + 4 * c), yy = load4_(y + 64 * u + 4 * c);
+      f32x4 xx = load4_(x + 64 * u + 4 * c);
+      if constexpr (sizeof(T) == 2) xx += load4_(z + 64 * u + 4 * c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      rx = __builtin_fmaf(dd[e], xx[e], rx);
-      ry = __builtin_fmaf(dd[e], yy[e], ry);
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (HALF) n2 = __builtin_fmaf(dd[e], dd[e], n2);
+        rx = __builtin_fmaf(dd[e], xx[e], rx);
+        ry = __builtin_fmaf(dd[e], yy[e], ry);
+      }
+    }
+    rx = tda::group_sum<16>(rx);
+    ry = tda::group_sum<16>(ry);
+    if constexpr (HALF) n2 = tda::group_sum<16>(n2);
+    if (c == 0) {
+      const float lam = lambda_of(P.lam, b, h, i), r1 = __builtin_fmaf(lam, ry, rx), inv = 1.0f / P.c;
+      P.stat[row] = -P.lse[row] * inv;
+      P.stat[rows + row] = -P.lse[rows + row] * inv;
+      P.stat[2 * rows + row] = -r1;
+      P.stat[3 * rows + row] = r1 - ry;
+      P.stat[4 * rows + row] = -lam;
+      if constexpr (HALF) {
+        const int len = len_of(P.see, b, P.Nk);
+        if ((P.see.causal ? min(len, off_of(P.see, b) + i + 1) : len) > 0) {  // a row that sees nothing counts for nothing
+          peak[0][threadIdx.x >> 4] = sqrtf(n2) * fmaxf(1.f, fabsf(lam));
+          peak[1][threadIdx.x >> 4] = fabsf(lam);
+        }
+      }
     }
   }
-  rx = tda::group_sum<16>(rx);
-  ry = tda::group_sum<16>(ry);
-  if (c == 0) {
-    const float lam = lambda_of(P.lam, b, h, i), r1 = __builtin_fmaf(lam, ry, rx), inv = 1.0f / P.c;
-    P.stat[row] = -P.lse[row] * inv;
-    P.stat[rows + row] = -P.lse[rows + row] * inv;
-    P.stat[2 * rows + row] = -r1;
-    P.stat[3 * rows + row] = r1 - ry;
-    P.stat[4 * rows + row] = -lam;
+  if constexpr (HALF) {
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      float top = 0.f;
+      for (int x = 0; x < 16; ++x) {
+        const float a = peak[threadIdx.x][x];
+        top = a != a ? a : top != top ? top : fmaxf(top, a);
+      }
+      raise(P.peak + 2 * threadIdx.x, top);
+    }
   }
 }
 
@@ -117,7 +204,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
   const int h0 = hk * GQ + part * P.gs;
   const int k0 = it.tile * S::KEYS, k0w = k0 + 32 * (wv % (NW / RH)), key = k0w + n32;
   const int len = len_of(P.see, b, P.Nk), off = off_of(P.see, b);
-  const bool live = key < len;
+  const bool live = key < (P.see.causal ? min(len, off + P.Nq) : len);  // some row sees it; others' rows may hold anything
   const int64_t rows = (int64_t)P.B * P.H * P.Nq;
 
   // query tiles of 32 rows, RH a step: from the first that sees the workgroup's first key on
@@ -168,6 +255,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
 #pragma unroll
   for (int x = 0; x < 2; ++x) load_frags<Tr, NT>(live ? row_of<T>(P.k[x], b, hk, key) : nullptr, g, kf[x]);
   load_frags<Tr, NV>(live ? row_of<T>(P.v, b, hk, key) : nullptr, g, vf);
+  const Scales by = scales<Tr>(P);
+  constexpr bool HALF = std::is_same_v<Tr, TrH>;
+  const float dsw = HALF ? by.ds * exp2_(-by.w) : 1.f;  // from a scaled weight to a scaled score gradient
   f32x16 dk[2][D / 32] = {}, dv[DV / 32] = {};
   pin(dk[0]);
   pin(dk[1]);
@@ -223,17 +313,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
       }
     };
     auto weight = [&](int x, int r) {
-      return START ? exp2_(P.c * s[x][r]) : exp2_(__builtin_fmaf(P.c, s[x][r], P.c * st[32 * x + crow(r, g)]));
+      return HALF ? exp2_(__builtin_fmaf(P.c, s[x][r], by.w)) : START ? exp2_(P.c * s[x][r]) : exp2_(__builtin_fmaf(P.c, s[x][r], P.c * st[32 * x + crow(r, g)]));
     };
     auto first_branch = [&](int r) {
       const float p = weight(0, r);
       w[r] = p;
       s[0][r] = p * (START ? dp[r] : dp[r] + st[64 + crow(r, g)]);
+      if constexpr (HALF) s[0][r] *= dsw;
     };
     auto second_branch = [&](int r) {
       const float p = lam[r] * weight(1, r);
       w[r] += p;
       s[1][r] = p * (START ? dp[r] + dif[r] : dp[r] + (dif[r] + st[64 + crow(r, g)]));
+      if constexpr (HALF) s[1][r] *= dsw;
     };
     constexpr int NG = E6 / G;
     times<NG>([&](auto i) {
@@ -320,8 +412,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
         if constexpr (!START) dp += rowstat(2), sc += rowstat(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          w[r] = exp2_(P.c * sc[r]);
+          w[r] = HALF ? exp2_(__builtin_fmaf(P.c, sc[r], by.w)) : exp2_(P.c * sc[r]);
           sc[r] = w[r] * dp[r];
+          if constexpr (HALF) sc[r] *= dsw;
         }
         ds[0] = pack8<Tr>(sc, 0), ds[1] = pack8<Tr>(sc, 1);
       }
@@ -335,9 +428,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * q + e;
-            const float p = lam[e] * exp2_(P.c * sc[r]);
+            const float p = lam[e] * (HALF ? exp2_(__builtin_fmaf(P.c, sc[r], by.w)) : exp2_(P.c * sc[r]));
             w[r] += p;
             sc[r] = p * dp[r];
+            if constexpr (HALF) sc[r] *= dsw;
           }
         }
         ds[0] = pack8<Tr>(sc, 0), ds[1] = pack8<Tr>(sc, 1);
@@ -397,17 +491,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
     });
   }
   if (key >= P.Nk) return;
-  // a key past the length met weights of its own making (of a zero row): its column holds nothing else
+  const float back = HALF ? P.scale / by.ds : P.scale, backw = HALF ? exp2_(-by.w) : 1.f;
+  // a key that no row sees met weights of its own making (of a zero row): its column holds nothing else
 #pragma unroll
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int y = 0; y < D / 32; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dk[x][y][r] = live ? dk[x][y][r] * P.scale : 0.f;
+      for (int r = 0; r < 16; ++r) dk[x][y][r] = live ? dk[x][y][r] * back : 0.f;
 #pragma unroll
   for (int y = 0; y < DV / 32; ++y)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dv[y][r] = live ? dv[y][r] : 0.f;
+    for (int r = 0; r < 16; ++r) dv[y][r] = live ? (HALF ? dv[y][r] * backw : dv[y][r]) : 0.f;
   constexpr int W = 2 * D + DV;
   float* pt = P.part ? P.part + (((int64_t)part * P.B * P.Hk + bk) * P.Nk + key) * W + 4 * g : nullptr;  // dk1, dk2, dv, f32
 #pragma unroll
@@ -531,6 +626,8 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
   }
   if (row) lam = -P.stat[4 * rows + at0];
   float more = 0.f;  // rowsum(P_2 (dP - r_2))
+  const float ds = scales<Tr>(P).ds;
+  constexpr bool HALF = std::is_same_v<Tr, TrH>;
   f32x16 dq[NB][D / 32] = {};
   if constexpr (!SPLIT) {
     pin(dq[0]);
@@ -557,7 +654,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     for (int x = 0; x < NB; ++x) {
       const int z = SPLIT ? br : x, kt = AT + x * KT::BYTES;
       f32x16 s = chain<Tr, NT>([&](int t) { return kr.read(kbuf, kt, t); }, qf[x]);
-      const float f = -lam;
+      const float f = HALF ? -lam * ds : -lam;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = exp2_(__builtin_fmaf(s[r], P.c, -lse[x]));
@@ -575,6 +672,9 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
           more += s[r];
           s[r] *= f;
         }
+      } else if constexpr (HALF) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= ds;
       }
       const frag e[2] = {pack8<Tr>(s, 0), pack8<Tr>(s, 1)};
       columns<Tr, D / 32>([&](int u, int y) { return kc.read(kbuf, kt, u, y); }, e, dq[x]);
@@ -611,6 +711,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
   more += __shfl_xor(more, 32);
   if (!row) return;
   if ((!SPLIT || br) && g == 0) P.stat[5 * rows + at0] = rs[NB - 1] + more;
+  const float back = HALF ? P.scale / ds : P.scale;
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
     T* to = row_of<T>(P.dq[SPLIT ? br : x], b, h, qi) + 4 * g;
@@ -618,7 +719,7 @@ __global__ void __launch_bounds__(SPLIT ? 512 : 256) __attribute__((amdgpu_waves
     for (int y = 0; y < D / 32; ++y)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        store4(to + 32 * y + 8 * r, f32x4{dq[x][y][4 * r] * P.scale, dq[x][y][4 * r + 1] * P.scale, dq[x][y][4 * r + 2] * P.scale, dq[x][y][4 * r + 3] * P.scale});
+        store4(to + 32 * y + 8 * r, f32x4{dq[x][y][4 * r] * back, dq[x][y][4 * r + 1] * back, dq[x][y][4 * r + 2] * back, dq[x][y][4 * r + 3] * back});
   }
 }
 
@@ -697,6 +798,12 @@ template <class Tr, int D, int DV>
 static int run(const BwdParams& p, hipStream_t st) {
   using T = typename Tr::T;
   const int64_t rows = (int64_t)p.B * p.H * p.Nq;
+  if constexpr (std::is_same_v<Tr, TrH>) {
+    bwd_clear<<<1, 64, 0, st>>>(p);
+    const int64_t keys = ((int64_t)p.B * p.Hk * p.Nk + 15) / 16;
+    bwd_peak<DV><<<(unsigned)(keys < 2048 ? keys : 2048), 256, 0, st>>>(p);
+    tda::launched(st, "sda_bwd_peak");
+  }
   bwd_rows<T, DV><<<tda::grid_of<256>((rows + 15) / 16), 256, 0, st>>>(p);
   tda::launched(st, "sda_bwd_rows");
   const int parts = p.H / p.Hk / p.gs;
@@ -737,7 +844,7 @@ static int pick(const BwdParams& p, int d, int dv, hipStream_t st) {
 }
 int launch_bwd(const BwdParams& p, int dtype, int d, int dv, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  return dtype == 1 ? pick<TrB>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
+  return dtype == 1 ? pick<TrB>(p, d, dv, st) : dtype == 2 ? pick<TrH>(p, d, dv, st) : pick<TrF>(p, d, dv, st);
 }
 
 }  // namespace sda

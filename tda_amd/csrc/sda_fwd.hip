@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(512) fwd_tiles(FwdParams P) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, w[e], o[y][4 * r + e] * inv);
         store4(to + 32 * y + 8 * r + 4 * g, z);
-        if constexpr (std::is_same_v<Tr, TrB>) {
+        if constexpr (sizeof(T) == 2) {
           if (low) {
             f32x4 rest;
 #pragma unroll

@@ -72,9 +72,9 @@ int32_t check_sizes(const A& a) {
              : TDA_ERR_SHAPE;
 }
 template <class A>
-int32_t check_common(const A& a, bool f16) {
+int32_t check_common(const A& a) {
   if (a.abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
-  if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16 && !(f16 && a.dtype == SDA_DTYPE_F16)) return TDA_ERR_DTYPE;
+  if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16 && a.dtype != SDA_DTYPE_F16) return TDA_ERR_DTYPE;
   if (a.causal != 0 && a.causal != 1) return TDA_ERR_CAUSAL;
   if (!check_scale(a.scale)) return SDA_ERR_SCALE;
   if (int32_t rc = check_sizes(a)) return rc;
@@ -87,7 +87,7 @@ int32_t check_common(const A& a, bool f16) {
 template <class A>
 int32_t check_kept(const A& a) {
   if (int32_t rc = check_rows(a.out2, 4)) return rc;
-  return a.dtype == TDA_DTYPE_BF16 ? check_rows(a.out_low, 2) : TDA_OK;
+  return a.dtype == TDA_DTYPE_F32 ? TDA_OK : check_rows(a.out_low, 2);
 }
 
 sda::Rows rows_of(const tda_tensor& t) { return {t.data, t.stride[0], t.stride[1], t.stride[2]}; }
@@ -142,7 +142,8 @@ int64_t key_group(const sda_bwd_args& a) {
     if (G % gs == 0 && base * (G / gs) >= 512) return gs;
   return 1;
 }
-int64_t stat_bytes(const sda_bwd_args& a) { return round256(6 * a.batch * a.heads * a.seq_len * 4); }
+int64_t peak_bytes(const sda_bwd_args& a) { return a.dtype == SDA_DTYPE_F16 ? 256 : 0; }
+int64_t stat_bytes(const sda_bwd_args& a) { return round256(6 * a.batch * a.heads * a.seq_len * 4) + peak_bytes(a); }
 int64_t part_bytes(const sda_bwd_args& a) {
   const int64_t G = a.heads / a.kv_heads, gs = key_group(a);
   return gs == G ? 0 : G / gs * a.batch * a.kv_heads * a.seq_len_kv * (2 * a.head_dim + a.v_head_dim) * 4;
@@ -238,7 +239,7 @@ size_t sda_fwd_workspace_bytes(const sda_fwd_args* a) {
 
 int32_t sda_validate_fwd(const sda_fwd_args* a) {
   if (!a) return TDA_ERR_NULL_POINTER;
-  if (int32_t rc = check_common(*a, !a->out2.data)) return rc;
+  if (int32_t rc = check_common(*a)) return rc;
   const int64_t es = bytes_of(a->dtype);
   for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out})
     if (int32_t rc = check_rows(*t, es)) return rc;
@@ -269,7 +270,7 @@ size_t sda_bwd_workspace_bytes(const sda_bwd_args* a) {
 
 int32_t sda_validate_bwd(const sda_bwd_args* a) {
   if (!a) return TDA_ERR_NULL_POINTER;
-  if (int32_t rc = check_common(*a, false)) return rc;
+  if (int32_t rc = check_common(*a)) return rc;
   const int64_t es = bytes_of(a->dtype);
   for (const tda_tensor* t : {&a->q1, &a->k1, &a->q2, &a->k2, &a->v, &a->out, &a->dout, &a->dq1, &a->dk1, &a->dq2,
                               &a->dk2, &a->dv})
@@ -294,6 +295,7 @@ int32_t sda_bwd(const sda_bwd_args* a, void* stream) {
   p.scale = a->scale;
   p.lse = a->lse;
   p.stat = static_cast<float*>(a->workspace);
+  if (peak_bytes(*a)) p.peak = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + stat_bytes(*a) - peak_bytes(*a));
   p.gs = (int)key_group(*a);
   p.part = part_bytes(*a) ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + stat_bytes(*a)) : nullptr;
   p.dlam = a->dlambda;

@@ -26,7 +26,7 @@ struct Sight {
 };
 
 struct FwdParams {
-  Rows q[2], k[2], v, out, out2, low;  // out2.p (f32) may be null; low: bf16 alone
+  Rows q[2], k[2], v, out, out2, low;  // out2.p (f32) may be null; low: with it, not for f32
   Lambda lam;
   Sight see;
   int B, H, Hk, Nq, Nk, nqt;      // nqt: query tiles (set by launch_fwd)
@@ -45,6 +45,7 @@ struct BwdParams {
   float c, scale;
   const float* lse;  // [2][B*H*Nq]
   float* stat;       // [6][B*H*Nq]: what the passes need of a row (bwd_rows), and r_2 (bwd_query)
+  float* peak;       // f16: [3], what its range has to hold (bwd_rows, bwd_peak); else null
   float* part;       // may be null: dk1, dk2, dv of each group of gs query heads, f32
   int gs;            // query heads a workgroup of the key pass sums over
   void* dlam;        // may be null

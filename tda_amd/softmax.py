@@ -3,8 +3,7 @@
     out = (softmax(s q1 k1^T + M) - lambda softmax(s q2 k2^T + M)) v
 
 beside the threshold form of api.py.  Forward and backward run in hand-written kernels behind
-include/sda.h (float32, bfloat16, and float16 without gradients; float16 with gradients, whose range would
-not hold them, and float64 are computed in float32, as by the threshold operators); a call of few query rows, such as a decoding step, takes kernels that split the
+include/sda.h (float32, bfloat16, float16; float64 is computed in float32, as by the threshold operators); a call of few query rows, such as a decoding step, takes kernels that split the
 key axis.  There is no CPU fallback.
 """
 from __future__ import annotations
@@ -21,7 +20,7 @@ from . import _abi, _sda_abi, ops
 
 _PUT = struct.Struct("<Q").pack_into
 _COMPUTE = {torch.float32: torch.float32, torch.bfloat16: torch.bfloat16,
-            torch.float16: torch.float32, torch.float64: torch.float32}
+            torch.float16: torch.float16, torch.float64: torch.float32}
 _CODE = {torch.float32: _abi.DTYPE_F32, torch.bfloat16: _abi.DTYPE_BF16, torch.float16: _sda_abi.DTYPE_F16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)  # the current stream's handle
@@ -255,7 +254,7 @@ def _forward(q1, q2, k1, k2, v, lam, scale, causal, q_offset, q_offsets, kv_lens
     out2 = low = lse = None
     if saving:
         out2 = _new_rows(q1, v.shape[3], torch.float32)
-        low = _new_rows(q1, v.shape[3]) if q1.dtype == torch.bfloat16 else None
+        low = _new_rows(q1, v.shape[3]) if q1.dtype != torch.float32 else None
         lse = torch.empty((2,) + q1.shape[:3], dtype=torch.float32, device=q1.device)
     rows = (q1, k1, q2, k2, v, out, out2, low)
     tpl, size = _template("sda_fwd", rows, _FWD_ROWS, _sda_abi.SdaFwdArgs, "sda_fwd_workspace_bytes", lam, scale,
@@ -353,12 +352,9 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     if any(t.numel() == 0 for t in tensors):  # no rows or no keys: zeros, connected to the inputs
         none = sum(t[:0].sum() for t in tensors) + lam.reshape(-1)[:0].sum().to(q1.dtype)
         return torch.zeros((b, h, n, dv), dtype=q1.dtype, device=dev) + none
-    train = torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors, lam))
-    if q1.dtype == torch.float16 and not train:
-        cdt = torch.float16
     rows = [t if t.dtype == cdt else t.to(cdt) for t in tensors]
     rows = [_pad(t, kd) for t in rows[:4]] + [_pad(rows[4], kv)]
-    if train:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*rows, lam)):
         out = _DifferentialAttention.apply(*rows, lam, s, bool(causal), off, q_offsets, lens)
     else:
         given = rows

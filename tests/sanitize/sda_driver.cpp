@@ -133,8 +133,14 @@ static void attention() {
   REFUSES(fwd_args(), sda_validate_fwd, a.abi_version = 7, TDA_ERR_ABI);
   REFUSES(fwd_args(), sda_validate_fwd, a.dtype = 3, TDA_ERR_DTYPE);
   REFUSES(fwd_args(), sda_validate_fwd, a.dtype = SDA_DTYPE_F16, TDA_OK);
-  REFUSES(fwd_args(), sda_validate_fwd, (a.dtype = SDA_DTYPE_F16, a.out2 = a.out), TDA_ERR_DTYPE);  // no training form
-  REFUSES(bwd_args(), sda_validate_bwd, a.dtype = SDA_DTYPE_F16, TDA_ERR_DTYPE);
+  REFUSES(bwd_args(), sda_validate_bwd, a.dtype = SDA_DTYPE_F16, TDA_ERR_WORKSPACE);  // its peaks take room
+  b = bwd_args();
+  b.dtype = SDA_DTYPE_F16;
+  const size_t without = b.workspace_bytes;
+  b.workspace_bytes = sda_bwd_workspace_bytes(&b);
+  CHECK(b.workspace_bytes == without + 256 && sda_bwd(&b, nullptr) == TDA_OK);
+  CHECK(reinterpret_cast<char*>(got::bwd.peak) == AT + 6 * 16 * 100 * 4 + (256 - 6 * 16 * 100 * 4 % 256) % 256);
+  CHECK(reinterpret_cast<char*>(got::bwd.part) == reinterpret_cast<char*>(got::bwd.peak) + 256);
   REFUSES(fwd_args(), sda_validate_fwd, a.causal = 2, TDA_ERR_CAUSAL);
   for (float s : {0.f, -1.f, std::nanf(""), std::numeric_limits<float>::infinity(), 1e-31f, 1e31f})
     REFUSES(fwd_args(), sda_validate_fwd, a.scale = s, SDA_ERR_SCALE);

@@ -36,26 +36,42 @@ def within(got, ref, name, u, extra=1e-30):
     assert far.max().item() <= 0, f"{name}: {far.max().item():.3g} past its bound of {off.flatten()[far.argmax()].item():.3g}"
 
 
+def tiny(xs, lam, dout=None):
+    """How far float16's smallest values may take a result, by name: below 2^-14 they are off by up to 2^-25.
+    Forward weights are shares of a row's largest; the backward's are scaled by 2^8 (|lambda| <= 1 here), its score
+    gradients by at least 2^12 / a, where a bounds them by half; the results themselves round last."""
+    q, k, v = (max(x.abs().max().item() for x in y) for y in (xs[:2], xs[2:4], xs[4:]))
+    most, last = float(torch.as_tensor(lam).abs().max()), 2.0 ** -25
+    b, h, n, d = xs[0].shape
+    nk, rows_of = xs[4].shape[2], n * h // xs[4].shape[1]
+    res = {"out": last + nk * 2.0 ** -25 * (1 + most) * v}
+    if dout is not None:
+        norm = lambda x: x.double().norm(dim=-1).max().item()  # noqa: E731
+        a = norm(dout) * norm(xs[4]) * max(1.0, most)
+        dq, dk = (last + m * a * 2.0 ** -37 * x / math.sqrt(d) for m, x in ((nk, k), (rows_of, q)))
+        res |= {"dq1": dq, "dq2": dq, "dk1": dk, "dk2": dk, "dv": last + rows_of * 2.0 ** -33 * dout.abs().max().item()}
+    return res
+
+
 def check(b, h, hk, n, nk, d, dv, dtype, lam, train=True, seq_major=False, **kw):
     xs = inputs(b, h, hk, n, nk, d, dv, dtype, seq_major)
-    u = U[dtype] if dtype != F16 else U[F32]
+    u = U[dtype]
     lam = lam if not isinstance(lam, torch.Tensor) else lam.cuda()
     ref_kw = {k: (v.cpu() if isinstance(v, torch.Tensor) else v) for k, v in kw.items()}
-    if not train:  # float16 in its own type: weights round to it, those below 2^-14 of a row's largest to 2^-25 of that
-        ref = oracle.attention(*xs, lam, u=U[dtype], **ref_kw)
-        most = float(torch.as_tensor(lam).abs().max())
-        tiny = nk * 2.0 ** -25 * (1 + most) * xs[4].abs().max().item() if dtype == F16 else 0.0
-        within(tda_amd.differential_attention(*xs, lam, **kw), ref, "out", U[dtype], 1e-30 + tiny)
+    dout = rows((b, h, n, dv), 6, dtype) if train else None
+    more = tiny(xs, lam, dout) if dtype == F16 else {}
+    if not train:
+        ref = oracle.attention(*xs, lam, u=u, **ref_kw)
+        within(tda_amd.differential_attention(*xs, lam, **kw), ref, "out", u, 1e-30 + more.get("out", 0.0))
         return
-    dout = rows((b, h, n, dv), 6, dtype)
     leaves = [x.requires_grad_(True) for x in xs]
     lam_leaf = lam.clone().requires_grad_(True) if isinstance(lam, torch.Tensor) else lam
     out = tda_amd.differential_attention(*leaves, lam_leaf, **kw)
     out.backward(dout)
     ref = oracle.attention(*xs, lam, u=u, dout=dout, **ref_kw)
-    within(out, ref, "out", U[dtype])
+    within(out, ref, "out", u, 1e-30 + more.get("out", 0.0))
     for x, name in zip(leaves, ("dq1", "dq2", "dk1", "dk2", "dv")):
-        within(x.grad, ref, name, U[dtype])
+        within(x.grad, ref, name, u, 1e-30 + more.get(name, 0.0))
     if isinstance(lam, torch.Tensor):
         assert lam_leaf.grad.dtype == lam.dtype
         within(lam_leaf.grad, ref, "dlam", U[lam.dtype])
@@ -515,16 +531,52 @@ def test_float16_without_gradients(d, dv, h, hk, n, nk, off):
 
 
 @gpu
-def test_float16_under_no_grad_and_with_gradients():
-    """Without gradients in float16's own kernels, with them in float32's: both within float16's rounding."""
-    xs = [x.requires_grad_() for x in inputs(1, 4, 2, 150, 150, 64, 64, F16)]
-    with torch.no_grad():
-        alone = tda_amd.differential_attention(*xs, 0.5)
-    out = tda_amd.differential_attention(*xs, 0.5)
-    assert out.requires_grad and not alone.requires_grad and out.dtype == alone.dtype == F16
-    ref = oracle.attention(*xs, 0.5, u=U[F16])
-    tiny = 150 * 2.0 ** -25 * 1.5 * xs[4].abs().max().item()
-    within(alone, ref, "out", U[F16], tiny)
-    within(out, ref, "out", U[F16], tiny)
-    out.sum().backward()
-    assert all(x.grad.dtype == F16 and x.grad.isfinite().all() for x in xs)
+@pytest.mark.parametrize("d, dv", DIMS)
+@pytest.mark.parametrize("h, hk, n, lam", [(2, 2, 1, 0.5), (4, 2, 129, torch.linspace(-0.9, 0.9, 4)), (6, 6, 300, torch.tensor(0.7))])
+def test_float16_training_step(d, dv, h, hk, n, lam):
+    check(3, h, hk, n, n, d, dv, F16, lam, kv_lens=torch.tensor([n, (n + 1) // 2, 0], dtype=torch.int32).cuda())
+
+
+@gpu
+@pytest.mark.parametrize("by", [2.0 ** -12, 2.0 ** 10])
+@pytest.mark.parametrize("lam", [0.5, 300.0])
+def test_float16_gradients_keep_their_bits_at_any_scale(by, lam):
+    """The same step with upstream gradients scaled by a power of two: the same gradients, scaled, to the bit where
+    float16 holds both (the passes' own scales take the power out again); below 2^-14 each is off by up to 2^-25."""
+    xs = [x * 0.25 for x in inputs(1, 4, 2, 200, 200, 64, 64, F16)]
+    dout = rows((1, 4, 200, 64), 6, F16, 2.0 ** -2 if by > 1 else 1.0)
+    dout = torch.where(dout.abs() < 2.0 ** -2, 0.0, dout)  # scaling stays exact
+    res = []
+    for y in (1.0, by):
+        leaves = [x.clone().requires_grad_() for x in xs]
+        tda_amd.differential_attention(*leaves, lam).backward(dout * y)
+        res.append([x.grad.double() for x in leaves])
+    for a, b in zip(*res):
+        # (a value just below 2^-14 may round up to it from the coarser steps there)
+        held = (b.abs() > 2.0 ** -14) & (a.abs() > 2.0 ** -14) & b.isfinite() & a.isfinite()
+        assert torch.equal(a[held] * by, b[held])
+        both = b.isfinite() & a.isfinite()
+        assert both.any() and ((a * by - b).abs() <= 2.0 ** -25 * (1 + by) + 2.0 ** -11 * b.abs())[both].all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+def test_rows_that_count_for_nothing(dtype):
+    """Keys behind every row's sight and rows that see no key take no part in the gradients (nor in float16's
+    scales), and get zeros."""
+    xs = inputs(2, 2, 2, 40, 60, 64, 64, dtype)
+    dout = rows((2, 2, 40, 64), 6, dtype)
+    off = torch.tensor([-5, 10]).cuda()  # rows 0 .. 4 of the first sequence see nothing; its last key seen is 34
+    res = []
+    for bad in (0.0, math.inf):
+        ys = [x.clone() for x in xs]
+        for x in ys[2:]:
+            x[0, :, 35:] = bad
+            x[1, :, 50:] = bad
+        d = dout.clone()
+        d[0, :, :5] *= 1024.0 if bad else 0.0
+        ys = [y.requires_grad_() for y in ys]
+        tda_amd.differential_attention(*ys, 0.5, q_offset=off).backward(d)
+        res.append([y.grad for y in ys])
+    assert all(torch.equal(a, b) and b.isfinite().all() for a, b in zip(*res))
+    assert not any(g[0, :, 35:].any() or g[1, :, 50:].any() for g in res[1][2:])
