@@ -22,7 +22,7 @@ extern "C" {
 
 #define SDA_ABI_VERSION 1
 
-/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 (not as lambda_dtype) */
+/* element types beyond TDA_DTYPE_F32 / TDA_DTYPE_BF16 */
 #define SDA_DTYPE_F16 2
 
 /* error codes beyond those of tda.h */
@@ -51,7 +51,7 @@ typedef struct sda_fwd_args {
                                that their own rounding has */
   const void* lambda_param; /* element (b, h, i) at b ls[0] + h ls[1] + i ls[2] */
   int64_t lambda_stride[3]; /* 0: the same along that axis */
-  int32_t lambda_dtype;     /* TDA_DTYPE_F32 or TDA_DTYPE_BF16 */
+  int32_t lambda_dtype;     /* as dtype, but of its own */
   int32_t reserved;
   int64_t q_offset;         /* off_b, unless q_offsets is given */
   const int32_t* q_offsets; /* optional (batch): off_b */

@@ -768,8 +768,9 @@ __global__ void __launch_bounds__(256) bwd_lambda(BwdParams P) {
     a = tda::wave_sum(a);
     if (id & 63) return;
   }
-  if (P.lam.bf16) static_cast<bf16*>(P.dlam)[e] = (bf16)a;
-  else static_cast<float*>(P.dlam)[e] = a;
+  if (P.lam.type == 0) static_cast<float*>(P.dlam)[e] = a;
+  else if (P.lam.type == 1) static_cast<bf16*>(P.dlam)[e] = (bf16)a;
+  else static_cast<_Float16*>(P.dlam)[e] = (_Float16)a;
 }
 
 // ------------------------------------------------------------------ launches

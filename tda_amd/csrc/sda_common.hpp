@@ -96,7 +96,9 @@ __device__ __forceinline__ T* row_of(const Rows& r, int b, int h, int64_t i) {
 }
 __device__ __forceinline__ float lambda_of(const Lambda& l, int b, int h, int i) {
   const int64_t at = (int64_t)b * l.sb + (int64_t)h * l.sh + (int64_t)i * l.si;
-  return l.bf16 ? (float)static_cast<const bf16*>(l.p)[at] : static_cast<const float*>(l.p)[at];
+  return l.type == 0   ? static_cast<const float*>(l.p)[at]
+         : l.type == 1 ? (float)static_cast<const bf16*>(l.p)[at]
+                       : (float)static_cast<const _Float16*>(l.p)[at];
 }
 __device__ __forceinline__ int len_of(const Sight& s, int b, int Nk) {
   return s.lens ? min(max(s.lens[b], 0), Nk) : Nk;

@@ -18,6 +18,7 @@ constexpr double kLog2e = 1.4426950408889634074;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
+bool any_dtype(int32_t t) { return t == TDA_DTYPE_F32 || t == TDA_DTYPE_BF16 || t == SDA_DTYPE_F16; }
 int64_t bytes_of(int32_t dtype) { return dtype == TDA_DTYPE_F32 ? 4 : 2; }
 
 // A (B, H, N, width) tensor whose rows the kernels read in 16-byte pieces (fine: any alignment of
@@ -38,7 +39,7 @@ bool head_dims(int64_t d, int64_t dv) {
 }
 int32_t check_lambda(const void* p, const int64_t (&s)[3], int32_t dtype) {
   if (!p) return TDA_ERR_NULL_POINTER;
-  if (dtype != TDA_DTYPE_F32 && dtype != TDA_DTYPE_BF16) return TDA_ERR_DTYPE;
+  if (!any_dtype(dtype)) return TDA_ERR_DTYPE;
   for (int64_t x : s)
     if (x < 0 || x > kMaxStride) return TDA_ERR_LAYOUT;
   return reinterpret_cast<uintptr_t>(p) % bytes_of(dtype) ? TDA_ERR_LAYOUT : TDA_OK;
@@ -74,7 +75,7 @@ int32_t check_sizes(const A& a) {
 template <class A>
 int32_t check_common(const A& a) {
   if (a.abi_version != SDA_ABI_VERSION) return TDA_ERR_ABI;
-  if (a.dtype != TDA_DTYPE_F32 && a.dtype != TDA_DTYPE_BF16 && a.dtype != SDA_DTYPE_F16) return TDA_ERR_DTYPE;
+  if (!any_dtype(a.dtype)) return TDA_ERR_DTYPE;
   if (a.causal != 0 && a.causal != 1) return TDA_ERR_CAUSAL;
   if (!check_scale(a.scale)) return SDA_ERR_SCALE;
   if (int32_t rc = check_sizes(a)) return rc;
@@ -92,7 +93,7 @@ int32_t check_kept(const A& a) {
 
 sda::Rows rows_of(const tda_tensor& t) { return {t.data, t.stride[0], t.stride[1], t.stride[2]}; }
 sda::Lambda lambda_of(const void* p, const int64_t (&s)[3], int32_t dtype) {
-  return {p, s[0], s[1], s[2], dtype == TDA_DTYPE_BF16 ? 1 : 0};
+  return {p, s[0], s[1], s[2], dtype};
 }
 
 // Few query rows go to the kernels that cut the key axis and read it once per 16 rows of the heads that share
@@ -184,7 +185,6 @@ int32_t check_cache(const sda_kv4& c) {
     if (reinterpret_cast<uintptr_t>(p) % 16) return TDA_ERR_LAYOUT;
   return reinterpret_cast<uintptr_t>(c.lengths) % 4 ? TDA_ERR_LAYOUT : TDA_OK;
 }
-bool any_dtype(int32_t t) { return t == TDA_DTYPE_F32 || t == TDA_DTYPE_BF16 || t == SDA_DTYPE_F16; }
 void fill_cache(sda::Kv4Params& p, const sda_kv4& c) {
   void* at[3] = {c.k1, c.k2, c.v};
   for (int z = 0; z < 3; ++z) {

@@ -14,7 +14,7 @@ struct Rows {     // a (B, H, N, width) tensor: element strides of the batch, he
 struct Lambda {   // element (b, h, i)
   const void* p;
   int64_t sb, sh, si;
-  int bf16;       // 1: bf16, 0: f32
+  int type;       // 0 f32, 1 bf16, 2 f16
 };
 
 // Who sees what: row i of sequence b stands at off(b) + i and sees key j when j < len(b) and

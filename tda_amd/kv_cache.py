@@ -89,9 +89,11 @@ class Int4KVCache:
 
     def _signature(self, *tensors):
         """What a call's plan goes by (the lengths' form among it), or None."""
-        for t in tensors:
+        for t in (self.lengths, *tensors):
             if t is not None and type(t) not in _TENSORS:
                 return None
+        if self.lengths is None:
+            return None
         return _sig(self.lengths), *[None if t is None else _sig(t) for t in tensors]
 
     def _planned(self, key, rows):

@@ -97,8 +97,8 @@ def _lambda(lam, b: int, h: int, n: int, device) -> torch.Tensor:
         raise ValueError(f"lambda_param must be a scalar, ({h},) or broadcast to ({b}, {h}, {n}), got {tuple(lam.shape)}")
     if not lam.dtype.is_floating_point:
         raise ValueError(f"lambda_param must be floating-point, got {lam.dtype}")
-    if lam.device != device or lam.dtype not in (torch.float32, torch.bfloat16):
-        lam = lam.to(device=device, dtype=lam.dtype if lam.dtype == torch.bfloat16 else torch.float32)
+    if lam.device != device or lam.dtype not in _CODE:
+        lam = lam.to(device=device, dtype=lam.dtype if lam.dtype in _CODE else torch.float32)
     return lam
 
 

@@ -113,7 +113,7 @@ static void attention() {
   sda_fwd_args f = fwd_args();
   f.q_offset = 200;
   CHECK(sda_fwd(&f, nullptr) == TDA_OK && got::forwards == 1 && got::fwd.see.qoff == 200 && got::fwd.Hk == 2);
-  CHECK(got::fwd.v.sb == f.v.stride[0] && got::fwd.part == nullptr && got::fwd.lam.bf16 == 0);
+  CHECK(got::fwd.v.sb == f.v.stride[0] && got::fwd.part == nullptr && got::fwd.lam.type == 0);
   f = fwd_args(1, 4000);  // one token: parts of the keys
   CHECK(f.workspace_bytes > 0 && sda_fwd(&f, nullptr) == TDA_OK && got::decodes == 1 && got::fwd.nsplit > 1);
   CHECK(got::fwd.chunk % 128 == 0 && (int64_t)got::fwd.chunk * got::fwd.nsplit >= 4000 &&
@@ -151,7 +151,7 @@ static void attention() {
   REFUSES(fwd_args(), sda_validate_fwd, a.q_offsets = reinterpret_cast<int32_t*>(AT + 2), TDA_ERR_LAYOUT);
   REFUSES(fwd_args(), sda_validate_fwd, a.kv_lens = reinterpret_cast<int32_t*>(AT + 1), TDA_ERR_LAYOUT);
   REFUSES(fwd_args(), sda_validate_fwd, a.lambda_param = nullptr, TDA_ERR_NULL_POINTER);
-  REFUSES(fwd_args(), sda_validate_fwd, a.lambda_dtype = SDA_DTYPE_F16, TDA_ERR_DTYPE);
+  REFUSES(fwd_args(), sda_validate_fwd, a.lambda_dtype = 3, TDA_ERR_DTYPE);
   REFUSES(fwd_args(), sda_validate_fwd, a.lambda_stride[2] = -1, TDA_ERR_LAYOUT);
   REFUSES(fwd_args(1, 4000), sda_validate_fwd, a.workspace = nullptr, TDA_ERR_WORKSPACE);
   REFUSES(fwd_args(1, 4000), sda_validate_fwd, --a.workspace_bytes, TDA_ERR_WORKSPACE);
@@ -276,7 +276,7 @@ static void held() {
   sda_kv4_read_args r = read_args();
   CHECK(sda_kv4_read(&r, nullptr) == TDA_OK && got::reads == 1 && got::kv4.rows == 70);
   sda_kv4_attend_args t = attend_args();
-  CHECK(t.workspace_bytes > 0 && sda_kv4_attend(&t, nullptr) == TDA_OK && got::attends == 1 && got::kv4.lam.bf16 == 1);
+  CHECK(t.workspace_bytes > 0 && sda_kv4_attend(&t, nullptr) == TDA_OK && got::attends == 1 && got::kv4.lam.type == 1);
   CHECK(got::kv4.chunk % 128 == 0 && (int64_t)got::kv4.chunk * got::kv4.nsplit >= 700);
   got::fail_with = 2;
   CHECK(sda_kv4_attend(&t, nullptr) == TDA_ERR_HIP);

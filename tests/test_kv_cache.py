@@ -362,9 +362,10 @@ def test_calls_of_one_signature_take_their_own_tensors():
     c.lengths.fill_(4)
     d.lengths.fill_(4)
     assert torch.equal(c.attend(q1, q2, lam), d.attend(q1, q2, lam))
-    c.lengths = c.lengths.long()
-    with pytest.raises(ValueError, match="lengths"):
-        c.attend(q1, q2, lam)
+    for wrong in (c.lengths.long(), None, [4, 4]):
+        c.lengths = wrong
+        with pytest.raises(ValueError, match="lengths"):
+            c.attend(q1, q2, lam)
     with pytest.raises(ValueError):
         d.attend(q1, q2, lam[:1].expand(3))
     with pytest.raises(ValueError):

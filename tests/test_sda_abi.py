@@ -101,7 +101,7 @@ BAD_ROWS = [
     (lambda a: setattr(a, "batch", 1 << 29), _abi.ERR_SHAPE),
     (lambda a: setattr(a, "lambda_param", None), _abi.ERR_NULL_POINTER),
     (lambda a: setattr(a, "lambda_param", FAKE + 2), _abi.ERR_LAYOUT),
-    (lambda a: setattr(a, "lambda_dtype", 2), _abi.ERR_DTYPE),
+    (lambda a: setattr(a, "lambda_dtype", 3), _abi.ERR_DTYPE),
     (lambda a: a.lambda_stride.__setitem__(1, -1), _abi.ERR_LAYOUT),
     (lambda a: setattr(a.q2, "data", None), _abi.ERR_NULL_POINTER),
     (lambda a: setattr(a.v, "data", FAKE + 8), _abi.ERR_LAYOUT),

@@ -163,7 +163,7 @@ def test_offsets_of_each_sequence(n, train):
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("shape", ["scalar", "one", "heads", "rows", "batch", "per_batch_head", "expanded"])
-@pytest.mark.parametrize("lam_dtype", [BF, F32])
+@pytest.mark.parametrize("lam_dtype", [BF, F32, F16])
 def test_lambda_of_every_shape(dtype, shape, lam_dtype):
     b, h, n = 2, 3, 45
     g = torch.Generator("cpu").manual_seed(9)
