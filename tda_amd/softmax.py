@@ -3,8 +3,9 @@
     out = (softmax(s q1 k1^T + M) - lambda softmax(s q2 k2^T + M)) v
 
 beside the threshold form of api.py.  Forward and backward run in hand-written kernels behind
-include/sda.h (float32, bfloat16, float16; float64 is computed in float32, as by the threshold operators); a call of few query rows, such as a decoding step, takes kernels that split the
-key axis.  There is no CPU fallback.
+include/sda.h (float32, bfloat16, float16; float64 is computed in float32, as by the threshold
+operators); a call of few query rows, such as a decoding step, takes kernels that split the key axis.
+There is no CPU fallback.
 """
 from __future__ import annotations
 

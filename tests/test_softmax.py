@@ -354,13 +354,13 @@ def test_same_bits_every_time():
 
 
 @gpu
-@pytest.mark.parametrize("n, nk", [(1, 3000), (260, 260)])
-def test_captured(n, nk):
+@pytest.mark.parametrize("n, nk, dtype", [(1, 3000, BF), (260, 260, BF), (260, 260, F16)])
+def test_captured(n, nk, dtype):
     """Graphs of the forward and of a training step, replayed between eager work and compared with it."""
-    xs = [x.requires_grad_(n > 1) for x in inputs(2, 4, 2, n, nk, 64, 64, BF)]
+    xs = [x.requires_grad_(n > 1) for x in inputs(2, 4, 2, n, nk, 64, 64, dtype)]
     lens = torch.tensor([nk, nk - 7], dtype=torch.int32).cuda()
     lam = torch.full((4,), 0.5, device="cuda", requires_grad=n > 1)
-    dout = rows((2, 4, n, 64), 6)
+    dout = rows((2, 4, n, 64), 6, dtype)
 
     def step():
         out = tda_amd.differential_attention(*xs, lam, kv_lens=lens)
