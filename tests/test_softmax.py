@@ -580,3 +580,62 @@ def test_rows_that_count_for_nothing(dtype):
         res.append([y.grad for y in ys])
     assert all(torch.equal(a, b) and b.isfinite().all() for a, b in zip(*res))
     assert not any(g[0, :, 35:].any() or g[1, :, 50:].any() for g in res[1][2:])
+
+
+def overlapping(x, step):
+    """Rows `step` values apart over x's first row (0: that row for every position)."""
+    b, h, n, d = x.shape
+    flat = torch.cat((x[:, :, 0], rows((b, h, n * step, 1), 77, x.dtype)[..., 0]), -1)
+    return flat.as_strided(x.shape, (flat.stride(0), flat.stride(1), step, 1))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+@pytest.mark.parametrize("d, dv", DIMS)
+@pytest.mark.parametrize("n", [1, 33, 50, 129])
+@pytest.mark.parametrize("causal", [True, False])
+def test_upstream_gradient_broadcast_along_the_sequence(dtype, d, dv, n, causal):
+    """As out.sum(2) or a mean over the sequence hands it down (rows with a stride of 0, or that overlap): the
+    gradients of its contiguous copy, to the bit."""
+    xs = inputs(2, 4, 2, n, n, d, dv, dtype)
+
+    def step(dout):
+        ys = [x.detach().requires_grad_() for x in xs]
+        return torch.autograd.grad(tda_amd.differential_attention(*ys, 0.5, causal=causal), ys, dout)
+
+    up = rows((2, 4, n, dv), 6, dtype)
+    for dout in (up[:, :, :1].expand(-1, -1, n, -1), overlapping(up, 8)):
+        assert all(torch.equal(a, b) for a, b in zip(step(dout), step(dout.contiguous())))
+
+
+@gpu
+def test_mean_over_the_sequence():
+    xs = [x.requires_grad_() for x in inputs(2, 4, 2, 50, 50, 64, 64, F32)]
+    up = rows((2, 4, 1, 64), 6, F32)
+    tda_amd.differential_attention(*xs, 0.5).mean(2).backward(up[:, :, 0])
+    ref = oracle.attention(*xs, 0.5, u=U[F32], dout=(up / 50).expand(-1, -1, 50, -1))
+    for x, name in zip(xs, ("dq1", "dq2", "dk1", "dk2", "dv")):
+        within(x.grad, ref, name, U[F32])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+@pytest.mark.parametrize("n, nk", [(1, 300), (50, 50), (129, 200)])
+@pytest.mark.parametrize("by", [1.0, 12.0])
+@pytest.mark.parametrize("step", [0, 8])
+def test_rows_that_overlap(dtype, n, nk, by, step):
+    """Every input with rows that are one row, or lie a few values apart; with scores of several hundreds too."""
+    xs = inputs(2, 4, 2, n, nk, 64, 128, dtype)
+    xs = [overlapping(x * by if k < 2 else x, step) for k, x in enumerate(xs)]
+    lens = torch.tensor([nk, nk - 7], dtype=torch.int32).cuda()
+    dout = rows((2, 4, n, 128), 6, dtype)
+
+    def run(ys):
+        ys = [y.detach().requires_grad_() for y in ys]
+        with torch.no_grad():
+            plain = tda_amd.differential_attention(*ys, 0.5, kv_lens=lens)
+        out = tda_amd.differential_attention(*ys, 0.5, kv_lens=lens)
+        return [plain, out.detach(), *torch.autograd.grad(out, ys, dout)]
+
+    got, want = run(xs), run([x.contiguous() for x in xs])
+    assert all(g.isfinite().all() and torch.equal(g, w) for g, w in zip(got, want))
