@@ -36,7 +36,8 @@ class Int4KVCache:
 
     `lengths` (int32, (batch,), on the device) counts the rows each sequence holds; the calls read and
     write it on the GPU, without synchronising, so they can be captured into a graph.  A program may set
-    it, to drop rows or to hand a place to another sequence.  The cache carries no gradient."""
+    it, to drop rows or to hand a place to another sequence.  The cache carries no gradient.  copy.deepcopy and
+    pickling give a cache with rows and lengths of its own."""
 
     def __init__(self, batch: int, kv_heads: int, capacity: int, head_dim: int, v_head_dim: int | None = None, *,
                  device="cuda"):
@@ -61,6 +62,15 @@ class Int4KVCache:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self._templates: dict = {}  # argument blocks by configuration
         self._plans: dict = {}      # of calls whose tensors need no copy, by their signature: no checks again
+
+    def __getstate__(self):
+        return {**self.__dict__, "_templates": {}, "_plans": {}}  # a copy has buffers of its own: their addresses too
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self._held[0].device  # a loaded cache may have been sent elsewhere
+        if self.device.type != "cuda":
+            raise ValueError(f"tda_amd runs on the GPU only (HIP); got a cache on {self.device}")
 
     # -------------------------------------------------------------- calls
     def _cache(self) -> _sda_abi.SdaKv4:

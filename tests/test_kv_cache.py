@@ -1,6 +1,8 @@
 """The 4-bit cache (tda_amd.Int4KVCache): what it holds against the definition, exactly; the attention over
 it against float64 on the values held, within the bounds of oracle/softmax.py."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -370,3 +372,34 @@ def test_calls_of_one_signature_take_their_own_tensors():
         d.attend(q1, q2, lam[:1].expand(3))
     with pytest.raises(ValueError):
         d.append(xs[0], xs[1].cpu(), xs[2])
+
+
+@gpu
+@pytest.mark.parametrize("fork", [copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))])
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_copy_has_its_own_rows(fork, n):
+    """A cache forked after calls of every kind: both go on by themselves, also with calls of signatures that the
+    original has seen."""
+    def step(c, seed):
+        c.append(*context(2, 2, n, 64, 128, BF, seed))
+        q = rows(2, 4, n, 64, seed + 5, BF)
+        return [c.attend(q, q * 0.5, lam), *c.read(), c.lengths.clone()]
+
+    lam = torch.tensor([0.1, 0.2, 0.3, 0.4]).cuda()
+    first = tda_amd.Int4KVCache(2, 2, 200, 64, 128)
+    step(first, 0)
+    second = fork(first)
+    got = [step(second, 10), step(first, 20), step(second, 30), step(first, 40)]
+    for k, seeds in enumerate(((0, 10, 30), (0, 20, 40))):
+        alone = tda_amd.Int4KVCache(2, 2, 200, 64, 128)
+        want = [step(alone, s) for s in seeds][1:]
+        assert all(torch.equal(a, b) for x, y in zip(got[k::2], want) for a, b in zip(x, y))
+
+
+def test_a_copy_keeps_no_addresses():
+    c = tda_amd.Int4KVCache.__new__(tda_amd.Int4KVCache)
+    c._held, c._templates, c._plans = [torch.zeros(8)], {"a": b"1"}, {"b": b"2"}
+    state = c.__getstate__()
+    assert state["_templates"] == state["_plans"] == {} and c._templates and c._plans
+    with pytest.raises(ValueError, match="GPU only"):
+        copy.deepcopy(c)  # rows on the CPU, as a cache loaded there would have
