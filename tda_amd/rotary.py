@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _sda_abi, ops
-from .softmax import _CODE, _TENSORS, _free_of_grad, _launch, _new_rows, _sig
+from .softmax import _CODE, _TENSORS, _free_of_grad, _launch, _new_rows, _refuse_tangents, _sig
 
 _PUT = struct.Struct("<Q").pack_into
 _OFF = {n: getattr(_sda_abi.SdaRotaryArgs, n).offset for n in ("x", "y", "positions", "inv_freq")}
@@ -89,9 +89,10 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
     each rotated pair.  sections: how many pairs turn by each axis, in order; pair p of a row turns by
     positions[axis of p] * inv_freq[p].  The 2 len(inv_freq) first values of a row are rotated, the rest
     copied.  A pair is (p, p + len(inv_freq)), with interleaved (2 p, 2 p + 1).  The angle is taken in 64
-    bits.  Gradients flow to xs."""
+    bits.  Gradients flow to xs; second derivatives and forward-mode derivatives raise."""
     one = isinstance(xs, torch.Tensor)
     ts = (xs,) if one else tuple(xs)
+    _refuse_tangents("rotary_axes", inv_freq, *ts)
     key = None
     if type(positions) is torch.Tensor and type(inv_freq) is torch.Tensor and all(type(t) in _TENSORS for t in ts):
         key = (tuple([_sig(t) for t in ts]), _sig(positions), _sig(inv_freq), tuple(sections), bool(interleaved))

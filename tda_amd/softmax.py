@@ -15,6 +15,7 @@ import struct
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _abi, _sda_abi, ops
@@ -194,6 +195,16 @@ def _free_of_grad(*tensors) -> bool:
     return not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors)
 
 
+def _refuse_tangents(what: str, *tensors):
+    """A forward-mode derivative is refused, not dropped: a dual tensor need not require a gradient, so the calls that
+    leave the autograd function out would return it without its tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _plan_key(rows, lam, scale, causal, q_offset, kv_lens):
     """The signature of a forward call that may have a plan, or None."""
     if type(lam) not in _TENSORS or not (q_offset is None or type(q_offset) is int) or not (scale is None or type(scale) is float):
@@ -319,8 +330,11 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     causal it sees the keys up to its position; with kv_lens (int32/int64, (batch,), clamped to [0,
     seq_len_kv]) only the first kv_lens[b].  A row that sees no key is zero, with zero gradients, and
     keys that no row of the call sees may hold anything.  (A NaN or infinite value row reaches the rows
-    that see it, and may reach other rows of the same call that stand before it.)"""
+    that see it, and may reach other rows of the same call that stand before it.)
+
+    Gradients flow to every tensor; second derivatives and forward-mode derivatives raise."""
     tensors, names = (q1, q2, k1, k2, v), ("q1", "q2", "k1", "k2", "v")
+    _refuse_tangents("differential_attention", *tensors, lambda_param)
     key = _plan_key(tensors, lambda_param, scale, causal, q_offset, kv_lens)
     plan = _plans.get(key) if key is not None else None
     if plan is not None and _free_of_grad(*tensors, lambda_param):

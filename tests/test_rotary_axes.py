@@ -155,3 +155,18 @@ def test_calls_of_one_signature_take_their_own_tensors():
         tda_amd.rotary_axes([xs[0], xs[1].half()], pos, freq, (32,))
     with pytest.raises(ValueError):
         tda_amd.rotary_axes(xs, pos, freq, (31,))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_is_refused(device):
+    from torch.autograd import forward_ad
+    x, pos, freq = torch.ones(1, 2, 3, 64, device=device), torch.ones(1, 1, 3, dtype=torch.int64, device=device), torch.ones(32, device=device)
+    if device == "cuda":
+        tda_amd.rotary_axes([x, x], pos, freq, (32,))  # later calls of this signature skip the checks
+    with forward_ad.dual_level():
+        y, f = forward_ad.make_dual(x, x), forward_ad.make_dual(freq, freq)
+        for xs, by in (([x, y], freq), ([y, x], freq), ([x, x], f), (y, freq)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                tda_amd.rotary_axes(xs, pos, by, (32,))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: tda_amd.rotary_axes(t, pos, freq, (32,)), (x,), (x,))

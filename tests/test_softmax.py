@@ -639,3 +639,27 @@ def test_rows_that_overlap(dtype, n, nk, by, step):
 
     got, want = run(xs), run([x.contiguous() for x in xs])
     assert all(g.isfinite().all() and torch.equal(g, w) for g, w in zip(got, want))
+
+
+def duals(device):
+    """Calls of differential_attention in which one argument has a tangent."""
+    from torch.autograd import forward_ad
+    xs = [torch.randn(1, 2, 5, 64, device=device) for _ in range(5)] + [torch.full((2,), 0.5, device=device)]
+    with torch.no_grad():
+        if device == "cuda":
+            tda_amd.differential_attention(*xs)  # later calls of this signature skip the checks
+    for i in range(6):
+        with forward_ad.dual_level():
+            yield [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate(xs)]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(device, grad):
+    with torch.set_grad_enabled(grad):
+        for xs in duals(device):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                tda_amd.differential_attention(*xs)
+        q, k, v = xs[0], xs[2], xs[4]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: tda_amd.differential_attention(t, q, k, k, v, 0.5), (q,), (q,))
