@@ -93,9 +93,10 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
     one = isinstance(xs, torch.Tensor)
     ts = (xs,) if one else tuple(xs)
     _refuse_tangents("rotary_axes", inv_freq, *ts)
+    sections = tuple([int(s) for s in sections])
     key = None
     if type(positions) is torch.Tensor and type(inv_freq) is torch.Tensor and all(type(t) in _TENSORS for t in ts):
-        key = (tuple([_sig(t) for t in ts]), _sig(positions), _sig(inv_freq), tuple(sections), bool(interleaved))
+        key = (tuple([_sig(t) for t in ts]), _sig(positions), _sig(inv_freq), sections, bool(interleaved))
         plan = _plans.get(key)
         if plan is not None and _free_of_grad(inv_freq, *ts):
             ys = tuple([torch.empty_strided(t.shape, st, dtype=t.dtype, device=t.device) for t, st in zip(ts, plan[1])])
@@ -118,7 +119,6 @@ def rotary_axes(xs, positions, inv_freq, sections, *, interleaved=False):
         raise ValueError(f"tda_amd runs on the GPU only (HIP); got tensors on {dev}")
     if ref.dtype not in _CODE:
         raise ValueError(f"xs must be float32, bfloat16 or float16, got {ref.dtype}")
-    sections = tuple(int(s) for s in sections)
     if not 1 <= len(sections) <= _sda_abi.MAX_AXES or min(sections) < 0:
         raise ValueError(f"sections must be 1 to {_sda_abi.MAX_AXES} counts of pairs, got {sections}")
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:

@@ -170,3 +170,11 @@ def test_forward_mode_is_refused(device):
                 tda_amd.rotary_axes(xs, pos, by, (32,))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: tda_amd.rotary_axes(t, pos, freq, (32,)), (x,), (x,))
+
+
+@gpu
+def test_sections_of_any_iterable():
+    xs, pos, freq = setup(2, (3,), 5, 64, 64, (16, 8, 8), torch.float32)
+    want = tda_amd.rotary_axes(xs[0], pos, freq, (16, 8, 8))
+    for sections in ([16, 8, 8], iter((16, 8, 8)), (n for n in (16, 8, 8)), torch.tensor([16, 8, 8])):
+        assert torch.equal(tda_amd.rotary_axes(xs[0], pos, freq, sections), want)
