@@ -29,7 +29,8 @@ extern "C" {
 #define SDA_ERR_HEADS   -20  /* heads not a multiple of kv_heads */
 #define SDA_ERR_SCALE   -21  /* scale not in 1e-30 .. 1e30 */
 #define SDA_ERR_AXES    -22  /* axes, sections or rotated width out of range */
-#define SDA_ERR_CACHE   -23  /* 4-bit cache: capacity, lengths or row count out of range */
+#define SDA_ERR_CACHE   -23  /* 4-bit cache: capacity, lengths or row count out of range, or start or
+                                counts overlapping lengths */
 
 /* Softmax differential attention.  Query row i of sequence b stands at position off_b + i and
  * sees key j when j < len_b and (causal) j <= off_b + i; a row that sees no key is zero.  Keys
@@ -133,7 +134,8 @@ typedef struct sda_kv4_append_args {
   const int32_t* counts;    /* optional (batch): rows of each sequence that count (clamped to
                                [0, n]); NULL: n */
 } sda_kv4_append_args;      /* rows at start + i < capacity are written; lengths becomes
-                               min(start + count, capacity) */
+                               min(start + count, capacity).  start and counts may be lengths, but no
+                               other array that overlaps it */
 
 typedef struct sda_kv4_read_args {
   int32_t abi_version;

@@ -219,7 +219,7 @@ const char* sda_error_string(int32_t code) {
     case SDA_ERR_HEADS: return "heads must be a multiple of kv_heads";
     case SDA_ERR_SCALE: return "scale must be finite and positive (1e-30 to 1e30)";
     case SDA_ERR_AXES: return "axes, sections or rotated width out of range";
-    case SDA_ERR_CACHE: return "4-bit cache: capacity, lengths or row count out of range";
+    case SDA_ERR_CACHE: return "4-bit cache: capacity, lengths or row count out of range, or start or counts overlapping lengths";
     case TDA_ERR_HEAD_DIM: return "(head_dim, v_head_dim) must be (64, 64), (64, 128), (128, 128) or (128, 256)";
     case TDA_ERR_CAUSAL: return "causal must be 0 or 1";
     case TDA_ERR_LAYOUT: return "rows must have a unit last stride, 16-byte alignment and at most 2^25 bytes between them";
@@ -375,7 +375,14 @@ int32_t sda_validate_kv4_append(const sda_kv4_append_args* a) {
   if (a->rows < 1 || a->rows > a->cache.capacity) return SDA_ERR_CACHE;
   for (const tda_tensor* t : {&a->k1, &a->k2, &a->v})
     if (int32_t rc = check_rows(*t, bytes_of(a->dtype))) return rc;
-  return check_words({a->start, a->counts});
+  if (int32_t rc = check_words({a->start, a->counts})) return rc;
+  // The call writes the lengths while others of its workgroups read start and counts: these may be the lengths
+  // themselves (a launch of its own then writes them), but no other part of them.
+  for (const int32_t* p : {a->start, a->counts}) {
+    const int64_t apart = (int64_t)(reinterpret_cast<intptr_t>(p) - reinterpret_cast<intptr_t>(a->cache.lengths));
+    if (p && apart && apart > -4 * a->cache.batch && apart < 4 * a->cache.batch) return SDA_ERR_CACHE;
+  }
+  return TDA_OK;
 }
 int32_t sda_kv4_append(const sda_kv4_append_args* a, void* stream) {
   if (int32_t rc = sda_validate_kv4_append(a)) return rc;

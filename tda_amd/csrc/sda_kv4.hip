@@ -161,14 +161,15 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P, int blocks) {
       if ((u & 7) == 0) pars[((uint32_t)at << (shift - 3)) + (u >> 3)] = bad ? 0x7fc0u : mb | sb << 16;
     }
   }
-  if (P.start && z == 0 && hk == 0 && i0 == 0 && u == 0)
+  if (P.start && P.counts != P.lengths && z == 0 && hk == 0 && i0 == 0 && u == 0)  // else kv4_lengths
     P.lengths[b] = (int)min(max((int64_t)start + count, (int64_t)0), (int64_t)P.cap);
 }
 __global__ void kv4_lengths(Kv4Params P) {
   const int b = blockIdx.x * 64 + threadIdx.x;
   if (b >= P.B) return;
+  const int64_t start = P.start ? P.start[b] : max(P.lengths[b], 0);
   const int count = P.counts ? min(max(P.counts[b], 0), P.rows) : P.rows;
-  P.lengths[b] = (int)min((int64_t)max(P.lengths[b], 0) + count, (int64_t)P.cap);
+  P.lengths[b] = (int)min(max(start + count, (int64_t)0), (int64_t)P.cap);
 }
 
 // ------------------------------------------------------------------ read
@@ -482,7 +483,7 @@ int launch_kv4_append(const Kv4Params& p, int dtype, void* stream) {
   else if (dtype == 1) append<bf16>(p, st);
   else append<_Float16>(p, st);
   tda::launched(st, "sda_kv4_append");
-  if (!p.start) {  // every workgroup above reads the lengths
+  if (!p.start || p.counts == p.lengths) {  // every workgroup above reads the lengths
     kv4_lengths<<<dim3((unsigned)((p.B + 63) / 64)), 64, 0, st>>>(p);
     tda::launched(st, "sda_kv4_lengths");
   }

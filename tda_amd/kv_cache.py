@@ -142,7 +142,8 @@ class Int4KVCache:
         Row i of sequence b goes to position lengths[b] + i, or start[b] + i where start (int32/int64,
         (batch,)) is given, for i < counts[b] (all n by default; rows past it are padding and are not
         read); lengths[b] becomes the position behind the last one.  Positions outside 0 .. capacity - 1
-        are dropped, and lengths stops at the capacity: a caller that must not lose rows keeps count."""
+        are dropped, and lengths stops at the capacity: a caller that must not lose rows keeps count.  start and
+        counts may be `lengths` itself, but no other tensor that overlaps it."""
         key = self._signature(k1, k2, v, start, counts)
         plan = self._planned(key, (k1, k2, v)) if key is not None else None
         if plan is not None:

@@ -403,3 +403,40 @@ def test_a_copy_keeps_no_addresses():
     assert state["_templates"] == state["_plans"] == {} and c._templates and c._plans
     with pytest.raises(ValueError, match="GPU only"):
         copy.deepcopy(c)  # rows on the CPU, as a cache loaded there would have
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 300])
+@pytest.mark.parametrize("given", [None, [0, 0, 0], [700, 5, 1], [900, 0, -4]])
+def test_append_counts_that_are_the_lengths(n, given):
+    """As with a copy of them, whichever workgroup comes last."""
+    caches = [tda_amd.Int4KVCache(3, 16, 1000, 128, 256) for _ in range(2)]
+    start = None if given is None else torch.tensor(given, dtype=torch.int32).cuda()
+    xs = context(3, 16, n, 128, 256, BF, 1)
+    for c in caches:
+        c.append(*context(3, 16, 1000, 128, 256, BF, 4))
+    for k in range(4):
+        for c in caches:
+            c.lengths.copy_(torch.tensor([n // 2, n, n // 3 + k]))
+        caches[0].append(*xs, counts=caches[0].lengths, start=start)
+        caches[1].append(*xs, counts=caches[1].lengths.clone(), start=start)
+        assert torch.equal(caches[0].lengths, caches[1].lengths)
+        if start is not None:
+            assert caches[0].lengths.tolist() == [min(max(s + m, 0), 1000) for s, m in zip(given, (n // 2, n, min(n // 3 + k, n)))]
+        for c in caches:
+            c.lengths.fill_(1000)
+        assert all(torch.equal(a, b) for a, b in zip(caches[0].read(), caches[1].read()))
+
+
+@gpu
+def test_append_lengths_as_part_of_another_tensor():
+    c = tda_amd.Int4KVCache(2, 1, 8, 64)
+    shared = torch.zeros(3, dtype=torch.int32).cuda()
+    c.lengths = shared[:2]
+    xs = context(2, 1, 1, 64, 64, BF)
+    c.append(*xs, start=shared[:2])
+    assert shared.tolist() == [1, 1, 0]
+    for kw in (dict(start=shared[1:]), dict(counts=shared[1:])):
+        with pytest.raises(ValueError, match="overlapping"):
+            c.append(*xs, **kw)
+    assert shared.tolist() == [1, 1, 0]

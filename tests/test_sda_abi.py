@@ -246,3 +246,13 @@ def test_cache_sizes_and_error_strings():
     assert so.sda_kv4_bytes(2, 3, 10, 96) == so.sda_kv4_bytes(0, 3, 10, 64) == 0
     texts = [so.sda_error_string(c).decode() for c in (*range(-13, 0), *range(-23, -19), -100)]
     assert all(texts) and len(set(texts[-5:])) == 5
+
+
+def test_append_refuses_arrays_that_overlap_the_lengths():
+    """The kernel writes the lengths while it reads start and counts."""
+    so = lib()
+    for name in ("start", "counts"):
+        for apart, code in ((0, _abi.OK), (4, _sda_abi.ERR_CACHE), (-4, _sda_abi.ERR_CACHE), (8, _abi.OK), (-8, _abi.OK)):
+            a = kv4(_sda_abi.SdaKv4AppendArgs)
+            setattr(a, name, FAKE + apart)
+            assert so.sda_validate_kv4_append(ctypes.byref(a)) == code, (name, apart)
