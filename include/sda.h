@@ -110,7 +110,7 @@ typedef struct sda_rotary_args {
 } sda_rotary_args;
 
 /* The 4-bit cache.  Each row of k1, k2 (d values) and v (dv values) is held in groups of 64
- * values x: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) in 32 bits, code =
+ * values x: m = bf16(min x), s = bf16((max x - m) / 15) in 32 bits, code =
  * min(max(rint((x - m) / s), 0), 15) (ties to even, 0 when s < 2^-100), value m + s code; a group with a NaN or an infinity, or whose
  * s is not finite, reads as NaN.  Three buffers of
  * sda_kv4_bytes() bytes each: for (b, head) the codes of capacity rows (rounded up to four; d / 2

@@ -124,10 +124,11 @@ def rotary(x, positions, inv_freq, sections, interleaved=False):
 
 def held4(x):
     """The values a 4-bit cache holds for rows x (..., width): groups of 64 with m = bf16(min), s =
-    bf16((max - m) (1 / 15)) rounded as 32-bit arithmetic rounds, codes decided in float64."""
+    bf16((max - m) / 15) rounded as 32-bit arithmetic rounds (the division in float64 first: torch multiplies 32-bit
+    values on a GPU by the rounded reciprocal of a number instead), codes decided in float64."""
     y = x.detach().float().unflatten(-1, (-1, 64))
     m = y.amin(-1, keepdim=True).bfloat16()
-    s = ((y.amax(-1, keepdim=True) - m.float()) * torch.tensor(1.0 / 15.0, dtype=torch.float32, device=x.device)).bfloat16()
+    s = ((y.amax(-1, keepdim=True) - m.float()).double() / 15.0).float().bfloat16()
     s = torch.where(s.float() >= 2.0 ** -100, s, 0.0).double()
     code = ((y.double() - m.double()) / torch.where(s > 0, s, 1.0)).round().clamp(0, 15) * (s > 0)
     val = m.double() + s * code

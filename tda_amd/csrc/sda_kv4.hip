@@ -1,6 +1,6 @@
 // sda_kv4.hip -- a key/value cache held in 4 bits: append, read, and the attention of few query rows.
 //
-// A row in groups of 64 values x: m = bf16(min), s = bf16((max - m) * (1 / 15)) in 32 bits,
+// A row in groups of 64 values x: m = bf16(min), s = bf16((max - m) / 15) in 32 bits,
 // code = rint((x - m) / s) clamped to 0 .. 15, value m + s code.  4.5 bits a value.
 //
 // Codes lie so that the attention's registers need no exchange between lanes and its loads are wide (the
@@ -48,6 +48,13 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     for (int e = 0; e < V; ++e) v[e] = (T)x[V * u + e];
     reinterpret_cast<vec*>(p)[u] = v;
   }
+}
+// x / 15, rounded once: the product by the rounded reciprocal, within a step of it, and its remainder, exact, by
+// the reciprocal again (compared with the division for every mantissa; that costs an append 3 % more).
+__device__ __forceinline__ float fifteenth(float x) {
+  constexpr float inv = 1.0f / 15.0f;
+  const float q = x * inv;
+  return x < __builtin_inff() ? __builtin_fmaf(__builtin_fmaf(-15.0f, q, x), inv, q) : x;
 }
 // rint((x - m) / s) with ties to the even code, decided exactly: x - m as an unevaluated sum hi + lo, the
 // nearest boundary p = (q + 1/2) s exact (q < 16, s of 8 bits), hi - p exact wherever its sign is in doubt.
@@ -138,7 +145,7 @@ __global__ void __launch_bounds__(256) kv4_append(Kv4Params P, int blocks) {
     hi = tda::group_max<8>(hi);
     const uint32_t mb = bf16_bits(lo);
     const float m = bf16_lo(mb);
-    uint32_t sb = bf16_bits((hi - m) * (1.0f / 15.0f));
+    uint32_t sb = bf16_bits(fifteenth(hi - m));
     float s = bf16_lo(sb);
     if (!(s >= kSmallStep)) s = 0.f, sb = 0;
     const bool bad = !(s < __builtin_inff()) || !(fabsf(m) < __builtin_inff());

@@ -30,7 +30,7 @@ def _from_codes(batch: int, kv_heads: int, rows: int, dtype) -> bool:
 class Int4KVCache:
     """The k1, k2 and v rows of up to `capacity` positions for each of `batch` sequences, 4.5 bits a value.
 
-    Every row is held in groups of 64 values x as m = bf16(min x), s = bf16((max x - m) * (1 / 15)) (in 32
+    Every row is held in groups of 64 values x as m = bf16(min x), s = bf16((max x - m) / 15) (in 32
     bits) and codes rint((x - m) / s) in 0 .. 15 (ties to even; all 0 when s < 2^-100); it stands for m + s
     code.  A group with a NaN or an infinity reads as NaN.  (head_dim, v_head_dim): (64, 64), (64, 128), (128, 128) or (128, 256).  capacity is at most 2^24.
 
