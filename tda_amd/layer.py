@@ -159,12 +159,25 @@ class DifferentialAttention(nn.Module):
         self.in_proj = nn.Linear(embed_dim, sum(h * w for h, w in zip(self._heads, self._widths)), bias=bias, **fk)
         self.out_proj = nn.Linear(num_heads * v_head_dim, embed_dim, bias=bias, **fk)
         self.lambda_param = nn.Parameter(torch.full((num_heads,), float(lambda_init), dtype=torch.float32, device=device))
-        self._inv_freq = float(rotary_base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        # on the CPU whatever the default device is: the frequencies have no copy in a checkpoint to come from
+        self._inv_freq = (float(rotary_base) ** (-torch.arange(pairs, dtype=torch.float64, device="cpu") / pairs)).float()
+        self._place()
 
-    def _frequencies(self, device) -> torch.Tensor:
-        """The pairs' frequencies, in 32 bits whatever type the module is cast to."""
-        if self._inv_freq.device != device or self._inv_freq.dtype != torch.float32:
-            self._inv_freq = self._inv_freq.to(device=device, dtype=torch.float32)
+    def _place(self):
+        """The pairs' frequencies, in 32 bits whatever type the module is cast to, beside the weights: a call must not
+        copy them from the host, which would make it wait and keep it out of a graph."""
+        device = self.in_proj.weight.device
+        if device.type != "meta" and self._inv_freq.device != device:
+            with torch.inference_mode(False):  # as a tensor that a training step may save
+                self._inv_freq = self._inv_freq.to(device)
+
+    def _apply(self, fn, *args, **kw):
+        super()._apply(fn, *args, **kw)
+        self._place()
+        return self
+
+    def _frequencies(self) -> torch.Tensor:
+        self._place()  # weights that were assigned, not moved
         return self._inv_freq
 
     def new_cache(self, batch: int, capacity: int) -> Int4KVCache:
@@ -206,7 +219,7 @@ class DifferentialAttention(nn.Module):
             positions = torch.arange(n, device=x.device).expand(len(self.rotary_sections), b, n)
             if cache is not None:
                 positions = positions + cache.lengths[:, None]
-        q1, q2, k1, k2 = rotary_axes((q1, q2, k1, k2), positions, self._frequencies(x.device), self.rotary_sections)
+        q1, q2, k1, k2 = rotary_axes((q1, q2, k1, k2), positions, self._frequencies(), self.rotary_sections)
         if cache is None:
             o = differential_attention(q1, q2, k1, k2, v, self.lambda_param, kv_lens=kv_lens)
         else:

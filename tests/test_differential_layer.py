@@ -220,3 +220,66 @@ def test_captured_decoding():
             assert torch.equal(out, m(now, cache=eager))
     assert own.lengths.tolist() == eager.lengths.tolist() == [12, 12]
     assert all(torch.equal(a, b) for a, b in zip(own.read(), eager.read()))
+
+
+# ------------------------------------------------------------------ the frequencies' place
+def test_frequencies_stay_beside_the_weights():
+    want = 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    with torch.device("meta"):
+        m = tda_amd.DifferentialAttention(96, 4, 64)
+    assert torch.equal(m._inv_freq, want.float())  # held on the CPU until the weights are somewhere
+    m = m.to_empty(device="cpu").to(BF)
+    assert m._inv_freq.dtype == F32 and torch.equal(m._frequencies(), want.float())
+    assert "_inv_freq" not in m.state_dict()
+
+
+@gpu
+def test_frequencies_move_with_the_module():
+    want = layer("cpu")._inv_freq
+    with torch.device("meta"):
+        empty = tda_amd.DifferentialAttention(96, 4, 64, kv_heads=2)
+    given = tda_amd.DifferentialAttention(96, 4, 64, kv_heads=2)
+    given.load_state_dict(layer().state_dict(), assign=True)
+    for m in (layer(), layer("cpu").cuda(), layer("cpu").to(device="cuda", dtype=BF), empty.to_empty(device="cuda"), given):
+        assert m._frequencies().is_cuda and m._inv_freq.dtype == F32 and torch.equal(m._inv_freq.cpu(), want)
+
+
+@gpu
+def test_the_first_call_neither_waits_nor_copies_from_the_host():
+    layer()(torch.zeros(1, 3, 96, device="cuda"))  # what the process sets up once
+    m = layer()
+    with torch.no_grad():
+        cache, other, x = m.new_cache(1, 8), m.new_cache(1, 8), torch.randn(1, 3, 96, device="cuda")
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            m(x, cache=cache)
+            m(x)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        fresh = layer()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = fresh(x, cache=other)
+        for k in range(3):
+            other.lengths.zero_()
+            x.mul_(0.9)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, m(x, cache=m.new_cache(1, 8)))
+
+
+@gpu
+def test_a_first_call_in_inference_mode_leaves_training_possible():
+    m = layer("cpu")
+    x = torch.randn(1, 3, 96, device="cuda")
+    with torch.inference_mode():
+        m = m.cuda()
+        m(x)
+    m = tda_amd.DifferentialAttention(96, 4, 64, device="cuda")
+    with torch.inference_mode():
+        want = m(x)
+    m(x).sum().backward()
+    assert all(p.grad.isfinite().all() for p in m.parameters())
+    with torch.no_grad():  # a training call takes other kernels
+        assert torch.equal(m(x), want)
