@@ -141,7 +141,8 @@ typedef struct sda_kv4_read_args {
   int32_t abi_version;
   int32_t dtype;
   sda_kv4 cache;
-  int64_t rows;             /* n <= capacity: rows 0 .. n - 1; rows past a length read as zeros */
+  int64_t rows;             /* n <= capacity: rows 0 .. n - 1; rows past a length read as zeros, in F16
+                               values past +-65504 as +-65504 */
   tda_tensor k1, k2, v;     /* outputs */
 } sda_kv4_read_args;
 

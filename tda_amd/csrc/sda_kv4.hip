@@ -228,6 +228,10 @@ __global__ void __launch_bounds__(256) kv4_read(Kv4Params P, int blocks) {
         x[4 + e] = __builtin_fmaf(s, (float)(d >> (4 * e) & 15), m);
       }
     }
+    if constexpr (std::is_same_v<T, _Float16>) {  // the largest float16 instead of infinity
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] > 65504.f ? 65504.f : x[e] < -65504.f ? -65504.f : x[e];
+    }
     store8(row_of<T>(P.x[z], b, hk, i) + 8 * u, x);
   }
 }

@@ -60,6 +60,7 @@ class Int4KVCache:
             raise ValueError(f"capacity must be at most 2^24 and batch kv_heads below 2^30, got {batch}, {kv_heads}, {capacity}")
         self._held = [torch.empty(n, dtype=torch.uint8, device=device) for n in sizes]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._wide = False          # rows of a wider range than float16's were appended
         self._templates: dict = {}  # argument blocks by configuration
         self._plans: dict = {}      # of calls whose tensors need no copy, by their signature: no checks again
 
@@ -162,6 +163,7 @@ class Int4KVCache:
             if start is not None:
                 self.lengths.copy_(start.clamp(0, self.capacity))
             return
+        self._wide |= k1.dtype != torch.float16
         rows = [_usable(t) for t in (k1, k2, v)]
 
         def build():
@@ -184,7 +186,8 @@ class Int4KVCache:
 
     def read(self, rows: int | None = None, dtype=torch.bfloat16):
         """The first `rows` (default: capacity) positions as tensors k1, k2, v of a dtype; positions a
-        sequence does not hold are zero."""
+        sequence does not hold are zero.  In float16 values past +-65504 (held from rows of a wider type, or a
+        step beyond float16 rows next to that) read as +-65504."""
         n = self.capacity if rows is None else int(rows)
         if not 1 <= n <= self.capacity:
             raise ValueError(f"rows must be 1 to {self.capacity}, got {n}")
@@ -214,7 +217,8 @@ class Int4KVCache:
         the same call that stand before it.)
 
         The rows of a decoding step or of a short chunk are computed from the codes; those of a long
-        one from the rows that read() gives in q1's dtype."""
+        one from the rows that read() gives in q1's dtype, unless that is float16 and the cache took rows of
+        another type, whose range float16 may not hold."""
         key = self._signature(q1, q2, lambda_param) if scale is None or type(scale) is float else None
         if key is not None:
             key = *key, scale
@@ -235,7 +239,8 @@ class Int4KVCache:
         lam = _lambda(lambda_param, b, h, n, self.device)
         if n == 0:
             return torch.zeros((b, h, 0, self.v_head_dim), dtype=q1.dtype, device=self.device)
-        if not _from_codes(b, hk, h // hk * n, q1.dtype):
+        narrow = q1.dtype == torch.float16 and self._wide
+        if not narrow and not _from_codes(b, hk, h // hk * n, q1.dtype):
             with torch.no_grad():
                 rows = self.read(dtype=q1.dtype)  # checks lengths
                 lens = self.lengths.clamp(0, self.capacity)

@@ -464,3 +464,44 @@ def test_many_groups(dtype):
     for got, x in zip(c.read(dtype=F32), xs):
         want = oracle.held4(x)
         assert ((got.double() - want).abs() <= 2.0 ** -24 * want.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("part", ["keys", "values"])
+@pytest.mark.parametrize("n", [1, 160])
+def test_float16_queries_over_rows_beyond_float16(dtype, part, n):
+    """Held values past 65504, whose scores and outputs float16 does hold, attended by a token and by many rows."""
+    c = tda_amd.Int4KVCache(4, 8, 160, 64)
+    k1, k2, v = context(4, 8, 160, 64, 64, dtype)
+    q1, q2 = rows(4, 8, n, 64, 50, F16), rows(4, 8, n, 64, 51, F16)
+    if part == "values":  # the two maps' averages of values around 90000
+        v = 90000 + 1000 * v
+    else:
+        k1, k2, q1, q2 = k1 * 7e4, k2 * 7e4, q1 * 2.0 ** -10, q2 * 2.0 ** -10
+    c.append(k1.to(dtype), k2.to(dtype), v.to(dtype))
+    assert n == 1 or not _from_codes(4, 8, n, F16)
+    got = c.attend(q1, q2, 1.0)
+    ref, ks = attend(c, q1, q2, 1.0)
+    assert max(x.abs().max().item() for x in ks) > 65520  # float16's infinity
+    close(got, ref, c, ks, q1, q2, F16)
+
+
+@gpu
+def test_float16_rows_next_to_the_end_of_float16():
+    """A group from -65504 to 65504 is held with a step that reaches beyond; read() and many rows stop at the end."""
+    c = tda_amd.Int4KVCache(4, 8, 160, 64)
+    x = torch.where(rows(4, 8, 160, 64, 1, F16) > 0, 65504.0, -65504.0).half()
+    c.append(x * 2.0 ** -14, x * 2.0 ** -14, x)
+    held = c.read(dtype=F32)[2]
+    assert held.abs().max().item() > 65520
+    ks = c.read(dtype=F16)
+    assert torch.equal(ks[2], held.clamp(-65504, 65504).half())
+    q = rows(4, 8, 160, 64, 2, F16)
+    got = c.attend(q, q * 0.5, 0.5)
+    want = tda_amd.differential_attention(q, q * 0.5, *ks, 0.5, q_offset=c.lengths - 160, kv_lens=c.lengths)
+    assert torch.equal(got, want) and got.isfinite().all()
+    x = x.float()
+    x[1, 3, 5, 7] = math.nan  # a group that is not finite stays so
+    c.append(x, x, x, start=torch.zeros(4, dtype=torch.int32).cuda())
+    assert torch.equal(c.read(dtype=F16)[2].isnan(), c.read(dtype=F32)[2].isnan()) and c.read(dtype=F16)[2].isnan().sum() == 64
