@@ -68,7 +68,9 @@ typedef struct sda_bwd_args {
   float   scale;
   int64_t batch, heads, kv_heads, seq_len, seq_len_kv, head_dim, v_head_dim;
   tda_tensor q1, k1, q2, k2, v;     /* the forward's */
-  tda_tensor out, out2, out_low, dout;  /* the forward's outputs and the upstream gradient */
+  tda_tensor out, out2, out_low, dout;  /* the forward's outputs and the upstream gradient.  Unless seq_len
+                               is a multiple of 32, rows of q1, q2 and dout may not overlap
+                               (stride[2] >= width) */
   tda_tensor dq1, dk1, dq2, dk2, dv;
   const void* lambda_param;
   int64_t lambda_stride[3];

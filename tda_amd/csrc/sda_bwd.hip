@@ -239,17 +239,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((kKeyT
     for (int u = 0; u < OL; ++u)
       if (OT::LOADS % NW == 0 || NW * u + wv < OT::LOADS) OT::load(r, reinterpret_cast<T*>(at + 2 * QT::BYTES), NW * u + wv, oo[u]);
     // the rows' statistics, two loads a wave (the last three bring the fifth again: every wave's loads of a
-    // stage are as many).  Rows past Nq get log-sums that weigh everything 0, and zeros else: their q and dO are
-    // zeros only where rows do not overlap (those of a gradient broadcast along the sequence do).
+    // stage are as many); rows past Nq read as zeros and meet zero rows of q and dO, whose rows do not
+    // overlap (sda_validate_bwd)
     const float* src = P.stat + ((int64_t)b * P.H + h) * P.Nq + i0;
 #pragma unroll
-    for (int z = 0; z < 8; z += NW) {
-      char* to = at + S::STAT + 128 * (z + wv);
-      const bool put = n < 32 && z + wv < 2;
-      if (l < (put ? n : 32))
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + min(z + wv, 4) * rows, 4 * n), LDS_PTR(void, to), 4, 4 * l, 0, 0, 0);
-      if (put && l >= n && l < 32) reinterpret_cast<float*>(to)[l] = -__builtin_inff();
-    }
+    for (int z = 0; z < 8; z += NW)
+      if (l < 32)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src + min(z + wv, 4) * rows, 4 * n), LDS_PTR(void, at + S::STAT + 128 * (z + wv)), 4, 4 * l, 0, 0, 0);
   };
   int nh = h0, nq = first;  // head and query tile of the next stage to send for
   auto send = [&](int slot) {

@@ -112,7 +112,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 // Descriptor over `rows` rows of `width` bytes, `stride` bytes apart: rows past them read as zeros, or, where rows
-// overlap (stride < width, 0 for a broadcast one), as bytes of the rows before: such rows need weights of zero.
+// overlap (stride < width, 0 for a broadcast one), as bytes of the rows before: then they need weights of zero.
 // rows * stride stays below 2^32 (tiles of up to 64 rows, strides of at most 2^25 bytes).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t stride, int rows, int width) {
   return rsrc_of(base, rows > 0 ? (uint32_t)((int64_t)(rows - 1) * stride + width) : 0u);

@@ -58,6 +58,13 @@ def _usable(t: torch.Tensor) -> torch.Tensor:
     return t if ok and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _apart(t: torch.Tensor) -> torch.Tensor:
+    """t itself, or a contiguous copy where its rows overlap (a stride of 0 along the sequence, as that of the gradient
+    of a sum or mean over it) and sda_bwd does not take them so."""
+    n, width = t.shape[2:]
+    return t.clone(memory_format=torch.contiguous_format) if n % 32 and t.stride(2) < width else t
+
+
 def _check_rows(tensors, names, shapes=None):
     """4-D floating tensors of one dtype on one GPU, the batch the same."""
     ref = tensors[0]
@@ -284,6 +291,8 @@ class _DifferentialAttention(torch.autograd.Function):
     def forward(ctx, q1, q2, k1, k2, v, lam, scale, causal, q_offset, q_offsets, kv_lens):
         saving = any(ctx.needs_input_grad[:6])
         rows = [_usable(t) for t in (q1, q2, k1, k2, v)]
+        if saving:
+            rows[:2] = _apart(rows[0]), _apart(rows[1])
         out, out2, low, lse = _forward(*rows, lam, scale, causal, q_offset, q_offsets, kv_lens, saving)
         if saving:
             ctx.save_for_backward(*rows, lam, out, out2, low, lse, q_offsets, kv_lens)
@@ -296,7 +305,7 @@ class _DifferentialAttention(torch.autograd.Function):
         q1, q2, k1, k2, v, lam, out, out2, low, lse, q_offsets, kv_lens = ctx.saved_tensors
         scale, causal, q_offset = ctx.cfg
         lib = _sda_abi.load()
-        dout = _usable(dout if dout.dtype == q1.dtype else dout.to(q1.dtype))
+        dout = _apart(_usable(dout if dout.dtype == q1.dtype else dout.to(q1.dtype)))
         dq1, dq2 = _new_rows(q1, q1.shape[3]), _new_rows(q2, q2.shape[3])
         dk1, dk2, dv = (_new_rows(t, t.shape[3]) for t in (k1, k2, v))
         dlam = torch.empty(lam.shape, dtype=lam.dtype, device=lam.device) if ctx.needs_input_grad[5] else None

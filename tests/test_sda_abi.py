@@ -256,3 +256,16 @@ def test_append_refuses_arrays_that_overlap_the_lengths():
             a = kv4(_sda_abi.SdaKv4AppendArgs)
             setattr(a, name, FAKE + apart)
             assert so.sda_validate_kv4_append(ctypes.byref(a)) == code, (name, apart)
+
+
+@pytest.mark.parametrize("name, width", [("q1", 64), ("q2", 64), ("dout", 128)])
+@pytest.mark.parametrize("n, code", [(1, _abi.ERR_LAYOUT), (33, _abi.ERR_LAYOUT), (100, _abi.ERR_LAYOUT), (32, _abi.OK), (96, _abi.OK)])
+def test_backward_refuses_query_rows_that_overlap(name, width, n, code):
+    """Its last tile of 32 rows reads past them, where overlapping rows are not zeros."""
+    so = lib()
+    for step in (0, 8, width - 8, width):
+        a = bwd(n=n)
+        t = _rows((2, 4, n, width))
+        t.stride[2] = step
+        setattr(a, name, t)
+        assert so.sda_validate_bwd(ctypes.byref(a)) == (_abi.OK if step == width else code)
