@@ -14,9 +14,9 @@
 //   bwd_lambda sums dlambda over the axes lambda is broadcast along
 // Both passes recompute the weights from the forward's log-sums: no atomics, so results do not depend
 // on the order of execution.  Bound by the matrix cores and, for narrow keys, the vector work between the
-// products.  bf16: (4, 16, 2048, 64/128) keys 267 us (0.51 PFLOP/s), queries 147 (0.70), rows 29, lambda 9;
-// (2, 16 over 4, 4096, 128) keys 577 (0.71), sum 21, queries 416 (0.83), rows 33.  f32 (2, 12, 1111, 64) keys
-// 141, queries 116 (0.08 PFLOP/s of 0.15).
+// products.  bf16: (4, 16, 2048, 64/128) keys 242 us (0.57 PFLOP/s), queries 139 (0.74), rows 29, lambda 9;
+// (2, 16 over 4, 4096, 128) keys 493 (0.84), sum 21, queries 392 (0.88), rows 36.  f32 (2, 12, 1111, 64) keys
+// 133, queries 109 (0.08 PFLOP/s of 0.15).
 #include "sda_common.hpp"
 
 namespace sda {
@@ -37,7 +37,7 @@ __device__ __forceinline__ f32x4 load4_(const T* p) {
 // them by powers of two: score gradients so that the largest possible, |dS| <= 2 max|dO_i| max(1, |lambda_i|)
 // max|v_j|, comes to 2^13 .. 2^14, weights by up to 2^8 (1 + max |lambda| leaves room).  peak holds the three
 // maxima; bits of floats that are not negative order as integers do, so an atomic maximum has one result.
-// Backward of (2, 16, 2048, 64): 250 us, bf16's 201; by f32 products it took 876.
+// Backward of (2, 16, 2048, 64): 236 us, bf16's 204; by f32 products it took 876.
 struct Scales {
   float ds, w;  // score gradients by ds, weights by 2^w
 };

@@ -6,8 +6,9 @@
 // that hold them: of a tile of 32 keys the second product takes, from lane quarter kq, keys 4 kq + j
 // and 16 + 4 kq + j (j = 0 .. 3), and the value fragments are read in that order.  Nothing is staged:
 // every key and value byte is used by one wave alone and goes straight to its registers.  Bound by
-// reading the cache: one token over bf16 (32, 32 over 8, 8192, 128) of unequal lengths, 1.22 GB, 253 us and
-// 4.5 us for the join (4.8 TB/s; a copy reaches 5.2).  The waves' sums meet in LDS, the parts' in a second
+// reading the cache: one token over bf16 (32, 32 over 8, 8192, 128) of unequal lengths, 1.22 GB, 256 us and
+// 4.8 us for the join (4.7 TB/s; a copy reaches 5.1 to 5.2), of full lengths 5.3 TB/s; f32 (16, 32 over 8, 8192, 128)
+// 4.1, (16, 32 over 8, 8192, 64) 5.1.  The waves' sums meet in LDS, the parts' in a second
 // launch.
 //
 // A source (Src) brings: D, DV, `Regs` (a tile's loads) and NBUF, load, scores, rescale (a branch's running

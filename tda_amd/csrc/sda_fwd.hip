@@ -13,10 +13,10 @@
 // Grids that would leave CUs idle take 64 query rows a workgroup (RG = 2 row groups): the other four waves
 // take the second half of each stage's keys, and the halves' maxima, sums and outputs meet in LDS first.
 //
-// bf16 (1, 16 over 4, 16384, 128) 1.97 ms, 1.1 PFLOP/s, where a product of 8192^3 reaches 1.23: bound by the
-// matrix cores.  Narrow keys leave fewer products to an exponential: (4, 16, 2048, 64/128), a training forward,
-// 161 us, 0.64 PFLOP/s, bound by both together (a stage's waits cost little: a third stage in LDS or waves
-// half a stage apart changed nothing).  f32 (2, 12, 1111, 64) 92 us, 0.1 PFLOP/s of 0.15.
+// bf16 (1, 16 over 4, 16384, 128) 1.98 ms (1.93 to 2.18 on several parts), 1.1 PFLOP/s, where a product of 8192^3
+// reaches 1.22: bound by the matrix cores.  Narrow keys leave fewer products to an exponential: (4, 16, 2048,
+// 64/128), a training forward, 148 us, 0.70 PFLOP/s, bound by both together (a stage's waits cost little: a third
+// stage in LDS or waves half a stage apart changed nothing).  f32 (2, 12, 1111, 64) 85 us, 0.09 PFLOP/s of 0.15.
 #include "sda_common.hpp"
 
 namespace sda {

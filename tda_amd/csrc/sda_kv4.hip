@@ -180,7 +180,7 @@ __global__ void kv4_lengths(Kv4Params P) {
 }
 
 // ------------------------------------------------------------------ read
-// Lanes and workgroups as above.  bf16 (4, 8, 2048, 128): 13.5 us for 64 MB, the memory's rate.
+// Lanes and workgroups as above.  bf16 (4, 8, 2048, 128): 13 us for 64 MB, the memory's rate.
 template <class T, int R>
 __global__ void __launch_bounds__(256) kv4_read(Kv4Params P, int blocks) {
   const int z = blockIdx.z, W = z < 2 ? P.D : P.DV, L = W / 8;
@@ -453,7 +453,8 @@ struct Kv4Src {
   __device__ __forceinline__ static int column(int t, int m) { return 64 * (t / 4) + 4 * m + t % 4; }
 };
 
-// One token over (32, 32 over 8, 8192, 128) of unequal lengths, 340 MB of codes: 95 us (3.6 TB/s), bound by the
+// One token over (32, 32 over 8, 8192, 128) of unequal lengths, 340 MB of codes: 94 to 104 us (3.3 to 3.6 TB/s), of full
+// lengths 107 us (f16 queries 176, f32 262: two and three products a code), bound by the
 // instructions that turn codes into operands as much as by reading them; two waves a SIMD cover each other's
 // loads (132 us; one, with the next tile's loads on their way, 188 us, both before the unpacking's last steps).
 template <class T, int NP, int D, int DV>

@@ -2,8 +2,9 @@
 //
 // A workgroup takes a few tokens: their cosines and sines go to LDS once (a table of tokens x pairs),
 // then the rows of every head of every tensor at those tokens stream through, each value read and
-// written once.  Bound by memory: four tensors of bf16 (4, 16, 4096, 128), 96 values rotated, 118 us for 537 MB
-// (4.5 TB/s).  The angle is a product of an integer and an f32 frequency taken in
+// written once.  Bound by memory: four tensors of bf16 (4, 16, 4096, 128), 96 values rotated, 120 us for 537 MB
+// (4.5 TB/s); all 128 rotated 104 us (5.2 TB/s).  Widths or strides that are no whole pieces of 16 bytes go by single
+// values: width 72, all rotated, 131 us for 302 MB (2.3 TB/s), width 80, 40 rotated, 198 us for 336 MB (1.7 TB/s).  The angle is a product of an integer and an f32 frequency taken in
 // 64 bits and reduced to a turn there, so far positions keep their accuracy; sine and cosine of the
 // reduced angle are f32.
 #include "sda_common.hpp"

@@ -23,7 +23,10 @@ def _from_codes(batch: int, kv_heads: int, rows: int, dtype) -> bool:
     reads the rows out first, for the attention that passes over them once per 128.  us, codes : rows, (batch, heads, kv_heads, n, keys) of width 128, bf16:
     (8, 16, 4, 16, 4096) 38 : 108, (32, 32, 8, 32, 4096) 344 : 767, (16, 8, 8, 128, 4096) 178 : 238,
     (16, 8, 8, 256, 4096) 331 : 261, (1, 16, 4, 256, 4096) 60 : 94, (1, 16, 4, 512, 4096) 92 : 96; float32:
-    (8, 8, 8, 128, 4096) 255 : 1257."""
+    (8, 8, 8, 128, 4096) 255 : 1257.  All with full caches: rows are read out for the whole capacity, which takes its time
+    and capacity (2 head_dim + v_head_dim) values a key head whatever is held: bf16 prompts of 512 rows into empty caches,
+    (32, 32, 8, 512) of capacity 8192 992 : 603, (8, 16, 16, 512) of 8192 and width 64 72 : 121, (1, 32, 8, 512) of 32768
+    40 : 58."""
     return rows <= (512 if dtype == torch.float32 else 128) or batch * kv_heads * -(-rows // 16) <= 256
 
 

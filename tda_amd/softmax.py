@@ -332,7 +332,8 @@ def differential_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=T
     place, others are padded with zeros.
 
     lambda_param: a float, or a tensor that is a scalar, (heads,) or broadcasts to (batch, heads,
-    seq_len); unclamped, differentiable.  scale: default 1 / sqrt(head_dim); 1e-30 to 1e30.
+    seq_len); unclamped, differentiable.  scale: default 1 / sqrt(head_dim); 1e-30 to 1e30, with scores
+    scale q k of up to 1e9 (32 bits hold them to 2^-24).
 
     M: row i of sequence b stands at position q_offset + i (q_offset an int, by default
     max(seq_len_kv - seq_len, 0), or an int32/int64 tensor (batch,), which may be negative).  With
