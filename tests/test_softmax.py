@@ -592,7 +592,7 @@ def overlapping(x, step):
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32, F16])
 @pytest.mark.parametrize("d, dv", DIMS)
-@pytest.mark.parametrize("n", [1, 33, 50, 129])
+@pytest.mark.parametrize("n", [1, 33, 50, 64, 129])
 @pytest.mark.parametrize("causal", [True, False])
 def test_upstream_gradient_broadcast_along_the_sequence(dtype, d, dv, n, causal):
     """As out.sum(2) or a mean over the sequence hands it down (rows with a stride of 0, or that overlap): the
@@ -663,3 +663,19 @@ def test_forward_mode_is_refused(device, grad):
         q, k, v = xs[0], xs[2], xs[4]
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda t: tda_amd.differential_attention(t, q, k, k, v, 0.5), (q,), (q,))
+
+
+@gpu
+@pytest.mark.parametrize("by", [2.0 ** -8, 2.0 ** -12])
+def test_float16_gradients_of_rows_of_unequal_size(by):
+    """One power of two scales all of a call's score gradients: every other upstream row far smaller than the rest, one
+    value row far larger; what float16's smallest values may take of the small rows is in tiny()."""
+    xs = inputs(2, 4, 2, 150, 150, 64, 64, F16)
+    dout = rows((2, 4, 150, 64), 6, F16)
+    dout[:, :, 1::2] *= by
+    xs[4][:, :, 5] *= 100
+    leaves = [x.requires_grad_() for x in xs]
+    tda_amd.differential_attention(*leaves, 0.5).backward(dout)
+    ref, more = oracle.attention(*xs, 0.5, u=U[F16], dout=dout), tiny(xs, 0.5, dout)
+    for x, name in zip(leaves, ("dq1", "dq2", "dk1", "dk2", "dv")):
+        within(x.grad, ref, name, U[F16], 1e-30 + more[name])
