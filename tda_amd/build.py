@@ -30,8 +30,8 @@ HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra"]
 
 HIP_SOURCES = ["tda_fwd.hip", "tda_fwd_sparse.hip", "tda_fwd_decode.hip", "tda_bwd.hip", "tda_bwd_fast.hip",
                "tda_wide.hip", "tda_noalloc.hip", "sda_fwd.hip", "sda_bwd.hip", "sda_decode.hip", "sda_kv4.hip",
-               "sda_rotary.hip"]
-HOST_SOURCES = ["tda_host.cpp", "sda_host.cpp"]
+               "sda_rotary.hip", "spa_append.hip", "spa_few.hip", "spa_many.hip", "sln.hip"]
+HOST_SOURCES = ["tda_host.cpp", "sda_host.cpp", "spa_host.cpp", "sln_host.cpp"]
 # host-only code that calls the HIP runtime API (no device code): g++ against the ROCm headers
 HIP_HOST_SOURCES = ["tda_timing.cpp"]
 HIP_HOST_FLAGS = [f"-I{ROCM}/include", "-D__HIP_PLATFORM_AMD__"]

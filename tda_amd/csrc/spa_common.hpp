@@ -1,0 +1,216 @@
+// spa_common.hpp -- device building blocks of the paged cache: the sequences of a call, the pages of a
+// sequence, and how the attention's work is dealt out.
+//
+// How many rows and keys each sequence has stands in device memory, so no launch knows its work: every
+// workgroup reads the sequences' lengths (a wave 64 of them at a time) and finds what falls to its number.
+#pragma once
+
+#include "sda_common.hpp"
+#include "spa_params.hpp"
+
+namespace spa {
+
+using sda::lane_id;
+using sda::rsrc_of;
+
+struct Seq {
+  int qb, row0, cnt;  // its rows: row0 .. row0 + cnt - 1 of batch entry qb
+  int held, len;      // the position of its first row; the positions that it has with its new rows
+};
+__device__ __forceinline__ Seq seq_of(const Seqs& Q, int s) {
+  Seq r;
+  if (Q.starts) {
+    r.qb = 0;
+    r.row0 = min(max(Q.starts[s], 0), Q.rows);
+    r.cnt = min(max(Q.starts[s + 1], r.row0), Q.rows) - r.row0;
+  } else {
+    r.qb = s;
+    r.row0 = 0;
+    r.cnt = Q.counts ? min(max(Q.counts[s], 0), Q.rows) : Q.rows;
+  }
+  r.held = min(max(Q.lengths[s], -(1 << 30)), 1 << 30);
+  r.len = min(max(r.held + r.cnt, 0), Q.tlen << Q.pshift);
+  return r;
+}
+
+// The same in scalar registers (s is the same in every lane): descriptors are made of it.
+__device__ __forceinline__ Seq uniform_seq(const Seqs& Q, int s) {
+  Seq r = seq_of(Q, s);
+  r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
+  r.cnt = __builtin_amdgcn_readfirstlane(r.cnt);
+  r.held = __builtin_amdgcn_readfirstlane(r.held);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
+  return r;
+}
+
+// The page numbers of 64 consecutive table entries in the lanes of a register, the next 64 on their way:
+// page() then costs a few scalar instructions.  Entries behind the table, and numbers that are no page,
+// are -1.
+struct Pages {
+  const int32_t* row;
+  int tlen, pages, base;
+  int now, next;
+  __device__ __forceinline__ int fetch(int at) const {
+    const int e = at + lane_id();
+    const int p = e < tlen ? row[e] : -1;
+    return p < pages ? p : -1;
+  }
+  __device__ __forceinline__ void begin(const Seqs& Q, int s, int slot) {
+    row = Q.table + (int64_t)s * Q.tstride;
+    tlen = Q.tlen;
+    pages = Q.pages;
+    base = slot;
+    now = fetch(slot);
+    next = fetch(slot + 64);
+  }
+  // Makes page() know the entries up to `last`, of which the earlier ones asked for so far stay known when they
+  // are at most 64 apart.  Slots only grow.
+  __device__ __forceinline__ void reach(int first) {
+    if (first >= base + 64) {
+      base += 64;
+      if (first >= base + 64) {  // a jump past what is on its way
+        base = first;
+        now = fetch(base);
+      } else {
+        now = next;
+      }
+      next = fetch(base + 64);
+    }
+  }
+  __device__ __forceinline__ int page(int slot) const {
+    const int e = slot - base;
+    return e < 64 ? __builtin_amdgcn_readlane(now, e) : __builtin_amdgcn_readlane(next, e - 64);
+  }
+};
+// Descriptor over `rows` rows (of `width` bytes, at most up to the page's end) from position `key` of a
+// page's head on; rows past them, and all rows of no page, read as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, int page, int Hk, int hk, int pshift, int key, int rows,
+                                                           int width) {
+  const int64_t at = (((int64_t)max(page, 0) * Hk + hk) << pshift) + (key & ((1 << pshift) - 1));
+  return rsrc_of(static_cast<const char*>(pool) + at * width, page >= 0 && rows > 0 ? (uint32_t)(rows * width) : 0u);
+}
+
+// ------------------------------------------------------------------ work
+// Sums over the wave's lanes, and running sums.
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+__device__ __forceinline__ uint64_t wave_total(uint64_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor((unsigned long long)x, d);
+  return x;
+}
+__device__ __forceinline__ uint32_t running(uint32_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(x, d);
+    if (lane_id() >= d) x += y;
+  }
+  return x;
+}
+
+constexpr int kUnit = 128;  // keys; pieces are whole units
+
+// A tile of RT rows of sequence s (the rows of all heads that share a key head, token by token), and which of
+// the `parts` pieces of its keys; `first` is the number of its first piece (of one key head).
+struct Job {
+  int s, tile, part, parts, units;  // units of keys in a piece
+  uint32_t first;
+};
+// The tiles of a form (FEW: sequences of at most `bound` rows), in the order of the sequences, a sequence's last
+// tile first: it has the most keys.  With `room` each tile is cut into pieces of at most W / (room - N) units,
+// W the sum over N tiles of their units, so that there are no more than `room` pieces.
+// BY_PIECE: idx counts pieces; else tiles (for the launch that joins them).  False: there is no such one.
+template <int RT, bool FEW, bool BY_PIECE>
+__device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int room, uint32_t idx, Job& J) {
+  const int l = lane_id();
+  uint32_t t = 0, u = 0;
+  const auto sizes = [&](int s0) {
+    t = u = 0;
+    if (s0 + l < Q.S) {
+      const Seq q = seq_of(Q, s0 + l);
+      const int R = q.cnt * G;
+      if ((R <= bound) == FEW) t = (uint32_t)(R + RT - 1) / RT;
+      u = (uint32_t)(q.len + kUnit - 1) / kUnit;
+    }
+  };
+  uint32_t units = 0x7fffffffu;
+  if (room) {
+    uint32_t N = 0;
+    uint64_t W = 0;
+    for (int s0 = 0; s0 < Q.S; s0 += 64) {
+      sizes(s0);
+      N += t;
+      W += (uint64_t)t * u;
+    }
+    N = wave_total(N);
+    W = wave_total(W);
+    if ((uint32_t)room > N) {
+      const uint32_t by = (uint32_t)room - N, over = (uint32_t)(W >> 31);  // W in 31 bits, rounded up
+      const int shift = (W >> 63) ? 33 : over ? 32 - __builtin_clz(over) : 0;
+      const uint32_t w = ((uint32_t)(W >> shift) + (shift ? 1u : 0u) + by - 1) / by;
+      units = (uint32_t)min(max((uint64_t)w << shift, (uint64_t)1), (uint64_t)0x7fffffff);
+    }
+  }
+  uint32_t tiles = 0, pieces = 0;  // of the sequences before
+  for (int s0 = 0; s0 < Q.S; s0 += 64) {
+    if (!room || Q.S > 64) sizes(s0);
+    const uint32_t p = t * max((u + units - 1) / units, 1u);
+    const uint32_t tu = running(t), pu = running(p), mine = BY_PIECE ? pu : tu, before = BY_PIECE ? pieces : tiles;
+    const uint32_t sum = __builtin_amdgcn_readlane(mine, 63);
+    if (idx - before < sum) {
+      const int x = __builtin_ctzll(__ballot(mine > idx - before));
+      const uint32_t nt = __builtin_amdgcn_readlane(t, x), np = __builtin_amdgcn_readlane(p, x);
+      const uint32_t first = pieces + __builtin_amdgcn_readlane(pu, x) - np;
+      const uint32_t e = idx - before - (__builtin_amdgcn_readlane(mine, x) - (BY_PIECE ? np : nt));
+      J.s = s0 + x;
+      J.parts = (int)(np / nt);
+      const uint32_t at = BY_PIECE ? e / (uint32_t)J.parts : e;
+      J.part = BY_PIECE ? (int)(e % (uint32_t)J.parts) : 0;
+      J.tile = (int)(nt - 1 - at);
+      J.units = (int)units;
+      J.first = first + at * (uint32_t)J.parts;
+      return true;
+    }
+    tiles += __builtin_amdgcn_readlane(tu, 63);
+    pieces += __builtin_amdgcn_readlane(pu, 63);
+  }
+  return false;
+}
+// A piece's keys within the `lim` that its tile sees.
+__device__ __forceinline__ void keys_of(const Job& J, int lim, int& k0, int& k1) {
+  const int64_t per = (int64_t)J.units * kUnit;
+  k0 = (int)min((int64_t)J.part * per, (int64_t)lim);
+  k1 = (int)min((int64_t)k0 + per, (int64_t)lim);
+}
+
+// Zeros the rows of no sequence: workgroup `bid` of `blocks`.
+template <class T, int DV, int THREADS>
+__device__ __forceinline__ void clear_free_rows(const AttendParams& P, uint32_t bid, uint32_t blocks) {
+  constexpr int V = 16 / sizeof(T), PER = DV / V;
+  if (!P.seq.starts && !P.seq.counts) return;
+  const int64_t all = (int64_t)P.lead * P.seq.rows;
+  int64_t lo = 0, hi = all;  // where they may be
+  int s0 = 0, s1 = 0;        // packed: rows s0 .. s1 - 1 have a sequence
+  if (P.seq.starts) {
+    s0 = min(max(P.seq.starts[0], 0), P.seq.rows);
+    s1 = min(max(P.seq.starts[P.seq.S], s0), P.seq.rows);
+    hi = all - (s1 - s0);
+  }
+  for (int64_t e = lo + bid; e < hi; e += blocks) {
+    int b = 0, i;
+    if (P.seq.starts) {
+      i = (int)(e < s0 ? e : e + (s1 - s0));
+    } else {
+      b = (int)(e / P.seq.rows);
+      i = (int)(e % P.seq.rows);
+      if (i < min(max(P.seq.counts[b], 0), P.seq.rows)) continue;
+    }
+    for (int x = threadIdx.x; x < P.H * PER; x += THREADS)
+      *reinterpret_cast<sda::u32x4*>(sda::row_of<T>(P.out, b, x / PER, i) + x % PER * V) = sda::u32x4{};
+  }
+}
+
+}  // namespace spa

@@ -1,0 +1,301 @@
+"""A key/value cache of softmax differential attention in pages: rows of new positions enter it with their rotary
+positions applied on the way, and the new positions attend over it."""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from . import _sda_abi, _spa_abi
+from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _new_rows, _raw_stream, _scale,
+                      _sig, _usable)
+
+_PUT = struct.Struct("<Q").pack_into
+_DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+_AT = {n: _spa_abi.SpaAppendArgs.at.offset + getattr(_spa_abi.SpaRows, n).offset for n in ("table", "lengths", "starts", "counts")}
+_APPEND_OFF = {**_AT, **{n: getattr(_spa_abi.SpaAppendArgs, n).offset for n in
+                         ("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out", "positions", "inv_freq")}}
+_ATTEND_OFF = {**_AT, **{n: getattr(_spa_abi.SpaAttendArgs, n).offset for n in ("q1", "q2", "out", "lambda_param", "workspace")}}
+
+
+class PagedKVCache:
+    """The k1, k2 and v rows of many sequences in `pages` pages of `page_size` positions that a program hands out.
+
+    k1, k2 (pages, kv_heads, page_size, head_dim) and v (..., v_head_dim) are tensors of dtype: float32, bfloat16 or
+    float16.  page_size: 16, 32, 64, 128 or 256; (head_dim, v_head_dim): (64, 64), (64, 128), (128, 128) or
+    (128, 256).
+
+    Which pages are whose stands in the calls' arguments, all on the device and read there without synchronising, so
+    that every call can be captured into a graph.  Position p of sequence s is row p % page_size of page
+    table[s, p // page_size] (table: int32, (sequences, entries)); an entry that is no page of the cache stands for
+    rows of zeros, and rows appended there are dropped.  lengths (int32/int64, (sequences,)) are the positions that
+    each sequence held before the call's rows, of which row i stands at lengths[s] + i: the calls do not change them, so
+    that the layers of a model can share them.  The rows of a call come in one of three forms:
+
+      (sequences, heads, n, width)              n rows of every sequence
+      the same, with counts (sequences,)        the first counts[s] rows of entry s (clamped to [0, n])
+      (1, heads, rows, width), with starts      packed: sequence s has the rows starts[s] .. starts[s + 1] - 1
+                (sequences + 1,), not decreasing
+
+    counts and starts are int32 or int64.  Rows of no sequence are not read, and are zero in what a call returns.
+    The calls carry no gradient.  A cache's calls order themselves by their stream; two sequences that
+    write to one page are the caller's to keep apart (reading one is fine).  copy.deepcopy and pickling give a cache with
+    pages of its own."""
+
+    def __init__(self, pages: int, kv_heads: int, page_size: int, head_dim: int, v_head_dim: int | None = None, *,
+                 dtype=torch.bfloat16, device="cuda"):
+        v_head_dim = head_dim if v_head_dim is None else v_head_dim
+        for name, n in (("pages", pages), ("kv_heads", kv_heads)):
+            if n < 1:
+                raise ValueError(f"{name} must be at least 1, got {n}")
+        if page_size not in _PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {_PAGE_SIZES}, got {page_size}")
+        if (head_dim, v_head_dim) not in _DIMS:
+            raise ValueError(f"(head_dim, v_head_dim) must be one of {_DIMS}, got {(head_dim, v_head_dim)}")
+        if dtype not in _CODE:
+            raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"tda_amd runs on the GPU only (HIP); got {device}")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.pages, self.kv_heads, self.page_size = int(pages), int(kv_heads), int(page_size)
+        self.head_dim, self.v_head_dim, self.dtype, self.device = int(head_dim), int(v_head_dim), dtype, device
+        self._held = [torch.empty((pages, kv_heads, page_size, w), dtype=dtype, device=device) for w in (head_dim, head_dim, v_head_dim)]
+        self._plans: dict = {}  # argument blocks of calls whose tensors need no copy, by their signature: no checks again
+
+    k1 = property(lambda self: self._held[0])
+    k2 = property(lambda self: self._held[1])
+    v = property(lambda self: self._held[2])
+
+    def __getstate__(self):
+        return {**self.__dict__, "_plans": {}}  # a copy has pages of its own: their addresses too
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self._held[0].device  # a loaded cache may have been sent elsewhere
+        if self.device.type != "cuda":
+            raise ValueError(f"tda_amd runs on the GPU only (HIP); got a cache on {self.device}")
+
+    # -------------------------------------------------------------- calls
+    def _start_block(self, args_type, at):
+        """A call's argument block with the cache, the sequences' shapes, and a mark at each array there is."""
+        table, _, starts, counts, rows = at
+        a = args_type()
+        a.abi_version, a.dtype = _spa_abi.ABI_VERSION, _CODE[self.dtype]
+        c = a.cache
+        c.pages, c.kv_heads, c.page_size, c.head_dim, c.v_head_dim = self.pages, self.kv_heads, self.page_size, self.head_dim, self.v_head_dim
+        c.k1, c.k2, c.v = (t.data_ptr() for t in self._held)
+        a.at.sequences, a.at.rows, a.at.table_len = table.shape[0], rows, table.shape[1]
+        a.at.table_stride = table.stride(0)
+        a.at.table = a.at.lengths = 4
+        a.at.starts, a.at.counts = (None if t is None else 4 for t in (starts, counts))
+        return a
+
+    @staticmethod
+    def _signature(*tensors):
+        """What a call's plan goes by, or None."""
+        for t in tensors:
+            if t is not None and type(t) not in _TENSORS:
+                return None
+        return tuple([None if t is None else _sig(t) for t in tensors])
+
+    def _plan(self, key, *plan):
+        if len(self._plans) > 64:
+            self._plans.clear()
+        self._plans[key] = plan
+
+    def _sequences(self, first, table, lengths, starts, counts):
+        """The checked (table, lengths, starts, counts, rows) of a call whose row tensors are like `first`."""
+        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.int32:
+            raise ValueError("table must be an int32 tensor of shape (sequences, entries)")
+        if table.device != self.device:
+            raise ValueError(f"table must be on {self.device}, got {table.device}")
+        s = table.shape[0]
+        if s and table.shape[1] < 1:
+            raise ValueError("table must have an entry for every sequence at least")
+        if starts is not None and counts is not None:
+            raise ValueError("starts and counts exclude each other")
+        lengths = _ints(lengths, s, self.device, "lengths")
+        starts = None if starts is None else _ints(starts, s + 1, self.device, "starts")
+        counts = None if counts is None else _ints(counts, s, self.device, "counts")
+        lead = s if starts is None else 1
+        if first.shape[0] != lead:
+            raise ValueError(f"rows of {s} sequences" + ("" if starts is None else ", packed,") + f" must have a batch of {lead}, got {first.shape[0]}")
+        if s and (table.stride(1) != 1 and table.shape[1] > 1 or table.stride(0) < 0):
+            table = table.contiguous()
+        return table, lengths, starts, counts, first.shape[2]
+
+    def _check(self, tensors, names, shapes):
+        _check_rows(tensors, names)
+        for t, n, s in zip(tensors, names, shapes):
+            if t.shape != s:
+                raise ValueError(f"{n} must have shape {tuple(s)}, got {tuple(t.shape)}")
+        if tensors[0].device != self.device:
+            raise ValueError(f"device mismatch: the cache is on {self.device}, {names[0]} on {tensors[0].device}")
+        if tensors[0].dtype != self.dtype:
+            raise ValueError(f"dtype mismatch: the cache holds {self.dtype}, {names[0]} is {tensors[0].dtype}")
+
+    def _call(self, fn, args_type, buf, what):
+        a = args_type.from_buffer(buf)
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(ctypes.byref(a), _raw_stream(self.device.index))
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(ctypes.byref(a), _raw_stream(self.device.index))
+        if rc:
+            _spa_abi.check(rc, what)
+
+    def append(self, k1, k2, v, table, lengths, q1=None, q2=None, *, starts=None, counts=None, inv_freq=None, sections=None,
+               positions=None, interleaved=False):
+        """The rows of new positions enter their pages: k1, k2 (batch, kv_heads, n, head_dim), v (..., v_head_dim) of the
+        cache's dtype.  With q1, q2 (batch, heads, n, head_dim) returns them as attend() wants them, else None.
+        Positions below 0, or for which the table has no entry, are dropped.
+
+        With inv_freq (float32, (pairs,), pairs at most head_dim / 2) k1, k2 and q1, q2 are turned on the way as
+        rotary_axes() turns them: pair p by positions[axis of p] inv_freq[p], a pair being (p, p + pairs) or, with
+        interleaved, (2 p, 2 p + 1).  positions: int32 or int64, (axes, batch, n); by default a row's place in its
+        sequence, on every axis.  sections: how many pairs turn by each axis (default: all by one).  Without
+        inv_freq rows enter as they are."""
+        given = k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions
+        key = self._signature(*given)
+        if key is not None:
+            key = "append", key, None if sections is None else tuple([int(s) for s in sections]), bool(interleaved)
+            plan = self._plans.get(key)
+            if plan is not None and not any(t.data_ptr() % 16 for t in (k1, k2, v, q1, q2) if t is not None):
+                return self._append(plan, given)
+        _check_rows((k1,), ("k1",))
+        b, hk, n, d, dv = k1.shape[0], self.kv_heads, k1.shape[2], self.head_dim, self.v_head_dim
+        self._check((k1, k2, v), ("k1", "k2", "v"), ((b, hk, n, d), (b, hk, n, d), (b, hk, n, dv)))
+        if (q1 is None) != (q2 is None):
+            raise ValueError("q1 and q2 are given together or not at all")
+        h = 0
+        if q1 is not None:
+            h = q1.shape[1] if isinstance(q1, torch.Tensor) and q1.dim() == 4 else hk
+            self._check((q1, q2), ("q1", "q2"), ((b, h, n, d),) * 2)
+            if h < 1:
+                raise ValueError("q1 has no heads")
+        at = self._sequences(k1, table, lengths, starts, counts)
+        sections, inv_freq, positions = self._turns(sections, inv_freq, positions, b, n)
+        if n == 0 or table.shape[0] == 0:
+            return None if q1 is None else (torch.zeros_like(q1), torch.zeros_like(q2))
+        rows = [t if t is None else _usable(t) for t in (k1, k2, v, q1, q2)]
+        a = self._start_block(_spa_abi.SpaAppendArgs, at)
+        a.heads = h
+        out = [] if q1 is None else [_new_rows(t, d) for t in rows[3:]]
+        for name, t in zip(("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out"), rows + out):
+            if t is not None:
+                getattr(a, name).stride[:] = t.stride()
+        if inv_freq is not None:
+            a.rot, a.axes, a.interleaved = 2 * inv_freq.shape[0], len(sections), int(interleaved)
+            a.sections[:len(sections)] = sections
+            if positions is not None:
+                a.position_stride[:] = positions.stride()
+                a.position_dtype = positions.element_size()
+        plan = bytes(a), [(t.shape, t.stride()) for t in out]
+        now = (*rows, *at[:4], inv_freq, positions)
+        if key is not None and all(x is y for x, y in zip(now, given)):
+            self._plan(key, *plan)
+        return self._append(plan, now)
+
+    def _turns(self, sections, inv_freq, positions, b, n):
+        if inv_freq is None:
+            if sections is not None or positions is not None:
+                raise ValueError("sections and positions need inv_freq")
+            return None, None, None
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+            raise ValueError("inv_freq must be a 1-D float32 tensor")
+        pairs = inv_freq.shape[0]
+        sections = (pairs,) if sections is None else tuple([int(s) for s in sections])
+        if not 1 <= len(sections) <= _sda_abi.MAX_AXES or min(sections) < 0:
+            raise ValueError(f"sections must be 1 to {_sda_abi.MAX_AXES} counts of pairs, got {sections}")
+        if pairs < 1 or sum(sections) != pairs or 2 * pairs > self.head_dim:
+            raise ValueError(f"sections {sections} must add up to inv_freq's {pairs} pairs, at most half of head_dim {self.head_dim}")
+        if positions is not None:
+            if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+                raise ValueError("positions must be an int32 or int64 tensor")
+            if positions.shape != (len(sections), b, n):
+                raise ValueError(f"positions must have shape {(len(sections), b, n)}, got {tuple(positions.shape)}")
+        if inv_freq.device != self.device or positions is not None and positions.device != self.device:
+            raise ValueError(f"positions and inv_freq must be on {self.device}")
+        return sections, inv_freq.contiguous(), positions
+
+    def _append(self, plan, tensors):
+        k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions = tensors
+        buf = bytearray(plan[0])
+        out = tuple([torch.empty_strided(shape, st, dtype=self.dtype, device=self.device) for shape, st in plan[1]])
+        for name, t in zip(("k1", "k2", "v", "table", "lengths"), (k1, k2, v, table, lengths)):
+            _PUT(buf, _APPEND_OFF[name], t.data_ptr())
+        for name, t in (("starts", starts), ("counts", counts), ("inv_freq", inv_freq), ("positions", positions)):
+            if t is not None:
+                _PUT(buf, _APPEND_OFF[name], t.data_ptr())
+        if out:
+            for name, t in zip(("q1", "q2", "q1_out", "q2_out"), (q1, q2, *out)):
+                _PUT(buf, _APPEND_OFF[name], t.data_ptr())
+        self._call(_spa_abi.load().spa_append, _spa_abi.SpaAppendArgs, buf, "spa_append")
+        return out or None
+
+    def attend(self, q1, q2, lambda_param, table, lengths, scale=None, *, starts=None, counts=None, most=None):
+        """Softmax differential attention of the new positions, whose keys and values append() has put in place:
+        q1, q2 (batch, heads, n, head_dim), heads a multiple of kv_heads.  Row i of sequence s sees the positions up
+        to lengths[s] + i that the table has entries for; a row that sees none is zero.  What lies behind may be anything.
+        (A NaN or infinite value row reaches the rows that see it, and may reach other rows of the same call
+        that stand before it.)  Returns (batch, heads, n, v_head_dim); no gradient.
+
+        lambda_param: a float, or a tensor that is a scalar, (heads,) or broadcasts to (batch, heads, n).
+        scale: default 1 / sqrt(head_dim).  most: the rows that any one sequence has, at most, where the caller
+        knows them to be fewer than n; a wrong number costs time, not results."""
+        given = q1, q2, lambda_param, table, lengths, starts, counts
+        key = self._signature(*given) if (scale is None or type(scale) is float) and (most is None or type(most) is int) else None
+        if key is not None:
+            key = "attend", key, scale, most
+            plan = self._plans.get(key)
+            if plan is not None and not (q1.data_ptr() % 16 or q2.data_ptr() % 16):
+                return self._attend(plan, given)
+        _check_rows((q1,), ("q1",))
+        b, h, n = q1.shape[:3]
+        self._check((q1, q2), ("q1", "q2"), ((b, h, n, self.head_dim),) * 2)
+        if h < 1:
+            raise ValueError("q1 has no heads")
+        _check_heads(h, self.kv_heads)
+        s = _scale(scale, self.head_dim)
+        most = 0 if most is None else int(most)
+        if most < 0:
+            raise ValueError(f"most must be at least 0, got {most}")
+        at = self._sequences(q1, table, lengths, starts, counts)
+        lam = _lambda(lambda_param, b, h, n, self.device)
+        if n == 0 or table.shape[0] == 0:
+            return torch.zeros((b, h, n, self.v_head_dim), dtype=self.dtype, device=self.device)
+        q1, q2 = _usable(q1), _usable(q2)
+        out = _new_rows(q1, self.v_head_dim)
+        a = self._start_block(_spa_abi.SpaAttendArgs, at)
+        a.heads, a.most, a.scale = h, most, s
+        for name, t in zip(("q1", "q2", "out"), (q1, q2, out)):
+            getattr(a, name).stride[:] = t.stride()
+        a.lambda_stride[:] = _lambda_strides(lam)
+        a.lambda_dtype = _CODE[lam.dtype]
+        a.workspace_bytes = _spa_abi.load().spa_attend_workspace_bytes(ctypes.byref(a))
+        plan = bytes(a), out.shape, out.stride(), a.workspace_bytes
+        now = (q1, q2, lam, *at[:4])
+        if key is not None and all(x is y for x, y in zip(now, given)):
+            self._plan(key, *plan)
+        return self._attend(plan, now)
+
+    def _attend(self, plan, tensors):
+        q1, q2, lam, table, lengths, starts, counts = tensors
+        block, shape, strides, size = plan
+        buf = bytearray(block)
+        out = torch.empty_strided(shape, strides, dtype=self.dtype, device=self.device)
+        for name, t in zip(("q1", "q2", "out", "lambda_param", "table", "lengths"), (q1, q2, out, lam, table, lengths)):
+            _PUT(buf, _ATTEND_OFF[name], t.data_ptr())
+        if starts is not None:
+            _PUT(buf, _ATTEND_OFF["starts"], starts.data_ptr())
+        if counts is not None:
+            _PUT(buf, _ATTEND_OFF["counts"], counts.data_ptr())
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            _PUT(buf, _ATTEND_OFF["workspace"], ws.data_ptr())
+        self._call(_spa_abi.load().spa_attend, _spa_abi.SpaAttendArgs, buf, "spa_attend")
+        return out
