@@ -13,6 +13,13 @@ namespace spa {
 using sda::lane_id;
 using sda::rsrc_of;
 
+// A value that every lane has, in a scalar register: descriptors are made of such, and one that the compiler cannot see
+// to be the same everywhere, or works out in vector registers (a quotient, a comparison of 64 bits), costs a loop.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return (uint32_t)uniform((int)(uint32_t)x) | ((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
 struct Seq {
   int qb, row0, cnt;  // its rows: row0 .. row0 + cnt - 1 of batch entry qb
   int held, len;      // the position of its first row; the positions that it has with its new rows
@@ -33,14 +40,9 @@ __device__ __forceinline__ Seq seq_of(const Seqs& Q, int s) {
   return r;
 }
 
-// The same in scalar registers (s is the same in every lane): descriptors are made of it.
 __device__ __forceinline__ Seq uniform_seq(const Seqs& Q, int s) {
-  Seq r = seq_of(Q, s);
-  r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
-  r.cnt = __builtin_amdgcn_readfirstlane(r.cnt);
-  r.held = __builtin_amdgcn_readfirstlane(r.held);
-  r.len = __builtin_amdgcn_readfirstlane(r.len);
-  return r;
+  const Seq r = seq_of(Q, s);
+  return {uniform(r.qb), uniform(r.row0), uniform(r.cnt), uniform(r.held), uniform(r.len)};
 }
 
 // The page numbers of 64 consecutive table entries in the lanes of a register, the next 64 on their way:
@@ -82,26 +84,25 @@ struct Pages {
     return e < 64 ? __builtin_amdgcn_readlane(now, e) : __builtin_amdgcn_readlane(next, e - 64);
   }
 };
-// Descriptor over `rows` rows (of `width` bytes, at most up to the page's end) from position `key` of a
-// page's head on; rows past them, and all rows of no page, read as zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, int page, int Hk, int hk, int pshift, int key, int rows,
-                                                           int width) {
-  const int64_t at = (((int64_t)max(page, 0) * Hk + hk) << pshift) + (key & ((1 << pshift) - 1));
-  return rsrc_of(static_cast<const char*>(pool) + at * width, page >= 0 && rows > 0 ? (uint32_t)(rows * width) : 0u);
+// Row of a pool (of one of its heads, counted over all pages) where position `key` of a page stands.
+__device__ __forceinline__ uint64_t pool_row(int page, int Hk, int hk, int pshift, int key) {
+  return ((uint64_t)(uint32_t)(max(page, 0) * Hk + hk) << pshift) + (uint32_t)(key & ((1 << pshift) - 1));
+}
+// How many of the n rows from position `key` on stand before `lim` (a negative number: none).
+__device__ __forceinline__ int rows_before(int key, int n, int lim) {
+  int rows = min(n, lim - key);
+  asm("" : "+s"(rows));  // this minimum and page_rsrc's maximum in one would be a vector instruction
+  return rows;
+}
+// Descriptor over `rows` rows (of WIDTH bytes, at most up to the page's end) from a row of the pool on; rows
+// past them, and all rows of no page, read as zeros.
+template <int WIDTH>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, uint64_t row, int page, int rows) {
+  return rsrc_of(static_cast<const char*>(pool) + row * WIDTH, page >= 0 ? (uint32_t)(max(rows, 0) * WIDTH) : 0u);
 }
 
 // ------------------------------------------------------------------ work
-// Sums over the wave's lanes, and running sums.
-__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ __forceinline__ uint64_t wave_total(uint64_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor((unsigned long long)x, d);
-  return x;
-}
+// Running sums over the wave's lanes, and their totals.
 __device__ __forceinline__ uint32_t running(uint32_t x) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -109,6 +110,12 @@ __device__ __forceinline__ uint32_t running(uint32_t x) {
     if (lane_id() >= d) x += y;
   }
   return x;
+}
+
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)running(x), 63); }
+__device__ __forceinline__ uint64_t wave_total(uint64_t x) {  // of values below 2^58
+  const uint32_t low = wave_total((uint32_t)(x & 0x3ffffff)), mid = wave_total((uint32_t)(x >> 26) & 0x3ffffff);
+  return low + ((uint64_t)mid << 26) + ((uint64_t)wave_total((uint32_t)(x >> 52)) << 52);
 }
 
 constexpr int kUnit = 128;  // keys; pieces are whole units
@@ -120,8 +127,8 @@ struct Job {
   uint32_t first;
 };
 // The tiles of a form (FEW: sequences of at most `bound` rows), in the order of the sequences, a sequence's last
-// tile first: it has the most keys.  With `room` each tile is cut into pieces of at most W / (room - N) units,
-// W the sum over N tiles of their units, so that there are no more than `room` pieces.
+// tile first: it has the most keys.  With `room` each tile is cut into pieces of the fewest units that leave no more
+// than `room` of them: from W / room on, W the sum over N tiles of their units, up to W / (room - N), which always do.
 // BY_PIECE: idx counts pieces; else tiles (for the launch that joins them).  False: there is no such one.
 template <int RT, bool FEW, bool BY_PIECE>
 __device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int room, uint32_t idx, Job& J) {
@@ -148,10 +155,23 @@ __device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int ro
     N = wave_total(N);
     W = wave_total(W);
     if ((uint32_t)room > N) {
-      const uint32_t by = (uint32_t)room - N, over = (uint32_t)(W >> 31);  // W in 31 bits, rounded up
-      const int shift = (W >> 63) ? 33 : over ? 32 - __builtin_clz(over) : 0;
-      const uint32_t w = ((uint32_t)(W >> shift) + (shift ? 1u : 0u) + by - 1) / by;
-      units = (uint32_t)min(max((uint64_t)w << shift, (uint64_t)1), (uint64_t)0x7fffffff);
+      const auto share = [&](uint32_t by) {  // W / by rounded up, of W in 31 bits
+        const uint32_t over = (uint32_t)(W >> 31);
+        const int shift = (W >> 63) ? 33 : over ? 32 - __builtin_clz(over) : 0;
+        const uint32_t w = ((uint32_t)(W >> shift) + (shift ? 1u : 0u) + by - 1) / by;
+        return (uint32_t)min(max((uint64_t)w << shift, (uint64_t)1), (uint64_t)0x7fffffff);
+      };
+      const uint32_t most = share((uint32_t)room - N);  // at most `room` pieces for sure
+      units = share((uint32_t)room);                    // the least there could be
+      while (units < most) {
+        uint32_t n = 0;
+        for (int s0 = 0; s0 < Q.S; s0 += 64) {
+          if (Q.S > 64) sizes(s0);
+          n += t * max((u + units - 1) / units, 1u);
+        }
+        if (wave_total(n) <= (uint32_t)room) break;
+        units = min(units + max(units / 8, 1u), most);
+      }
     }
   }
   uint32_t tiles = 0, pieces = 0;  // of the sequences before
@@ -182,8 +202,8 @@ __device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int ro
 // A piece's keys within the `lim` that its tile sees.
 __device__ __forceinline__ void keys_of(const Job& J, int lim, int& k0, int& k1) {
   const int64_t per = (int64_t)J.units * kUnit;
-  k0 = (int)min((int64_t)J.part * per, (int64_t)lim);
-  k1 = (int)min((int64_t)k0 + per, (int64_t)lim);
+  k0 = uniform((int)min((int64_t)J.part * per, (int64_t)lim));
+  k1 = uniform((int)min((int64_t)k0 + per, (int64_t)lim));
 }
 
 // Zeros the rows of no sequence: workgroup `bid` of `blocks`.

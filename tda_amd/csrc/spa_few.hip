@@ -40,14 +40,15 @@ struct PagedSrc : sda::DenseSrc<Tr, D_, DV_> {
     if (t0 < lim) pages.reach(t0 >> ps);
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      const int key = t0 + 16 * y, rows = min(16, lim - key), pg = pages.page(key >> ps);
+      const int key = t0 + 16 * y, rows = rows_before(key, 16, lim), pg = pages.page(key >> ps);
+      const uint64_t at = pool_row(pg, A->Hk, hk, ps, key);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const auto r = page_rsrc(A->k[x], pg, A->Hk, hk, ps, key, rows, D * ES);
+        const auto r = page_rsrc<D * ES>(A->k[x], at, pg, rows);
 #pragma unroll
         for (int t = 0; t < NT; ++t) g.k[x][y][t] = Base::load8(r, (uint32_t)(n * D * ES + (32 * t + 8 * kq) * ES));
       }
-      const auto r = page_rsrc(A->v, pg, A->Hk, hk, ps, key, rows, DV * ES);
+      const auto r = page_rsrc<DV * ES>(A->v, at, pg, rows);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll

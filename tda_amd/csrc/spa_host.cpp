@@ -35,7 +35,8 @@ int32_t check_cache_sizes(const spa_cache& c) {
   if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1))) return SPA_ERR_PAGES;
   if (c.pages < 1 || c.pages > kMaxPos) return SPA_ERR_PAGES;
   if (c.kv_heads < 1 || c.kv_heads > (1 << 20)) return TDA_ERR_SHAPE;
-  return (double)c.pages * c.kv_heads * c.page_size * c.v_head_dim > (double)kMaxStride ? SPA_ERR_PAGES : TDA_OK;
+  // a page's heads are counted in 32 bits
+  return c.pages * c.kv_heads > kMaxPos || (double)c.pages * c.kv_heads * c.page_size * c.v_head_dim > (double)kMaxStride ? SPA_ERR_PAGES : TDA_OK;
 }
 int32_t check_cache(const spa_cache& c) {
   if (int32_t rc = check_cache_sizes(c)) return rc;
@@ -99,7 +100,7 @@ int32_t check_attend_sizes(const spa_attend_args& a) {
 }
 
 // Workgroups that a call is cut into where its tiles are fewer, by splitting the keys.
-constexpr int64_t kFewTarget = 1024, kManyTarget = 256;
+constexpr int64_t kFewTarget = 256, kManyTarget = 256;
 
 void deal(const spa_attend_args& a, spa::AttendParams& p) {
   const int64_t G = a.heads / a.cache.kv_heads, S = a.at.sequences, hk = a.cache.kv_heads, rows = a.at.rows;

@@ -52,10 +52,10 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv & 3, br = wv >> 2;
   const int r0 = J.tile * kManyRows, r0w = r0 + 32 * rg;
   // positions that the workgroup's, the wave's last rows and the wave's first row see
-  const auto sight = [&](int r) { return max(min(sq.len, sq.held + min(r, R - 1) / G + 1), 0); };
+  const auto sight = [&](int r) { return max(min(sq.len, sq.held + min(r, R - 1) / G + 1), 0); };  // 0 .. 2^30
   int k0p, lim;
   keys_of(J, sight(r0 + kManyRows - 1), k0p, lim);
-  const int limw = min(sight(r0w + 31), lim), clear = sight(r0w);
+  const int limw = uniform(min(sight(r0w + 31), lim)), clear = uniform(sight(r0w));
   const int nst = (lim - k0p + BN - 1) / BN;
   const int r = r0w + n32;  // this lane's row
   const bool live = r < R;
@@ -69,26 +69,50 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
   for (int u = 0; u < VL; ++u) vo[u] = VT::source(8 * u + wv, DV * VT::ES) - (uint32_t)((8 * u + wv) * VR * DV * VT::ES);
   Pages pages;
   pages.begin(P.seq, J.s, k0p >> ps);
-  // Stage j into buffer j % 2; rows behind every row's sight read as zeros (a weight of zero times
-  // whatever lies there must stay zero).
-  auto issue = [&](int j) {
-    char* at = lds + (j & 1) * S::STAGE;
+  // Stage j goes into buffer j % 2; rows behind every row's sight read as zeros (a weight of zero times whatever lies
+  // there must stay zero).  Where its rows stand is worked out a stage ahead of its loads, in the middle of the
+  // products, and kept in scalar registers.
+  constexpr bool SAME = KR == VR;  // keys' and values' loads take the same rows
+  uint64_t krow[KL], vrow[VL];
+  int krows[KL], vrows[VL];
+  auto prepare = [&](int j) {
     const int key = k0p + j * BN;
     pages.reach(key >> ps);
+    const auto place = [&](int k, int n, uint64_t& row, int& rows) {
+      const int pg = pages.page(k >> ps);
+      row = pool_row(pg, P.Hk, hk, ps, k);
+      rows = pg >= 0 ? rows_before(k, n, lim) : 0;
+    };
 #pragma unroll
-    for (int u = 0; u < KL; ++u) {
-      const int k = key + (8 * u + wv) * KR, rows = min(KR, lim - k), pg = pages.page(k >> ps);
+    for (int u = 0; u < KL; ++u) place(key + (8 * u + wv) * KR, KR, krow[u], krows[u]);
+    if constexpr (!SAME) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        KT::load(page_rsrc(P.k[x], pg, P.Hk, hk, ps, k, rows, D * KT::ES), reinterpret_cast<T*>(at + x * KT::BYTES), 8 * u + wv, ko[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < VL; ++u) {
-      const int k = key + (8 * u + wv) * VR, rows = min(VR, lim - k), pg = pages.page(k >> ps);
-      VT::load(page_rsrc(P.v, pg, P.Hk, hk, ps, k, rows, DV * VT::ES), reinterpret_cast<T*>(at + 2 * KT::BYTES), 8 * u + wv, vo[u]);
+      for (int u = 0; u < VL; ++u) place(key + (8 * u + wv) * VR, VR, vrow[u], vrows[u]);
     }
   };
-  if (nst > 0) issue(0);
+  auto issue = [&](int j) {
+    char* at = lds + (j & 1) * S::STAGE;
+#pragma unroll
+    for (int u = 0; u < KL; ++u) {
+      const uint64_t row = uniform(krow[u]);
+      const int rows = uniform(krows[u]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        KT::load(page_rsrc<D * KT::ES>(P.k[x], row, 0, rows), reinterpret_cast<T*>(at + x * KT::BYTES), 8 * u + wv, ko[u]);
+      if constexpr (SAME)
+        VT::load(page_rsrc<DV * VT::ES>(P.v, row, 0, rows), reinterpret_cast<T*>(at + 2 * KT::BYTES), 8 * u + wv, vo[u]);
+    }
+    if constexpr (!SAME) {
+#pragma unroll
+      for (int u = 0; u < VL; ++u)
+        VT::load(page_rsrc<DV * VT::ES>(P.v, uniform(vrow[u]), 0, uniform(vrows[u])), reinterpret_cast<T*>(at + 2 * KT::BYTES), 8 * u + wv, vo[u]);
+    }
+  };
+  if (nst > 0) {
+    prepare(0);
+    issue(0);
+    prepare(1);
+  }
 
   frag qf[NT];
   sda::load_frags<Tr, NT>(live ? sda::row_of<T>(P.q[br], sq.qb, h, qi) : nullptr, g, qf);
@@ -107,7 +131,10 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
     tda::lds_barrier();  // stage j is in place, and every wave is done with stage j - 1
     if (j + 1 < nst) issue(j + 1);
     const int k0 = k0p + j * BN;
-    if (k0 >= limw) return;
+    if (k0 >= limw) {
+      prepare(j + 2);
+      return;
+    }
     // one sequence of NS NT key fragments, then 2 NS NO value fragments, read a group ahead of their use
     frag f[2][G4];
     auto read = [&](int i) {
@@ -164,6 +191,7 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
     frag p[2 * NS];
 #pragma unroll
     for (int x = 0; x < 2 * NS; ++x) p[x] = sda::pack8<Tr>(s[x / 2], x % 2);
+    prepare(j + 2);  // behind the last stage: rows of none
     constexpr int first = NS * NT / G4, last = first + 2 * NS * NO / G4;
 #pragma unroll
     for (int i = first; i < last; ++i) {
