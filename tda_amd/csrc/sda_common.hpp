@@ -200,7 +200,12 @@ struct RowReader {
       return Tile<Tr, 32, W>::row(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, t);
   }
 };
-template <class Tr, int W>
+// A transposing read that the compiler takes to be apart from the direct loads to LDS on their way.  It knows no more of
+// this read than that it reads LDS, and would wait for every such load before it (that of the next stage, issued a
+// moment ago): a pass that uses it has to wait for the loads of what it reads itself.
+typedef __attribute__((address_space(3))) tda::s16x4 quad;
+__device__ __forceinline__ tda::s16x4 read_apart(quad* __restrict p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
+template <class Tr, int W, bool APART = false>
 struct ColReader {
   static constexpr int NY = W / 32;
   uint32_t a[2][NY];
@@ -221,12 +226,12 @@ struct ColReader {
   // Step s (16 rows) of the tile at `at`, column block y.
   __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int s, int y) const {
     if constexpr (sizeof(typename Tr::T) == 2) {
-      typedef __attribute__((address_space(3))) tda::s16x4 quad;
       typedef typename Tr::T half4 __attribute__((ext_vector_type(4)));
       typename Tr::frag f;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        const half4 w = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<quad*>(a[hh][y] + at + 32 * W * s)));
+        quad* p = reinterpret_cast<quad*>(a[hh][y] + at + 32 * W * s);
+        const half4 w = __builtin_bit_cast(half4, APART ? read_apart(p) : __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[4 * hh + e] = w[e];
       }

@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
   float m = sda::kNoMax, sums[4] = {};
 
   sda::RowReader<Tr, D> kr;
-  sda::ColReader<Tr, DV> vr;
+  sda::ColReader<Tr, DV, true> vr;  // a stage is waited for before its barrier
   const char* kbuf = lds + br * KT::BYTES;
   const char* vbuf = lds + 2 * KT::BYTES;
   kr.init(kbuf);
