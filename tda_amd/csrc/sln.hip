@@ -5,7 +5,8 @@
 //
 // A row stays in the registers of the lanes that share it: 8 to 64 lanes of a wave for rows of up to 4 KB, with the
 // row's sums by lane moves, and 256 or 1024 threads beyond, whose waves' sums meet in LDS.  A lane's pieces are the same columns of every row, so it keeps the sums of dw and db in registers over all
-// its rows; a workgroup leaves one row of them, and a second launch adds those up in order.  All sums are 32 bits;
+// its rows; a workgroup leaves one row of them, and a second launch adds those up in order (where there are few rows, one
+// workgroup takes them all and writes the result).  All sums are 32 bits;
 // the variance is taken around the mean (of a wave, joined by the waves' means).
 #include "sda_common.hpp"
 #include "sln_params.hpp"
@@ -59,6 +60,12 @@ __device__ __forceinline__ void weights(const void* p, int type, int64_t row, in
 #pragma unroll
     for (int e = 0; e < V; ++e) w[e] = (float)x[e];
   }
+}
+
+template <class T>
+__device__ __forceinline__ void put_sum(void* p, int type, int64_t at, float x) {
+  if (type == 0) static_cast<float*>(p)[at] = x;
+  else static_cast<T*>(p)[at] = (T)x;
 }
 
 // Sum over the L lanes that share a row (of a wave, if they are more).
@@ -292,7 +299,7 @@ __global__ void __launch_bounds__(bwd_threads(L)) norm_bwd(Params P) {
       }
     }
   }
-  if (!P.part) return;
+  if (!P.dweight && !P.dbias) return;
   // the rows that a wave has side by side, then the waves, in order
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -321,8 +328,15 @@ __global__ void __launch_bounds__(bwd_threads(L)) norm_bwd(Params P) {
     }
     __syncthreads();
   }
-  float* to = P.part + ((int64_t)grp * P.blocks + blk) * 2 * width;
-  for (int e = threadIdx.x; e < 2 * width; e += TH) to[e] = sums[e];
+  if (P.part) {
+    float* to = P.part + ((int64_t)grp * P.blocks + blk) * 2 * width;
+    for (int e = threadIdx.x; e < 2 * width; e += TH) to[e] = sums[e];
+    return;
+  }
+  for (int e = threadIdx.x; e < width; e += TH) {
+    if (P.dweight) put_sum<T>(P.dweight, P.weight_type, (int64_t)grp * width + e, sums[e]);
+    if (P.dbias) put_sum<T>(P.dbias, P.weight_type, (int64_t)grp * width + e, sums[width + e]);
+  }
 }
 
 // Adds up the workgroups' rows of sums: 32 columns a workgroup, every eighth row a thread, then those eight.
@@ -354,9 +368,7 @@ __global__ void __launch_bounds__(256) norm_sums(Params P) {
   float all = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) all += lds[k][x];
-  const int64_t to = (int64_t)grp * P.width + col;
-  if (P.weight_type == 0) static_cast<float*>(out)[to] = all;
-  else static_cast<T*>(out)[to] = (T)all;
+  put_sum<T>(out, P.weight_type, (int64_t)grp * P.width + col, all);
 }
 
 // ------------------------------------------------------------------ launches
@@ -372,7 +384,7 @@ static int fwd(const Params& p, hipStream_t st) {
 template <class T, bool WHOLE, int L, int C, int U>
 static int bwd(const Params& p, hipStream_t st) {
   constexpr int TH = bwd_threads(L);
-  const int lds = p.part ? 2 * p.width * 4 : 0;
+  const int lds = p.dweight || p.dbias ? 2 * p.width * 4 : 0;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&norm_bwd<T, WHOLE, L, C, U>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;

@@ -143,7 +143,7 @@ size_t sln_bwd_workspace_bytes(const sln_bwd_args* a) {
   if (!a || check_sizes(*a) || !(a->dweight || a->dbias)) return 0;
   const int64_t groups = a->weight_heads ? a->heads : 1;
   const int64_t blocks = sln::bwd_blocks((int)a->width, a->dtype, (int)groups, (int)(a->batch * a->heads * a->rows / groups));
-  return (size_t)(groups * blocks * 2 * a->width * 4);
+  return blocks == 1 ? 0 : (size_t)(groups * blocks * 2 * a->width * 4);
 }
 
 int32_t sln_validate_bwd(const sln_bwd_args* a) {
@@ -172,7 +172,7 @@ int32_t sln_bwd(const sln_bwd_args* a, void* stream) {
   p.dweight = a->dweight;
   p.dbias = a->dbias;
   p.blocks = sln::bwd_blocks(p.width, a->dtype, p.groups, p.rows);
-  if (a->dweight || a->dbias) p.part = static_cast<float*>(a->workspace);
+  if ((a->dweight || a->dbias) && p.blocks > 1) p.part = static_cast<float*>(a->workspace);
   tda::timing_begin(stream);
   return done(sln::launch_bwd(p, a->dtype, stream));
 }

@@ -44,6 +44,7 @@ inline int bwd_blocks(int width, int dtype, int groups, int rows) {
   const Split s = split_of(width, dtype);
   const int at_once = bwd_threads(s.lanes) / s.lanes, chip = s.pieces == 1 ? 1024 : s.lanes == 1024 ? 256 : 512;
   const int most = (rows + at_once - 1) / at_once, want = (chip + groups - 1) / groups;
+  if (most <= 8) return 1;  // a workgroup's few rounds cost less than the second launch
   return most < want ? most : want;
 }
 

@@ -40,11 +40,6 @@ __device__ __forceinline__ Seq seq_of(const Seqs& Q, int s) {
   return r;
 }
 
-__device__ __forceinline__ Seq uniform_seq(const Seqs& Q, int s) {
-  const Seq r = seq_of(Q, s);
-  return {uniform(r.qb), uniform(r.row0), uniform(r.cnt), uniform(r.held), uniform(r.len)};
-}
-
 // The page numbers of 64 consecutive table entries in the lanes of a register, the next 64 on their way:
 // page() then costs a few scalar instructions.  Entries behind the table, and numbers that are no page,
 // are -1.
@@ -102,16 +97,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, ui
 }
 
 // ------------------------------------------------------------------ work
-// Running sums over the wave's lanes, and their totals.
+// Running sums over the wave's lanes (lane moves: four within rows of 16 lanes, two from row to row), and their totals.
+// Call with every lane active.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {  // 0 where nothing comes from
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true);
+}
 __device__ __forceinline__ uint32_t running(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t y = __shfl_up(x, d);
-    if (lane_id() >= d) x += y;
-  }
+  x += moved<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x += moved<0x112, 0xF>(x);
+  x += moved<0x114, 0xF>(x);
+  x += moved<0x118, 0xF>(x);
+  x += moved<0x142, 0xA>(x);  // row_bcast 15 into rows 1 and 3
+  x += moved<0x143, 0xC>(x);  // row_bcast 31 into rows 2 and 3
   return x;
 }
-
 __device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)running(x), 63); }
 __device__ __forceinline__ uint64_t wave_total(uint64_t x) {  // of values below 2^58
   const uint32_t low = wave_total((uint32_t)(x & 0x3ffffff)), mid = wave_total((uint32_t)(x >> 26) & 0x3ffffff);
@@ -125,6 +125,7 @@ constexpr int kUnit = 128;  // keys; pieces are whole units
 struct Job {
   int s, tile, part, parts, units;  // units of keys in a piece
   uint32_t first;
+  Seq seq;
 };
 // The tiles of a form (FEW: sequences of at most `bound` rows), in the order of the sequences, a sequence's last
 // tile first: it has the most keys.  With `room` each tile is cut into pieces of the fewest units that leave no more
@@ -134,10 +135,11 @@ template <int RT, bool FEW, bool BY_PIECE>
 __device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int room, uint32_t idx, Job& J) {
   const int l = lane_id();
   uint32_t t = 0, u = 0;
+  Seq q{};
   const auto sizes = [&](int s0) {
     t = u = 0;
     if (s0 + l < Q.S) {
-      const Seq q = seq_of(Q, s0 + l);
+      q = seq_of(Q, s0 + l);
       const int R = q.cnt * G;
       if ((R <= bound) == FEW) t = (uint32_t)(R + RT - 1) / RT;
       u = (uint32_t)(q.len + kUnit - 1) / kUnit;
@@ -192,6 +194,8 @@ __device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int ro
       J.tile = (int)(nt - 1 - at);
       J.units = (int)units;
       J.first = first + at * (uint32_t)J.parts;
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x); };
+      J.seq = {of(q.qb), of(q.row0), of(q.cnt), of(q.held), of(q.len)};
       return true;
     }
     tiles += __builtin_amdgcn_readlane(tu, 63);

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) few_rows(DecParams P, AttendParams A) {
   clear_free_rows<T, DV, 256>(A, bid, A.few.grid);
   Job J;
   if (!find_job<kFewRows, true, true>(A.seq, A.H / A.Hk, A.bound, A.few.room, bid / (uint32_t)A.Hk, J)) return;
-  const Seq s = uniform_seq(A.seq, J.s);
+  const Seq s = J.seq;
   DecWork W;
   W.b = J.s;
   W.hk = (int)(bid % (uint32_t)A.Hk);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
     Job J;
     if (!find_job<kFewRows, true, false>(A.seq, G, A.bound, A.few.room, bid / (uint32_t)A.Hk, J) || J.parts < 2) return;
     const int hk = (int)(bid % (uint32_t)A.Hk);
-    const Seq s = uniform_seq(A.seq, J.s);
+    const Seq s = J.seq;
     const int rows = min(kFewRows, s.cnt * G - kFewRows * J.tile);
     const float* base = A.few.part + ((int64_t)J.first * A.Hk + hk) * few_floats(DV);
     const int64_t step = (int64_t)A.Hk * few_floats(DV);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
   Job J;
   if (!find_job<kManyRows, false, false>(A.seq, G, A.bound, A.many.room, item / (uint32_t)A.Hk, J) || J.parts < 2) return;
   const int hk = (int)(item % (uint32_t)A.Hk);
-  const Seq s = uniform_seq(A.seq, J.s);
+  const Seq s = J.seq;
   // the second form's pieces: [branch][m, l][128], then [branch][32 rows][4 of a lane's values][lane]
   const float* base = A.many.part + ((int64_t)J.first * A.Hk + hk) * many_floats(DV);
   const int64_t step = (int64_t)A.Hk * many_floats(DV);
@@ -174,23 +174,49 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
   const int h = hk * G + q % G, i = s.row0 + q / G;
   const float lam = sda::lambda_of(A.lam, s.qb, h, i);
   T* to = sda::row_of<T>(A.out, s.qb, h, i);
-  for (int x = tid >> 6; x < 4 * NO; x += 4) {
-    float a[2][4];
-    Joined j[2];
+  // each branch's maximum and sum over the pieces, then the pieces' values under them, in order
+  float top[2], inv[2];
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
-      join_parts(J.parts, [&](int u, float& m, float& z) {
-          m = base[u * step + 2 * kManyRows * y + 32 * rg + (l & 31)];
-          z = base[u * step + 2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
-        }, [&](int u, float(&v)[4]) {
-          const f32x4 w = *reinterpret_cast<const f32x4*>(base + u * step + 4 * kManyRows + (int64_t)(((y * RG + rg) * NO * 4 + x) * 64 + l) * 4);
+  for (int y = 0; y < 2; ++y) {
+    Joined j;
+    float none[1];
+    join_parts(J.parts, [&](int u, float& m, float& z) {
+        m = base[u * step + 2 * kManyRows * y + 32 * rg + (l & 31)];
+        z = base[u * step + 2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
+      }, [](int, float(&v)[1]) { v[0] = 0.f; }, none, j);
+    top[y] = j.m;
+    inv[y] = j.l > 0.f || j.l != j.l ? 1.0f / j.l : 0.f;
+  }
+  inv[1] *= -lam;
+  constexpr int XS = NO < 4 ? NO : 4;  // quads of values a thread has in hand
+  f32x4 z[XS] = {};
+  const int x0 = (tid >> 6) * NO;
+  for (int xs = 0; xs < NO; xs += XS) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = w[e];
-        }, a[y], j[y]);
-    f32x4 z;
+    for (int k = 0; k < XS; ++k) z[k] = f32x4{};
+    for (int u = 0; u < J.parts; ++u) {
+      const float* part = base + u * step;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, over(a[1][e], j[1].l), over(a[0][e], j[0].l));
-    sda::store4(to + 32 * (x / 4) + 8 * (x % 4) + 4 * (l >> 5), z);
+      for (int y = 0; y < 2; ++y) {
+        const float sum = part[2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
+        const float w = sda::exp2_(part[2 * kManyRows * y + 32 * rg + (l & 31)] - top[y]) * inv[y];
+        f32x4 v[XS];
+#pragma unroll
+        for (int k = 0; k < XS; ++k)
+          v[k] = *reinterpret_cast<const f32x4*>(part + 4 * kManyRows + (int64_t)(((y * RG + rg) * NO * 4 + x0 + xs + k) * 64 + l) * 4);
+        if (sum != 0.f) {  // else no key of this piece: its sums are not written
+#pragma unroll
+          for (int k = 0; k < XS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[k][e] = __builtin_fmaf(w, v[k][e], z[k][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < XS; ++k) {
+      const int x = x0 + xs + k;
+      sda::store4(to + 32 * (x / 4) + 8 * (x % 4) + 4 * (l >> 5), z[k]);
+    }
   }
 }
 

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(512) many_rows(AttendParams P) {
   const int G = P.H / P.Hk, hk = (int)(bid % (uint32_t)P.Hk), ps = P.seq.pshift;
   Job J;
   if (!find_job<kManyRows, false, true>(P.seq, G, P.bound, P.many.room, bid / (uint32_t)P.Hk, J)) return;
-  const Seq sq = uniform_seq(P.seq, J.s);
+  const Seq sq = J.seq;
   const int R = sq.cnt * G;
   const int l = lane_id(), n32 = l & 31, g = l >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wv & 3, br = wv >> 2;

@@ -9,36 +9,18 @@ import struct
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _sln_abi, ops
-from .softmax import _CODE, _COMPUTE, _TENSORS, _free_of_grad, _new_rows, _raw_stream, _refuse_tangents, _sig
+from . import _sln_abi
+from .softmax import _CODE, _COMPUTE, _TENSORS, _new_rows, _raw_stream, _refuse_tangents, _sig
 
 _PUT = struct.Struct("<Q").pack_into
-_FWD_OFF = {n: getattr(_sln_abi.SlnFwdArgs, n).offset for n in ("x", "y", "weight", "bias", "stats")}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_FWD_X, _FWD_Y, _FWD_W, _FWD_B, _FWD_S = (getattr(_sln_abi.SlnFwdArgs, n).offset for n in ("x", "y", "weight", "bias", "stats"))
 _BWD_OFF = {n: getattr(_sln_abi.SlnBwdArgs, n).offset for n in ("x", "dy", "dx", "weight", "stats", "dweight", "dbias", "workspace")}
-
-_plans: dict = {}  # of calls without gradients whose tensors need no copy, by signature: no checks again
-
-
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
-
-
-def _strides(t: torch.Tensor):
-    return (*t.stride()[:3], 1)
-
-
-def _rows4(x: torch.Tensor) -> torch.Tensor:
-    """x as (batch, heads, rows, width), a view where its strides allow one."""
-    if x.dim() == 4:
-        return x
-    if x.dim() == 3:
-        return x.unsqueeze(1)
-    return x.reshape(1, 1, -1, x.shape[-1])
 
 
 def _call(fn, args_type, buf, device, what):
     a = args_type.from_buffer(buf)
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         rc = fn(ctypes.byref(a), _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
@@ -47,78 +29,121 @@ def _call(fn, args_type, buf, device, what):
         _sln_abi.check(rc, what)
 
 
-def _head(a, x, weight, bias, center):
-    w = weight if weight is not None else bias
-    a.abi_version, a.dtype, a.center = _sln_abi.ABI_VERSION, _CODE[x.dtype], int(center)
-    a.batch, a.heads, a.rows, a.width = x.shape
-    a.weight_dtype = _CODE[w.dtype if w is not None else x.dtype]
-    a.weight_heads = int(w is not None and w.dim() == 2)
-    a.x.stride[:] = _strides(x)
+class _Plan:
+    """What a call's signature settles: its argument blocks but for the device pointers, the shape and strides of its
+    result.  Rows are (batch, heads, rows, width), axes that x lacks being of one element."""
+
+    __slots__ = ("block", "shape", "strides", "rows", "center", "weight_dtype", "weight_heads", "bwd")
+
+    def __init__(self, x, weight, bias, eps, center):
+        w = weight if weight is not None else bias
+        self.shape, self.center = x.shape, center
+        self.rows = (1,) * (4 - x.dim()) + tuple(x.shape)
+        self.strides = (_new_rows(x, x.shape[3]) if x.dim() == 4 else torch.empty(x.shape, device="meta")).stride()
+        self.weight_dtype = _CODE[w.dtype if w is not None else x.dtype]
+        self.weight_heads = int(w is not None and w.dim() == 2)
+        self.bwd: dict = {}  # argument block and workspace, by the gradient's strides and the gradients wanted
+        a = _sln_abi.SlnFwdArgs()
+        self.head(a, x)
+        a.eps = eps
+        a.y.stride[:] = self.four(self.strides)
+        self.block = bytes(a)
+
+    def head(self, a, x):
+        a.abi_version, a.dtype, a.center = _sln_abi.ABI_VERSION, _CODE[x.dtype], int(self.center)
+        a.batch, a.heads, a.rows, a.width = self.rows
+        a.weight_dtype, a.weight_heads = self.weight_dtype, self.weight_heads
+        a.x.stride[:] = self.four(x.stride())
+
+    @staticmethod
+    def four(strides):
+        return (*(0,) * (4 - len(strides)), *strides[:-1], 1)
+
+    def backward_block(self, x, dy, want):
+        a = _sln_abi.SlnBwdArgs()
+        self.head(a, x)
+        a.dy.stride[:] = self.four(dy.stride())
+        if want[0]:
+            a.dx.stride[:] = self.four(self.strides)
+        a.dweight, a.dbias = (4 if w else None for w in want[1:])
+        a.workspace_bytes = _sln_abi.load().sln_bwd_workspace_bytes(ctypes.byref(a))
+        if len(self.bwd) > 64:
+            self.bwd.clear()
+        got = self.bwd[dy.stride(), want] = bytes(a), a.workspace_bytes
+        return got
+
+    def forward(self, x, weight, bias, stats):
+        y = torch.empty_strided(self.shape, self.strides, dtype=x.dtype, device=x.device)
+        buf = bytearray(self.block)
+        _PUT(buf, _FWD_X, x.data_ptr())
+        _PUT(buf, _FWD_Y, y.data_ptr())
+        if weight is not None:
+            _PUT(buf, _FWD_W, weight.data_ptr())
+        if bias is not None:
+            _PUT(buf, _FWD_B, bias.data_ptr())
+        if stats is not None:
+            _PUT(buf, _FWD_S, stats.data_ptr())
+        _call(_sln_abi.load().sln_fwd, _sln_abi.SlnFwdArgs, buf, x.device, "sln_fwd")
+        return y
+
+    def run(self, x, weight, bias):
+        if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                        or bias is not None and bias.requires_grad):
+            return _LayerNorm.apply(x, weight, bias, self)
+        return self.forward(x, weight, bias, None)
 
 
-def _fwd_block(x, y, weight, bias, eps, center) -> bytes:
-    a = _sln_abi.SlnFwdArgs()
-    _head(a, x, weight, bias, center)
-    a.eps = eps
-    a.y.stride[:] = _strides(y)
-    return bytes(a)
+_plans: dict = {}  # by signature, of calls whose tensors need no copy: no checks again
 
 
-def _forward(block, x, y, weight, bias, stats):
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    plan, bias = ctx.cfg
+    want = ctx.needs_input_grad[:3]
+    if dy.dtype != x.dtype:
+        dy = dy.to(x.dtype)
+    if dy.stride(-1) != 1 and dy.shape[-1] > 1:
+        dy = dy.contiguous()
+    block, size = ctx.block if dy.stride() == plan.strides and ctx.block else plan.bwd.get((dy.stride(), want)) or plan.backward_block(x, dy, want)
     buf = bytearray(block)
-    for name, t in (("x", x), ("y", y), ("weight", weight), ("bias", bias), ("stats", stats)):
-        if t is not None:
-            _PUT(buf, _FWD_OFF[name], t.data_ptr())
-    _call(_sln_abi.load().sln_fwd, _sln_abi.SlnFwdArgs, buf, x.device, "sln_fwd")
+    dx = dw = db = None
+    if want[0]:
+        dx = torch.empty_strided(plan.shape, plan.strides, dtype=x.dtype, device=x.device)
+        _PUT(buf, _BWD_OFF["dx"], dx.data_ptr())
+    if weight is not None:
+        _PUT(buf, _BWD_OFF["weight"], weight.data_ptr())
+        if want[1]:
+            dw = torch.empty_like(weight)
+            _PUT(buf, _BWD_OFF["dweight"], dw.data_ptr())
+    if want[2]:
+        db = torch.empty(bias[0], dtype=bias[1], device=x.device)
+        _PUT(buf, _BWD_OFF["dbias"], db.data_ptr())
+    if size:
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        _PUT(buf, _BWD_OFF["workspace"], ws.data_ptr())
+    _PUT(buf, _BWD_OFF["x"], x.data_ptr())
+    _PUT(buf, _BWD_OFF["dy"], dy.data_ptr())
+    _PUT(buf, _BWD_OFF["stats"], stats.data_ptr())
+    _call(_sln_abi.load().sln_bwd, _sln_abi.SlnBwdArgs, buf, x.device, "sln_bwd")
+    return dx, dw, db, None
 
 
-def _key(kind, rows, weight, bias, *more):
-    return (kind, rows[0].shape, rows[0].dtype, tuple([None if t is None else t.stride() for t in rows]),
-            tuple([None if t is None else (t.dtype, t.dim()) for t in (weight, bias)]), *more)
+_backward_once = once_differentiable(_backward)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, center):
-        x = _readable(x)
-        y = _new_rows(x, x.shape[3])
-        stats = torch.empty(x.shape[:3] + (2,), dtype=torch.float32, device=x.device)
-        block = ops._cached(_key("sln_fwd", (x, y), weight, bias, eps, center), lambda: _fwd_block(x, y, weight, bias, eps, center))
-        _forward(block, x, y, weight, bias, stats)
+    def forward(ctx, x, weight, bias, plan):
+        stats = torch.empty(plan.rows[:3] + (2,), dtype=torch.float32, device=x.device)
         ctx.save_for_backward(x, weight, stats)
-        ctx.cfg = (None if bias is None else (bias.shape, bias.dtype), center)
-        return y
+        ctx.cfg = plan, None if bias is None else (bias.shape, bias.dtype)
+        ctx.block = plan.bwd.get((plan.strides, ctx.needs_input_grad[:3]))
+        return plan.forward(x, weight, bias, stats)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        like_bias, center = ctx.cfg
-        dy = _readable(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-        want = ctx.needs_input_grad
-        dx = _new_rows(x, x.shape[3]) if want[0] else None
-        dw = torch.empty_like(weight) if want[1] else None
-        db = torch.empty(like_bias[0], dtype=like_bias[1], device=x.device) if want[2] else None
-
-        def build():
-            a = _sln_abi.SlnBwdArgs()
-            _head(a, x, weight, db, center)
-            a.dy.stride[:] = _strides(dy)
-            if dx is not None:
-                a.dx.stride[:] = _strides(dx)
-            a.dweight, a.dbias = (None if t is None else 4 for t in (dw, db))
-            a.workspace_bytes = _sln_abi.load().sln_bwd_workspace_bytes(ctypes.byref(a))
-            return bytes(a), a.workspace_bytes
-
-        block, size = ops._cached(_key("sln_bwd", (x, dy, dx), weight, db, center, want[:3]), build)
-        buf = bytearray(block)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        for name, t in (("x", x), ("dy", dy), ("dx", dx), ("weight", weight), ("stats", stats), ("dweight", dw), ("dbias", db),
-                        ("workspace", ws)):
-            if t is not None:
-                _PUT(buf, _BWD_OFF[name], t.data_ptr())
-        _call(_sln_abi.load().sln_bwd, _sln_abi.SlnBwdArgs, buf, x.device, "sln_bwd")
-        return dx, dw, db, None, None
+        # what refuses a second derivative is set up where one may be taken
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def _check_weight(w, name, x, other):
@@ -146,12 +171,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
     _refuse_tangents("layer_norm", x, weight, bias)
     key = None
     if type(x) in _TENSORS and (weight is None or type(weight) in _TENSORS) and (bias is None or type(bias) in _TENSORS):
-        key = _sig(x), None if weight is None else _sig(weight), None if bias is None else _sig(bias), eps, bool(center)
+        key = _sig(x), None if weight is None else _sig(weight), None if bias is None else _sig(bias), eps, center
         plan = _plans.get(key)
-        if plan is not None and _free_of_grad(*[t for t in (x, weight, bias) if t is not None]):
-            y = torch.empty_strided(plan[1], plan[2], dtype=x.dtype, device=x.device)
-            _forward(plan[0], x, y, weight, bias, None)
-            return y
+        if plan is not None:
+            return plan.run(x, weight, bias)
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
     if x.dim() < 1:
@@ -169,25 +192,16 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
         _check_weight(weight, "weight", x, None)
     if bias is not None:
         _check_weight(bias, "bias", x, weight)
-    given = x, weight, bias
     if x.dtype == torch.float64:
-        x, weight, bias = (None if t is None else t.to(torch.float32) for t in given)
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    if x.numel() == 0:
-        return x * 1 + sum((t.sum() * 0 for t in (weight, bias) if t is not None), torch.zeros((), dtype=x.dtype, device=x.device)).to(x.dtype)
-    rows = _rows4(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        y = _LayerNorm.apply(rows, weight, bias, e, bool(center))
-    else:
-        r = _readable(rows)
-        y = _new_rows(r, r.shape[3])
-        block = _fwd_block(r, y, weight, bias, e, bool(center))
-        _forward(block, r, y, weight, bias, None)
-        if key is not None and r is rows and x is given[0] and weight is given[1] and bias is given[2] and rows.data_ptr() == x.data_ptr():
-            if len(_plans) > 4096:
-                _plans.clear()
-            out = y.view(x.shape) if x.dim() != 4 else y
-            _plans[key] = block, out.shape, out.stride()
-    if y.shape != x.shape:
-        y = y.view(x.shape)
-    return y if y.dtype == given[0].dtype else y.to(given[0].dtype)
+        return layer_norm(x.float(), *(None if t is None else t.float() for t in (weight, bias)), e, center=center).double()
+    if x.numel() == 0:  # no rows: connected to the inputs
+        return x * 1 + sum((t.sum() * 0 for t in (weight, bias) if t is not None), torch.zeros((), device=x.device)).to(x.dtype)
+    rows = x.flatten(0, -2) if x.dim() > 4 else x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    now = rows, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
+    plan = _Plan(*now, e, bool(center))
+    if key is not None and all(a is b for a, b in zip(now, (x, weight, bias))):
+        if len(_plans) > 4096:
+            _plans.clear()
+        _plans[key] = plan
+    y = plan.run(*now)
+    return y if y.shape == x.shape else y.view(x.shape)
