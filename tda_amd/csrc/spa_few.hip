@@ -194,23 +194,31 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
   for (int xs = 0; xs < NO; xs += XS) {
 #pragma unroll
     for (int k = 0; k < XS; ++k) z[k] = f32x4{};
-    for (int u = 0; u < J.parts; ++u) {
-      const float* part = base + u * step;
+    for (int u0 = 0; u0 < J.parts; u0 += 2) {  // two pieces' values on their way
+      f32x4 v[2][2][XS];
+      float w[2][2];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float sum = part[2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
-        const float w = sda::exp2_(part[2 * kManyRows * y + 32 * rg + (l & 31)] - top[y]) * inv[y];
-        f32x4 v[XS];
+      for (int u = 0; u < 2; ++u) {
+        const float* part = base + min(u0 + u, J.parts - 1) * step;
 #pragma unroll
-        for (int k = 0; k < XS; ++k)
-          v[k] = *reinterpret_cast<const f32x4*>(part + 4 * kManyRows + (int64_t)(((y * RG + rg) * NO * 4 + x0 + xs + k) * 64 + l) * 4);
-        if (sum != 0.f) {  // else no key of this piece: its sums are not written
+        for (int y = 0; y < 2; ++y) {
+          const float sum = part[2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
+          w[u][y] = u0 + u < J.parts && sum != 0.f  // else no key of this piece: its sums are not written
+                        ? sda::exp2_(part[2 * kManyRows * y + 32 * rg + (l & 31)] - top[y]) * inv[y] : 0.f;
 #pragma unroll
           for (int k = 0; k < XS; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[k][e] = __builtin_fmaf(w, v[k][e], z[k][e]);
+            v[u][y][k] = *reinterpret_cast<const f32x4*>(part + 4 * kManyRows + (int64_t)(((y * RG + rg) * NO * 4 + x0 + xs + k) * 64 + l) * 4);
         }
       }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (w[u][y] != 0.f)
+#pragma unroll
+            for (int k = 0; k < XS; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) z[k][e] = __builtin_fmaf(w[u][y], v[u][y][k][e], z[k][e]);
     }
 #pragma unroll
     for (int k = 0; k < XS; ++k) {
