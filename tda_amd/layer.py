@@ -1,5 +1,5 @@
 """Multi-head differential attention as nn.Modules: the threshold form, and the softmax form with rotary
-positions and decoding over a 4-bit cache (DifferentialAttention).
+positions, a norm of the heads' outputs and decoding over a 4-bit or a paged cache (DifferentialAttention).
 
 The reference ships only the functional operator (snap-research/TDA
 triton_threshold_attention.py, TTA:472-519); the layer of the paper it accompanies (README.md:10)
@@ -22,6 +22,8 @@ from torch import nn
 
 from .api import differential_threshold_rela_triton, threshold_rela_triton
 from .kv_cache import Int4KVCache
+from .norm import layer_norm
+from .paged_cache import PagedKVCache
 from .rotary import rotary_axes
 from .softmax import differential_attention
 
@@ -115,10 +117,12 @@ class ThresholdDifferentialAttention(nn.Module):
 
 class DifferentialAttention(nn.Module):
     """Causal multi-head softmax differential attention with rotary positions, for training and for decoding
-    over a 4-bit cache:
+    over a 4-bit or a paged cache:
 
         x (B, N, E) --fused projection--> q1, q2 (B, N, H, d), k1, k2 (B, N, Hk, d), v (B, N, Hk, dv)
           --> rotary_axes on q1, q2, k1, k2 --> differential_attention, or Int4KVCache.append and attend
+              (or PagedKVCache.append, which turns them on the way, and attend)
+          --> with head_norm: layer_norm of each head's output, without the mean
           --> (B, N, H*dv) --output projection--> (B, N, E)
 
     The projected tensors are strided views of one projection output and every operator keeps the
@@ -133,11 +137,14 @@ class DifferentialAttention(nn.Module):
         rotary_base: pair p of P turns by rotary_base^(-p / P) a position.
         lambda_init: initial weight of the second branch, learned per head.
         bias: biases on the projections.
+        head_norm: normalise each head's output by its root mean square (with norm_eps) and weigh its values, alike in
+            every head; the weights are learned and start at 1 - lambda_init, the scale of a difference of maps.
     """
 
     def __init__(self, embed_dim: int, num_heads: int, head_dim: int | None = None, *, kv_heads: int | None = None,
                  v_head_dim: int | None = None, rotary_sections=None, rotary_base: float = 10000.0,
-                 lambda_init: float = 0.5, bias: bool = False, device=None, dtype=None):
+                 lambda_init: float = 0.5, bias: bool = False, head_norm: bool = False, norm_eps: float = 1e-5, device=None,
+                 dtype=None):
         super().__init__()
         head_dim = head_dim if head_dim is not None else embed_dim // num_heads
         v_head_dim = v_head_dim if v_head_dim is not None else head_dim
@@ -159,6 +166,8 @@ class DifferentialAttention(nn.Module):
         self.in_proj = nn.Linear(embed_dim, sum(h * w for h, w in zip(self._heads, self._widths)), bias=bias, **fk)
         self.out_proj = nn.Linear(num_heads * v_head_dim, embed_dim, bias=bias, **fk)
         self.lambda_param = nn.Parameter(torch.full((num_heads,), float(lambda_init), dtype=torch.float32, device=device))
+        self.norm_eps = float(norm_eps)
+        self.register_parameter("norm_weight", nn.Parameter(torch.full((v_head_dim,), 1.0 - float(lambda_init), **fk)) if head_norm else None)
         # on the CPU whatever the default device is: the frequencies have no copy in a checkpoint to come from
         self._inv_freq = (float(rotary_base) ** (-torch.arange(pairs, dtype=torch.float64, device="cpu") / pairs)).float()
         self._place()
@@ -185,6 +194,11 @@ class DifferentialAttention(nn.Module):
         return Int4KVCache(batch, self.kv_heads, capacity, self.head_dim, self.v_head_dim,
                            device=self.in_proj.weight.device)
 
+    def new_paged_cache(self, pages: int, page_size: int = 64) -> PagedKVCache:
+        """Pages for this layer's keys and values, of its weights' type and on their device."""
+        w = self.in_proj.weight
+        return PagedKVCache(pages, self.kv_heads, page_size, self.head_dim, self.v_head_dim, dtype=w.dtype, device=w.device)
+
     def project(self, x: torch.Tensor):
         """The (B, H or Hk, N, d or dv) views of the projected q1, q2, k1, k2, v.  They come from one split,
         whose backward joins the parts' gradients in one pass; autograd forbids editing them in place."""
@@ -193,7 +207,9 @@ class DifferentialAttention(nn.Module):
         return [p.view(b, n, h, w).transpose(1, 2) for p, h, w in zip(parts, self._heads, self._widths)]
 
     def forward(self, x: torch.Tensor, positions: torch.Tensor | None = None, kv_lens: torch.Tensor | None = None,
-                cache: Int4KVCache | None = None) -> torch.Tensor:
+                cache: Int4KVCache | PagedKVCache | None = None, *, table: torch.Tensor | None = None,
+                lengths: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                counts: torch.Tensor | None = None) -> torch.Tensor:
         """x: (batch, seq_len, embed_dim), causal over seq_len; positions: int32 or int64, (axes, batch,
         seq_len), by default the same count on every axis.  kv_lens (batch,) hides the rows of a padded
         batch from then on.
@@ -202,31 +218,49 @@ class DifferentialAttention(nn.Module):
         and the attention runs over all that the cache holds, without gradients; positions count from
         the cache's lengths by default.  Rows past the cache's capacity are dropped, as append() drops them: a
         caller keeps count.  A prompt padded at its end is decoded on from after cache.lengths
-        is set to the sequences' own lengths."""
+        is set to the sequences' own lengths.
+
+        A PagedKVCache needs table and lengths, and takes x in any of its three forms (with counts a padded batch, with
+        starts a packed one, (1, rows, embed_dim)): see there.  lengths are what the sequences held before, and are
+        the caller's to add to once every layer has run.  Rows of no sequence give the output projection's bias."""
         if x.dim() != 3 or x.shape[-1] != self.embed_dim:
             raise ValueError(f"x must have shape (batch, seq_len, {self.embed_dim}), got {tuple(x.shape)}")
+        paged = isinstance(cache, PagedKVCache)
+        if paged and (table is None or lengths is None):
+            raise ValueError("a paged cache needs table and lengths")
+        if not paged and any(t is not None for t in (table, lengths, starts, counts)):
+            raise ValueError("table, lengths, starts and counts go with a paged cache")
+        where = {"table": table, "lengths": lengths, "starts": starts, "counts": counts}
         if cache is not None:
             if kv_lens is not None:
                 raise ValueError("kv_lens and cache exclude each other: a cache has its own lengths")
-            if x.shape[0] != cache.batch:
+            if not paged and x.shape[0] != cache.batch:
                 raise ValueError(f"the cache holds {cache.batch} sequences, x has {x.shape[0]}")
             if torch.is_grad_enabled():
                 with torch.no_grad():
-                    return self.forward(x, positions, None, cache)
+                    return self.forward(x, positions, None, cache, **where)
         b, n, _ = x.shape
         q1, q2, k1, k2, v = self.project(x)
+        if paged:
+            q1, q2 = cache.append(k1, k2, v, q1=q1, q2=q2, **where, inv_freq=self._frequencies(), sections=self.rotary_sections,
+                                  positions=positions)
+            return self._output(cache.attend(q1, q2, self.lambda_param, **where))
         if positions is None:
             positions = torch.arange(n, device=x.device).expand(len(self.rotary_sections), b, n)
             if cache is not None:
                 positions = positions + cache.lengths[:, None]
         q1, q2, k1, k2 = rotary_axes((q1, q2, k1, k2), positions, self._frequencies(), self.rotary_sections)
         if cache is None:
-            o = differential_attention(q1, q2, k1, k2, v, self.lambda_param, kv_lens=kv_lens)
-        else:
-            cache.append(k1, k2, v)
-            o = cache.attend(q1, q2, self.lambda_param)
-        return self.out_proj(o.transpose(1, 2).reshape(b, n, self.num_heads * self.v_head_dim))
+            return self._output(differential_attention(q1, q2, k1, k2, v, self.lambda_param, kv_lens=kv_lens))
+        cache.append(k1, k2, v)
+        return self._output(cache.attend(q1, q2, self.lambda_param))
+
+    def _output(self, o: torch.Tensor) -> torch.Tensor:
+        if self.norm_weight is not None:
+            o = layer_norm(o, self.norm_weight, eps=self.norm_eps, center=False)
+        return self.out_proj(o.transpose(1, 2).flatten(2))
 
     def extra_repr(self) -> str:
         return (f"embed_dim={self.embed_dim}, num_heads={self.num_heads}, kv_heads={self.kv_heads}, "
-                f"head_dim={self.head_dim}, v_head_dim={self.v_head_dim}, rotary_sections={self.rotary_sections}")
+                f"head_dim={self.head_dim}, v_head_dim={self.v_head_dim}, rotary_sections={self.rotary_sections}"
+                + ("" if self.norm_weight is None else f", head_norm=True, norm_eps={self.norm_eps}"))
