@@ -30,7 +30,8 @@ HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra"]
 
 HIP_SOURCES = ["tda_fwd.hip", "tda_fwd_sparse.hip", "tda_fwd_decode.hip", "tda_bwd.hip", "tda_bwd_fast.hip",
                "tda_wide.hip", "tda_noalloc.hip", "sda_fwd.hip", "sda_bwd.hip", "sda_decode.hip", "sda_kv4.hip",
-               "sda_rotary.hip", "spa_append.hip", "spa_few.hip", "spa_many.hip", "sln.hip"]
+               "sda_rotary.hip", "spa_append.hip", "spa_attend_f32.hip", "spa_attend_bf16.hip",
+               "spa_attend_f16.hip", "sln.hip"]
 HOST_SOURCES = ["tda_host.cpp", "sda_host.cpp", "spa_host.cpp", "sln_host.cpp"]
 # host-only code that calls the HIP runtime API (no device code): g++ against the ROCm headers
 HIP_HOST_SOURCES = ["tda_timing.cpp"]

@@ -141,8 +141,8 @@ struct Tile {
     else return r & 15;
   }
   // Byte offset (from the tile's first row in memory) that this lane loads in instruction u.
-  __device__ __forceinline__ static uint32_t source(int u, uint32_t stride) {
-    const int ci = 64 * u + lane_id(), r = ci / CPR, c = ci % CPR;
+  __device__ __forceinline__ static uint32_t source(int u, uint32_t stride, int lane = lane_id()) {
+    const int ci = 64 * u + lane, r = ci / CPR, c = ci % CPR;
     return (uint32_t)r * stride + 16u * (uint32_t)(c ^ swz(r));
   }
   __device__ __forceinline__ static void load(__amdgpu_buffer_rsrc_t r, T* lds, int u, uint32_t off) {
@@ -182,8 +182,8 @@ template <class Tr, int W>
 struct RowReader {
   static constexpr int NT = W / 16;
   uint32_t a[NT];
-  __device__ __forceinline__ void init(const void* lds) {
-    const int r = lane_id() & 31, g = lane_id() >> 5;
+  __device__ __forceinline__ void init(const void* lds, int lane = lane_id()) {
+    const int r = lane & 31, g = lane >> 5;
     const uint32_t base = lds_address(lds);
     if constexpr (sizeof(typename Tr::T) == 2) {
 #pragma unroll
@@ -209,8 +209,8 @@ template <class Tr, int W, bool APART = false>
 struct ColReader {
   static constexpr int NY = W / 32;
   uint32_t a[2][NY];
-  __device__ __forceinline__ void init(const void* lds) {
-    const int l = lane_id(), bk = l >> 4, j = l & 15;
+  __device__ __forceinline__ void init(const void* lds, int l = lane_id()) {
+    const int bk = l >> 4, j = l & 15;
     const uint32_t base = lds_address(lds);
     if constexpr (sizeof(typename Tr::T) == 2) {
 #pragma unroll

@@ -287,14 +287,14 @@ struct Kv4Src {
     }
   }
 
-  __device__ __forceinline__ void begin(const DecParams& P, const DecWork& W, int h, int i, bool live) {
+  __device__ __forceinline__ void begin(const DecParams& P, int b, int hk, int h, int i, bool live) {
     const int kq = lane_id() >> 4;
-    const int64_t row0 = ((int64_t)W.b * P.Hk + W.hk) * C->cap4;
+    const int64_t row0 = ((int64_t)b * P.Hk + hk) * C->cap4;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       kc[x] = reinterpret_cast<const uint32_t*>(C->codes[x]) + row0 * (D / 8);
       kpar[x] = C->pars[x] + row0 * GK;
-      const T* r = row_of<const T>(P.q[x], W.qb, h, W.row0 + i);
+      const T* r = row_of<const T>(P.q[x], b, h, i);
 #pragma unroll
       for (int y = 0; y < GK; ++y) {
         float a = 0.f;
@@ -462,8 +462,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((DV <=
   extern __shared__ float lds[];
   Kv4Src<T, NP, D, DV> src;
   src.C = &C;
-  DecWork W;
-  if (dec_work(P, W)) decode_body(P, W, src, lds);
+  decode_body(P, src, lds);
 }
 
 // ------------------------------------------------------------------ launches

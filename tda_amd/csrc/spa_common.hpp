@@ -20,6 +20,20 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   return (uint32_t)uniform((int)(uint32_t)x) | ((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
 }
 
+// The lane's number as something new: what a loop's passes make of it is not kept in registers from one to the next.
+__device__ __forceinline__ int fresh_lane() {
+  int l = lane_id();
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+// Zero, likewise.
+__device__ __forceinline__ float fresh_zero() {
+  float z = 0.f;
+  asm volatile("" : "+v"(z));
+  return z;
+}
+
 struct Seq {
   int qb, row0, cnt;  // its rows: row0 .. row0 + cnt - 1 of batch entry qb
   int held, len;      // the position of its first row; the positions that it has with its new rows
@@ -49,11 +63,11 @@ struct Pages {
   int now, next;
   __device__ __forceinline__ int fetch(int at) const {
     const int e = at + lane_id();
-    const int p = e < tlen ? row[e] : -1;
-    return p < pages ? p : -1;
+    const int p = row[min(e, tlen - 1)];  // no branch: see many_rows' queries
+    return e < tlen && p < pages ? p : -1;
   }
   __device__ __forceinline__ void begin(const Seqs& Q, int s, int slot) {
-    row = Q.table + (int64_t)s * Q.tstride;
+    row = Q.table + (int64_t)uniform(s) * Q.tstride;
     tlen = Q.tlen;
     pages = Q.pages;
     base = slot;
@@ -97,6 +111,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, ui
 }
 
 // ------------------------------------------------------------------ work
+constexpr int kUnit = 128;  // keys
+// Tiles of 16 rows are cut until there are this many for each workgroup: their parts' sums are small.
+constexpr int kFewCut = 8;
+
 // Running sums over the wave's lanes (lane moves: four within rows of 16 lanes, two from row to row), and their totals.
 // Call with every lane active.
 template <int CTRL, int ROWS>
@@ -118,101 +136,125 @@ __device__ __forceinline__ uint64_t wave_total(uint64_t x) {  // of values below
   return low + ((uint64_t)mid << 26) + ((uint64_t)wave_total((uint32_t)(x >> 52)) << 52);
 }
 
-constexpr int kUnit = 128;  // keys; pieces are whole units
-
-// A tile of RT rows of sequence s (the rows of all heads that share a key head, token by token), and which of
-// the `parts` pieces of its keys; `first` is the number of its first piece (of one key head).
+// A part of a tile of rows of one sequence (the rows of all heads that share a key head, token by token): units from ..
+// from + count - 1 of the tile's `units`.
 struct Job {
-  int s, tile, part, parts, units;  // units of keys in a piece
-  uint32_t first;
+  int s, tile;
+  uint32_t at, from, count, units;  // at: the tile's place on its form's line
   Seq seq;
 };
-// The tiles of a form (FEW: sequences of at most `bound` rows), in the order of the sequences, a sequence's last
-// tile first: it has the most keys.  With `room` each tile is cut into pieces of the fewest units that leave no more
-// than `room` of them: from W / room on, W the sum over N tiles of their units, up to W / (room - N), which always do.
-// BY_PIECE: idx counts pieces; else tiles (for the launch that joins them).  False: there is no such one.
-template <int RT, bool FEW, bool BY_PIECE>
-__device__ __forceinline__ bool find_job(const Seqs& Q, int G, int bound, int room, uint32_t idx, Job& J) {
-  const int l = lane_id();
-  uint32_t t = 0, u = 0;
-  Seq q{};
-  const auto sizes = [&](int s0) {
+
+// How the work of a key head is dealt out.  Sequences of at most `bound` rows have tiles of 16 (form 0), the others of
+// 128 (form 1).  The tiles of a form stand on a line, in the order of the sequences, a sequence's last tile first (it has the
+// most keys), each as long as its keys in units of 128.  Workgroups take equal stretches of the line: a stretch may
+// end in one tile and begin in another, and what it has of either goes to a place of its own, to be joined.  Two forms
+// share the workgroups by their units' costs, `cost` to 1.
+// Where the tiles are enough to fill the chip each is one unit, and one workgroup's.
+// Everything is whole numbers, so that every workgroup of both launches finds the same.
+struct Deal {
+  const Seqs& Q;
+  int G, bound, l;
+  bool cut;
+  uint32_t groups[2], per[2], line[2];  // workgroups of a form, units of each, units in all
+  uint32_t t, u;                        // this lane's sequence: tiles, units of each
+  int form;
+  Seq q;
+
+  __device__ __forceinline__ void sizes(int s0) {
     t = u = 0;
+    form = 0;
     if (s0 + l < Q.S) {
       q = seq_of(Q, s0 + l);
       const int R = q.cnt * G;
-      if ((R <= bound) == FEW) t = (uint32_t)(R + RT - 1) / RT;
-      u = (uint32_t)(q.len + kUnit - 1) / kUnit;
+      form = R > bound;
+      t = (uint32_t)(R + (form ? kManyRows : kFewRows) - 1) / (form ? kManyRows : kFewRows);
+      u = max((uint32_t)(q.len + kUnit - 1) / kUnit, 1u);
     }
-  };
-  uint32_t units = 0x7fffffffu;
-  if (room) {
-    uint32_t N = 0;
-    uint64_t W = 0;
+  }
+  __device__ __forceinline__ Deal(const Seqs& Q_, int G_, int bound_, int room, int cost) : Q(Q_), G(G_), bound(bound_), l(lane_id()) {
+    q = Seq{};
+    uint32_t n0 = 0, n1 = 0;
+    uint64_t w0 = 0, w1 = 0;
     for (int s0 = 0; s0 < Q.S; s0 += 64) {
       sizes(s0);
-      N += t;
-      W += (uint64_t)t * u;
+      const uint64_t w = (uint64_t)t * u;
+      n0 += form ? 0 : t;
+      n1 += form ? t : 0;
+      w0 += form ? 0 : w;
+      w1 += form ? w : 0;
     }
-    N = wave_total(N);
-    W = wave_total(W);
-    if ((uint32_t)room > N) {
-      const auto share = [&](uint32_t by) {  // W / by rounded up, of W in 31 bits
-        const uint32_t over = (uint32_t)(W >> 31);
-        const int shift = (W >> 63) ? 33 : over ? 32 - __builtin_clz(over) : 0;
-        const uint32_t w = ((uint32_t)(W >> shift) + (shift ? 1u : 0u) + by - 1) / by;
-        return (uint32_t)min(max((uint64_t)w << shift, (uint64_t)1), (uint64_t)0x7fffffff);
-      };
-      const uint32_t most = share((uint32_t)room - N);  // at most `room` pieces for sure
-      units = share((uint32_t)room);                    // the least there could be
-      while (units < most) {
-        uint32_t n = 0;
-        for (int s0 = 0; s0 < Q.S; s0 += 64) {
-          if (Q.S > 64) sizes(s0);
-          n += t * max((u + units - 1) / units, 1u);
+    groups[0] = line[0] = wave_total(n0);
+    groups[1] = line[1] = wave_total(n1);
+    per[0] = per[1] = 1;
+    cut = false;
+    if (room && line[0] + line[1] < (uint32_t)(line[1] ? room : kFewCut * room)) {
+      const uint64_t w[2] = {wave_total(w0), wave_total(w1)};
+      cut = w[0] + w[1] < 0x40000000u;  // fewer tiles than that are longer than a cache can be
+      if (cut) {
+        uint32_t to[2] = {(uint32_t)room, (uint32_t)room};
+        if (w[0] && w[1]) {
+          const uint64_t a = w[0], b = w[1] * (uint64_t)cost;
+          const int shift = max(44 - (int)__builtin_clzll(a + b + 1), 0);  // the sum in 20 bits
+          const uint32_t x = (uint32_t)(a >> shift), y = (uint32_t)(b >> shift);
+          to[1] = min(max(((uint32_t)room * y + (x + y) / 2) / max(x + y, 1u), 1u), (uint32_t)room - 1);
+          to[0] = (uint32_t)room - to[1];
         }
-        if (wave_total(n) <= (uint32_t)room) break;
-        units = min(units + max(units / 8, 1u), most);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          line[f] = (uint32_t)w[f];
+          per[f] = max((line[f] + to[f] - 1) / to[f], 1u);
+          groups[f] = (line[f] + per[f] - 1) / per[f];
+        }
       }
     }
   }
-  uint32_t tiles = 0, pieces = 0;  // of the sequences before
-  for (int s0 = 0; s0 < Q.S; s0 += 64) {
-    if (!room || Q.S > 64) sizes(s0);
-    const uint32_t p = t * max((u + units - 1) / units, 1u);
-    const uint32_t tu = running(t), pu = running(p), mine = BY_PIECE ? pu : tu, before = BY_PIECE ? pieces : tiles;
-    const uint32_t sum = __builtin_amdgcn_readlane(mine, 63);
-    if (idx - before < sum) {
-      const int x = __builtin_ctzll(__ballot(mine > idx - before));
-      const uint32_t nt = __builtin_amdgcn_readlane(t, x), np = __builtin_amdgcn_readlane(p, x);
-      const uint32_t first = pieces + __builtin_amdgcn_readlane(pu, x) - np;
-      const uint32_t e = idx - before - (__builtin_amdgcn_readlane(mine, x) - (BY_PIECE ? np : nt));
-      J.s = s0 + x;
-      J.parts = (int)(np / nt);
-      const uint32_t at = BY_PIECE ? e / (uint32_t)J.parts : e;
-      J.part = BY_PIECE ? (int)(e % (uint32_t)J.parts) : 0;
-      J.tile = (int)(nt - 1 - at);
-      J.units = (int)units;
-      J.first = first + at * (uint32_t)J.parts;
-      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x); };
-      J.seq = {of(q.qb), of(q.row0), of(q.cnt), of(q.held), of(q.len)};
-      return true;
-    }
-    tiles += __builtin_amdgcn_readlane(tu, 63);
-    pieces += __builtin_amdgcn_readlane(pu, 63);
+  // What stands at unit `at` of a form's line, or with TILE the tile number `at`; up to `end` or the tile's end.  False:
+  // nothing.
+  template <int FORM, bool TILE>
+  __device__ __forceinline__ bool find(uint32_t at, uint32_t end, Job& J) const {
+    Deal d = *this;
+    return d.look<FORM, TILE>(at, end, J);
   }
-  return false;
-}
-// A piece's keys within the `lim` that its tile sees.
-__device__ __forceinline__ void keys_of(const Job& J, int lim, int& k0, int& k1) {
-  const int64_t per = (int64_t)J.units * kUnit;
-  k0 = uniform((int)min((int64_t)J.part * per, (int64_t)lim));
-  k1 = uniform((int)min((int64_t)k0 + per, (int64_t)lim));
-}
+  template <int FORM, bool TILE>
+  __device__ __forceinline__ bool look(uint32_t at, uint32_t end, Job& J) {
+    uint32_t tiles = 0, units = 0;  // of the sequences before
+    for (int s0 = 0; s0 < Q.S; s0 += 64) {
+      if (Q.S > 64) sizes(s0);
+      const uint32_t each = cut ? u : 1u, n = form == FORM ? t : 0, w = n * each;
+      const uint32_t nu = running(n), wu = running(w);
+      const auto lane = [&](uint32_t v, int x) { return (uint32_t)__builtin_amdgcn_readlane((int)v, x); };
+      const uint32_t sum = lane(TILE ? nu : wu, 63), rest = at - (TILE ? tiles : units);
+      if (rest < sum) {
+        const int x = __builtin_ctzll(__ballot((TILE ? nu : wu) > rest));
+        const uint32_t e = rest - (lane(TILE ? nu : wu, x) - lane(TILE ? n : w, x));  // within the sequence
+        J.units = lane(each, x);
+        const uint32_t tile = TILE ? e : e / J.units;
+        J.s = s0 + x;
+        J.tile = (int)(lane(n, x) - 1 - tile);
+        J.at = units + lane(wu, x) - lane(w, x) + tile * J.units;
+        J.from = TILE ? 0 : at - J.at;
+        J.count = TILE ? J.units : min(J.units - J.from, end - at);
+        const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x); };
+        J.seq = {of(q.qb), of(q.row0), of(q.cnt), of(q.held), of(q.len)};
+        return true;
+      }
+      tiles += lane(nu, 63);
+      units += lane(wu, 63);
+    }
+    return false;
+  }
+  // A part's keys within the `lim` that its tile sees.
+  __device__ __forceinline__ static void keys(const Job& J, int lim, int& k0, int& k1) {
+    const bool whole = J.count == J.units;
+    k0 = uniform(whole ? 0 : min((int)(J.from * kUnit), lim));
+    k1 = uniform(whole ? lim : min((int)((J.from + J.count) * kUnit), lim));
+  }
+};
 
-// Zeros the rows of no sequence: workgroup `bid` of `blocks`.
+// Zeros the rows of no sequence, each workgroup some.
 template <class T, int DV, int THREADS>
-__device__ __forceinline__ void clear_free_rows(const AttendParams& P, uint32_t bid, uint32_t blocks) {
+__device__ __forceinline__ void clear_free_rows(const AttendParams& P, uint32_t bid) {
+  const uint32_t blocks = P.grid;
   constexpr int V = 16 / sizeof(T), PER = DV / V;
   if (!P.seq.starts && !P.seq.counts) return;
   const int64_t all = (int64_t)P.lead * P.seq.rows;

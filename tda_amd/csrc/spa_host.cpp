@@ -99,17 +99,17 @@ int32_t check_attend_sizes(const spa_attend_args& a) {
              : TDA_ERR_SHAPE;
 }
 
-// Workgroups that a call is cut into where its tiles are fewer, by splitting the keys.
-constexpr int64_t kFewTarget = 256, kManyTarget = 256;
+// Workgroups that share a call's tiles where these are fewer: one a CU.
+constexpr int64_t kTarget = 256;
 
 void deal(const spa_attend_args& a, spa::AttendParams& p) {
-  const int64_t G = a.heads / a.cache.kv_heads, S = a.at.sequences, hk = a.cache.kv_heads, rows = a.at.rows;
+  const int64_t G = a.heads / a.cache.kv_heads, S = a.at.sequences, hk = a.cache.kv_heads, rows = a.at.rows, dv = a.cache.v_head_dim;
   const bool exact = !a.at.starts && !a.at.counts;  // every sequence has `rows` rows
   const int64_t most = !exact && a.most && a.most < rows ? a.most : rows;
   const int64_t total = (a.at.starts ? 1 : S) * rows * G;  // rows of all sequences, of the heads of a key head
   int64_t few = 0, many = 0;                         // tiles at most
   if (most * G <= spa::kFewRows) {
-    p.bound = 0x7fffffff;  // the first form takes every sequence, however many rows it has after all
+    p.bound = 0x7fffffff;  // every sequence has small tiles, however many rows it has after all
     few = a.at.starts ? total / spa::kFewRows + (S < total ? S : total) : S * ceil_div(rows * G, spa::kFewRows);
   } else if (exact) {
     p.bound = 0;
@@ -120,22 +120,18 @@ void deal(const spa_attend_args& a, spa::AttendParams& p) {
     const int64_t big = total / (spa::kFewRows + 1);  // sequences with more rows than that
     many = total / spa::kManyRows + (S < big ? S : big);
   }
-  const auto form = [&](spa::Form& f, int64_t tiles, int64_t target, int per) {
-    const int64_t n = tiles * hk;
-    const bool cut = n > 0 && 4 * n <= 3 * target;
-    f.grid = (uint32_t)(cut ? target : n);
-    f.room = cut ? (int)(target / hk) : 0;
-    f.join = cut ? (uint32_t)(n * per) : 0;
-  };
-  form(p.few, few, kFewTarget, 1);
-  form(p.many, many, kManyTarget, spa::kManyRows / 32);
+  // whether there are few enough tiles to be cut: known of an exact call, else taken to be so when whole tiles of all rows
+  // would be
+  const int64_t tiles = many ? (exact ? many : total / spa::kManyRows) : ceil_div(total / spa::kFewRows, 8);
+  const bool cut = 4 * tiles * hk <= 3 * kTarget && hk <= kTarget;
+  p.room = cut ? (int)(kTarget / hk) : 0;
+  const int64_t most_tiles = few + many;
+  p.grid = (uint32_t)(hk * (most_tiles > p.room ? most_tiles : p.room));
+  p.join[0] = cut ? (uint32_t)(few * hk) : 0;
+  p.join[1] = cut ? (uint32_t)(many * hk * (spa::kManyRows / 32)) : 0;
+  p.stride = many ? spa::many_floats(dv) : spa::few_floats(dv);
 }
-int64_t few_bytes(const spa::AttendParams& p, int64_t dv) {
-  return p.few.room ? (int64_t)p.few.grid * spa::few_floats((int)dv) * 4 : 0;
-}
-int64_t many_bytes(const spa::AttendParams& p, int64_t dv) {
-  return p.many.room ? (int64_t)p.many.grid * spa::many_floats((int)dv) * 4 : 0;
-}
+int64_t part_bytes(const spa::AttendParams& p, int64_t hk) { return 2 * p.room * hk * p.stride * 4; }
 
 }  // namespace
 
@@ -229,7 +225,7 @@ size_t spa_attend_workspace_bytes(const spa_attend_args* a) {
   spa::AttendParams p;
   std::memset(&p, 0, sizeof(p));
   deal(*a, p);
-  return (size_t)(few_bytes(p, a->cache.v_head_dim) + many_bytes(p, a->cache.v_head_dim));
+  return (size_t)part_bytes(p, a->cache.kv_heads);
 }
 
 int32_t spa_validate_attend(const spa_attend_args* a) {
@@ -268,9 +264,7 @@ int32_t spa_attend(const spa_attend_args* a, void* stream) {
   p.Hk = (int)a->cache.kv_heads;
   p.lead = (int)lead_of(a->at);
   p.c = (float)(a->scale * kLog2e);
-  const int64_t first = few_bytes(p, a->cache.v_head_dim);
-  if (p.few.room) p.few.part = static_cast<float*>(a->workspace);
-  if (p.many.room) p.many.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + first);
+  if (p.room) p.part = static_cast<float*>(a->workspace);
   tda::timing_begin(stream);
   return done(spa::launch_attend(p, a->dtype, (int)a->cache.head_dim, (int)a->cache.v_head_dim, stream));
 }

@@ -29,14 +29,9 @@ struct AppendParams {
   const float* inv_freq;
 };
 
-// One of the two forms of the attention: `few` takes the sequences of at most `bound` rows (a row: a query
-// row of one of the heads that share a key head), `many` the others.
-struct Form {
-  uint32_t grid;         // workgroups; 0: not launched
-  uint32_t join;         // workgroups of its joining launch; 0: none
-  int room;              // pieces a key head may be cut into; 0: whole tiles only
-  float* part;           // grid pieces' sums, when room is not 0
-};
+// The attention takes sequences of at most `bound` rows (a row: a query row of one of the heads that share a key head)
+// in tiles of 16 rows, the others in tiles of 128.
+constexpr int kFewRows = 16, kManyRows = 128;
 struct AttendParams {
   Seqs seq;
   const void* k[2];
@@ -45,17 +40,23 @@ struct AttendParams {
   Lambda lam;
   int H, Hk, lead, bound;
   float c;               // scale * log2(e)
-  Form few, many;
+  int room;              // workgroups that may share a key head's tiles; 0: whole tiles only
+  uint32_t grid;         // workgroups of all key heads, at most
+  uint32_t join[2];      // workgroups of the joining launch: a small tile each, 32 rows of a large one each
+  float* part;           // two places for each of room workgroups of every key head, `stride` floats each
+  int64_t stride;
 };
 
-constexpr int kFewRows = 16, kManyRows = 128;  // rows of a tile of each form
-constexpr int64_t few_floats(int dv) { return 64 + 2 * kFewRows * (int64_t)dv; }     // a piece's sums
-constexpr int64_t many_floats(int dv) { return 4 * kManyRows + 2 * kManyRows * (int64_t)dv; }
+// The sums of a part of a tile.  Few rows: [branch][m, l][16], then [branch][row][dv].  Many: [branch][m, l][128], then
+// [branch][32 rows][4 of a lane's values][lane][4].
+constexpr int64_t few_floats(int64_t dv) { return 64 + 2 * kFewRows * dv; }
+constexpr int64_t many_floats(int64_t dv) { return 4 * kManyRows + 2 * kManyRows * dv; }
 
 int launch_append(const AppendParams& p, int dtype, void* stream);
 int launch_attend(const AttendParams& p, int dtype, int d, int dv, void* stream);
-// the two forms, one to a file so that they compile side by side
-int launch_few(const AttendParams& p, int dtype, int d, int dv, void* stream);
-int launch_many(const AttendParams& p, int dtype, int d, int dv, void* stream);
+// one type to a file, so that they compile side by side
+int launch_attend_f32(const AttendParams& p, int d, int dv, void* stream);
+int launch_attend_bf16(const AttendParams& p, int d, int dv, void* stream);
+int launch_attend_f16(const AttendParams& p, int d, int dv, void* stream);
 
 }  // namespace spa

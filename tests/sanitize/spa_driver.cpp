@@ -144,27 +144,28 @@ static void paged() {
   CHECK(spa_append(&ap, nullptr) == TDA_ERR_HIP && tda_last_hip_error() == 77);
   extremes(append_args(), {&spa_append_args::heads, &spa_append_args::rot}, [](const spa_append_args& a) { spa_append(&a, nullptr); });
 
-  // few rows of every sequence: one form; cut where the tiles are few
+  // few rows of every sequence: small tiles; cut where they are few
+  const int64_t few = spa::few_floats(128) * 4, many = spa::many_floats(128) * 4;
   spa_attend_args at = attend_args(3, 1);
   CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attends == 1);
-  CHECK(got::attend.bound == 0x7fffffff && got::attend.many.grid == 0 && got::attend.few.join == 6);
-  CHECK(got::attend.few.room > 3 && got::attend.few.grid >= (uint32_t)got::attend.few.room * 2);
-  CHECK(at.workspace_bytes == (size_t)got::attend.few.grid * spa::few_floats(128) * 4 && got::attend.few.part);
-  at = attend_args(400, 1);  // whole tiles
-  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.few.grid == 800 && !got::attend.few.room && !got::attend.few.join && !at.workspace_bytes);
+  CHECK(got::attend.bound == 0x7fffffff && got::attend.join[0] == 6 && got::attend.join[1] == 0);
+  CHECK(got::attend.room > 3 && got::attend.grid == (uint32_t)got::attend.room * 2 && got::attend.part);
+  CHECK((int64_t)at.workspace_bytes == got::attend.room * 4 * few);
+  at = attend_args(20000, 1);  // whole tiles
+  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.grid == 40000 && !got::attend.room && !got::attend.join[0] && !at.workspace_bytes);
   at = attend_args(2, 1000);  // 4000 rows of a key head are 32 tiles
-  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.bound == 0 && !got::attend.few.grid && got::attend.many.join == 2 * 32 * 2 * 4);
+  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.bound == 0 && !got::attend.join[0] && got::attend.join[1] == 2 * 32 * 2 * 4);
   at = attend_args(8, 1000);
-  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.many.grid == 8 * 32 * 2 && !got::attend.many.room && !at.workspace_bytes);
+  CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.grid == 8 * 32 * 2 && !got::attend.room && !at.workspace_bytes);
   at = attend_args(8, 1000);  // packed: either form
   at.at.starts = INTS;
   at.workspace_bytes = spa_attend_workspace_bytes(&at);
   CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.lead == 1 && got::attend.bound == spa::kFewRows);
-  CHECK(got::attend.few.join == 8 * 2 && got::attend.many.join == (4000 / 128 + 8) * 2 * 4);
-  CHECK(reinterpret_cast<char*>(got::attend.many.part) == AT + (size_t)got::attend.few.grid * spa::few_floats(128) * 4);
-  at.most = 4;  // one form, which has room for any rows
+  CHECK(got::attend.join[0] == 8 * 2 && got::attend.join[1] == (4000 / 128 + 8) * 2 * 4);
+  CHECK((int64_t)at.workspace_bytes == got::attend.room * 4 * many);
+  at.most = 4;  // small tiles alone, which have room for any rows
   at.workspace_bytes = spa_attend_workspace_bytes(&at);
-  CHECK(spa_attend(&at, nullptr) == TDA_OK && !got::attend.many.grid && got::attend.few.grid >= (4000 / 16 + 8) * 2);
+  CHECK(spa_attend(&at, nullptr) == TDA_OK && !got::attend.join[1] && got::attend.grid >= (4000 / 16 + 8) * 2);
   extremes(attend_args(3, 5), {&spa_attend_args::heads, &spa_attend_args::most}, [](spa_attend_args a) {
     a.workspace_bytes = spa_attend_workspace_bytes(&a);
     spa_attend(&a, nullptr);
@@ -180,7 +181,7 @@ static void paged() {
         a.workspace_bytes = spa_attend_workspace_bytes(&a);
         if (spa_attend(&a, nullptr) != TDA_OK) continue;
         const double need = packed ? (double)n * 4 / 16 : (double)s * ((n * 4 + 127) / 128);
-        CHECK((double)got::attend.few.grid + got::attend.many.grid >= (got::attend.many.grid ? need / 8 : need));
+        CHECK((double)got::attend.grid >= need / 8);
       }
 }
 

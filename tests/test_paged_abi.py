@@ -156,16 +156,16 @@ def test_starts_and_counts_exclude_each_other_and_null_is_refused():
 
 
 def test_attend_workspaces():
-    """None where the tiles fill the chip; a piece's sums for each workgroup where they do not, of either form of rows."""
+    """None where the tiles fill the chip; two places for sums for each workgroup where they do not, of either form of rows."""
     few, many = (64 + 2 * 16 * 128) * 4, (4 * 128 + 2 * 128 * 128) * 4
-    assert attend(s=3, n=5).workspace_bytes == 256 * few
-    assert attend(s=3, n=100).workspace_bytes == 256 * many
-    assert attend(s=300, n=5).workspace_bytes == attend(s=300, n=100).workspace_bytes == 0
+    assert attend(s=3, n=5).workspace_bytes == 512 * few
+    assert attend(s=3, n=100).workspace_bytes == 512 * many
+    assert attend(s=30000, n=5).workspace_bytes == attend(s=300, n=100).workspace_bytes == 0
     a = attend(s=3, n=100)
     a.at.counts = FAKE
-    assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == 256 * (few + many)
+    assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == 512 * many
     a.most = 8
-    assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == 256 * few
+    assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == 512 * few
     a.heads = 3
     assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == lib().spa_attend_workspace_bytes(None) == 0
 

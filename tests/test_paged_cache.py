@@ -143,9 +143,17 @@ def test_many_sequences(dtype):
 @gpu
 def test_long_sequences_are_cut_and_joined():
     for new, held, form in (([1], [9000], "even"), ([1, 1], [9000, 10], "even"), ([40], [7000], "even"), ([1, 60], [300, 6000], "packed"),
-                            ([20, 60], [3000, 20], "packed")):
+                            ([20, 60], [3000, 20], "packed"), ([3], [5000], "even"), ([4, 2, 0], [4000, 100, 9], "counts")):
         for dtype, (d, dv) in ((BF, (128, 128)), (F32, (64, 128)), (F16, (128, 256))):
             Setup(new, held, 4, 2, d, dv, 64, dtype, form).spoil().attend()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, d, dv", [(BF, 64, 128), (F16, 128, 128), (F32, 128, 256)])
+def test_tiles_with_every_row_are_cut(dtype, d, dv):
+    """Tiles of 16 and of 128 rows without a spare one, whose parts end before any row's sight does."""
+    for new, held, h, hk in (([8], [5000], 4, 2), ([1, 1], [4321, 77], 32, 2), ([4, 8], [2500, 900], 8, 2), ([32], [6011], 8, 2), ([16, 4], [3500, 4097], 8, 1)):
+        Setup(new, held, h, hk, d, dv, 64, dtype, "packed").spoil().attend()
 
 
 @gpu
