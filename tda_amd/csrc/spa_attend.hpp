@@ -533,17 +533,19 @@ struct FewRows {
   }
 };
 
-// What a launch has: tiles of 16 rows alone, or of both kinds.
-template <class Tr, int D, int DV, bool BOTH>
+// What a launch may have: tiles of 16 rows, of 128, or both.
+enum { FEW = 1, MANY = 2, BOTH = 3 };
+template <class Tr, int D, int DV, int TILES>
 struct Kind {
-  using Few = FewRows<Tr, D, DV, BOTH ? 8 : 4>;
-  static constexpr int THREADS = BOTH ? 512 : 256;
-  static constexpr int LDS = BOTH && Shape<Tr, D, DV>::LDS > Few::LDS ? Shape<Tr, D, DV>::LDS : Few::LDS;
+  using Few = FewRows<Tr, D, DV, TILES == FEW ? 4 : 8>;
+  static constexpr int THREADS = TILES == FEW ? 256 : 512;
+  static constexpr int FEW_LDS = TILES & FEW ? Few::LDS : 0, MANY_LDS = TILES & MANY ? Shape<Tr, D, DV>::LDS : 0;
+  static constexpr int LDS = FEW_LDS > MANY_LDS ? FEW_LDS : MANY_LDS;
 };
 
-template <class Tr, int D, int DV, bool BOTH>
-__global__ void __launch_bounds__(BOTH ? 512 : 256) attend(AttendParams P) {
-  using K = Kind<Tr, D, DV, BOTH>;
+template <class Tr, int D, int DV, int TILES>
+__global__ void __launch_bounds__(TILES == FEW ? 256 : 512) attend(AttendParams P) {
+  using K = Kind<Tr, D, DV, TILES>;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const uint32_t bid = tda::grid_bid<K::THREADS>();
   if (bid >= P.grid) return;
@@ -553,9 +555,9 @@ __global__ void __launch_bounds__(BOTH ? 512 : 256) attend(AttendParams P) {
   do {  // the tiles of a stretch; each looks at the sequences anew, which costs no registers meanwhile
     const Deal deal(P.seq, P.H / P.Hk, P.bound, P.room, kManyCost<typename Tr::T>);
     uint32_t group = bid / (uint32_t)P.Hk;
-    const bool many = BOTH && group < deal.groups[1];
+    const bool many = TILES == MANY || (TILES == BOTH && group < deal.groups[1]);
     if (!many) group -= deal.groups[1];
-    if (!many && group >= deal.groups[0]) return;
+    if (group >= (many ? deal.groups[1] : deal.groups[0])) return;
     const uint32_t per = many ? deal.per[1] : deal.per[0], begin = group * per, end = min(begin + per, many ? deal.line[1] : deal.line[0]);
     all = end - begin;
     Job J;
@@ -565,189 +567,189 @@ __global__ void __launch_bounds__(BOTH ? 512 : 256) attend(AttendParams P) {
     float* part = uniform(J.count < J.units) ? P.part + place : nullptr;
     if (done) __syncthreads();  // the tile before is done with the LDS
     done += J.count;
-    if constexpr (BOTH) {
-      if (many) {
-        many_rows<Tr, D, DV>(P, J, hk, part, lds);
-        continue;
-      }
-    }
-    K::Few::run(P, J, hk, part, reinterpret_cast<float*>(lds));
+    if constexpr (TILES & MANY)
+      if (many) many_rows<Tr, D, DV>(P, J, hk, part, lds);
+    if constexpr (TILES & FEW)
+      if (!many) K::Few::run(P, J, hk, part, reinterpret_cast<float*>(lds));
   } while (done < all);
 }
 
-// ------------------------------------------------------------------ joining pieces
-// Parts u = 0 .. n - 1 of one value: maximum, sum and weighted sum, in order, eight at a time so that their
-// loads are on their way together.
-struct Joined { float m, l; };
-template <class Stat, class Val, int N>
-__device__ __forceinline__ void join_parts(int n, Stat&& stat, Val&& val, float (&a)[N], Joined& j) {
-  j.m = sda::kNoMax;
-  j.l = 0.f;
+// ------------------------------------------------------------------ joining parts
+// One branch of some values: maximum, sum and weighted sums of the parts so far, taken on in order.
+template <int N>
+struct Joined {
+  float m = sda::kNoMax, l = 0.f, a[N] = {};
+  // Parts with maxima mm, sums ll (0: no key, its values are not written) and values v.
+  template <int B>
+  __device__ __forceinline__ void take(const float (&mm)[B], const float (&ll)[B], const float (&v)[B][N]) {
+    float top = m;
 #pragma unroll
-  for (int e = 0; e < N; ++e) a[e] = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 8) {
-    float mm[8], ll[8], aa[8][N];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int s = min(s0 + u, n - 1);
-      stat(s, mm[u], ll[u]);
-      val(s, aa[u]);
-      if (s0 + u >= n) ll[u] = 0.f;
-    }
-    float top = j.m;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) top = fmaxf(top, mm[u]);
-    const float f = sda::exp2_(j.m - top);
-    j.l *= f;
-    j.m = top;
+    for (int u = 0; u < B; ++u) top = fmaxf(top, mm[u]);
+    const float f = sda::exp2_(m - top);
+    l *= f;
+    m = top;
 #pragma unroll
     for (int e = 0; e < N; ++e) a[e] *= f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (ll[u] == 0.f) continue;  // no key of this piece: its sums are not written
+    for (int u = 0; u < B; ++u) {
       const float w = sda::exp2_(mm[u] - top);
-      j.l = __builtin_fmaf(ll[u], w, j.l);
+      l = __builtin_fmaf(ll[u], w, l);
 #pragma unroll
-      for (int e = 0; e < N; ++e) a[e] = __builtin_fmaf(aa[u][e], w, a[e]);
+      for (int e = 0; e < N; ++e) a[e] = ll[u] == 0.f ? a[e] : __builtin_fmaf(v[u][e], w, a[e]);
     }
   }
-}
+  // Takes on another lane's.
+  __device__ __forceinline__ void with(int lanes) {
+    const float om = __shfl_xor(m, lanes), top = fmaxf(m, om), f = sda::exp2_(m - top), g = sda::exp2_(om - top);
+    m = top;
+    const float ol = __shfl_xor(l, lanes);
+    l = l * f + ol * g;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float o = __shfl_xor(a[e], lanes);
+      a[e] = a[e] * f + o * g;
+    }
+  }
+};
 
-// Workgroups 0 .. join[0] - 1: a small tile each; then 32 rows of a large one each.
+// How a tile is joined.  Of a small one each wave takes a row, four columns a lane; where a row fills a part of the wave only, the
+// other lanes take other parts.  Of a large one each wave takes 32 rows, XS times four columns a lane.  The parts' sums and values are loaded
+// eight or four parts at a time, all together: a launch of this is a few waits for memory, and little else.
+template <int DV>
+struct Join {
+  static constexpr int W = DV / 4, SLICES = 64 / W;         // lanes of a row, its parts at a time
+  static constexpr int XS = 2, RG = kManyRows / 32, COLS = DV / 8 / XS / 4;  // workgroups that 32 rows take
+};
+
+// Workgroups of four rows of a small tile each; then of some columns of 32 rows of a large one each.
 template <class T, int DV>
 __global__ void __launch_bounds__(256) join(AttendParams A) {
-  const int G = A.H / A.Hk, tid = threadIdx.x;
+  using K = Join<DV>;
+  const int G = A.H / A.Hk, l = lane_id(), wv = uniform((int)threadIdx.x >> 6);
   uint32_t bid = tda::grid_bid<256>();
   Deal deal(A.seq, G, A.bound, A.room, kManyCost<T>);
   Job J;
   if (!deal.cut) return;
   // the parts of a tile: workgroups first .. first + n - 1 of its form, each in its first place unless the tile is where
   // its stretch ends
-  const auto parts_of = [&](int form, int hk, uint32_t& first, int& n) {
-    const uint32_t per = deal.per[form], last = (J.at + J.units - 1) / per;
-    first = J.at / per;
-    n = (int)(last - first) + 1;
+  const float *head, *tail;
+  int parts;
+  const int64_t step = 2 * A.Hk * A.stride;
+  const auto parts_of = [&](int form, int hk) {
+    const uint32_t per = deal.per[form], first = J.at / per, last = (J.at + J.units - 1) / per;
+    parts = (int)(last - first) + 1;
     const uint32_t place = first * per < J.at;  // of the first part; the others begin with this tile
     const uint32_t group = first + (form ? 0 : deal.groups[1]);
-    return A.part + (2 * ((int64_t)group * A.Hk + hk) + place) * A.stride;
+    tail = A.part + 2 * ((int64_t)group * A.Hk + hk) * A.stride;
+    head = tail + place * A.stride;
   };
-  uint32_t first;
-  int parts;
-  if (bid < A.join[0]) {
-    const int hk = (int)(bid % (uint32_t)A.Hk);
-    if (!deal.find<0, true>(bid / (uint32_t)A.Hk, 0, J)) return;
-    const float* head = parts_of(0, hk, first, parts);
-    if (parts < 2) return;
+  const auto part = [&](int u) { return u ? tail + u * step : head; };
+  const uint32_t per = (uint32_t)(A.join_rows + 3) / 4;  // workgroups of a small tile
+  if (bid < A.join[0] * per) {
+    const uint32_t tile = bid / per;
+    const int hk = (int)(tile % (uint32_t)A.Hk), n = 4 * (int)(bid % per) + wv;
+    if (!deal.find<0, true>(tile / (uint32_t)A.Hk, 0, J)) return;
     const Seq s = J.seq;
-    const int rows = min(kFewRows, s.cnt * G - kFewRows * J.tile);
-    const float* tail = A.part + 2 * ((int64_t)(first + deal.groups[1]) * A.Hk + hk) * A.stride;
-    const int64_t step = 2 * A.Hk * A.stride;
-    const auto part = [&](int u) { return u ? tail + u * step : head; };
-    for (int e = tid; e < rows * DV; e += 256) {
-      const int n = e / DV, c = e % DV, q = kFewRows * J.tile + n, h = hk * G + q % G, i = s.row0 + q / G;
-      float res[2];
+    parts_of(0, hk);
+    if (parts < 2 || n >= s.cnt * G - kFewRows * J.tile) return;
+    const int q = kFewRows * J.tile + n, h = hk * G + q % G, i = s.row0 + q / G, c = 4 * (l % K::W);
+    const float lam = sda::lambda_of(A.lam, s.qb, h, i);
+    Joined<4> j[2];
+    for (int u0 = l / K::W; u0 < parts; u0 += 8 * K::SLICES) {
+      float mm[2][8], ll[2][8], v[2][8][4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        Joined j;
-        float a[1];
-        join_parts(parts, [&](int u, float& m, float& l) { m = part(u)[32 * x + n]; l = part(u)[32 * x + 16 + n]; },
-                   [&](int u, float(&v)[1]) { v[0] = part(u)[64 + (x * kFewRows + n) * DV + c]; }, a, j);
-        res[x] = over(a[0], j.l);
-      }
-      sda::row_of<T>(A.out, s.qb, h, i)[c] = (T)__builtin_fmaf(-sda::lambda_of(A.lam, s.qb, h, i), res[1], res[0]);
-    }
-    return;
-  }
-  bid -= A.join[0];
-  if (bid >= A.join[1]) return;
-  constexpr int NO = DV / 32, RG = kManyRows / 32;
-  const int rg = (int)(bid % RG);
-  const uint32_t item = bid / RG;
-  if (!deal.find<1, true>(item / (uint32_t)A.Hk, 0, J)) return;
-  const int hk = (int)(item % (uint32_t)A.Hk);
-  const float* head = parts_of(1, hk, first, parts);
-  if (parts < 2) return;
-  const Seq s = J.seq;
-  const float* tail = A.part + 2 * ((int64_t)first * A.Hk + hk) * A.stride;
-  const int64_t step = 2 * A.Hk * A.stride;
-  const auto part_at = [&](int u) { return u ? tail + u * step : head; };
-  const int l = lane_id(), q = kManyRows * J.tile + 32 * rg + (l & 31);
-  if (q >= s.cnt * G) return;
-  const int h = hk * G + q % G, i = s.row0 + q / G;
-  const float lam = sda::lambda_of(A.lam, s.qb, h, i);
-  T* to = sda::row_of<T>(A.out, s.qb, h, i);
-  // each branch's maximum and sum over the pieces, then the pieces' values under them, in order
-  float top[2], inv[2];
+      for (int u = 0; u < 8; ++u) {
+        const int at = u0 + u * K::SLICES;
+        const float* p = part(min(at, parts - 1));
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    Joined j;
-    float none[1];
-    join_parts(parts, [&](int u, float& m, float& z) {
-        m = part_at(u)[2 * kManyRows * y + 32 * rg + (l & 31)];
-        z = part_at(u)[2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
-      }, [](int, float(&v)[1]) { v[0] = 0.f; }, none, j);
-    top[y] = j.m;
-    inv[y] = j.l > 0.f || j.l != j.l ? 1.0f / j.l : 0.f;
-  }
-  inv[1] *= -lam;
-  constexpr int XS = NO < 4 ? NO : 4;  // quads of values a thread has in hand
-  f32x4 z[XS] = {};
-  const int x0 = (tid >> 6) * NO;
-  for (int xs = 0; xs < NO; xs += XS) {
+        for (int x = 0; x < 2; ++x) {
+          mm[x][u] = p[32 * x + n];
+          ll[x][u] = p[32 * x + 16 + n];
+          const f32x4 y = *reinterpret_cast<const f32x4*>(p + 64 + (x * kFewRows + n) * DV + c);
 #pragma unroll
-    for (int k = 0; k < XS; ++k) z[k] = f32x4{};
-    for (int u0 = 0; u0 < parts; u0 += 2) {  // two pieces' values on their way
-      f32x4 v[2][2][XS];
-      float w[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float* part = part_at(min(u0 + u, parts - 1));
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float sum = part[2 * kManyRows * y + kManyRows + 32 * rg + (l & 31)];
-          w[u][y] = u0 + u < parts && sum != 0.f  // else no key of this piece: its sums are not written
-                        ? sda::exp2_(part[2 * kManyRows * y + 32 * rg + (l & 31)] - top[y]) * inv[y] : 0.f;
-#pragma unroll
-          for (int k = 0; k < XS; ++k)
-            v[u][y][k] = *reinterpret_cast<const f32x4*>(part + 4 * kManyRows + (int64_t)(((y * RG + rg) * NO * 4 + x0 + xs + k) * 64 + l) * 4);
+          for (int e = 0; e < 4; ++e) v[x][u][e] = y[e];
+          if (at >= parts) ll[x][u] = 0.f;
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (w[u][y] != 0.f)
-#pragma unroll
-            for (int k = 0; k < XS; ++k)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) z[k][e] = __builtin_fmaf(w[u][y], v[u][y][k][e], z[k][e]);
+      for (int x = 0; x < 2; ++x) j[x].take(mm[x], ll[x], v[x]);
     }
 #pragma unroll
-    for (int k = 0; k < XS; ++k) {
-      const int x = x0 + xs + k;
-      sda::store4(to + 32 * (x / 4) + 8 * (x % 4) + 4 * (l >> 5), z[k]);
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int d = K::W; d < 64; d *= 2) j[x].with(d);
+    if (l >= K::W) return;
+    f32x4 z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, over(j[1].a[e], j[1].l), over(j[0].a[e], j[0].l));
+    sda::store4(sda::row_of<T>(A.out, s.qb, h, i) + c, z);
+    return;
+  }
+  bid -= A.join[0] * per;
+  if (bid >= A.join[1] * K::COLS) return;
+  constexpr int NO = DV / 32;
+  const int x0 = (4 * (int)(bid % K::COLS) + wv) * K::XS, rg = (int)(bid / K::COLS % K::RG);
+  const uint32_t item = bid / (K::COLS * K::RG);
+  const int hk = (int)(item % (uint32_t)A.Hk);
+  if (!deal.find<1, true>(item / (uint32_t)A.Hk, 0, J)) return;
+  const Seq s = J.seq;
+  parts_of(1, hk);
+  const int row = 32 * rg + (l & 31), q = kManyRows * J.tile + row;
+  if (parts < 2 || q >= s.cnt * G) return;
+  const int h = hk * G + q % G, i = s.row0 + q / G;
+  const float lam = sda::lambda_of(A.lam, s.qb, h, i);
+  Joined<4 * K::XS> j[2];
+  for (int u0 = 0; u0 < parts; u0 += 4) {
+    float mm[2][4], ll[2][4], v[2][4][4 * K::XS];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* p = part(min(u0 + u, parts - 1));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mm[x][u] = p[2 * kManyRows * x + row];
+        ll[x][u] = p[2 * kManyRows * x + kManyRows + row];
+        if (u0 + u >= parts) ll[x][u] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K::XS; ++k) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(p + 4 * kManyRows + (int64_t)(((x * K::RG + rg) * NO * 4 + x0 + k) * 64 + l) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[x][u][4 * k + e] = y[e];
+        }
+      }
     }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) j[x].take(mm[x], ll[x], v[x]);
+  }
+  T* to = sda::row_of<T>(A.out, s.qb, h, i);
+#pragma unroll
+  for (int k = 0; k < K::XS; ++k) {
+    f32x4 z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(-lam, over(j[1].a[4 * k + e], j[1].l), over(j[0].a[4 * k + e], j[0].l));
+    const int x = x0 + k;
+    sda::store4(to + 32 * (x / 4) + 8 * (x % 4) + 4 * (l >> 5), z);
   }
 }
 
 // ------------------------------------------------------------------ launches
-template <class Tr, int D, int DV, bool BOTH>
+template <class Tr, int D, int DV, int TILES>
 static int launch(const AttendParams& p, hipStream_t st) {
-  using K = Kind<Tr, D, DV, BOTH>;
+  using K = Kind<Tr, D, DV, TILES>;
   if (K::LDS > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend<Tr, D, DV, BOTH>), hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend<Tr, D, DV, TILES>), hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return (int)e;
   }
-  attend<Tr, D, DV, BOTH><<<tda::grid_of<K::THREADS>(p.grid), K::THREADS, K::LDS, st>>>(p);
-  tda::launched(st, BOTH ? "spa_attend" : "spa_attend_few");
+  attend<Tr, D, DV, TILES><<<tda::grid_of<K::THREADS>(p.grid), K::THREADS, K::LDS, st>>>(p);
+  tda::launched(st, TILES == FEW ? "spa_attend_few" : TILES == MANY ? "spa_attend_many" : "spa_attend");
   return 0;
 }
 template <class Tr, int D, int DV>
 static int run(const AttendParams& p, hipStream_t st) {
-  const int e = p.bound < 0x7fffffff ? launch<Tr, D, DV, true>(p, st) : launch<Tr, D, DV, false>(p, st);
+  const int e = p.bound == 0 ? launch<Tr, D, DV, MANY>(p, st) : p.bound == 0x7fffffff ? launch<Tr, D, DV, FEW>(p, st) : launch<Tr, D, DV, BOTH>(p, st);
   if (e) return e;
   if (p.room) {
-    join<typename Tr::T, DV><<<tda::grid_of<256>((int64_t)p.join[0] + p.join[1]), 256, 0, st>>>(p);
+    const int64_t blocks = (int64_t)p.join[0] * ((p.join_rows + 3) / 4) + (int64_t)p.join[1] * Join<DV>::COLS;
+    join<typename Tr::T, DV><<<tda::grid_of<256>(blocks), 256, 0, st>>>(p);
     tda::launched(st, "spa_join");
   }
   return (int)hipGetLastError();

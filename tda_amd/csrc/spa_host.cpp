@@ -129,6 +129,7 @@ void deal(const spa_attend_args& a, spa::AttendParams& p) {
   p.grid = (uint32_t)(hk * (most_tiles > p.room ? most_tiles : p.room));
   p.join[0] = cut ? (uint32_t)(few * hk) : 0;
   p.join[1] = cut ? (uint32_t)(many * hk * (spa::kManyRows / 32)) : 0;
+  p.join_rows = (int)(exact && rows * G < spa::kFewRows ? rows * G : spa::kFewRows);
   p.stride = many ? spa::many_floats(dv) : spa::few_floats(dv);
 }
 int64_t part_bytes(const spa::AttendParams& p, int64_t hk) { return 2 * p.room * hk * p.stride * 4; }

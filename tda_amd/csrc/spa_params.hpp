@@ -42,7 +42,8 @@ struct AttendParams {
   float c;               // scale * log2(e)
   int room;              // workgroups that may share a key head's tiles; 0: whole tiles only
   uint32_t grid;         // workgroups of all key heads, at most
-  uint32_t join[2];      // workgroups of the joining launch: a small tile each, 32 rows of a large one each
+  uint32_t join[2];      // what the joining launch may have to join: small tiles; groups of 32 rows of large ones
+  int join_rows;         // rows of a small tile, at most
   float* part;           // two places for each of room workgroups of every key head, `stride` floats each
   int64_t stride;
 };
