@@ -149,8 +149,8 @@ struct Tile {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(void, reinterpret_cast<char*>(lds) + 1024 * u), 16, off, 0, 0, 0);
   }
   // Row fragment step t: lane (m, g) gets row r0 + m, values 16 t + 8 g + [0, 8).
-  __device__ __forceinline__ static typename Tr::frag row(const T* lds, int r0, int t) {
-    const int l = lane_id(), r = r0 + (l & 31), g = l >> 5;
+  __device__ __forceinline__ static typename Tr::frag row(const T* lds, int r0, int t, int l = lane_id()) {
+    const int r = r0 + (l & 31), g = l >> 5;
     static_assert(ES == 4, "16-bit types: RowReader");
     const int c = 4 * t + 2 * g;
     const f32x4 a = *reinterpret_cast<const f32x4*>(lds + r * W + 4 * (c ^ swz(r)));
@@ -159,9 +159,9 @@ struct Tile {
   }
   // Transposed fragment, step s (16 rows from r0 + 16 s): lane (n, g) gets column 32 cs + n at rows
   // r0 + crow(8 s + j, g), j = 0 .. 7, which is the order of a score tile's values.
-  __device__ __forceinline__ static typename Tr::frag col(const T* lds, int r0, int s, int cs) {
+  __device__ __forceinline__ static typename Tr::frag col(const T* lds, int r0, int s, int cs, int l = lane_id()) {
     static_assert(ES == 4, "16-bit types: ColReader");
-    const int l = lane_id(), g = l >> 5, n = 32 * cs + (l & 31);
+    const int g = l >> 5, n = 32 * cs + (l & 31);
     f32x8 f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -193,11 +193,11 @@ struct RowReader {
       }
     }
   }
-  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int t) const {
+  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int t, int lane = lane_id()) const {
     if constexpr (sizeof(typename Tr::T) == 2)
       return *reinterpret_cast<const __attribute__((address_space(3))) typename Tr::frag*>(a[t] + at);
     else
-      return Tile<Tr, 32, W>::row(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, t);
+      return Tile<Tr, 32, W>::row(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, t, lane);
   }
 };
 // A transposing read that the compiler takes to be apart from the direct loads to LDS on their way.  It knows no more of
@@ -224,7 +224,7 @@ struct ColReader {
     }
   }
   // Step s (16 rows) of the tile at `at`, column block y.
-  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int s, int y) const {
+  __device__ __forceinline__ typename Tr::frag read(const void* lds, int at, int s, int y, int lane = lane_id()) const {
     if constexpr (sizeof(typename Tr::T) == 2) {
       typedef typename Tr::T half4 __attribute__((ext_vector_type(4)));
       typename Tr::frag f;
@@ -237,7 +237,7 @@ struct ColReader {
       }
       return f;
     } else {
-      return Tile<Tr, 32, W>::col(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, s, y);
+      return Tile<Tr, 32, W>::col(reinterpret_cast<const float*>(static_cast<const char*>(lds) + at), 0, s, y, lane);
     }
   }
 };

@@ -140,10 +140,16 @@ __device__ __forceinline__ void many_rows(const AttendParams& P, const Job& J, i
     prepare(1);
   }
 
-  frag qf[NT];
-  const T* qr = sda::row_of<T>(P.q[br], sq.qb, h, qi);
+  // What registers do not hold of the widest fp32 rows (left to the compiler it went to memory and back in every stage: 1000 rows behind
+  // 3000, (16, 4 heads, 128, 256): 1750 us, so 980): the queries, read again in each stage, a few ahead of their products and
+  // before the next stage's loads, which they would else wait for; and the reads' addresses, worked out at each read.
+  constexpr bool TIGHT = sizeof(T) == 4 && D == 128, AGAIN = sizeof(T) == 4 && DV == 256;
+  constexpr int NQ = AGAIN ? 4 : NT;
+  frag qf[NQ];
+  const T* qr = sda::row_of<T>(P.q[br], sq.qb, h, qi) + 8 * g;
+  if constexpr (!AGAIN)
 #pragma unroll
-  for (int t = 0; t < NT; ++t) qf[t] = load8<Tr>(qr + 16 * t + 8 * g);
+    for (int t = 0; t < NT; ++t) qf[t] = load8<Tr>(qr + 16 * t);
   f32x16 o[NO];
   const float none = fresh_zero();
 #pragma unroll
@@ -160,23 +166,31 @@ __device__ __forceinline__ void many_rows(const AttendParams& P, const Job& J, i
     constexpr int AT = half * S::STAGE;
     sda::wait_vm<0>();
     tda::lds_barrier();  // stage j is in place, and every wave is done with stage j - 1
-    if (j + 1 < nst) issue(j + 1);
+    if (!AGAIN && j + 1 < nst) issue(j + 1);
     const int k0 = k0p + j * BN;
     if (k0 >= limw) {
+      if (AGAIN && j + 1 < nst) issue(j + 1);
       prepare(j + 2);
       return;
     }
     // one sequence of NS NT key fragments, then 2 NS NO value fragments, read a group ahead of their use
     frag f[2][G4];
+    const int ls = TIGHT ? fresh_lane() : l;
     auto read = [&](int i) {
 #pragma unroll
       for (int u = 0; u < G4; ++u) {
         const int e = i * G4 + u, w = e - NS * NT;
-        if (e < NS * NT) f[i & 1][u] = kr.read(kbuf, AT + 32 * D * KT::ES * (e % NS), e / NS);
-        else f[i & 1][u] = vr.read(vbuf, AT + 32 * DV * VT::ES * (w / (2 * NO)), w / NO % 2, w % NO);
+        if (e < NS * NT) f[i & 1][u] = kr.read(kbuf, AT + 32 * D * KT::ES * (e % NS), e / NS, ls);
+        else f[i & 1][u] = vr.read(vbuf, AT + 32 * DV * VT::ES * (w / (2 * NO)), w / NO % 2, w % NO, ls);
       }
     };
     f32x16 s[NS] = {};
+    const T* qs = qr;
+    if constexpr (AGAIN) {
+      asm volatile("" : "+v"(qs));
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) qf[t] = load8<Tr>(qs + 16 * t);
+    }
     read(0);
 #pragma unroll
     for (int i = 0; i < NS * NT / G4; ++i) {
@@ -184,9 +198,12 @@ __device__ __forceinline__ void many_rows(const AttendParams& P, const Job& J, i
 #pragma unroll
       for (int u = 0; u < G4; ++u) {
         const int e = i * G4 + u;
-        s[e % NS] = Tr::mma32(f[i & 1][u], qf[e / NS], s[e % NS]);
+        s[e % NS] = Tr::mma32(f[i & 1][u], qf[e / NS % NQ], s[e % NS]);
+        if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+        if (AGAIN && e % NS == NS - 1 && e / NS + NQ < NT) qf[e / NS % NQ] = load8<Tr>(qs + 16 * (e / NS + NQ));
       }
     }
+    if (AGAIN && j + 1 < nst) issue(j + 1);
     if (k0 + BN > clear) {
       asm volatile("");  // a branch: few stages need this
 #pragma unroll
@@ -231,6 +248,7 @@ __device__ __forceinline__ void many_rows(const AttendParams& P, const Job& J, i
       for (int u = 0; u < G4; ++u) {
         const int w = i * G4 + u - NS * NT;
         o[w % NO] = Tr::mma32(f[i & 1][u], p[w / NO], o[w % NO]);
+        if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -300,7 +318,7 @@ struct FewRows {
   typedef T row __attribute__((ext_vector_type(CW)));
   // 4-byte registers of a lane that holds both branches: a tile's keys and values; queries and sums
   static constexpr int TILE = (D / 2 + DV / 4) * (ES / 2), REST = D / 4 * (ES / 2) + DV / 2;
-  static constexpr bool SPLIT = WAVES == 8 && TILE + REST > 210;
+  static constexpr bool SPLIT = TILE + REST > (WAVES == 8 ? 210 : 420);
   static constexpr int DEPTH = WAVES == 4 && 2 * TILE + REST <= 400 ? 2 : 1;
   static constexpr int NBR = SPLIT ? 1 : 2, SETS = SPLIT ? WAVES / 2 : WAVES;  // branches of a wave, waves that share a branch's keys
   static constexpr int LROW = DV + 4;  // LDS row stride: rows start in different banks
