@@ -40,10 +40,6 @@ __device__ __forceinline__ typename Tr::frag load8(__amdgpu_buffer_rsrc_t r, uin
   }
 }
 
-// What a unit of a large tile costs next to one of a small one (Deal).
-template <class T>
-constexpr int kManyCost = sizeof(T) == 2 ? 2 : 7;
-
 // ------------------------------------------------------------------ many rows
 // sda_fwd.hip's pass over the keys: 128 rows a workgroup, 8 waves (four groups of 32 rows times the two
 // branches), transposed scores, keys and values by direct loads to LDS a stage ahead.  A stage's rows come from pages: one
@@ -571,7 +567,7 @@ __global__ void __launch_bounds__(TILES == FEW ? 256 : 512) attend(AttendParams 
   const int hk = (int)(bid % (uint32_t)P.Hk);
   uint32_t done = 0, all;
   do {  // the tiles of a stretch; each looks at the sequences anew, which costs no registers meanwhile
-    const Deal deal(P.seq, P.H / P.Hk, P.bound, P.room, kManyCost<typename Tr::T>);
+    const Deal deal(P.seq, P.H / P.Hk, P.bound, P.room, P.cost);
     uint32_t group = bid / (uint32_t)P.Hk;
     const bool many = TILES == MANY || (TILES == BOTH && group < deal.groups[1]);
     if (!many) group -= deal.groups[1];
@@ -645,7 +641,7 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
   using K = Join<DV>;
   const int G = A.H / A.Hk, l = lane_id(), wv = uniform((int)threadIdx.x >> 6);
   uint32_t bid = tda::grid_bid<256>();
-  Deal deal(A.seq, G, A.bound, A.room, kManyCost<T>);
+  Deal deal(A.seq, G, A.bound, A.room, A.cost);
   Job J;
   if (!deal.cut) return;
   // the parts of a tile: workgroups first .. first + n - 1 of its form, each in its first place unless the tile is where

@@ -112,8 +112,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const void* pool, ui
 
 // ------------------------------------------------------------------ work
 constexpr int kUnit = 128;  // keys
-// Tiles of 16 rows are cut until there are this many for each workgroup: their parts' sums are small.
-constexpr int kFewCut = 8;
+// Tiles of 16 rows are cut until there are this many for each workgroup: whole tiles that workgroups take as they come save the joining
+// and the second tile's start (newest tokens of 128 sequences of up to 1500, (32 over 8 heads, 128): 171 us, cut 186; of 64 of
+// up to 2000: 114, cut 119), while a tile a workgroup leaves the last ones alone (32 of up to 8192: 231, cut 223).
+constexpr int kFewCut = 2;
 
 // Running sums over the wave's lanes (lane moves: four within rows of 16 lanes, two from row to row), and their totals.
 // Call with every lane active.

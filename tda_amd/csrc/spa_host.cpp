@@ -102,6 +102,15 @@ int32_t check_attend_sizes(const spa_attend_args& a) {
 // Workgroups that share a call's tiles where these are fewer: one a CU.
 constexpr int64_t kTarget = 256;
 
+// What 128 keys of 128 rows cost next to 128 keys of 16: products and exponentials against bytes.  One long chunk among
+// tokens of 23 to 39 sequences behind up to 3000 to 5000, µs at the cost taken and at those beside it: bf16 (64, 64) 81 (86 at 1, 101 at 3),
+// (64, 128) 85 (94, 88), (128, 128) 130 (138 at 2), (128, 256) 162 (182 at 2); fp32 (64, 64) 118 (134 at 4, 140 at 8), (128, 128) 242 (279, 263),
+// (128, 256) 575 (694 at 6).
+int cost_of(int32_t dtype, int64_t d, int64_t dv) {
+  if (dtype == TDA_DTYPE_F32) return dv == 256 ? 4 : 6;
+  return d == 64 ? 2 : 1;
+}
+
 void deal(const spa_attend_args& a, spa::AttendParams& p) {
   const int64_t G = a.heads / a.cache.kv_heads, S = a.at.sequences, hk = a.cache.kv_heads, rows = a.at.rows, dv = a.cache.v_head_dim;
   const bool exact = !a.at.starts && !a.at.counts;  // every sequence has `rows` rows
@@ -130,6 +139,7 @@ void deal(const spa_attend_args& a, spa::AttendParams& p) {
   p.join[0] = cut ? (uint32_t)(few * hk) : 0;
   p.join[1] = cut ? (uint32_t)(many * hk * (spa::kManyRows / 32)) : 0;
   p.join_rows = (int)(exact && rows * G < spa::kFewRows ? rows * G : spa::kFewRows);
+  p.cost = cost_of(a.dtype, a.cache.head_dim, dv);
   p.stride = many ? spa::many_floats(dv) : spa::few_floats(dv);
 }
 int64_t part_bytes(const spa::AttendParams& p, int64_t hk) { return 2 * p.room * hk * p.stride * 4; }

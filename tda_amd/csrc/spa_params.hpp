@@ -40,6 +40,7 @@ struct AttendParams {
   Lambda lam;
   int H, Hk, lead, bound;
   float c;               // scale * log2(e)
+  int cost;              // what 128 keys of a large tile cost next to those of a small one
   int room;              // workgroups that may share a key head's tiles; 0: whole tiles only
   uint32_t grid;         // workgroups of all key heads, at most
   uint32_t join[2];      // what the joining launch may have to join: small tiles; groups of 32 rows of large ones
