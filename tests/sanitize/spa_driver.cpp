@@ -72,7 +72,7 @@ static void place(A& a, int64_t s, int64_t n) {
   a.abi_version = SPA_ABI_VERSION;
   a.dtype = TDA_DTYPE_BF16;
   a.cache = {100, 2, 32, 64, 128, AT, AT, AT};
-  a.at = {s, n, INTS, 9, 9, INTS, nullptr, nullptr};
+  a.at = {s, n, INTS, 90, 90, INTS, nullptr, nullptr};
   a.heads = 8;
   a.q1 = a.q2 = rows(8, n, 64);
 }
@@ -151,6 +151,8 @@ static void paged() {
   CHECK(got::attend.bound == 0x7fffffff && got::attend.join[0] == 6 && got::attend.join[1] == 0);
   CHECK(got::attend.room > 3 && got::attend.grid == (uint32_t)got::attend.room * 2 && got::attend.part);
   CHECK((int64_t)at.workspace_bytes == got::attend.room * 4 * few);
+  at.at.table_len = 31;  // over short tables: whole
+  CHECK(spa_attend(&at, nullptr) == TDA_OK && !got::attend.room && !spa_attend_workspace_bytes(&at));
   at = attend_args(20000, 1);  // whole tiles
   CHECK(spa_attend(&at, nullptr) == TDA_OK && got::attend.grid == 40000 && !got::attend.room && !got::attend.join[0] && !at.workspace_bytes);
   at = attend_args(2, 1000);  // 4000 rows of a key head are 32 tiles

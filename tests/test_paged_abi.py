@@ -64,7 +64,7 @@ def _cache(a, pages=10, hk=2, page=16, d=64, dv=128):
     c.k1 = c.k2 = c.v = FAKE
 
 
-def _at(a, s=3, n=5, table_len=4):
+def _at(a, s=3, n=5, table_len=100):
     a.at.sequences, a.at.rows, a.at.table, a.at.table_stride, a.at.table_len, a.at.lengths = s, n, FAKE, table_len, table_len, FAKE
 
 
@@ -160,6 +160,9 @@ def test_attend_workspaces():
     few, many = (64 + 2 * 16 * 128) * 4, (4 * 128 + 2 * 128 * 128) * 4
     assert attend(s=3, n=5).workspace_bytes == 512 * few
     assert attend(s=3, n=100).workspace_bytes == 512 * many
+    a = attend(s=3, n=5)
+    a.at.table_len = 4  # 256 positions
+    assert lib().spa_attend_workspace_bytes(ctypes.byref(a)) == 0
     assert attend(s=30000, n=5).workspace_bytes == attend(s=300, n=100).workspace_bytes == 0
     a = attend(s=3, n=100)
     a.at.counts = FAKE

@@ -195,6 +195,19 @@ def test_lambda_scale_and_layouts():
 
 
 @gpu
+@pytest.mark.parametrize("dtype, d, dv", [(BF, 64, 64), (F16, 128, 128), (F32, 128, 256)])
+def test_room_for_more_than_is_held(dtype, d, dv):
+    """Tables of 2048 positions, of which a few are held: small tiles are cut, and joined, or have one unit of keys."""
+    for new, held, form in (([1] * 5, [5, 16, 15, 0, 300], "even"), ([3, 0, 2], [129, 700, 126], "counts"), ([2, 1, 3], [900, 0, 128], "packed")):
+        s = Setup(new, held, 8, 2, d, dv, 16, dtype, form).spoil()
+        wide = torch.full((s.table.shape[0], 128), -1, dtype=torch.int32, device="cuda")
+        wide[:, : s.table.shape[1]] = s.table
+        s.table = wide
+        s.attend()
+        s.attend(most=3)
+
+
+@gpu
 def test_shared_pages_and_pages_that_are_none():
     """Two sequences read one prefix; table entries out of range stand for rows of zeros."""
     s = Setup([1, 1, 20], [70, 75, 90], 4, 2, 64, 64, 16, BF, "packed")
