@@ -16,10 +16,13 @@ s_cbranch_execnz edge is not followed when no instruction between the MFMA and t
 writes EXEC: the branch then tests the EXEC the MFMA ran under, which is never empty in
 these whole-wave loops.
 
+A second scan (masked_spills) looks for spills that only a part of the lanes stores.
+
     python -m tda_amd.isa_check          # compile and scan every kernel source
 """
 from __future__ import annotations
 
+import functools
 import os
 import re
 import subprocess
@@ -61,12 +64,13 @@ def _functions(asm: str) -> dict:
         if not s:
             continue
         if s.startswith("."):
-            if re.match(r"^\.LBB\S*:", s):
+            if s.startswith(".Lfunc_end"):
+                cur = None
+            elif re.match(r"^\.LBB\S*:", s):
                 funcs[cur].append(("label", s[:-1]))
             continue
-        if s.startswith("s_endpgm"):
+        if s.startswith("s_endpgm"):  # a kernel may end in more than one place
             funcs[cur].append(("end", s))
-            cur = None
             continue
         funcs[cur].append(("ins", s))
     return funcs
@@ -132,6 +136,29 @@ def scan_function(body: list) -> list:
     return found
 
 
+def masked_spills(body: list) -> list:
+    """Spills that a join of control flow places before the lanes that skipped the branch are back: those lanes would reload
+    what they never stored.  hipcc was seen to do so at the end of a branch of the lanes around loads, in a kernel out of
+    registers, with an address."""
+    joins = {_split(s)[1][0] for kind, s in body if kind == "ins" and s.startswith("s_cbranch_execz")}
+    out, at = [], None
+    for kind, s in body:
+        if kind == "label":
+            at = s if s in joins else None
+            seen = []
+        elif at and kind == "ins":
+            if s.startswith("scratch_store"):
+                seen.append((at, s))
+            elif s.startswith("s_or_b64 exec, exec,"):
+                out += seen
+                at = None
+            elif "exec" in s.split(",")[0] or s.startswith(("s_branch", "s_cbranch")):
+                at = None
+        else:
+            at = None
+    return out
+
+
 def scan(asm: str) -> dict:
     """{kernel symbol: hazards} for every kernel in one assembly file with a hazard."""
     out = {}
@@ -154,14 +181,26 @@ def compile_asm(src: str, outdir: str) -> str:
         return f.read()
 
 
-def check_all(sources=None) -> dict:
-    """Compile every kernel source and scan it.  Returns {source: {kernel: hazards}}."""
-    sources = sources or _build.HIP_SOURCES
+@functools.lru_cache(maxsize=1)
+def _assemblies(sources: tuple) -> tuple:
     with tempfile.TemporaryDirectory() as d:
         paths = [os.path.join(_build.CSRC, s) for s in sources]
         with ThreadPoolExecutor(max_workers=min(len(paths), os.cpu_count() or 1)) as ex:
-            asms = list(ex.map(lambda p: compile_asm(p, d), paths))
-    return {s: r for s, r in ((s, scan(a)) for s, a in zip(sources, asms)) if r}
+            return tuple(ex.map(lambda p: compile_asm(p, d), paths))
+
+
+def check_all(sources=None) -> dict:
+    """Compile every kernel source and scan it.  Returns {source: {kernel: hazards}}."""
+    sources = tuple(sources or _build.HIP_SOURCES)
+    return {s: r for s, r in ((s, scan(a)) for s, a in zip(sources, _assemblies(sources))) if r}
+
+
+def check_spills(sources=None) -> dict:
+    """The same for spills under a mask.  Returns {source: {kernel: spills}}."""
+    sources = tuple(sources or _build.HIP_SOURCES)
+    found = ((s, {k: h for k, h in ((k, masked_spills(b)) for k, b in _functions(a).items()) if h})
+             for s, a in zip(sources, _assemblies(sources)))
+    return {s: r for s, r in found if r}
 
 
 if __name__ == "__main__":
@@ -172,4 +211,9 @@ if __name__ == "__main__":
                 print(f"{src} {name}\n   {kind} after {ws} wait states via {path or 'fall-through'}\n"
                       f"   {mfma}\n   {use}")
     print("hazards:", sum(len(h) for k in res.values() for h in k.values()))
-    sys.exit(1 if res else 0)
+    spills = check_spills()
+    for src, kernels in spills.items():
+        for name, found in kernels.items():
+            print(f"{src} {name}\n   spill under a mask at {found[0][0]}: {found[0][1]}")
+    print("spills under a mask:", sum(len(h) for k in spills.values() for h in k.values()))
+    sys.exit(1 if res or spills else 0)
