@@ -4,10 +4,12 @@
 //   dx = rstd (g - mean(g) - xhat mean(g xhat)),  g = dy w;   dw = sum dy xhat,  db = sum dy
 //
 // A row stays in the registers of the lanes that share it: 8 to 64 lanes of a wave for rows of up to 4 KB, with the
-// row's sums by lane moves, and 256 or 1024 threads beyond, whose waves' sums meet in LDS.  A lane's pieces are the same columns of every row, so it keeps the sums of dw and db in registers over all
-// its rows; a workgroup leaves one row of them, and a second launch adds those up in order (where there are few rows, one
-// workgroup takes them all and writes the result).  All sums are 32 bits;
-// the variance is taken around the mean (of a wave, joined by the waves' means).
+// row's sums by lane moves, and 256 or 1024 threads beyond, whose waves' sums meet in LDS.  A lane's pieces are the same
+// columns of every row, so it keeps the sums of dw and db in registers over all its rows; a workgroup leaves one row of
+// them, and a second launch adds those up in order (where there are few rows, one workgroup takes them all and writes the
+// result).  All sums are 32 bits; the variance is taken around the mean (of a wave, joined by the waves' means).
+// Bound by memory, each value read and written once a pass: rows of 128, bf16, 2^18 of them, 32 us forward and 46 backward (4.2
+// TB/s); rows of 4096, 16384 of them, 60 and 82 (4.5 TB/s).
 #include "sda_common.hpp"
 #include "sln_params.hpp"
 
