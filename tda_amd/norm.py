@@ -4,7 +4,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -12,10 +11,11 @@ from torch.autograd.function import once_differentiable
 from . import _sln_abi
 from .softmax import _CODE, _COMPUTE, _TENSORS, _new_rows, _raw_stream, _refuse_tangents, _sig
 
-_PUT = struct.Struct("<Q").pack_into
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-_FWD_X, _FWD_Y, _FWD_W, _FWD_B, _FWD_S = (getattr(_sln_abi.SlnFwdArgs, n).offset for n in ("x", "y", "weight", "bias", "stats"))
-_BWD_OFF = {n: getattr(_sln_abi.SlnBwdArgs, n).offset for n in ("x", "dy", "dx", "weight", "stats", "dweight", "dbias", "workspace")}
+# where a call's arrays stand in its argument block, in pointers
+_FX, _FY, _FW, _FB, _FS = (getattr(_sln_abi.SlnFwdArgs, n).offset // 8 for n in ("x", "y", "weight", "bias", "stats"))
+_BX, _BDY, _BDX, _BW, _BS, _BDW, _BDB, _BWS = (getattr(_sln_abi.SlnBwdArgs, n).offset // 8
+                                               for n in ("x", "dy", "dx", "weight", "stats", "dweight", "dbias", "workspace"))
 
 
 def _call(fn, args_type, buf, device, what):
@@ -75,14 +75,14 @@ class _Plan:
     def forward(self, x, weight, bias, stats):
         y = torch.empty_strided(self.shape, self.strides, dtype=x.dtype, device=x.device)
         buf = bytearray(self.block)
-        _PUT(buf, _FWD_X, x.data_ptr())
-        _PUT(buf, _FWD_Y, y.data_ptr())
+        put = memoryview(buf).cast("Q")
+        put[_FX], put[_FY] = x.data_ptr(), y.data_ptr()
         if weight is not None:
-            _PUT(buf, _FWD_W, weight.data_ptr())
+            put[_FW] = weight.data_ptr()
         if bias is not None:
-            _PUT(buf, _FWD_B, bias.data_ptr())
+            put[_FB] = bias.data_ptr()
         if stats is not None:
-            _PUT(buf, _FWD_S, stats.data_ptr())
+            put[_FS] = stats.data_ptr()
         _call(_sln_abi.load().sln_fwd, _sln_abi.SlnFwdArgs, buf, x.device, "sln_fwd")
         return y
 
@@ -106,24 +106,23 @@ def _backward(ctx, dy):
         dy = dy.contiguous()
     block, size = ctx.block if dy.stride() == plan.strides and ctx.block else plan.bwd.get((dy.stride(), want)) or plan.backward_block(x, dy, want)
     buf = bytearray(block)
+    put = memoryview(buf).cast("Q")
     dx = dw = db = None
     if want[0]:
         dx = torch.empty_strided(plan.shape, plan.strides, dtype=x.dtype, device=x.device)
-        _PUT(buf, _BWD_OFF["dx"], dx.data_ptr())
+        put[_BDX] = dx.data_ptr()
     if weight is not None:
-        _PUT(buf, _BWD_OFF["weight"], weight.data_ptr())
+        put[_BW] = weight.data_ptr()
         if want[1]:
             dw = torch.empty_like(weight)
-            _PUT(buf, _BWD_OFF["dweight"], dw.data_ptr())
+            put[_BDW] = dw.data_ptr()
     if want[2]:
         db = torch.empty(bias[0], dtype=bias[1], device=x.device)
-        _PUT(buf, _BWD_OFF["dbias"], db.data_ptr())
+        put[_BDB] = db.data_ptr()
     if size:
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        _PUT(buf, _BWD_OFF["workspace"], ws.data_ptr())
-    _PUT(buf, _BWD_OFF["x"], x.data_ptr())
-    _PUT(buf, _BWD_OFF["dy"], dy.data_ptr())
-    _PUT(buf, _BWD_OFF["stats"], stats.data_ptr())
+        put[_BWS] = ws.data_ptr()
+    put[_BX], put[_BDY], put[_BS] = x.data_ptr(), dy.data_ptr(), stats.data_ptr()
     _call(_sln_abi.load().sln_bwd, _sln_abi.SlnBwdArgs, buf, x.device, "sln_bwd")
     return dx, dw, db, None
 

@@ -3,21 +3,28 @@ positions applied on the way, and the new positions attend over it."""
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
 from . import _sda_abi, _spa_abi
 from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _new_rows, _raw_stream, _scale,
-                      _sig, _usable)
+                      _usable)
 
-_PUT = struct.Struct("<Q").pack_into
 _DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
 _PAGE_SIZES = (16, 32, 64, 128, 256)
-_AT = {n: _spa_abi.SpaAppendArgs.at.offset + getattr(_spa_abi.SpaRows, n).offset for n in ("table", "lengths", "starts", "counts")}
-_APPEND_OFF = {**_AT, **{n: getattr(_spa_abi.SpaAppendArgs, n).offset for n in
-                         ("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out", "positions", "inv_freq")}}
-_ATTEND_OFF = {**_AT, **{n: getattr(_spa_abi.SpaAttendArgs, n).offset for n in ("q1", "q2", "out", "lambda_param", "workspace")}}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _words(args_type, names):
+    """Where a call's arrays stand in its argument block, in pointers."""
+    at = [args_type.at.offset + getattr(_spa_abi.SpaRows, n).offset for n in ("table", "lengths", "starts", "counts")]
+    return [o // 8 for o in (*at, *(getattr(args_type, n).offset for n in names))]
+
+
+(_A_TABLE, _A_LENGTHS, _A_STARTS, _A_COUNTS, _A_K1, _A_K2, _A_V, _A_Q1, _A_Q2, _A_O1, _A_O2, _A_POS, _A_FREQ) = _words(
+    _spa_abi.SpaAppendArgs, ("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out", "positions", "inv_freq"))
+(_T_TABLE, _T_LENGTHS, _T_STARTS, _T_COUNTS, _T_Q1, _T_Q2, _T_OUT, _T_LAM, _T_WS) = _words(
+    _spa_abi.SpaAttendArgs, ("q1", "q2", "out", "lambda_param", "workspace"))
 
 
 class PagedKVCache:
@@ -97,10 +104,19 @@ class PagedKVCache:
     @staticmethod
     def _signature(*tensors):
         """What a call's plan goes by, or None."""
+        out = []
+        add = out.append
         for t in tensors:
-            if t is not None and type(t) not in _TENSORS:
+            if t is None:
+                add(None)
+            elif type(t) in _TENSORS:
+                add(t.shape)
+                add(t.stride())
+                add(t.dtype)
+                add(t.device)
+            else:
                 return None
-        return tuple([None if t is None else _sig(t) for t in tensors])
+        return tuple(out)
 
     def _plan(self, key, *plan):
         if len(self._plans) > 64:
@@ -140,7 +156,7 @@ class PagedKVCache:
 
     def _call(self, fn, args_type, buf, what):
         a = args_type.from_buffer(buf)
-        if torch.cuda.current_device() == self.device.index:
+        if _current_device() == self.device.index:
             rc = fn(ctypes.byref(a), _raw_stream(self.device.index))
         else:
             with torch.cuda.device(self.device):
@@ -164,7 +180,8 @@ class PagedKVCache:
         if key is not None:
             key = "append", key, None if sections is None else tuple([int(s) for s in sections]), bool(interleaved)
             plan = self._plans.get(key)
-            if plan is not None and not any(t.data_ptr() % 16 for t in (k1, k2, v, q1, q2) if t is not None):
+            if plan is not None and not (k1.data_ptr() | k2.data_ptr() | v.data_ptr()
+                                         | (0 if q1 is None else q1.data_ptr() | q2.data_ptr())) % 16:
                 return self._append(plan, given)
         _check_rows((k1,), ("k1",))
         b, hk, n, d, dv = k1.shape[0], self.kv_heads, k1.shape[2], self.head_dim, self.v_head_dim
@@ -225,17 +242,23 @@ class PagedKVCache:
     def _append(self, plan, tensors):
         k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions = tensors
         buf = bytearray(plan[0])
-        out = tuple([torch.empty_strided(shape, st, dtype=self.dtype, device=self.device) for shape, st in plan[1]])
-        for name, t in zip(("k1", "k2", "v", "table", "lengths"), (k1, k2, v, table, lengths)):
-            _PUT(buf, _APPEND_OFF[name], t.data_ptr())
-        for name, t in (("starts", starts), ("counts", counts), ("inv_freq", inv_freq), ("positions", positions)):
-            if t is not None:
-                _PUT(buf, _APPEND_OFF[name], t.data_ptr())
-        if out:
-            for name, t in zip(("q1", "q2", "q1_out", "q2_out"), (q1, q2, *out)):
-                _PUT(buf, _APPEND_OFF[name], t.data_ptr())
+        put = memoryview(buf).cast("Q")
+        put[_A_K1], put[_A_K2], put[_A_V] = k1.data_ptr(), k2.data_ptr(), v.data_ptr()
+        put[_A_TABLE], put[_A_LENGTHS] = table.data_ptr(), lengths.data_ptr()
+        if starts is not None:
+            put[_A_STARTS] = starts.data_ptr()
+        if counts is not None:
+            put[_A_COUNTS] = counts.data_ptr()
+        if inv_freq is not None:
+            put[_A_FREQ] = inv_freq.data_ptr()
+        if positions is not None:
+            put[_A_POS] = positions.data_ptr()
+        out = None
+        if plan[1]:
+            out = tuple([torch.empty_strided(shape, st, dtype=self.dtype, device=self.device) for shape, st in plan[1]])
+            put[_A_Q1], put[_A_Q2], put[_A_O1], put[_A_O2] = q1.data_ptr(), q2.data_ptr(), out[0].data_ptr(), out[1].data_ptr()
         self._call(_spa_abi.load().spa_append, _spa_abi.SpaAppendArgs, buf, "spa_append")
-        return out or None
+        return out
 
     def attend(self, q1, q2, lambda_param, table, lengths, scale=None, *, starts=None, counts=None, most=None):
         """Softmax differential attention of the new positions, whose keys and values append() has put in place:
@@ -252,7 +275,7 @@ class PagedKVCache:
         if key is not None:
             key = "attend", key, scale, most
             plan = self._plans.get(key)
-            if plan is not None and not (q1.data_ptr() % 16 or q2.data_ptr() % 16):
+            if plan is not None and not (q1.data_ptr() | q2.data_ptr()) % 16:
                 return self._attend(plan, given)
         _check_rows((q1,), ("q1",))
         b, h, n = q1.shape[:3]
@@ -287,15 +310,16 @@ class PagedKVCache:
         q1, q2, lam, table, lengths, starts, counts = tensors
         block, shape, strides, size = plan
         buf = bytearray(block)
+        put = memoryview(buf).cast("Q")
         out = torch.empty_strided(shape, strides, dtype=self.dtype, device=self.device)
-        for name, t in zip(("q1", "q2", "out", "lambda_param", "table", "lengths"), (q1, q2, out, lam, table, lengths)):
-            _PUT(buf, _ATTEND_OFF[name], t.data_ptr())
+        put[_T_Q1], put[_T_Q2], put[_T_OUT], put[_T_LAM] = q1.data_ptr(), q2.data_ptr(), out.data_ptr(), lam.data_ptr()
+        put[_T_TABLE], put[_T_LENGTHS] = table.data_ptr(), lengths.data_ptr()
         if starts is not None:
-            _PUT(buf, _ATTEND_OFF["starts"], starts.data_ptr())
+            put[_T_STARTS] = starts.data_ptr()
         if counts is not None:
-            _PUT(buf, _ATTEND_OFF["counts"], counts.data_ptr())
+            put[_T_COUNTS] = counts.data_ptr()
         if size:
             ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _PUT(buf, _ATTEND_OFF["workspace"], ws.data_ptr())
+            put[_T_WS] = ws.data_ptr()
         self._call(_spa_abi.load().spa_attend, _spa_abi.SpaAttendArgs, buf, "spa_attend")
         return out
