@@ -639,7 +639,7 @@ struct Joined {
 template <int DV>
 struct Join {
   static constexpr int W = DV / 4, SLICES = 64 / W;         // lanes of a row, its parts at a time
-  static constexpr int XS = 2, RG = kManyRows / 32, COLS = DV / 8 / XS / 4;  // workgroups that 32 rows take
+  static constexpr int XS = DV >= 128 ? 4 : 2, PB = 8 / XS, RG = kManyRows / 32, COLS = DV / 8 / XS / 4;  // workgroups that 32 rows take
 };
 
 // Workgroups of four rows of a small tile each; then of some columns of 32 rows of a large one each.
@@ -720,10 +720,10 @@ __global__ void __launch_bounds__(256) join(AttendParams A) {
   const int h = hk * G + q % G, i = s.row0 + q / G;
   const float lam = sda::lambda_of(A.lam, s.qb, h, i);
   Joined<4 * K::XS> j[2];
-  for (int u0 = 0; u0 < parts; u0 += 4) {
-    float mm[2][4], ll[2][4], v[2][4][4 * K::XS];
+  for (int u0 = 0; u0 < parts; u0 += K::PB) {
+    float mm[2][K::PB], ll[2][K::PB], v[2][K::PB][4 * K::XS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < K::PB; ++u) {
       const float* p = part(min(u0 + u, parts - 1));
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
