@@ -133,17 +133,13 @@ __device__ __forceinline__ uint32_t running(uint32_t x) {
   return x;
 }
 __device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)running(x), 63); }
-__device__ __forceinline__ uint64_t wave_total(uint64_t x) {  // of values below 2^58
-  const uint32_t low = wave_total((uint32_t)(x & 0x3ffffff)), mid = wave_total((uint32_t)(x >> 26) & 0x3ffffff);
-  return low + ((uint64_t)mid << 26) + ((uint64_t)wave_total((uint32_t)(x >> 52)) << 52);
-}
 
 // A part of a tile of rows of one sequence (the rows of all heads that share a key head, token by token): units from ..
 // from + count - 1 of the tile's `units`.
 struct Job {
   int s, tile;
   uint32_t at, from, count, units;  // at: the tile's place on its form's line
-  uint32_t per;                     // the stretches' length where the tile begins with one, else 0
+  uint32_t per, parts;              // where the tile begins with a stretch: its length, and how many the tile has; else 0
   Seq seq;
 };
 
@@ -179,63 +175,67 @@ struct Deal {
   }
   __device__ __forceinline__ static uint32_t fill(uint32_t units, uint32_t per) { return (units + per - 1) / per; }
   __device__ __forceinline__ Deal(const Seqs& Q_, int G_, int bound_, int room, int cost) : Q(Q_), G(G_), bound(bound_), l(lane_id()) {
+    // Sums that matter while they are small are held small: a lane's units end at 2^24 (that many keys in fewer tiles than are
+    // cut would be 2^31), its stretches at 1023, of two lengths in one number.
+    constexpr uint32_t kUnits = 1 << 24, kParts = 1023;
     q = Seq{};
-    uint32_t n0 = 0, n1 = 0;
-    uint64_t w0 = 0, w1 = 0;
+    uint32_t n[2] = {0, 0}, w[2] = {0, 0};
     for (int s0 = 0; s0 < Q.S; s0 += 64) {
       sizes(s0);
-      const uint64_t w = (uint64_t)t * u;
-      n0 += form ? 0 : t;
-      n1 += form ? t : 0;
-      w0 += form ? 0 : w;
-      w1 += form ? w : 0;
-    }
-    groups[0] = line[0] = wave_total(n0);
-    groups[1] = line[1] = wave_total(n1);
-    per[0] = per[1] = 1;
-    own[0] = own[1] = cut = false;
-    if (room && line[0] + line[1] < (uint32_t)(line[1] ? room : kFewCut * room)) {
-      const uint64_t w[2] = {wave_total(w0), wave_total(w1)};
-      cut = w[0] + w[1] < 0x40000000u;  // fewer tiles than that are longer than a cache can be
-      if (cut) {
-        uint32_t to[2] = {(uint32_t)room, (uint32_t)room};
-        if (w[0] && w[1]) {
-          const uint64_t a = w[0], b = w[1] * (uint64_t)cost;
-          const int shift = max(44 - (int)__builtin_clzll(a + b + 1), 0);  // the sum in 20 bits
-          const uint32_t x = (uint32_t)(a >> shift), y = (uint32_t)(b >> shift);
-          to[1] = min(max(((uint32_t)room * y + (x + y) / 2) / max(x + y, 1u), 1u), (uint32_t)room - 1);
-          to[0] = (uint32_t)room - to[1];
-        }
+      const uint32_t x = (uint32_t)min((uint64_t)t * u, (uint64_t)kUnits);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          line[f] = (uint32_t)w[f];
-          per[f] = max((line[f] + to[f] - 1) / to[f], 1u);
-          groups[f] = (line[f] + per[f] - 1) / per[f];
-        }
-        uint32_t longer[2];
-#pragma unroll
-        for (int f = 0; f < 2; ++f) longer[f] = per[f] + (per[f] + 7) / 8;
-        uint32_t n[4] = {0, 0, 0, 0};  // stretches that tiles of their own take, of either length
-        for (int s0 = 0; s0 < Q.S; s0 += 64) {
-          if (Q.S > 64) sizes(s0);
-          const uint32_t a = t * fill(u, form ? per[1] : per[0]), b = t * fill(u, form ? longer[1] : longer[0]);
-          n[0] += form ? 0 : a;
-          n[1] += form ? a : 0;
-          n[2] += form ? 0 : b;
-          n[3] += form ? b : 0;
-        }
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const uint32_t a = wave_total(n[f]), b = wave_total(n[2 + f]);
-          own[f] = min(a, b) <= to[f];
-          if (own[f]) {
-            if (a > to[f]) per[f] = longer[f];
-            groups[f] = a > to[f] ? b : a;
-            line[f] = groups[f] * per[f];
-          }
-        }
+      for (int f = 0; f < 2; ++f) {
+        n[f] += form == f ? t : 0;
+        w[f] = min(w[f] + (form == f ? x : 0), kUnits);
       }
     }
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      groups[f] = line[f] = wave_total(n[f]);
+      per[f] = 1;
+      own[f] = false;
+    }
+    cut = room && line[0] + line[1] < (uint32_t)(line[1] ? room : kFewCut * room) && !__any(w[0] >= kUnits || w[1] >= kUnits);
+    if (!cut) return;
+    uint32_t all[2] = {0, 0}, to[2] = {(uint32_t)room, (uint32_t)room}, longer[2] = {1, 1};
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+      if (line[f]) all[f] = wave_total(w[f]);
+    if (line[0] && line[1]) {
+      const uint64_t a = all[0], b = all[1] * (uint64_t)cost;
+      const int shift = max(44 - (int)__builtin_clzll(a + b + 1), 0);  // the sum in 20 bits
+      const uint32_t x = (uint32_t)(a >> shift), y = (uint32_t)(b >> shift);
+      to[1] = min(max(((uint32_t)room * y + (x + y) / 2) / max(x + y, 1u), 1u), (uint32_t)room - 1);
+      to[0] = (uint32_t)room - to[1];
+    }
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+      if (line[f]) {
+        per[f] = max((all[f] + to[f] - 1) / to[f], 1u);
+        longer[f] = per[f] + (per[f] + 7) / 8;
+      }
+    uint32_t m[2] = {0, 0};  // stretches that tiles of their own take, of either length
+    for (int s0 = 0; s0 < Q.S; s0 += 64) {
+      if (Q.S > 64) sizes(s0);
+      const uint32_t a = min(t * fill(u, form ? per[1] : per[0]), kParts), b = min(t * fill(u, form ? longer[1] : longer[0]), kParts);
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+        if (form == f) m[f] = min((m[f] & 0xffff) + a, kParts) | min((m[f] >> 16) + b, kParts) << 16;
+    }
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+      if (line[f]) {
+        const uint32_t both = wave_total(m[f]), a = both & 0xffff, b = both >> 16;
+        own[f] = min(a, b) <= to[f];
+        if (own[f]) {
+          if (a > to[f]) per[f] = longer[f];
+          groups[f] = a > to[f] ? b : a;
+          line[f] = groups[f] * per[f];
+        } else {
+          line[f] = all[f];
+          groups[f] = (all[f] + per[f] - 1) / per[f];
+        }
+      }
   }
   // What stands at unit `at` of a form's line, or with TILE the tile number `at`; up to `end` or the tile's end.  False:
   // nothing.
@@ -249,7 +249,12 @@ struct Deal {
     uint32_t tiles = 0, units = 0;  // of the sequences before
     for (int s0 = 0; s0 < Q.S; s0 += 64) {
       if (Q.S > 64) sizes(s0);
-      const uint32_t each = !cut ? 1u : own[FORM] ? fill(u, per[FORM]) * per[FORM] : u, n = form == FORM ? t : 0, w = n * each;
+      uint32_t each = cut ? u : 1u, parts = 0;
+      if (own[FORM]) {
+        parts = fill(u, per[FORM]);
+        each = parts * per[FORM];
+      }
+      const uint32_t n = form == FORM ? t : 0, w = n * each;
       const uint32_t nu = running(n), wu = running(w);
       const auto lane = [&](uint32_t v, int x) { return (uint32_t)__builtin_amdgcn_readlane((int)v, x); };
       const uint32_t sum = lane(TILE ? nu : wu, 63), rest = at - (TILE ? tiles : units);
@@ -264,6 +269,7 @@ struct Deal {
         J.from = TILE ? 0 : at - J.at;
         J.count = TILE ? J.units : min(J.units - J.from, end - at);
         J.per = own[FORM] ? per[FORM] : 0;
+        J.parts = lane(parts, x);
         const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x); };
         J.seq = {of(q.qb), of(q.row0), of(q.cnt), of(q.held), of(q.len)};
         return true;
@@ -277,9 +283,9 @@ struct Deal {
   __device__ __forceinline__ static void keys(const Job& J, int lim, int& k0, int& k1) {
     uint32_t from = J.from, to = J.from + J.count;
     if (J.per) {
-      const uint32_t parts = J.units / J.per, part = from / J.per, units = (uint32_t)(lim + kUnit - 1) / kUnit;
-      from = part * units / parts;
-      to = (part + 1) * units / parts;
+      const uint32_t part = from / J.per, units = (uint32_t)(lim + kUnit - 1) / kUnit, each = units / J.parts, more = units - each * J.parts;
+      from = part * each + min(part, more);
+      to = from + each + (part < more);
     }
     const bool whole = J.count == J.units;
     k0 = uniform(whole ? 0 : min((int)(from * kUnit), lim));
