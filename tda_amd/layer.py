@@ -172,6 +172,11 @@ class DifferentialAttention(nn.Module):
         self._inv_freq = (float(rotary_base) ** (-torch.arange(pairs, dtype=torch.float64, device="cpu") / pairs)).float()
         self._place()
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._parameters.setdefault("norm_weight", None)  # a layer that was pickled before it had a norm
+        self.__dict__.setdefault("norm_eps", 1e-5)
+
     def _place(self):
         """The pairs' frequencies, in 32 bits whatever type the module is cast to, beside the weights: a call must not
         copy them from the host, which would make it wait and keep it out of a graph."""
@@ -238,7 +243,7 @@ class DifferentialAttention(nn.Module):
                 raise ValueError(f"the cache holds {cache.batch} sequences, x has {x.shape[0]}")
             if torch.is_grad_enabled():
                 with torch.no_grad():
-                    return self.forward(x, positions, None, cache, **where)
+                    return self.forward(x, positions, None, cache, **(where if paged else {}))
         b, n, _ = x.shape
         q1, q2, k1, k2, v = self.project(x)
         if paged:

@@ -200,3 +200,32 @@ def test_refusals():
         m(x[:1], cache=cache, table=table, lengths=lengths)
     with pytest.raises(ValueError, match="holds"):
         m(x, cache=layer(dtype=BF).new_paged_cache(4, 16), table=table, lengths=lengths)
+
+
+# ------------------------------------------------------------------ what layers without these could do
+def test_layers_pickled_without_a_norm():
+    m = tda_amd.DifferentialAttention(128, 2, bias=True)
+    state = copy.deepcopy(m.__dict__)
+    del state["norm_eps"], state["_parameters"]["norm_weight"]
+    old = tda_amd.DifferentialAttention.__new__(tda_amd.DifferentialAttention)
+    old.__setstate__(state)
+    assert old.norm_weight is None and old.norm_eps == 1e-5 and repr(old) == repr(m)
+    assert list(old.state_dict()) == list(m.state_dict()) and "norm_weight" not in old.state_dict()
+    assert old.load_state_dict(m.state_dict()).missing_keys == []
+
+
+def test_subclasses_with_the_arguments_of_a_4_bit_cache():
+    """A forward of four arguments is called again without gradients as it was called."""
+    calls = []
+
+    class Mine(tda_amd.DifferentialAttention):
+        def forward(self, x, positions=None, kv_lens=None, cache=None):
+            calls.append((positions, kv_lens, cache, torch.is_grad_enabled()))
+            return x if len(calls) == 2 else super().forward(x, positions, kv_lens, cache)
+
+    class Cache:
+        batch = 3
+
+    cache, x = Cache(), torch.zeros(3, 1, 128)
+    assert Mine(128, 2)(x, cache=cache) is x
+    assert calls == [(None, None, cache, True), (None, None, cache, False)]
