@@ -6,7 +6,7 @@
 // is hidden, and its keys are read once.  Where the tiles are fewer than the CUs their keys are cut into stretches
 // (Deal), so that a batch of unequal conversations, or of tokens and chunks, is even work: a chunk keeps some CUs' matrix
 // cores busy while others read the caches of the tokens beside it (a chunk of 700 rows and 23 tokens behind up to 5000, fp16, 16 over 4
-// heads of (64, 128): 101 us; as launches of their own for tokens and chunk 132).
+// heads of (64, 128): 98 us; as launches of their own for tokens and chunk 132).
 #pragma once
 
 #include "spa_common.hpp"
@@ -634,8 +634,8 @@ struct Joined {
 
 // How a tile is joined.  Of a small one each wave takes a row, four columns a lane; where a row fills a part of the wave only, the
 // other lanes take other parts.  Of a large one each wave takes 32 rows, XS times four columns a lane.  The parts' sums and values are loaded
-// eight or four parts at a time, all together: a launch of this is a few waits for memory, and little else (4.7 us for one
-// token's eight parts, 7.2 for 32 parts of 32000 keys, 10.7 for a chunk's 34 MB).
+// eight or four parts at a time, all together: a launch of this is a few waits for memory, and little else (4.4 us for one
+// token's eight parts, 7.0 for 32 parts of 32000 keys, 9.8 for a chunk's 34 MB).
 template <int DV>
 struct Join {
   static constexpr int W = DV / 4, SLICES = 64 / W;         // lanes of a row, its parts at a time
