@@ -63,7 +63,9 @@ struct Pages {
   int now, next;
   __device__ __forceinline__ int fetch(int at) const {
     const int e = at + lane_id();
-    const int p = row[min(e, tlen - 1)];  // no branch: see many_rows' queries
+    // The compiler loads under the first condition and waits for the load there.  Checked in page() instead, every stage would wait for
+    // all loads on their way (a chunk among tokens 103 -> 113 us).
+    const int p = row[min(e, tlen - 1)];
     return e < tlen && p < pages ? p : -1;
   }
   __device__ __forceinline__ void begin(const Seqs& Q, int s, int slot) {
