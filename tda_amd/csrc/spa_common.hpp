@@ -118,6 +118,7 @@ constexpr int kUnit = 128;  // keys
 // and the second tile's start (newest tokens of 128 sequences of up to 1500, (32 over 8 heads, 128): 171 us, cut 186; of 64 of
 // up to 2000: 114, cut 119), while a tile a workgroup leaves the last ones alone (32 of up to 8192: 231, cut 223).
 constexpr int kFewCut = 2;
+constexpr int kManyCut = 3;
 
 // Running sums over the wave's lanes (lane moves: four within rows of 16 lanes, two from row to row), and their totals.
 // Call with every lane active.
@@ -182,9 +183,11 @@ struct Deal {
     constexpr uint32_t kUnits = 1 << 24, kParts = 1023;
     q = Seq{};
     uint32_t n[2] = {0, 0}, w[2] = {0, 0};
+    bool early = false;  // large tiles whose keys are far fewer than their sequence's last one's
     for (int s0 = 0; s0 < Q.S; s0 += 64) {
       sizes(s0);
       const uint32_t x = (uint32_t)min((uint64_t)t * u, (uint64_t)kUnits);
+      early |= form && 3 * (int64_t)q.cnt > q.len;
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         n[f] += form == f ? t : 0;
@@ -197,7 +200,16 @@ struct Deal {
       per[f] = 1;
       own[f] = false;
     }
-    cut = room && line[0] + line[1] < (uint32_t)(line[1] ? room : kFewCut * room) && !__any(w[0] >= kUnits || w[1] >= kUnits);
+    const uint32_t tiles = line[0] + line[1];
+    cut = room && tiles < (uint32_t)(line[1] ? room : kFewCut * room);
+    // Two or three rounds of large tiles are cut too where a quarter of the rounds' places would be idle: stretches are then a tile or more and a
+    // part (1200 rows behind 3000, 32 over 8 heads of 128: 184 us, whole 203; 2100 behind 8000: 697, 801).  Not among small tiles, nor where
+    // tiles have unlike keys: workgroups take these as they come, the longest first (1600 behind 2000: 171, cut 201).
+    if (room && !line[0] && !cut && tiles < (uint32_t)(kManyCut * room)) {
+      const uint32_t rounds = 1 + (tiles > (uint32_t)room) + (tiles > (uint32_t)(2 * room));
+      cut = 4 * tiles < 3 * rounds * (uint32_t)room && !__any(early);
+    }
+    cut = cut && !__any(w[0] >= kUnits || w[1] >= kUnits);
     if (!cut) return;
     uint32_t all[2] = {0, 0}, to[2] = {(uint32_t)room, (uint32_t)room}, longer[2] = {1, 1};
 #pragma unroll

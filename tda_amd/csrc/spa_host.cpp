@@ -135,7 +135,10 @@ void deal(const spa_attend_args& a, spa::AttendParams& p) {
   // Small tiles over short tables are taken whole: what the joining launch costs, six microseconds, their other keys cost too from about 1024
   // on (newest tokens of 8 x 250, (16 over 4 heads, 128): 13.0 us, cut 18.2; 8 x 500: 16.7, 18.5; 2 x 1000: 17.7, 18.1).
   const bool brief = !many && a.at.table_len < 1024 / a.cache.page_size;
-  const bool cut = 4 * tiles * hk <= 3 * kTarget && hk <= kTarget && !brief;
+  // ... or too many by so few that a last round of them leaves CUs idle; how full the rounds are is known of an exact call
+  const int64_t all = tiles * hk, rounds = ceil_div(all, kTarget);
+  const bool ragged = many && all <= 3 * kTarget && (!exact || 4 * all < 3 * rounds * kTarget);
+  const bool cut = (4 * all <= 3 * kTarget || ragged) && hk <= kTarget && !brief;
   p.room = cut ? (int)(kTarget / hk) : 0;
   const int64_t most_tiles = few + many;
   p.grid = (uint32_t)(hk * (most_tiles > p.room ? most_tiles : p.room));

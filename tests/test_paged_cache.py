@@ -157,6 +157,14 @@ def test_tiles_with_every_row_are_cut(dtype, d, dv):
 
 
 @gpu
+@pytest.mark.parametrize("dtype, d, dv", [(BF, 128, 128), (F16, 64, 128), (F32, 64, 64)])
+def test_a_few_tiles_more_than_fit_at_once(dtype, d, dv):
+    """Stretches of more than one large tile, alone and among tokens; and prompts from the start, whose tiles stay whole."""
+    for new, held, form in (([600], [1500], "even"), ([600], [1303], "packed"), ([600, 0], [1500, 7], "counts"), ([600, 1, 3], [1500, 300, 0], "packed"), ([600], [0], "even")):
+        Setup(new, held, 64, 64, d, dv, 64, dtype, form).spoil().attend()
+
+
+@gpu
 def test_the_rows_bound_costs_no_results():
     s = Setup([1, 50, 1], [40, 300, 1000], 8, 2, 64, 64, 16, BF, "packed").spoil()
     want = s.attend()
