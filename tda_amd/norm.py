@@ -55,9 +55,9 @@ class _Plan:
         a.weight_dtype, a.weight_heads = self.weight_dtype, self.weight_heads
         a.x.stride[:] = self.four(x.stride())
 
-    @staticmethod
-    def four(strides):
-        return (*(0,) * (4 - len(strides)), *strides[:-1], 1)
+    def four(self, strides):
+        """The strides of four axes.  The last one as it is, for sln_fwd and sln_bwd to check; along one value any will do."""
+        return (*(0,) * (4 - len(strides)), *strides[:-1], strides[-1] if self.rows[3] > 1 else 1)
 
     def backward_block(self, x, dy, want):
         a = _sln_abi.SlnBwdArgs()
@@ -159,6 +159,13 @@ def _check_weight(w, name, x, other):
         raise ValueError(f"weight and bias must be alike, got {tuple(other.shape)} {other.dtype} and {tuple(w.shape)} {w.dtype}")
 
 
+def _in_rows(x):
+    """x with up to four axes, and rows that the kernels read in place (x itself or a view where they can), else copied."""
+    if x.dim() > 4:
+        x = x.flatten(0, -2)
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
     """(x - mean) / sqrt(var + eps) weight + bias over the last axis; with center=False the mean is left out: x /
     sqrt(mean(x^2) + eps) weight + bias (RMS norm).
@@ -195,8 +202,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
         return layer_norm(x.float(), *(None if t is None else t.float() for t in (weight, bias)), e, center=center).double()
     if x.numel() == 0:  # no rows: connected to the inputs
         return x * 1 + sum((t.sum() * 0 for t in (weight, bias) if t is not None), torch.zeros((), device=x.device)).to(x.dtype)
-    rows = x.flatten(0, -2) if x.dim() > 4 else x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-    now = rows, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
+    now = _in_rows(x), None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
     plan = _Plan(*now, e, bool(center))
     if key is not None and all(a is b for a, b in zip(now, (x, weight, bias))):
         if len(_plans) > 4096:

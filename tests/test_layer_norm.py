@@ -1,5 +1,6 @@
 """Layer norm and RMS norm (tda_amd.layer_norm): refusals on the CPU, and on the GPU every output and gradient against
 the definition in float64, within the bounds of oracle/norm.py, which count half a step of the type for each rounding."""
+import ctypes
 import math
 
 import pytest
@@ -7,6 +8,7 @@ import torch
 
 import tda_amd
 from oracle import norm as oracle
+from tda_amd import _abi, _sln_abi, norm
 
 BF, F32, F16 = torch.bfloat16, torch.float32, torch.float16
 U = {BF: 2.0 ** -8, F32: 2.0 ** -24, F16: 2.0 ** -11, torch.float64: 2.0 ** -24}
@@ -117,6 +119,44 @@ def test_shapes():
         y = tda_amd.layer_norm(x, leaf)
         y.sum().backward()
         assert y.shape == shape and x.grad.shape == shape and not leaf.grad.any()
+
+
+def stepped(n, dtype=F32, device="cpu"):
+    """n axes, the last of every second value; and n axes whose last is one value, expanded."""
+    return (rows((2, 1, 3, 2, 4, 5)[6 - n + 1:] + (16,), 1, dtype, device)[..., ::2],
+            rows((2, 1, 3, 2, 4, 5)[6 - n + 1:] + (1,), 2, dtype, device).expand(*(2, 1, 3, 2, 4, 5)[6 - n + 1:], 8))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32, F16])
+@pytest.mark.parametrize("n", [2, 4, 5, 6])
+def test_a_last_axis_that_is_no_row(dtype, n):
+    """Every second value, and one value for all columns: whatever the number of axes, those are the values that are read
+    (axes beyond the fourth merge into a view, which keeps the last axis' stride)."""
+    w, b = rows((8,), 3, dtype), rows((8,), 4, dtype)
+    for x in stepped(n, dtype, "cuda"):
+        assert x.dim() == n and x.stride(-1) != 1
+        for dy in (rows(x.shape, 5, dtype), rows((*x.shape[:-1], 16), 6, dtype)[..., ::2], rows((), 7, dtype).expand(x.shape)):
+            check(x, w, b, dy)
+        check(x, None, None, dy, center=False)
+        assert torch.equal(tda_amd.layer_norm(x, w, b), tda_amd.layer_norm(x.contiguous(), w, b))
+
+
+@pytest.mark.parametrize("n", [2, 3, 4, 5, 6])
+def test_rows_for_the_kernels(n):
+    """The rows handed on have a unit last stride and hold x's values; a block of rows that do not is refused."""
+    for x in (*stepped(n), rows((2, 1, 3, 2, 4, 5)[6 - n + 1:] + (8,), 1, F32, "cpu").transpose(0, 1)):
+        r = norm._in_rows(x)
+        assert r.dim() <= 4 and r.stride(-1) == 1 and torch.equal(r.reshape(x.shape), x)
+    for x in stepped(n):
+        flat = x.flatten(0, -2) if n > 4 else x
+        a = _sln_abi.SlnFwdArgs.from_buffer_copy(norm._Plan(flat, None, None, 1e-5, True).block)
+        a.x.data = a.y.data = 64
+        assert a.x.stride[3] == flat.stride(-1) and _sln_abi.load().sln_validate_fwd(ctypes.byref(a)) == _abi.ERR_LAYOUT
+    one = rows((2, 1, 3, 2, 4, 5)[6 - n + 1:] + (16,), 1, F32, "cpu")[..., 3:4]
+    r = norm._in_rows(one)
+    a = _sln_abi.SlnFwdArgs.from_buffer_copy(norm._Plan(r, None, None, 1e-5, True).block)
+    assert list(a.x.stride)[-2:] == [16, 1] and r.data_ptr() == one.data_ptr()  # one value a row: read in place
 
 
 @gpu
