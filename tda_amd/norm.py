@@ -175,6 +175,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
     (batch, heads, seq_len, width): each head's own; x's dtype or float32, both alike.  Means and sums are
     float32.  Gradients flow to all three; second derivatives and forward-mode derivatives raise."""
     _refuse_tangents("layer_norm", x, weight, bias)
+    eps, center = float(eps), bool(center)  # their values: a plan must not go by which tensor holds them
     key = None
     if type(x) in _TENSORS and (weight is None or type(weight) in _TENSORS) and (bias is None or type(bias) in _TENSORS):
         key = _sig(x), None if weight is None else _sig(weight), None if bias is None else _sig(bias), eps, center
@@ -191,19 +192,18 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, center=True):
         raise ValueError(f"x must be float32, bfloat16, float16 or float64, got {x.dtype}")
     if not 1 <= x.shape[-1] <= _sln_abi.MAX_WIDTH:
         raise ValueError(f"the last axis must have 1 to {_sln_abi.MAX_WIDTH} values, got {x.shape[-1]}")
-    e = float(eps)
-    if not (e >= 0 and math.isfinite(e)):
+    if not (eps >= 0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     if weight is not None:
         _check_weight(weight, "weight", x, None)
     if bias is not None:
         _check_weight(bias, "bias", x, weight)
     if x.dtype == torch.float64:
-        return layer_norm(x.float(), *(None if t is None else t.float() for t in (weight, bias)), e, center=center).double()
+        return layer_norm(x.float(), *(None if t is None else t.float() for t in (weight, bias)), eps, center=center).double()
     if x.numel() == 0:  # no rows: connected to the inputs
         return x * 1 + sum((t.sum() * 0 for t in (weight, bias) if t is not None), torch.zeros((), device=x.device)).to(x.dtype)
     now = _in_rows(x), None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
-    plan = _Plan(*now, e, bool(center))
+    plan = _Plan(*now, eps, center)
     if key is not None and all(a is b for a, b in zip(now, (x, weight, bias))):
         if len(_plans) > 4096:
             _plans.clear()

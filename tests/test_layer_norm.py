@@ -285,6 +285,21 @@ def test_repeated_calls_look_at_their_arguments():
     assert tda_amd.layer_norm(x, same).grad_fn is not None
 
 
+@gpu
+def test_eps_and_center_held_by_tensors():
+    """A tensor whose value changes between two calls is read in each."""
+    x = rows((4, 96), 1, F32)
+    for device in ("cpu", "cuda"):
+        eps, center = torch.tensor(1e-5, dtype=torch.float64, device=device), torch.tensor(True, device=device)
+        for e, c in ((1e-5, True), (0.5, True), (0.5, False), (1e-5, False)):
+            eps.fill_(e), center.fill_(c)
+            for _ in range(2):
+                assert torch.equal(tda_amd.layer_norm(x, eps=eps, center=center), tda_amd.layer_norm(x, eps=e, center=c))
+        eps.fill_(-1.0)
+        with pytest.raises(ValueError, match="eps"):
+            tda_amd.layer_norm(x, eps=eps, center=center)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals_on_the_cpu():
     x = torch.zeros(2, 3, 4, 8)
