@@ -18,12 +18,13 @@ _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice
 def _words(args_type, names):
     """Where a call's arrays stand in its argument block, in pointers."""
     at = [args_type.at.offset + getattr(_spa_abi.SpaRows, n).offset for n in ("table", "lengths", "starts", "counts")]
-    return [o // 8 for o in (*at, *(getattr(args_type, n).offset for n in names))]
+    pools = [args_type.cache.offset + getattr(_spa_abi.SpaCache, n).offset for n in ("k1", "k2", "v")]
+    return [o // 8 for o in (*pools, *at, *(getattr(args_type, n).offset for n in names))]
 
 
-(_A_TABLE, _A_LENGTHS, _A_STARTS, _A_COUNTS, _A_K1, _A_K2, _A_V, _A_Q1, _A_Q2, _A_O1, _A_O2, _A_POS, _A_FREQ) = _words(
+(_A_POOL1, _A_POOL2, _A_POOLV, _A_TABLE, _A_LENGTHS, _A_STARTS, _A_COUNTS, _A_K1, _A_K2, _A_V, _A_Q1, _A_Q2, _A_O1, _A_O2, _A_POS, _A_FREQ) = _words(
     _spa_abi.SpaAppendArgs, ("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out", "positions", "inv_freq"))
-(_T_TABLE, _T_LENGTHS, _T_STARTS, _T_COUNTS, _T_Q1, _T_Q2, _T_OUT, _T_LAM, _T_WS) = _words(
+(_T_POOL1, _T_POOL2, _T_POOLV, _T_TABLE, _T_LENGTHS, _T_STARTS, _T_COUNTS, _T_Q1, _T_Q2, _T_OUT, _T_LAM, _T_WS) = _words(
     _spa_abi.SpaAttendArgs, ("q1", "q2", "out", "lambda_param", "workspace"))
 
 
@@ -48,7 +49,8 @@ class PagedKVCache:
 
     counts and starts are int32 or int64.  Rows of no sequence are not read, and are zero in what a call returns.
     The calls carry no gradient.  A cache's calls order themselves by their stream; two sequences that
-    write to one page are the caller's to keep apart (reading one is fine).  copy.deepcopy and pickling give a cache with
+    write to one page are the caller's to keep apart (reading one is fine).  A program may give the pages another storage of
+    their shape and type (cache.k1.data = ...): the next call uses it.  copy.deepcopy and pickling give a cache with
     pages of its own."""
 
     def __init__(self, pages: int, kv_heads: int, page_size: int, head_dim: int, v_head_dim: int | None = None, *,
@@ -73,12 +75,13 @@ class PagedKVCache:
         self._held = [torch.empty((pages, kv_heads, page_size, w), dtype=dtype, device=device) for w in (head_dim, head_dim, v_head_dim)]
         self._plans: dict = {}  # argument blocks of calls whose tensors need no copy, by their signature: no checks again
 
+    _at = None  # the pools' addresses when they were last looked at
     k1 = property(lambda self: self._held[0])
     k2 = property(lambda self: self._held[1])
     v = property(lambda self: self._held[2])
 
     def __getstate__(self):
-        return {**self.__dict__, "_plans": {}}  # a copy has pages of its own: their addresses too
+        return {**self.__dict__, "_plans": {}, "_at": None}  # a copy has pages of its own: their addresses too
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -87,14 +90,27 @@ class PagedKVCache:
             raise ValueError(f"tda_amd runs on the GPU only (HIP); got a cache on {self.device}")
 
     # -------------------------------------------------------------- calls
+    def _pools(self):
+        """The addresses of k1, k2 and v as they are now: a program may have given them another storage."""
+        k1, k2, v = self._held
+        at = k1.data_ptr(), k2.data_ptr(), v.data_ptr()
+        if at != self._at:
+            for t, name, w in zip(self._held, ("k1", "k2", "v"), (self.head_dim, self.head_dim, self.v_head_dim)):
+                shape = self.pages, self.kv_heads, self.page_size, w
+                if t.shape != shape or t.dtype != self.dtype or t.device != self.device or not t.is_contiguous():
+                    raise ValueError(f"the cache's {name} must be a contiguous {self.dtype} tensor of shape {shape} on {self.device}")
+                if t.untyped_storage().nbytes() < t.storage_offset() * t.element_size() + t.nbytes:
+                    raise ValueError(f"the cache's {name} has no storage")
+            self._at = at
+        return at
+
     def _start_block(self, args_type, at):
-        """A call's argument block with the cache, the sequences' shapes, and a mark at each array there is."""
+        """A call's argument block with the cache's and the sequences' shapes, and a mark at each array that not every call has."""
         table, _, starts, counts, rows = at
         a = args_type()
         a.abi_version, a.dtype = _spa_abi.ABI_VERSION, _CODE[self.dtype]
         c = a.cache
         c.pages, c.kv_heads, c.page_size, c.head_dim, c.v_head_dim = self.pages, self.kv_heads, self.page_size, self.head_dim, self.v_head_dim
-        c.k1, c.k2, c.v = (t.data_ptr() for t in self._held)
         a.at.sequences, a.at.rows, a.at.table_len = table.shape[0], rows, table.shape[1]
         a.at.table_stride = table.stride(0)
         a.at.table = a.at.lengths = 4
@@ -243,6 +259,7 @@ class PagedKVCache:
         k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions = tensors
         buf = bytearray(plan[0])
         put = memoryview(buf).cast("Q")
+        put[_A_POOL1], put[_A_POOL2], put[_A_POOLV] = self._pools()
         put[_A_K1], put[_A_K2], put[_A_V] = k1.data_ptr(), k2.data_ptr(), v.data_ptr()
         put[_A_TABLE], put[_A_LENGTHS] = table.data_ptr(), lengths.data_ptr()
         if starts is not None:
@@ -312,6 +329,7 @@ class PagedKVCache:
         buf = bytearray(block)
         put = memoryview(buf).cast("Q")
         out = torch.empty_strided(shape, strides, dtype=self.dtype, device=self.device)
+        put[_T_POOL1], put[_T_POOL2], put[_T_POOLV] = self._pools()
         put[_T_Q1], put[_T_Q2], put[_T_OUT], put[_T_LAM] = q1.data_ptr(), q2.data_ptr(), out.data_ptr(), lam.data_ptr()
         put[_T_TABLE], put[_T_LENGTHS] = table.data_ptr(), lengths.data_ptr()
         if starts is not None:

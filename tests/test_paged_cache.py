@@ -457,6 +457,43 @@ def test_copies_and_pickles_have_pages_of_their_own():
 
 
 @gpu
+def test_pages_that_get_another_storage():
+    """Calls of a signature that was seen before read and write where k1, k2 and v are now, not where they were; without
+    a storage, or with one of another shape or type, they are refused."""
+    s = Setup([1, 1], [10, 30], 4, 2, 64, 128, 16, BF, "even")
+    c, freq = s.cache, torch.rand(32).cuda()
+    run = lambda: step(s, s, freq)  # noqa: E731
+    want = [run() for _ in range(3)][-1]
+    filled = [t.clone() for t in s.pools()]
+    old = [t.detach() for t in s.pools()]  # the storages that they had, still in use
+    for t, x in zip(s.pools(), filled):
+        t.data = x.clone()
+    for t in old:
+        t.fill_(math.nan)
+    assert torch.equal(run(), want) and all(t.isnan().all() for t in old)
+    assert all(torch.equal(t, x) for t, x in zip(s.pools(), filled))
+    for t in s.pools():
+        t.untyped_storage().resize_(0)  # given back ...
+        with pytest.raises(ValueError, match="storage"):
+            run()
+        with pytest.raises(ValueError, match="storage"):
+            c.attend(s.q1, s.q2, 0.4, s.table, s.lengths)
+    for t, x in zip(s.pools(), filled):
+        t.untyped_storage().resize_(x.nbytes)  # ... and taken again
+        t.copy_(x)
+    assert torch.equal(run(), want)
+    for i, x in enumerate(filled):
+        for bad in (x[:2], x.float(), x.transpose(1, 2).contiguous().transpose(1, 2), x.cpu()):
+            c._held[i] = bad
+            with pytest.raises(ValueError, match="must be a contiguous"):
+                run()
+            with pytest.raises(ValueError, match="must be a contiguous"):
+                c.attend(s.q1, s.q2, 0.4, s.table, s.lengths)
+        c._held[i] = x
+    assert torch.equal(run(), want)
+
+
+@gpu
 def test_results_repeat():
     s = Setup([300, 1, 1, 40], [900, 5000, 3, 2000], 8, 2, 128, 128, 64, BF, "packed").spoil()
     want = s.attend()
