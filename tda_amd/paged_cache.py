@@ -192,9 +192,11 @@ class PagedKVCache:
         sequence, on every axis.  sections: how many pairs turn by each axis (default: all by one).  Without
         inv_freq rows enter as they are."""
         given = k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions
+        if sections is not None:
+            sections = tuple([int(s) for s in sections])
         key = self._signature(*given)
         if key is not None:
-            key = "append", key, None if sections is None else tuple([int(s) for s in sections]), bool(interleaved)
+            key = "append", key, sections, bool(interleaved)
             plan = self._plans.get(key)
             if plan is not None and not (k1.data_ptr() | k2.data_ptr() | v.data_ptr()
                                          | (0 if q1 is None else q1.data_ptr() | q2.data_ptr())) % 16:
@@ -241,7 +243,8 @@ class PagedKVCache:
         if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
             raise ValueError("inv_freq must be a 1-D float32 tensor")
         pairs = inv_freq.shape[0]
-        sections = (pairs,) if sections is None else tuple([int(s) for s in sections])
+        if sections is None:
+            sections = (pairs,)
         if not 1 <= len(sections) <= _sda_abi.MAX_AXES or min(sections) < 0:
             raise ValueError(f"sections must be 1 to {_sda_abi.MAX_AXES} counts of pairs, got {sections}")
         if pairs < 1 or sum(sections) != pairs or 2 * pairs > self.head_dim:

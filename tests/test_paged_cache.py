@@ -336,6 +336,22 @@ def test_append_positions():
 
 
 @gpu
+def test_append_sections_of_any_kind():
+    """A list, a tensor, something that can be gone through once: the first call of a kind and a planned one alike."""
+    kinds = [list, iter, lambda x: (n for n in x), torch.tensor, lambda x: map(int, x)]
+    want = None
+    for make in [tuple, *kinds, *kinds]:
+        s = Setup([30, 10], [3, 40], 2, 1, 64, 64, 32, F32, "packed")
+        for _ in range(2):
+            out = s.cache.append(s.k1, s.k2, s.v, s.table, s.lengths, s.q1, s.q2, **s.where, inv_freq=torch.rand(32, generator=torch.Generator().manual_seed(1)).cuda(),
+                                 sections=make((8, 12, 12)), positions=torch.arange(120).view(3, 1, 40).cuda())
+            want = want or [*out, *s.pools()]
+            assert all(torch.equal(a, b) for a, b in zip([*out, *s.pools()], want))
+    with pytest.raises(ValueError, match="add up"):
+        s.cache.append(s.k1, s.k2, s.v, s.table, s.lengths, **s.where, inv_freq=torch.rand(32).cuda(), sections=iter((8, 12)))
+
+
+@gpu
 def test_append_drops_what_has_no_place():
     s = Setup([9, 20, 6, 4], [10, 10, 40, 0], 4, 2, 64, 64, 16, BF, "packed")
     s.table[0, 0], s.table[1, 1], s.table[3, 0] = -1, s.cache.pages, 2 ** 31 - 1
