@@ -7,8 +7,8 @@ import ctypes
 import torch
 
 from . import _sda_abi, _spa_abi
-from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _new_rows, _raw_stream, _scale,
-                      _usable)
+from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _new_rows, _raw_stream,
+                      _refuse_tangents, _scale, _usable)
 
 _DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
 _PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -48,7 +48,7 @@ class PagedKVCache:
                 (sequences + 1,), not decreasing
 
     counts and starts are int32 or int64.  Rows of no sequence are not read, and are zero in what a call returns.
-    The calls carry no gradient.  A cache's calls order themselves by their stream; two sequences that
+    The calls carry no gradient, and refuse tensors with a forward-mode derivative.  A cache's calls order themselves by their stream; two sequences that
     write to one page are the caller's to keep apart (reading one is fine).  A program may give the pages another storage of
     their shape and type (cache.k1.data = ...): the next call uses it.  copy.deepcopy and pickling give a cache with
     pages of its own."""
@@ -192,6 +192,7 @@ class PagedKVCache:
         sequence, on every axis.  sections: how many pairs turn by each axis (default: all by one).  Without
         inv_freq rows enter as they are."""
         given = k1, k2, v, q1, q2, table, lengths, starts, counts, inv_freq, positions
+        _refuse_tangents("PagedKVCache.append", k1, k2, v, q1, q2, inv_freq)
         if sections is not None:
             sections = tuple([int(s) for s in sections])
         key = self._signature(*given)
@@ -291,6 +292,7 @@ class PagedKVCache:
         scale: default 1 / sqrt(head_dim).  most: the rows that any one sequence has, at most, where the caller
         knows them to be fewer than n; a wrong number costs time, not results."""
         given = q1, q2, lambda_param, table, lengths, starts, counts
+        _refuse_tangents("PagedKVCache.attend", q1, q2, lambda_param, *self._held)
         key = self._signature(*given) if (scale is None or type(scale) is float) and (most is None or type(most) is int) else None
         if key is not None:
             key = "attend", key, scale, most

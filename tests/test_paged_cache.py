@@ -510,6 +510,38 @@ def test_pages_that_get_another_storage():
 
 
 @gpu
+def test_forward_mode_derivatives_are_refused():
+    """Not dropped: the calls would return their results without a tangent."""
+    s = Setup([1, 1], [10, 30], 4, 2, 64, 64, 16, BF, "even")
+    names, lam, freq = ("k1", "k2", "v", "q1", "q2"), torch.tensor(0.4).cuda(), torch.rand(32).cuda()
+
+    def append(rows, freq):
+        return s.cache.append(rows["k1"], rows["k2"], rows["v"], s.table, s.lengths, rows["q1"], rows["q2"], inv_freq=freq)
+
+    def attend(rows, lam):
+        return s.cache.attend(rows["q1"], rows["q2"], lam, s.table, s.lengths)
+
+    plain = {n: getattr(s, n) for n in names}
+    append(plain, freq), attend(plain, lam)
+    want = [*s.pools(), attend(plain, lam)]
+    want = [t.clone() for t in want]
+    dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+    with torch.autograd.forward_ad.dual_level():
+        for n in names:
+            with pytest.raises(NotImplementedError, match="append"):
+                append({**plain, n: dual(plain[n])}, freq)
+        with pytest.raises(NotImplementedError, match="append"):
+            append(plain, dual(freq))
+        for n in ("q1", "q2"):
+            with pytest.raises(NotImplementedError, match="attend"):
+                attend({**plain, n: dual(plain[n])}, lam)
+        with pytest.raises(NotImplementedError, match="attend"):
+            attend(plain, dual(lam))
+        assert torch.equal(attend(plain, lam), want[3])  # tensors without one
+    assert all(torch.equal(a, b) for a, b in zip(s.pools(), want))
+
+
+@gpu
 def test_results_repeat():
     s = Setup([300, 1, 1, 40], [900, 5000, 3, 2000], 8, 2, 128, 128, 64, BF, "packed").spoil()
     want = s.attend()
