@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _sln_abi
-from .softmax import _CODE, _COMPUTE, _TENSORS, _new_rows, _raw_stream, _refuse_tangents, _sig
+from .softmax import _CODE, _COMPUTE, _TENSORS, _raw_stream, _refuse_tangents, _row_strides, _sig
 
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 # where a call's arrays stand in its argument block, in pointers
@@ -39,7 +39,7 @@ class _Plan:
         w = weight if weight is not None else bias
         self.shape, self.center = x.shape, center
         self.rows = (1,) * (4 - x.dim()) + tuple(x.shape)
-        self.strides = (_new_rows(x, x.shape[3]) if x.dim() == 4 else torch.empty(x.shape, device="meta")).stride()
+        self.strides = _row_strides(x, x.shape[3]) if x.dim() == 4 else torch.empty(x.shape, device="meta").stride()
         self.weight_dtype = _CODE[w.dtype if w is not None else x.dtype]
         self.weight_heads = int(w is not None and w.dim() == 2)
         self.bwd: dict = {}  # argument block and workspace, by the gradient's strides and the gradients wanted

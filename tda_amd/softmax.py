@@ -151,12 +151,17 @@ def _pad(t: torch.Tensor, d: int) -> torch.Tensor:
     return t if t.shape[-1] == d else F.pad(t, (0, d - t.shape[-1]))
 
 
+def _row_strides(like: torch.Tensor, width: int):
+    """Strides of dense (B, H, N, width) rows in like's memory order."""
+    h, n = max(like.shape[1], 1), max(like.shape[2], 1)
+    if h > 1 and n > 1 and like.stride(1) < like.stride(2):
+        return h * n * width, width, h * width, 1
+    return h * n * width, n * width, width, 1
+
+
 def _new_rows(like: torch.Tensor, width: int, dtype=None) -> torch.Tensor:
     """Uninitialised (B, H, N, width) rows in like's memory order."""
-    b, h, n, _ = like.shape
-    if h > 1 and n > 1 and like.stride(1) < like.stride(2):
-        return torch.empty((b, n, h, width), dtype=dtype or like.dtype, device=like.device).transpose(1, 2)
-    return torch.empty((b, h, n, width), dtype=dtype or like.dtype, device=like.device)
+    return torch.empty_strided((*like.shape[:3], width), _row_strides(like, width), dtype=dtype or like.dtype, device=like.device)
 
 
 # ------------------------------------------------------------------ calls

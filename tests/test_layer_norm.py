@@ -286,6 +286,25 @@ def test_repeated_calls_look_at_their_arguments():
 
 
 @gpu
+def test_memory_of_a_call():
+    """A call takes its result and the copy of rows that it cannot read in place, and no more: neither the first of its kind
+    nor one that is planned anew each time."""
+    size = 2 * 8 * 1024 * 128 * 2
+
+    def taken(x):
+        total = lambda: torch.cuda.memory_stats()["allocated_bytes.all.allocated"]  # noqa: E731
+        before = total()
+        assert tda_amd.layer_norm(x).nbytes == size
+        return total() - before
+
+    x = rows((2, 8, 1024, 256), 1, BF)
+    whole = x[..., :128].contiguous()
+    for _ in range(2):
+        assert taken(whole) == size and taken(whole.transpose(1, 2)) == size
+        assert taken(x[..., :128]) == size and taken(x[..., ::2]) == 2 * size
+
+
+@gpu
 def test_eps_and_center_held_by_tensors():
     """A tensor whose value changes between two calls is read in each."""
     x = rows((4, 96), 1, F32)
