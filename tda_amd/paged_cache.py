@@ -7,8 +7,8 @@ import ctypes
 import torch
 
 from . import _sda_abi, _spa_abi
-from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _new_rows, _raw_stream,
-                      _refuse_tangents, _scale, _usable)
+from .softmax import (_CODE, _TENSORS, _check_heads, _check_rows, _ints, _lambda, _lambda_strides, _raw_stream,
+                      _refuse_tangents, _row_strides, _scale, _usable)
 
 _DIMS = ((64, 64), (64, 128), (128, 128), (128, 256))
 _PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -220,17 +220,19 @@ class PagedKVCache:
         rows = [t if t is None else _usable(t) for t in (k1, k2, v, q1, q2)]
         a = self._start_block(_spa_abi.SpaAppendArgs, at)
         a.heads = h
-        out = [] if q1 is None else [_new_rows(t, d) for t in rows[3:]]
-        for name, t in zip(("k1", "k2", "v", "q1", "q2", "q1_out", "q2_out"), rows + out):
+        out = [] if q1 is None else [(t.shape, _row_strides(t, d)) for t in rows[3:]]
+        for name, t in zip(("k1", "k2", "v", "q1", "q2"), rows):
             if t is not None:
                 getattr(a, name).stride[:] = t.stride()
+        for name, (_, strides) in zip(("q1_out", "q2_out"), out):
+            getattr(a, name).stride[:] = strides
         if inv_freq is not None:
             a.rot, a.axes, a.interleaved = 2 * inv_freq.shape[0], len(sections), int(interleaved)
             a.sections[:len(sections)] = sections
             if positions is not None:
                 a.position_stride[:] = positions.stride()
                 a.position_dtype = positions.element_size()
-        plan = bytes(a), [(t.shape, t.stride()) for t in out]
+        plan = bytes(a), out
         now = (*rows, *at[:4], inv_freq, positions)
         if key is not None and all(x is y for x, y in zip(now, given)):
             self._plan(key, *plan)
@@ -314,15 +316,15 @@ class PagedKVCache:
         if n == 0 or table.shape[0] == 0:
             return torch.zeros((b, h, n, self.v_head_dim), dtype=self.dtype, device=self.device)
         q1, q2 = _usable(q1), _usable(q2)
-        out = _new_rows(q1, self.v_head_dim)
+        strides = _row_strides(q1, self.v_head_dim)
         a = self._start_block(_spa_abi.SpaAttendArgs, at)
         a.heads, a.most, a.scale = h, most, s
-        for name, t in zip(("q1", "q2", "out"), (q1, q2, out)):
-            getattr(a, name).stride[:] = t.stride()
+        for name, st in zip(("q1", "q2", "out"), (q1.stride(), q2.stride(), strides)):
+            getattr(a, name).stride[:] = st
         a.lambda_stride[:] = _lambda_strides(lam)
         a.lambda_dtype = _CODE[lam.dtype]
         a.workspace_bytes = _spa_abi.load().spa_attend_workspace_bytes(ctypes.byref(a))
-        plan = bytes(a), out.shape, out.stride(), a.workspace_bytes
+        plan = bytes(a), (b, h, n, self.v_head_dim), strides, a.workspace_bytes
         now = (q1, q2, lam, *at[:4])
         if key is not None and all(x is y for x, y in zip(now, given)):
             self._plan(key, *plan)

@@ -510,6 +510,30 @@ def test_pages_that_get_another_storage():
 
 
 @gpu
+@pytest.mark.parametrize("form", ["packed", "counts"])
+def test_memory_of_a_call(form):
+    """The first call of a kind takes as much as the next ones: its results, and the attention's workspace."""
+    s = Setup([301, 1], [70, 600], 8, 2, 64, 128, 64, BF, form)
+    size = s.lead * 8 * s.n * 2
+
+    def peak(call):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = call()
+        taken = torch.cuda.max_memory_allocated() - before
+        assert len(got) in (1, 2)
+        return taken
+
+    rounded = lambda n: -(-n // 512) * 512  # noqa: E731
+    append = [peak(lambda: s.cache.append(s.k1, s.k2, s.v, s.table, s.lengths, s.q1, s.q2, **s.where)) for _ in range(3)]
+    assert append == [2 * rounded(64 * size)] * 3
+    lam = torch.tensor(0.4).cuda()
+    attend = [peak(lambda: [s.cache.attend(s.q1, s.q2, lam, s.table, s.lengths, **s.where)]) for _ in range(3)]
+    assert attend == [attend[-1]] * 3 and attend[0] >= rounded(128 * size)
+
+
+@gpu
 def test_forward_mode_derivatives_are_refused():
     """Not dropped: the calls would return their results without a tangent."""
     s = Setup([1, 1], [10, 30], 4, 2, 64, 64, 16, BF, "even")
