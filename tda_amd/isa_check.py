@@ -34,6 +34,7 @@ from . import build as _build
 
 STORES = ("ds_write", "ds_store", "global_store", "buffer_store", "flat_store", "global_atomic",
           "buffer_atomic", "flat_atomic", "ds_add", "ds_bpermute", "ds_permute")
+RESTORES = ("s_or_b64 exec, exec,", "s_or_saveexec_b64", "s_mov_b64 exec,")  # of lanes that a branch left out
 
 
 def _regs(tok: str) -> set:
@@ -139,7 +140,13 @@ def scan_function(body: list) -> list:
 def masked_spills(body: list) -> list:
     """Spills that a join of control flow places before the lanes that skipped the branch are back: those lanes would reload
     what they never stored.  hipcc was seen to do so at the end of a branch of the lanes around loads, in a kernel out of
-    registers, with an address."""
+    registers, with an address.
+
+    Found are stores to scratch memory and writes of a vector register to an accumulator register (both leave out the lanes
+    that are off) between the label that a branch on an empty mask leads to and the instruction that brings lanes back: an
+    s_or_b64 of the mask with the lanes left out, an s_or_saveexec_b64 (the way into an else), an s_mov_b64 to the mask.  Not found
+    are copies from one vector register to another, which are what a branch's results look like, and spills behind a
+    further branch.  A spill of a scalar register (v_writelane_b32) takes no notice of the mask."""
     joins = {_split(s)[1][0] for kind, s in body if kind == "ins" and s.startswith("s_cbranch_execz")}
     out, at = [], None
     for kind, s in body:
@@ -147,9 +154,9 @@ def masked_spills(body: list) -> list:
             at = s if s in joins else None
             seen = []
         elif at and kind == "ins":
-            if s.startswith("scratch_store"):
+            if s.startswith("scratch_store") or s.startswith("v_accvgpr_write") and _split(s)[1][1].startswith("v"):
                 seen.append((at, s))
-            elif s.startswith("s_or_b64 exec, exec,"):
+            elif s.startswith(RESTORES):
                 out += seen
                 at = None
             elif "exec" in s.split(",")[0] or s.startswith(("s_branch", "s_cbranch")):

@@ -42,6 +42,23 @@ def test_scanner_accepts_spills_of_all_lanes_and_of_a_branch():
 \ts_or_b64 exec, exec, s[4:5]""") == []
 
 
+def test_scanner_flags_spills_to_accumulator_registers():
+    assert _spills(BRANCH + """\tv_accvgpr_write_b32 a12, v98
+\tv_accvgpr_write_b32 a13, 0
+\tv_accvgpr_write_b32 a14, s3
+\tv_writelane_b32 v255, s34, 2
+\tv_accvgpr_read_b32 v4, a9
+\ts_or_b64 exec, exec, s[6:7]
+\tv_accvgpr_write_b32 a15, v99""") == [(".LBB0_2", "v_accvgpr_write_b32 a12, v98")]
+
+
+@pytest.mark.parametrize("back", ["s_or_b64 exec, exec, s[6:7]", "s_or_saveexec_b64 s[4:5], s[6:7]", "s_mov_b64 exec, s[6:7]"])
+@pytest.mark.parametrize("spill", ["scratch_store_dword off, v98, off", "v_accvgpr_write_b32 a12, v98"])
+def test_scanner_knows_each_way_back(back, spill):
+    assert _spills(BRANCH + f"\t{spill}\n\t{back}") == [(".LBB0_2", spill)]
+    assert _spills(BRANCH + f"\t{back}\n\t{spill}") == []
+
+
 def test_kernels_are_read_to_their_end():
     body = isa_check._functions("_Z1kv:\n\ts_cbranch_scc1 .LBB0_2\n\ts_endpgm\n.LBB0_2:\n\tv_mov_b32_e32 v3, 0\n\ts_endpgm\n.Lfunc_end0:\n\tv_nop\n")["_Z1kv"]
     assert [kind for kind, _ in body] == ["ins", "end", "label", "ins", "end"]
