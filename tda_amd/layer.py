@@ -199,10 +199,11 @@ class DifferentialAttention(nn.Module):
         return Int4KVCache(batch, self.kv_heads, capacity, self.head_dim, self.v_head_dim,
                            device=self.in_proj.weight.device)
 
-    def new_paged_cache(self, pages: int, page_size: int = 64) -> PagedKVCache:
-        """Pages for this layer's keys and values, of its weights' type and on their device."""
+    def new_paged_cache(self, pages: int, page_size: int = 64, *, dtype=None) -> PagedKVCache:
+        """Pages for this layer's keys and values, on its weights' device and of their type, or of dtype: that in which the
+        projection comes out, where the layer runs under torch.autocast."""
         w = self.in_proj.weight
-        return PagedKVCache(pages, self.kv_heads, page_size, self.head_dim, self.v_head_dim, dtype=w.dtype, device=w.device)
+        return PagedKVCache(pages, self.kv_heads, page_size, self.head_dim, self.v_head_dim, dtype=dtype or w.dtype, device=w.device)
 
     def project(self, x: torch.Tensor):
         """The (B, H or Hk, N, d or dv) views of the projected q1, q2, k1, k2, v.  They come from one split,

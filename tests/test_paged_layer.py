@@ -130,6 +130,32 @@ def test_serving_gives_what_the_whole_sequences_give(kw, form):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_serving_under_autocast(dtype):
+    """A float32 layer whose projections come out in 16 bits, over pages of that type: the operators one by one give the
+    same.  Pages of the weights' type are refused."""
+    m = layer(head_norm=True, v_head_dim=128, rotary_sections=(16, 8))
+    x = torch.randn(1, 45, 96, generator=torch.Generator().manual_seed(8)).cuda()
+    where = {"table": ints(3, 1, 0, 4).view(2, 2), "lengths": ints(0, 9), "starts": ints(0, 30, 45)}
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        caches = [m.new_paged_cache(6, 16, dtype=dtype) for _ in range(2)]
+        assert caches[0].dtype == dtype and m.new_paged_cache(6, 16).dtype == F32
+        for c in caches:
+            for t in (c.k1, c.k2, c.v):
+                t.fill_(0.25)
+        got = m(x, cache=caches[0], **where)
+        q1, q2, k1, k2, v = m.project(x)
+        assert q1.dtype == dtype and got.dtype == dtype
+        q1, q2 = caches[1].append(k1, k2, v, q1=q1, q2=q2, **where, inv_freq=m._frequencies(), sections=(16, 8))
+        o = caches[1].attend(q1, q2, m.lambda_param, **where)
+        o = tda_amd.layer_norm(o, m.norm_weight, eps=m.norm_eps, center=False)
+        assert torch.equal(got, m.out_proj(o.transpose(1, 2).flatten(2)))
+        assert all(torch.equal(a, b) for a, b in zip(caches[0]._held, caches[1]._held))
+        with pytest.raises(ValueError, match="holds"):
+            m(x, cache=m.new_paged_cache(6, 16), **where)
+
+
+@gpu
 def test_padding_gives_the_bias():
     m = layer(bias=True, head_norm=True)
     x = torch.randn(1, 12, 96, device="cuda")
