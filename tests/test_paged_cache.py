@@ -566,6 +566,37 @@ def test_forward_mode_derivatives_are_refused():
 
 
 @gpu
+@pytest.mark.parametrize("dtype, hk, page, d, dv", [(BF, 8, 256, 128, 128), (F32, 1, 16, 64, 128)])
+def test_pools_past_31_bits(dtype, hk, page, d, dv):
+    """Pages behind 2^31 values (and 2^32 bytes) of the pools, next to the first ones: rows land there and are read from
+    there, as in a small cache whose pages hold the same."""
+    far = 2 ** 31 // (hk * page * d) + 9
+    at = [0, far - 1, 1, far - 2, *range(far - 3, far - 9, -1)]  # where the pages of the small one stand
+    s = Setup([90, 1, 1], [40, 130, 7], 8, hk, d, dv, page, dtype, "packed", spare=3)
+    small, n = s.cache, s.cache.pages
+    at += range(far - 9, far - 9 - n, -1)
+    big = tda_amd.PagedKVCache(far, hk, page, d, dv, dtype=dtype)
+    assert all(t.numel() > 2 ** 31 and t[far - 8:].data_ptr() - t.data_ptr() > 2 ** 32 - 1 for t in (big.k1, big.k2, big.v))
+    idx = torch.tensor(at[:n]).cuda()
+    for a, b in zip((small.k1, small.k2, small.v), (big.k1, big.k2, big.v)):
+        for i in range(n):
+            b[at[i]] = a[i]
+    table = torch.where(s.table >= 0, idx.to(torch.int32)[s.table.clamp_min(0).long()], -1)
+    freq = torch.rand(d // 2).cuda()
+    for new in ([90, 1, 1], [1, 1, 1]):
+        where = {"starts": ints(*[sum(new[:i]) for i in range(4)])}
+        x = [t[:, :, :sum(new)] for t in (s.k1, s.k2, s.v, s.q1, s.q2)]
+        got = [c.append(*x[:3], t, s.lengths, *x[3:], **where, inv_freq=freq) for c, t in ((small, s.table), (big, table))]
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        for a, b in zip((small.k1, small.k2, small.v), (big.k1, big.k2, big.v)):
+            assert all(torch.equal(a[i], b[at[i]]) for i in range(n))
+        want = small.attend(*got[0], 0.4, s.table, s.lengths, **where)
+        assert want.any() and torch.equal(big.attend(*got[1], 0.4, table, s.lengths, **where), want)
+    del big, a, b
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_results_repeat():
     s = Setup([300, 1, 1, 40], [900, 5000, 3, 2000], 8, 2, 128, 128, 64, BF, "packed").spoil()
     want = s.attend()
