@@ -42,7 +42,7 @@ class _Plan:
         self.strides = _row_strides(x, x.shape[3]) if x.dim() == 4 else torch.empty(x.shape, device="meta").stride()
         self.weight_dtype = _CODE[w.dtype if w is not None else x.dtype]
         self.weight_heads = int(w is not None and w.dim() == 2)
-        self.bwd: dict = {}  # argument block and workspace, by the gradient's strides and the gradients wanted
+        self.bwd: dict = {}  # argument block and workspace, by what _backward finds
         a = _sln_abi.SlnFwdArgs()
         self.head(a, x)
         a.eps = eps
@@ -59,7 +59,7 @@ class _Plan:
         """The strides of four axes.  The last one as it is, for sln_fwd and sln_bwd to check; along one value any will do."""
         return (*(0,) * (4 - len(strides)), *strides[:-1], strides[-1] if self.rows[3] > 1 else 1)
 
-    def backward_block(self, x, dy, want):
+    def backward_block(self, key, x, dy, want):
         a = _sln_abi.SlnBwdArgs()
         self.head(a, x)
         a.dy.stride[:] = self.four(dy.stride())
@@ -69,7 +69,7 @@ class _Plan:
         a.workspace_bytes = _sln_abi.load().sln_bwd_workspace_bytes(ctypes.byref(a))
         if len(self.bwd) > 64:
             self.bwd.clear()
-        got = self.bwd[dy.stride(), want] = bytes(a), a.workspace_bytes
+        got = self.bwd[key] = bytes(a), a.workspace_bytes
         return got
 
     def forward(self, x, weight, bias, stats):
@@ -99,12 +99,15 @@ _plans: dict = {}  # by signature, of calls whose tensors need no copy: no check
 def _backward(ctx, dy):
     x, weight, stats = ctx.saved_tensors
     plan, bias = ctx.cfg
+    # as they are now: a hook on saved tensors may have brought back copies with other strides
+    x, weight, stats = _in_rows(x), None if weight is None else weight.contiguous(), stats.contiguous()
     want = ctx.needs_input_grad[:3]
     if dy.dtype != x.dtype:
         dy = dy.to(x.dtype)
     if dy.stride(-1) != 1 and dy.shape[-1] > 1:
         dy = dy.contiguous()
-    block, size = ctx.block if dy.stride() == plan.strides and ctx.block else plan.bwd.get((dy.stride(), want)) or plan.backward_block(x, dy, want)
+    key = x.stride(), x.dtype, dy.stride(), want
+    block, size = plan.bwd.get(key) or plan.backward_block(key, x, dy, want)
     buf = bytearray(block)
     put = memoryview(buf).cast("Q")
     dx = dw = db = None
@@ -136,7 +139,6 @@ class _LayerNorm(torch.autograd.Function):
         stats = torch.empty(plan.rows[:3] + (2,), dtype=torch.float32, device=x.device)
         ctx.save_for_backward(x, weight, stats)
         ctx.cfg = plan, None if bias is None else (bias.shape, bias.dtype)
-        ctx.block = plan.bwd.get((plan.strides, ctx.needs_input_grad[:3]))
         return plan.forward(x, weight, bias, stats)
 
     @staticmethod

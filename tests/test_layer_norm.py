@@ -1,5 +1,6 @@
 """Layer norm and RMS norm (tda_amd.layer_norm): refusals on the CPU, and on the GPU every output and gradient against
 the definition in float64, within the bounds of oracle/norm.py, which count half a step of the type for each rounding."""
+import contextlib
 import ctypes
 import math
 
@@ -283,6 +284,47 @@ def test_repeated_calls_look_at_their_arguments():
     assert tda_amd.layer_norm(x, leaf).requires_grad
     same = torch.nn.Parameter(w.clone())
     assert tda_amd.layer_norm(x, same).grad_fn is not None
+
+
+def test_backward_block_of_saved_rows():
+    """The argument block goes by the strides of the rows that the backward is given."""
+    x = rows((4, 30, 6, 80), 1, F32, "cpu").transpose(1, 2)[..., 3:40]
+    plan = norm._Plan(x, None, None, 1e-5, True)
+    dy, want = torch.empty_strided(plan.shape, plan.strides), (True, False, False)
+    for t in (x, x.contiguous(), x):
+        key = t.stride(), t.dtype, dy.stride(), want
+        block, _ = plan.bwd.get(key) or plan.backward_block(key, t, dy, want)
+        assert list(_sln_abi.SlnBwdArgs.from_buffer_copy(block).x.stride) == list(t.stride())
+
+
+@gpu
+@pytest.mark.parametrize("first", ["plain", "moved"])
+def test_saved_tensors_that_hooks_move(first):
+    """Rows kept on the host (or anywhere) between the passes come back with other strides: the gradients are those of rows
+    that stayed, for a call of either kind after the other."""
+    w, b = rows((6, 37), 2, BF), rows((6, 37), 3, BF)
+    base = rows((4, 30, 6, 80), 1, BF)
+    for x in (base.transpose(1, 2)[..., 3:40], base.transpose(1, 2)[:, :, ::2, 5:42], base[0, 0, :, :37]):
+        args = (x, w, b) if x.dim() == 4 else (x, w[0], b[0])
+        dy = rows(x.shape, 4, BF)
+        dy = dy.transpose(1, 2).contiguous().transpose(1, 2) if x.dim() == 4 else dy
+
+        def grads(hooks):
+            leaves = [t.detach().requires_grad_(True) for t in args]
+            with hooks:
+                y = tda_amd.layer_norm(*leaves)
+            return torch.autograd.grad(y, leaves, dy)
+
+        moved = lambda: torch.autograd.graph.save_on_cpu()  # noqa: E731
+        wide = lambda: torch.autograd.graph.saved_tensors_hooks(  # noqa: E731
+            lambda t: t, lambda t: torch.nn.functional.pad(t, (0, 11))[..., :-11] if t.shape == x.shape else t)
+        apart = lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack((t, t), -1)[..., 0])  # noqa: E731
+        stay = contextlib.nullcontext
+        want = None
+        for hooks in ([stay, moved, wide, apart, stay] if first == "plain" else [moved, apart, wide, stay, moved]):
+            got = grads(hooks())
+            want = want or got
+            assert all(torch.equal(a, c) for a, c in zip(got, want))
 
 
 @gpu
