@@ -8,8 +8,9 @@
 // columns of every row, so it keeps the sums of dw and db in registers over all its rows; a workgroup leaves one row of
 // them, and a second launch adds those up in order (where there are few rows, one workgroup takes them all and writes the
 // result).  All sums are 32 bits; the variance is taken around the mean (of a wave, joined by the waves' means).
-// Bound by memory, each value read and written once a pass: rows of 128, bf16, 2^18 of them, 31 us forward and 46 backward (4.3
-// TB/s); rows of 4096, 16384 of them, 60 and 82 (4.5 TB/s).
+// Bound by memory, each value read and written once a pass.  bf16, kernels within training steps, one run: 2^18 rows of 128, forward 24 us
+// (134 MB, 5.5 TB/s), backward 44 (201 MB, 4.6 TB/s); 16384 rows of 4096, 58 (268 MB, 4.6 TB/s) and 79 (403 MB, 5.1 TB/s).  Another
+// part took 31 and 47, 60 and 80.
 #include "sda_common.hpp"
 #include "sln_params.hpp"
 
@@ -377,8 +378,9 @@ __global__ void __launch_bounds__(256) norm_sums(Params P) {
 template <class T, bool WHOLE, int L, int C, int U>
 static int fwd(const Params& p, hipStream_t st) {
   constexpr int TH = L <= 64 ? 256 : L, PER = TH / L * U;
-  // Workgroups that each take a few rows: the loads of one are on their way while others sum (2^18 rows of 128: 31.0 us, with 2048 32.6;
-  // 16384 rows of 4096, whose weights each workgroup reads: 62.6 with 4096, 65 with half as many, 88 with four times).
+  // Workgroups that each take a few rows: the loads of one are on their way while others sum.  The run of the figures above: 2^18 rows of 128
+  // 24.3 us, with 2048 workgroups 25.0; 16384 rows of 4096, whose weights each workgroup reads, 58 with 4096, 56 with half as many, 80 with
+  // four times (the other part: 62.6, 65 and 88).
   const int64_t most = ((int64_t)p.rows + PER - 1) / PER, want = ((L <= 64 ? 16384 : 4096 * 256 / TH) + p.groups - 1) / p.groups;
   const int blocks = (int)(most < want ? most : want);
   norm_fwd<T, WHOLE, L, C, U><<<tda::grid_of<TH>((int64_t)blocks * p.groups), TH, 0, st>>>(p, blocks);

@@ -46,6 +46,9 @@ __device__ __forceinline__ typename Tr::frag load8(__amdgpu_buffer_rsrc_t r, uin
 // branches), transposed scores, keys and values by direct loads to LDS a stage ahead.  A stage's rows come from pages: one
 // load instruction takes 1 KB, 1 to 8 rows that lie in one page (pages are 16 rows or more), whose number a wave has in a
 // register of 64 table entries.
+// Weights are rounded to the rows' type for their product with the values, in both forms, as sda_fwd.hip rounds them: a product of 32 bits has
+// an eighth of the rate or less.  With the output's own rounding that is 2.4e-3 of the output's norm in bf16 (weights in 32 bits: 1.7e-3) and 3.0e-4
+// in fp16 (2.1e-4).  Sums of weights are taken before the rounding, in 32 bits.
 // Bound by the matrix cores and the exponentials and LDS reads between their products, at the clock that the card's power leaves: 2048 rows
 // behind 30000, bf16, 16 over 4 heads of 128: 985 us, 1.06 PFLOP/s, where a large library product reaches 1.23 to 1.32.  128 keys of
 // a tile take a CU 3.9 us at (128, 128) and 4.3 at (64, 128), whose exponentials are as many.
