@@ -138,7 +138,8 @@ class DifferentialAttention(nn.Module):
         lambda_init: initial weight of the second branch, learned per head.
         bias: biases on the projections.
         head_norm: normalise each head's output by its root mean square (with norm_eps, above 0: a row that saw no key
-            is zeros, and zero by zero is NaN) and weigh its values, alike in every head; the weights are learned and start at 1 - lambda_init, the scale of a difference of maps.
+            is zeros, and zero by zero is NaN) and weigh its values, alike in every head; the weights are learned and
+            start at 1 - lambda_init, the scale of a difference of maps.
     """
 
     def __init__(self, embed_dim: int, num_heads: int, head_dim: int | None = None, *, kv_heads: int | None = None,

@@ -165,6 +165,18 @@ def test_a_few_tiles_more_than_fit_at_once(dtype, d, dv):
 
 
 @gpu
+@pytest.mark.parametrize("dtype, d, dv", [(BF, 128, 128), (F16, 64, 128)])
+def test_tiles_that_stay_whole(dtype, d, dv):
+    """A padded batch too large for its tiles to be cut, most of it padding; one long sequence among as many short ones as
+    are taken whole."""
+    s = Setup([700] + [1] * 23, [3000 - 60 * i for i in range(24)], 8, 2, d, dv, 32, dtype, "counts").spoil()
+    got = s.attend()
+    assert not got[1:, :, 1:].any()
+    Setup([1] * 64, [20 + i for i in range(63)] + [20000], 16, 8, d, dv, 64, dtype, "even").spoil().attend()
+    Setup([1] * 64, [20000] + [20 + i for i in range(63)], 16, 8, d, dv, 64, dtype, "packed").spoil().attend()
+
+
+@gpu
 def test_the_rows_bound_costs_no_results():
     s = Setup([1, 50, 1], [40, 300, 1000], 8, 2, 64, 64, 16, BF, "packed").spoil()
     want = s.attend()
